@@ -55,6 +55,15 @@ EXPORTED_SYMBOLS = (
     "altob200_spread_rows",
     "altob200_swiglu_forward",
     "altob200_swiglu_backward",
+    "altob200_swiglu_keep_forward",
+    "altob200_swiglu_kept_backward",
+    "altob200_rms_norm_forward",
+    "altob200_rms_norm_backward_work_bytes",
+    "altob200_rms_norm_backward",
+    "altob200_route_forward",
+    "altob200_route_backward",
+    "altob200_expert_plan_work_bytes",
+    "altob200_expert_plan",
     "altob200_dge_scale",
     "altob200_deosc_accumulate",
     "altob200_linear_backward_work_bytes",
@@ -138,6 +147,26 @@ class LinearBackwardArgs(C.Structure):
         (n, C.c_int32) for n in ("format", "dtype", "use_outer", "use_sr", "rht_n")]
 
 
+class RmsNormArgs(C.Structure):
+    """``altob200_rms_norm_args`` of the header."""
+    _fields_ = [(n, C.c_int64) for n in ("rows", "cols", "ld_x", "ld_residual")] + [
+        (n, C.c_void_p) for n in ("x", "residual", "weight", "out", "stream_out", "scale_plain", "scale_packed")] + [
+        ("eps", C.c_float)] + [(n, C.c_int32) for n in ("dtype", "weight_dtype", "format")]
+
+
+class RmsNormGradArgs(C.Structure):
+    """``altob200_rms_norm_grad_args`` of the header."""
+    _fields_ = [(n, C.c_int64) for n in ("rows", "cols", "ld_grad", "ld_stream", "ld_grad_stream")] + [
+        (n, C.c_void_p) for n in ("grad_out", "stream", "grad_stream", "weight", "grad_in", "grad_weight")] + [
+        ("eps", C.c_float)] + [(n, C.c_int32) for n in ("dtype", "weight_dtype")]
+
+
+class RouteParams(C.Structure):
+    """``altob200_route_params`` of the header."""
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "experts", "top_k", "sigmoid", "num_groups", "groups_kept", "group_top",
+                                         "renormalize")] + [("scale", C.c_float)]
+
+
 class Altob200Error(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -218,6 +247,24 @@ def _declare_more(lib):
     lib.altob200_deosc_accumulate.argtypes = [vp, vp, vp, vp, vp, vp, i64, i32, vp]
     lib.altob200_dge_scale.restype = C.c_int
     lib.altob200_dge_scale.argtypes = [vp, i32, i64, i64, i64, vp, C.POINTER(C.c_float), vp]
+    lib.altob200_swiglu_keep_forward.restype = C.c_int
+    lib.altob200_swiglu_keep_forward.argtypes = [vp, i64, i64, i64, i32, vp, vp, vp, vp]
+    lib.altob200_swiglu_kept_backward.restype = C.c_int
+    lib.altob200_swiglu_kept_backward.argtypes = [vp, vp, vp, i64, i64, i32, vp, vp]
+    lib.altob200_rms_norm_forward.restype = C.c_int
+    lib.altob200_rms_norm_forward.argtypes = [C.POINTER(RmsNormArgs), vp]
+    lib.altob200_rms_norm_backward_work_bytes.restype = i64
+    lib.altob200_rms_norm_backward_work_bytes.argtypes = [C.POINTER(RmsNormGradArgs)]
+    lib.altob200_rms_norm_backward.restype = C.c_int
+    lib.altob200_rms_norm_backward.argtypes = [C.POINTER(RmsNormGradArgs), vp, vp]
+    lib.altob200_route_forward.restype = C.c_int
+    lib.altob200_route_forward.argtypes = [C.POINTER(RouteParams), vp, i64, i64, vp, vp, vp, vp]
+    lib.altob200_route_backward.restype = C.c_int
+    lib.altob200_route_backward.argtypes = [C.POINTER(RouteParams), vp, i64, i64, vp, vp, vp, vp]
+    lib.altob200_expert_plan_work_bytes.restype = i64
+    lib.altob200_expert_plan_work_bytes.argtypes = [i64, i32]
+    lib.altob200_expert_plan.restype = C.c_int
+    lib.altob200_expert_plan.argtypes = [vp, i32, i64, i32, i32, i32, i64, vp, vp, vp, vp, vp, vp, vp]
     ms = C.POINTER(MacroScaleDesc)
     lib.altob200_gemm_mxfp4_two_level.restype = C.c_int
     lib.altob200_gemm_mxfp4_two_level.argtypes = [i64, i64, i64, vp, vp, ms, vp, vp, ms, C.c_float, i32, vp, i64, vp]
@@ -283,6 +330,18 @@ def _require_cuda(*tensors: Optional[torch.Tensor]) -> None:
 def on_current_device(t: torch.Tensor) -> bool:
     """Whether a kernel launched here may read ``t``: launches go to the current device's stream."""
     return t.is_cuda and t.device.index == torch.cuda.current_device()
+
+
+def on_device_of(fn):
+    """Decorator: the call runs with the device of its first tensor argument current, so that its launches and
+    allocations go there and to that device's stream."""
+    @functools.wraps(fn)
+    def inner(t, *args, **kwargs):
+        if t.device.index == torch._C._cuda_getDevice():
+            return fn(t, *args, **kwargs)
+        with torch.cuda.device(t.device):
+            return fn(t, *args, **kwargs)
+    return inner
 
 
 def packed_scale_bytes(rows: int, ncols: int) -> int:
@@ -568,6 +627,82 @@ def pack_scales(scales: torch.Tensor, rows: int, block: int) -> torch.Tensor:
     return out
 
 
+@on_device_of
+def rms_norm_forward(x2: torch.Tensor, weight: torch.Tensor, eps: float, residual2: Optional[torch.Tensor] = None,
+                     fmt: int = -1, packed: bool = False):
+    """(out, stream, scales): x2 [rows, cols] with unit column stride, rows of any stride that do not overlap; ``stream`` is
+    None without a residual, ``scales`` without an 8-bit format (plain, or the packed layout)."""
+    rows, cols = x2.shape
+    out = torch.empty(rows, cols, dtype=x2.dtype if fmt < 0 else torch.uint8, device=x2.device)
+    stream = None if residual2 is None else torch.empty(rows, cols, dtype=x2.dtype, device=x2.device)
+    scales = None
+    a = RmsNormArgs(rows, cols, x2.stride(0), 0, x2.data_ptr(), None, weight.data_ptr(), out.data_ptr(), None, None, None,
+                    eps, _dt(x2.dtype), _dt(weight.dtype), fmt)
+    if residual2 is not None:
+        a.ld_residual, a.residual, a.stream_out = residual2.stride(0), residual2.data_ptr(), stream.data_ptr()
+    if fmt >= 0:
+        if packed:
+            scales = torch.empty(packed_scale_bytes(rows, cols // 32), dtype=torch.uint8, device=x2.device)
+            a.scale_packed = scales.data_ptr()
+        else:
+            scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x2.device)
+            a.scale_plain = scales.data_ptr()
+    _check(lib().altob200_rms_norm_forward(C.byref(a), _stream()), "altob200_rms_norm_forward")
+    return out, stream, scales
+
+
+@on_device_of
+def rms_norm_backward(grad2: torch.Tensor, stream2: torch.Tensor, weight: torch.Tensor, eps: float,
+                      grad_stream2: Optional[torch.Tensor], need_weight: bool):
+    """(grad of the rows, grad of the weight or None); operands as in ``rms_norm_forward``."""
+    rows, cols = stream2.shape
+    grad_in = torch.empty(rows, cols, dtype=stream2.dtype, device=stream2.device)
+    grad_w = torch.empty(cols, dtype=weight.dtype, device=stream2.device) if need_weight else None
+    a = RmsNormGradArgs(rows, cols, grad2.stride(0), stream2.stride(0), 0, grad2.data_ptr(), stream2.data_ptr(), None,
+                        weight.data_ptr(), grad_in.data_ptr(), _ptr(grad_w), eps, _dt(stream2.dtype), _dt(weight.dtype))
+    if grad_stream2 is not None:
+        a.ld_grad_stream, a.grad_stream = grad_stream2.stride(0), grad_stream2.data_ptr()
+    work = None
+    if need_weight and rows > 0:
+        work = torch.empty(lib().altob200_rms_norm_backward_work_bytes(C.byref(a)), dtype=torch.uint8, device=stream2.device)
+    _check(lib().altob200_rms_norm_backward(C.byref(a), _ptr(work), _stream()), "altob200_rms_norm_backward")
+    return grad_in, grad_w
+
+
+@on_device_of
+def route_forward(logits2: torch.Tensor, p: RouteParams, bias: Optional[torch.Tensor]):
+    """(ids int32 [tokens, k], weights fp32 [tokens, k]) of logits [tokens, experts] with unit column stride."""
+    tokens = logits2.shape[0]
+    ids = torch.empty(tokens, p.top_k, dtype=torch.int32, device=logits2.device)
+    weights = torch.empty(tokens, p.top_k, dtype=torch.float32, device=logits2.device)
+    _check(lib().altob200_route_forward(C.byref(p), logits2.data_ptr(), tokens, logits2.stride(0), _ptr(bias), ids.data_ptr(),
+                                        weights.data_ptr(), _stream()), "altob200_route_forward")
+    return ids, weights
+
+
+@on_device_of
+def route_backward(logits2: torch.Tensor, p: RouteParams, ids: torch.Tensor, grad: torch.Tensor) -> torch.Tensor:
+    tokens, experts = logits2.shape
+    out = torch.empty(tokens, experts, dtype=logits2.dtype, device=logits2.device)
+    _check(lib().altob200_route_backward(C.byref(p), logits2.data_ptr(), tokens, logits2.stride(0), ids.data_ptr(),
+                                         grad.data_ptr(), out.data_ptr(), _stream()), "altob200_route_backward")
+    return out
+
+
+@on_device_of
+def expert_plan(ids: torch.Tensor, tokens: int, k: int, experts: int, align: int, rows: int):
+    """(token [rows], position [rows], slot [tokens k], offs [experts], counts [experts]), all int32; ids contiguous."""
+    n, dev = tokens * k, ids.device
+    token, position, slot, offs, counts = (torch.empty(m, dtype=torch.int32, device=dev)
+                                           for m in (rows, rows, n, experts, experts))
+    nbytes = lib().altob200_expert_plan_work_bytes(n, experts)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _check(lib().altob200_expert_plan(ids.data_ptr(), ids.element_size() * 8, tokens, k, experts, align, rows, token.data_ptr(),
+                                      position.data_ptr(), slot.data_ptr(), offs.data_ptr(), counts.data_ptr(), _ptr(work),
+                                      _stream()), "altob200_expert_plan")
+    return token, position, slot, offs, counts
+
+
 def gather_rows(src: torch.Tensor, index: torch.Tensor, out_rows: Optional[int] = None) -> torch.Tensor:
     """out[i] = src[index[i]] for index[i] >= 0, else a zero row.  src: [rows, cols] contiguous with
     rows of a multiple of 16 bytes; index: int32 on the same device."""
@@ -626,6 +761,27 @@ def swiglu_backward(h: torch.Tensor, grad_out: torch.Tensor) -> torch.Tensor:
     grad_h = torch.empty_like(h)
     _check(lib().altob200_swiglu_backward(h.data_ptr(), grad_out.data_ptr(), rows, H, 2 * H, grad_h.data_ptr(),
                                           _stream()), "altob200_swiglu_backward")
+    return grad_h
+
+
+@on_device_of
+def swiglu_keep_forward(h: torch.Tensor, fmt: int):
+    """(out [rows, H], codes uint8 [rows, 2H], scales uint8 [rows, 2H / 32]) of a contiguous bf16 h [rows, 2H]."""
+    rows, two_h = h.shape
+    out = torch.empty(rows, two_h // 2, dtype=h.dtype, device=h.device)
+    codes = torch.empty(rows, two_h, dtype=torch.uint8, device=h.device)
+    scales = torch.empty(rows, two_h // 32, dtype=torch.uint8, device=h.device)
+    _check(lib().altob200_swiglu_keep_forward(h.data_ptr(), rows, two_h // 2, h.stride(0), fmt, out.data_ptr(),
+                                              codes.data_ptr(), scales.data_ptr(), _stream()), "altob200_swiglu_keep_forward")
+    return out, codes, scales
+
+
+@on_device_of
+def swiglu_kept_backward(codes: torch.Tensor, scales: torch.Tensor, grad_out: torch.Tensor, fmt: int) -> torch.Tensor:
+    rows, two_h = codes.shape
+    grad_h = torch.empty(rows, two_h, dtype=torch.bfloat16, device=codes.device)
+    _check(lib().altob200_swiglu_kept_backward(codes.data_ptr(), scales.data_ptr(), grad_out.data_ptr(), rows, two_h // 2, fmt,
+                                               grad_h.data_ptr(), _stream()), "altob200_swiglu_kept_backward")
     return grad_h
 
 

@@ -1,0 +1,566 @@
+// Root-mean-square norm of rows, with the residual's addition in front of it and with its result in the type of x or as
+// MXFP8 codes and scales, and its backward pass.
+//
+//   r = T(x + residual)                     (r = x without one; T the type of x, because r is the stream that is stored)
+//   y = T(r * rstd * w),  rstd = 1 / sqrt(mean(r^2) + eps)
+//   dr = T(rstd * (dy w - xhat * mean(dy w xhat)) + d_stream),  dw = sum over rows of dy xhat,  xhat = r rstd
+//
+// Sums, rstd and dw are fp32; y is rounded once.  The 8-bit result is what altob200_quantize_rowwise makes of y (blocks
+// of 32 along the row), so that both ways to the block-scaled product give the same codes.
+//
+// Both directions are HBM streams: forward reads x (and the residual) and writes y (and r), backward reads dy, r (and
+// d_stream) and writes dr.  rstd is not kept: backward reads r anyway, and one more sum costs less than the launch-time
+// allocation of a vector.
+//
+// A row is held in registers, 16-byte vectors of it per thread (lane-adjacent, so that four (bf16) or eight (fp32)
+// neighbouring lanes hold a block of 32); rows of up to 1024 threads x 4 vectors take this path, other widths,
+// alignments and strides the element-wise kernels, which read a row a second time.
+#include "common.cuh"
+
+namespace altob200 {
+
+struct NormArgs {
+  const void* x;
+  const void* res;      // NULL: none
+  const void* w;
+  void* y;              // T [rows, cols], or the codes
+  void* r;              // T [rows, cols], only with res
+  uint8_t* scale_plain; // [rows, cols / 32] or NULL
+  uint8_t* scale_packed;
+  int64_t rows, cols, ld_x, ld_res;
+  float eps, inv_cols;
+  int32_t w_f32, e5m2;
+};
+
+template <bool BF16>
+struct NormType;
+template <>
+struct NormType<true> {
+  using T = __nv_bfloat16;
+  static constexpr int V = 8;
+};
+template <>
+struct NormType<false> {
+  using T = float;
+  static constexpr int V = 4;
+};
+
+// the elements of a 16-byte vector
+template <bool BF16>
+__device__ __forceinline__ void unpack_vec(const uint4& w, float* v) {
+  if constexpr (BF16) {
+    v[0] = bf16lo_to_f32(w.x); v[1] = bf16hi_to_f32(w.x); v[2] = bf16lo_to_f32(w.y); v[3] = bf16hi_to_f32(w.y);
+    v[4] = bf16lo_to_f32(w.z); v[5] = bf16hi_to_f32(w.z); v[6] = bf16lo_to_f32(w.w); v[7] = bf16hi_to_f32(w.w);
+  } else {
+    v[0] = u2f(w.x); v[1] = u2f(w.y); v[2] = u2f(w.z); v[3] = u2f(w.w);
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 pack_vec(const float* v) {
+  if constexpr (BF16) {
+    return make_uint4(f32_to_bf16_bits(v[0]) | (f32_to_bf16_bits(v[1]) << 16), f32_to_bf16_bits(v[2]) | (f32_to_bf16_bits(v[3]) << 16),
+                      f32_to_bf16_bits(v[4]) | (f32_to_bf16_bits(v[5]) << 16), f32_to_bf16_bits(v[6]) | (f32_to_bf16_bits(v[7]) << 16));
+  } else {
+    return make_uint4(f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3]));
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ float load_elem(const void* p, int64_t i) {
+  if constexpr (BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  else return reinterpret_cast<const float*>(p)[i];
+}
+template <bool BF16>
+__device__ __forceinline__ void store_elem(void* p, int64_t i, float v) {
+  if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<float*>(p)[i] = v;
+}
+template <bool BF16>
+__device__ __forceinline__ float round_elem(float v) {
+  return BF16 ? u2f(f32_to_bf16_bits(v) << 16) : v;
+}
+__device__ __forceinline__ float weight_elem(const void* w, int64_t i, int f32) {
+  return f32 ? __ldg(reinterpret_cast<const float*>(w) + i) : __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16*>(w) + i));
+}
+
+// V weights from column c, which is a multiple of V
+template <int V>
+__device__ __forceinline__ void load_weights(const void* w, int64_t c, int f32, float* out) {
+  if (f32) {
+#pragma unroll
+    for (int q = 0; q < V; q += 4) {
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(w) + c + q));
+      unpack_vec<false>(a, out + q);
+    }
+  } else if constexpr (V == 8) {
+    unpack_vec<true>(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(w) + c)), out);
+  } else {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(w) + c));
+    out[0] = bf16lo_to_f32(a.x); out[1] = bf16hi_to_f32(a.x); out[2] = bf16lo_to_f32(a.y); out[3] = bf16hi_to_f32(a.y);
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+
+// Sum over the CTA (every thread gets it).  `part` holds 32 values; callers that come again alternate between two.
+__device__ __forceinline__ float block_sum(float v, float* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  v = warp_sum(v);
+  if (lane == 0) part[warp] = v;
+  __syncthreads();
+  return warp_sum(lane < warps ? part[lane] : 0.0f);
+}
+
+// Codes of V values of one block of 32 that neighbouring lanes hold: amax over the lanes, scale, encode.
+template <bool BF16, int V>
+__device__ __forceinline__ uint32_t encode_block(const float* v, int e5m2, uint32_t* code /* V / 4 words */) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) m = max(m, f2u(v[j]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int o = 1; o < 32 / V; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  const uint32_t e = BF16 ? e8m0_from_amax_bits<true>(m >> 16, e5m2 ? 2 : 3, e5m2 ? 15 : 8)
+                          : e8m0_from_amax_bits<false>(m, e5m2 ? 2 : 3, e5m2 ? 15 : 8);
+  const float q = u2f(e << 23), rq = u2f((254u - e) << 23);
+  float s[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) s[j] = e <= 253u ? __fmul_rn(v[j], rq) : __fdiv_rn(v[j], q);
+#pragma unroll
+  for (int j = 0; j < V; j += 4)
+    code[j / 4] = e5m2 ? (fp8x2_rtn_hw<true>(s[j], s[j + 1]) | (fp8x2_rtn_hw<true>(s[j + 2], s[j + 3]) << 16))
+                       : (fp8x2_rtn_hw<false>(s[j], s[j + 1]) | (fp8x2_rtn_hw<false>(s[j + 2], s[j + 3]) << 16));
+  return e;
+}
+
+// Scale bytes of the packed layout that belong to no block: rows up to a multiple of 128, columns up to one of 4.
+__device__ __forceinline__ void zero_packed_padding(const NormArgs& a, int64_t row, int thread, int threads) {
+  const int64_t nkb = a.cols >> 5, tiles = (nkb + 3) >> 2;
+  const int64_t first = row < a.rows ? nkb : 0;
+  for (int64_t c = first + thread; c < tiles * 4; c += threads) a.scale_packed[packed_scale_offset(row, c, tiles)] = 0;
+}
+
+// One row per warp (WARP) or per CTA, NV vectors per thread.
+template <bool BF16, bool MX, bool WARP, int NV>
+__global__ void __launch_bounds__(WARP ? 128 : 1024) norm_forward_kernel(NormArgs a) {
+  using T = typename NormType<BF16>::T;
+  constexpr int V = NormType<BF16>::V;
+  __shared__ float part[32];
+  grid_dependency_wait();
+  const int threads = WARP ? 32 : blockDim.x, t = WARP ? (threadIdx.x & 31) : threadIdx.x;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (MX && a.scale_packed != nullptr && row < ((a.rows + 127) & ~127ll)) zero_packed_padding(a, row, t, threads);
+  if (row >= a.rows) return;
+  const int units = (int)(a.cols / V);
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
+  uint4 raw[NV];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int u = t + i * threads;
+    raw[i] = u < units ? __ldg(reinterpret_cast<const uint4*>(x) + u) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (a.res != nullptr) {
+    const T* res = reinterpret_cast<const T*>(a.res) + row * a.ld_res;
+    T* r = reinterpret_cast<T*>(a.r) + row * a.cols;
+    uint4 add[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int u = t + i * threads;
+      add[i] = u < units ? __ldg(reinterpret_cast<const uint4*>(res) + u) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int u = t + i * threads;
+      float p[V], q[V];
+      unpack_vec<BF16>(raw[i], p);
+      unpack_vec<BF16>(add[i], q);
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[j] = __fadd_rn(p[j], q[j]);
+      raw[i] = pack_vec<BF16>(p);
+      if (u < units) reinterpret_cast<uint4*>(r)[u] = raw[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float p[V];
+    unpack_vec<BF16>(raw[i], p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) ss = __fmaf_rn(p[j], p[j], ss);
+  }
+  ss = WARP ? warp_sum(ss) : block_sum(ss, part);
+  const float rstd = rsqrtf(__fmaf_rn(ss, a.inv_cols, a.eps));
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int u = t + i * threads;
+    float p[V], w[V] = {};
+    unpack_vec<BF16>(raw[i], p);
+    if (u < units) load_weights<V>(a.w, (int64_t)u * V, a.w_f32, w);
+#pragma unroll
+    for (int j = 0; j < V; ++j) p[j] = p[j] * rstd * w[j];
+    if constexpr (MX) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[j] = round_elem<BF16>(p[j]);
+      uint32_t code[V / 4];
+      const uint32_t e = encode_block<BF16, V>(p, a.e5m2, code);
+      if (u < units) {
+        uint8_t* y = reinterpret_cast<uint8_t*>(a.y) + row * a.cols + (int64_t)u * V;
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(y) = make_uint2(code[0], code[1]);
+        else *reinterpret_cast<uint32_t*>(y) = code[0];
+        constexpr int LANES = 32 / V;   // that hold one block
+        if ((u & (LANES - 1)) == 0) {
+          const int64_t nkb = a.cols >> 5, kb = u / LANES;
+          if (a.scale_plain != nullptr) a.scale_plain[row * nkb + kb] = (uint8_t)e;
+          if (a.scale_packed != nullptr) a.scale_packed[packed_scale_offset(row, kb, (nkb + 3) >> 2)] = (uint8_t)e;
+        }
+      }
+    } else {
+      if (u < units) reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.y) + row * a.cols)[u] = pack_vec<BF16>(p);
+    }
+  }
+}
+
+// Any width, stride and alignment: one row per CTA, elements one by one, the row read again for the result.
+template <bool BF16, bool MX>
+__global__ void __launch_bounds__(256) norm_forward_any_kernel(NormArgs a) {
+  __shared__ float part[32];
+  grid_dependency_wait();
+  const int64_t row = blockIdx.x;
+  if (MX && a.scale_packed != nullptr) zero_packed_padding(a, row, threadIdx.x, 256);
+  if (row >= a.rows) return;
+  const auto stream = [&](int64_t c) {
+    const float v = load_elem<BF16>(a.x, row * a.ld_x + c);
+    return a.res == nullptr ? v : round_elem<BF16>(__fadd_rn(v, load_elem<BF16>(a.res, row * a.ld_res + c)));
+  };
+  float ss = 0.0f;
+  for (int64_t c = threadIdx.x; c < a.cols; c += 256) {
+    const float v = stream(c);
+    if (a.res != nullptr) store_elem<BF16>(a.r, row * a.cols + c, v);
+    ss = __fmaf_rn(v, v, ss);
+  }
+  ss = block_sum(ss, part);
+  const float rstd = rsqrtf(__fmaf_rn(ss, a.inv_cols, a.eps));
+  for (int64_t c = threadIdx.x; c < a.cols; c += 256) {   // MX: cols is a multiple of 32, so whole warps come here
+    const float v = stream(c) * rstd * weight_elem(a.w, c, a.w_f32);
+    if constexpr (MX) {
+      const float p = round_elem<BF16>(v);
+      uint32_t m = f2u(p) & 0x7FFFFFFFu;
+      m = __reduce_max_sync(0xFFFFFFFFu, m);
+      const uint32_t e = BF16 ? e8m0_from_amax_bits<true>(m >> 16, a.e5m2 ? 2 : 3, a.e5m2 ? 15 : 8)
+                              : e8m0_from_amax_bits<false>(m, a.e5m2 ? 2 : 3, a.e5m2 ? 15 : 8);
+      const float s = e <= 253u ? __fmul_rn(p, u2f((254u - e) << 23)) : __fdiv_rn(p, u2f(e << 23));
+      reinterpret_cast<uint8_t*>(a.y)[row * a.cols + c] =
+          (uint8_t)(a.e5m2 ? fp8x2_rtn_hw<true>(s, 0.0f) : fp8x2_rtn_hw<false>(s, 0.0f));
+      if ((threadIdx.x & 31) == 0) {
+        const int64_t nkb = a.cols >> 5, kb = c >> 5;
+        if (a.scale_plain != nullptr) a.scale_plain[row * nkb + kb] = (uint8_t)e;
+        if (a.scale_packed != nullptr) a.scale_packed[packed_scale_offset(row, kb, (nkb + 3) >> 2)] = (uint8_t)e;
+      }
+    } else {
+      store_elem<BF16>(a.y, row * a.cols + c, v);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------------------
+struct NormGradArgs {
+  const void* dy;
+  const void* r;
+  const void* ds;       // gradient of the stream, or NULL
+  const void* w;
+  void* dr;             // T [rows, cols]
+  float* partial;       // [CTAs, cols], or NULL: no gradient of w
+  int64_t rows, cols, ld_dy, ld_r, ld_ds;
+  float eps, inv_cols;
+  int32_t w_f32;
+};
+
+// Two sums over the CTA at once.
+__device__ __forceinline__ float2 block_sum2(float u, float v, float2* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  u = warp_sum(u);
+  v = warp_sum(v);
+  if (lane == 0) part[warp] = make_float2(u, v);
+  __syncthreads();
+  const float2 p = lane < warps ? part[lane] : make_float2(0.0f, 0.0f);
+  return make_float2(warp_sum(p.x), warp_sum(p.y));
+}
+
+// A CTA (or each of its four warps) walks over rows; a thread keeps its columns, so it sums their part of dw in
+// registers and writes it once.
+template <bool BF16, bool WARP, int NV>
+__global__ void __launch_bounds__(WARP ? 128 : 1024) norm_backward_kernel(NormGradArgs a) {
+  using T = typename NormType<BF16>::T;
+  constexpr int V = NormType<BF16>::V;
+  __shared__ float2 part[2][32];
+  extern __shared__ float joined[];   // WARP: [cols], the four warps' sums
+  grid_dependency_wait();
+  const int threads = WARP ? 32 : blockDim.x, t = WARP ? (threadIdx.x & 31) : threadIdx.x;
+  const int units = (int)(a.cols / V);
+  float acc[NV][V] = {};
+  int turn = 0;
+  const int64_t step = WARP ? (int64_t)gridDim.x * 4 : gridDim.x;
+  for (int64_t row = WARP ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x; row < a.rows; row += step) {
+    const uint4* dy = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.dy) + row * a.ld_dy);
+    const uint4* r = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.r) + row * a.ld_r);
+    uint4 g[NV], x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int u = t + i * threads;
+      g[i] = u < units ? __ldg(dy + u) : make_uint4(0u, 0u, 0u, 0u);
+      x[i] = u < units ? __ldg(r + u) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    float ss = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int u = t + i * threads;
+      float gv[V], xv[V], w[V] = {};
+      unpack_vec<BF16>(g[i], gv);
+      unpack_vec<BF16>(x[i], xv);
+      if (u < units) load_weights<V>(a.w, (int64_t)u * V, a.w_f32, w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        ss = __fmaf_rn(xv[j], xv[j], ss);
+        dot = __fmaf_rn(gv[j] * w[j], xv[j], dot);
+      }
+    }
+    if (WARP) {
+      ss = warp_sum(ss);
+      dot = warp_sum(dot);
+    } else {
+      const float2 s = block_sum2(ss, dot, part[turn]);
+      turn ^= 1;
+      ss = s.x;
+      dot = s.y;
+    }
+    const float rstd = rsqrtf(__fmaf_rn(ss, a.inv_cols, a.eps));
+    const float along = dot * rstd * rstd * a.inv_cols;   // mean(dy w xhat) rstd
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int u = t + i * threads;
+      if (u < units) {
+        float gv[V], xv[V], w[V], d[V] = {};
+        unpack_vec<BF16>(g[i], gv);
+        unpack_vec<BF16>(x[i], xv);
+        load_weights<V>(a.w, (int64_t)u * V, a.w_f32, w);
+        if (a.ds != nullptr) unpack_vec<BF16>(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.ds) + row * a.ld_ds) + u), d);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          acc[i][j] = __fmaf_rn(gv[j], xv[j] * rstd, acc[i][j]);
+          d[j] = __fmaf_rn(rstd, __fmaf_rn(-xv[j], along, gv[j] * w[j]), d[j]);
+        }
+        reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.dr) + row * a.cols)[u] = pack_vec<BF16>(d);
+      }
+    }
+  }
+  if (a.partial == nullptr) return;
+  float* out = a.partial + (int64_t)blockIdx.x * a.cols;
+  if (WARP) {
+    for (int c = threadIdx.x; c < (int)a.cols; c += 128) joined[c] = 0.0f;
+    for (int turn_of = 0; turn_of < 4; ++turn_of) {
+      __syncthreads();
+      if ((int)(threadIdx.x >> 5) == turn_of) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int u = t + i * threads;
+          if (u < units)
+#pragma unroll
+            for (int j = 0; j < V; ++j) joined[u * V + j] += acc[i][j];
+        }
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < (int)a.cols; c += 128) out[c] = joined[c];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int u = t + i * threads;
+      if (u < units)
+#pragma unroll
+        for (int j = 0; j < V; j += 4)
+          *reinterpret_cast<float4*>(out + (int64_t)u * V + j) = make_float4(acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]);
+    }
+  }
+}
+
+// Any width, stride and alignment: the gradient of the rows, and behind it dw with a thread per column.
+template <bool BF16>
+__global__ void __launch_bounds__(256) norm_backward_any_kernel(NormGradArgs a) {
+  __shared__ float2 part[2][32];
+  grid_dependency_wait();
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    float ss = 0.0f, dot = 0.0f;
+    for (int64_t c = threadIdx.x; c < a.cols; c += 256) {
+      const float g = load_elem<BF16>(a.dy, row * a.ld_dy + c), x = load_elem<BF16>(a.r, row * a.ld_r + c);
+      ss = __fmaf_rn(x, x, ss);
+      dot = __fmaf_rn(g * weight_elem(a.w, c, a.w_f32), x, dot);
+    }
+    const float2 s = block_sum2(ss, dot, part[turn]);
+    turn ^= 1;
+    const float rstd = rsqrtf(__fmaf_rn(s.x, a.inv_cols, a.eps)), along = s.y * rstd * rstd * a.inv_cols;
+    float* out = a.partial == nullptr ? nullptr : a.partial + (int64_t)blockIdx.x * a.cols;
+    for (int64_t c = threadIdx.x; c < a.cols; c += 256) {
+      const float g = load_elem<BF16>(a.dy, row * a.ld_dy + c), x = load_elem<BF16>(a.r, row * a.ld_r + c);
+      const float d = a.ds == nullptr ? 0.0f : load_elem<BF16>(a.ds, row * a.ld_ds + c);
+      store_elem<BF16>(a.dr, row * a.cols + c, __fmaf_rn(rstd, __fmaf_rn(-x, along, g * weight_elem(a.w, c, a.w_f32)), d));
+      // the thread's own columns: no other thread writes them
+      if (out != nullptr) out[c] = (row == (int64_t)blockIdx.x ? 0.0f : out[c]) + g * (x * rstd);
+    }
+  }
+}
+
+// dw[c] = sum of the CTAs' parts, in a fixed order: 32 columns a CTA, its eight warps over the parts.
+__global__ void __launch_bounds__(256) norm_join_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols,
+                                                        void* __restrict__ dw, int w_f32) {
+  __shared__ float sums[8][33];
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (c < cols)
+    for (int64_t p = warp; p < parts; p += 8) s += partial[p * cols + c];
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < cols) {
+    for (int i = 1; i < 8; ++i) s += sums[i][lane];
+    if (w_f32) reinterpret_cast<float*>(dw)[c] = s;
+    else reinterpret_cast<__nv_bfloat16*>(dw)[c] = __float2bfloat16_rn(s);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// How a row of `units` vectors is spread: over a warp up to 4 vectors a lane, else over a CTA.
+struct NormShape {
+  bool warp;
+  int threads, nv;
+};
+static NormShape norm_shape(int64_t units) {
+  if (units <= 128) return {true, 128, units <= 32 ? 1 : units <= 64 ? 2 : 4};
+  const int nv = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
+  if (units > 4096) return {false, 0, 0};
+  return {false, (int)(ceil_div(ceil_div(units, nv), 32) * 32), nv};
+}
+
+static int norm_blocks_backward(const NormShape& s, int64_t rows) {
+  if (s.threads == 0) return (int)(rows < 148 * 4 ? rows : 148 * 4);
+  const int64_t per_cta = s.warp ? 4 : 1, all = ceil_div(rows, per_cta);
+  const int64_t most = 148 * (s.warp ? 4 : s.threads >= 1024 ? 1 : 1024 / s.threads);
+  return (int)(all < most ? all : most);
+}
+
+static NormShape norm_shape_for(int64_t cols, int32_t dtype, bool vec) {
+  const int V = dtype == ALTOB200_DT_BF16 ? 8 : 4;
+  return vec ? norm_shape(cols / V) : NormShape{false, 0, 0};
+}
+
+}  // namespace altob200
+
+using namespace altob200;
+
+extern "C" int altob200_rms_norm_forward(const altob200_rms_norm_args* p, void* stream) {
+  if (p == nullptr || p->rows < 0 || p->cols <= 0) return ALTOB200_EINVAL_SHAPE;
+  if (p->rows == 0) return ALTOB200_OK;
+  const bool bf16 = p->dtype == ALTOB200_DT_BF16, mx = p->format >= 0;
+  if ((!bf16 && p->dtype != ALTOB200_DT_F32) || (p->weight_dtype != ALTOB200_DT_BF16 && p->weight_dtype != ALTOB200_DT_F32) ||
+      (mx && p->format != ALTOB200_FMT_MXFP8_E4M3 && p->format != ALTOB200_FMT_MXFP8_E5M2))
+    return ALTOB200_EUNSUPPORTED;
+  if (p->x == nullptr || p->weight == nullptr || p->out == nullptr || p->ld_x < p->cols ||
+      (p->residual != nullptr && (p->stream_out == nullptr || p->ld_residual < p->cols)) ||
+      (mx && (p->cols % 32 != 0 || (p->scale_plain == nullptr && p->scale_packed == nullptr))))
+    return ALTOB200_EINVAL_SHAPE;
+  if (p->rows >= (1ll << 31) - 128) return ALTOB200_ELIMIT;
+  const int V = bf16 ? 8 : 4;
+  const bool vec = p->cols % V == 0 && p->ld_x % V == 0 && aligned16(p->x) && aligned16(p->out) && aligned16(p->weight) &&
+                   (p->residual == nullptr || (p->ld_residual % V == 0 && aligned16(p->residual) && aligned16(p->stream_out)));
+  const NormShape s = norm_shape_for(p->cols, p->dtype, vec);
+  NormArgs a;
+  a.x = p->x; a.res = p->residual; a.w = p->weight; a.y = p->out; a.r = p->stream_out;
+  a.scale_plain = p->scale_plain; a.scale_packed = p->scale_packed;
+  a.rows = p->rows; a.cols = p->cols; a.ld_x = p->ld_x; a.ld_res = p->ld_residual;
+  a.eps = p->eps; a.inv_cols = (float)(1.0 / (double)p->cols);
+  a.w_f32 = p->weight_dtype == ALTOB200_DT_F32;
+  a.e5m2 = p->format == ALTOB200_FMT_MXFP8_E5M2;
+  const int64_t all_rows = mx && p->scale_packed != nullptr ? ceil_div(p->rows, 128) * 128 : p->rows;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (s.threads == 0) {
+#define ANY(B, M) (void)launch_after(norm_forward_any_kernel<B, M>, dim3((unsigned)all_rows), dim3(256), 0, st, a)
+    if (bf16) { if (mx) ANY(true, true); else ANY(true, false); }
+    else { if (mx) ANY(false, true); else ANY(false, false); }
+#undef ANY
+  } else {
+    const dim3 grid((unsigned)(s.warp ? ceil_div(all_rows, 4) : all_rows)), block(s.threads);
+#define ONE(B, M, W, N) (void)launch_after(norm_forward_kernel<B, M, W, N>, grid, block, 0, st, a)
+#define BY_NV(B, M, W) { if (s.nv == 1) ONE(B, M, W, 1); else if (s.nv == 2) ONE(B, M, W, 2); else ONE(B, M, W, 4); }
+#define BY_WARP(B, M) { if (s.warp) BY_NV(B, M, true) else BY_NV(B, M, false) }
+    if (bf16) { if (mx) BY_WARP(true, true) else BY_WARP(true, false) }
+    else { if (mx) BY_WARP(false, true) else BY_WARP(false, false) }
+#undef BY_WARP
+#undef BY_NV
+#undef ONE
+  }
+  return cudaGetLastError() == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
+}
+
+static bool norm_backward_vec(const altob200_rms_norm_grad_args* p) {
+  const int V = p->dtype == ALTOB200_DT_BF16 ? 8 : 4;
+  return p->cols % V == 0 && p->ld_grad % V == 0 && p->ld_stream % V == 0 && aligned16(p->grad_out) && aligned16(p->stream) &&
+         aligned16(p->weight) && aligned16(p->grad_in) &&
+         (p->grad_stream == nullptr || (p->ld_grad_stream % V == 0 && aligned16(p->grad_stream)));
+}
+
+extern "C" int64_t altob200_rms_norm_backward_work_bytes(const altob200_rms_norm_grad_args* p) {
+  if (p == nullptr || p->rows <= 0 || p->cols <= 0 || p->grad_weight == nullptr) return 0;
+  const NormShape s = norm_shape_for(p->cols, p->dtype, norm_backward_vec(p));
+  return (int64_t)norm_blocks_backward(s, p->rows) * p->cols * 4;
+}
+
+extern "C" int altob200_rms_norm_backward(const altob200_rms_norm_grad_args* p, void* work, void* stream) {
+  if (p == nullptr || p->rows < 0 || p->cols <= 0) return ALTOB200_EINVAL_SHAPE;
+  const bool bf16 = p->dtype == ALTOB200_DT_BF16;
+  if ((!bf16 && p->dtype != ALTOB200_DT_F32) || (p->weight_dtype != ALTOB200_DT_BF16 && p->weight_dtype != ALTOB200_DT_F32))
+    return ALTOB200_EUNSUPPORTED;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int w_f32 = p->weight_dtype == ALTOB200_DT_F32;
+  if (p->rows == 0) {   // a sum over no rows
+    if (p->grad_weight != nullptr) ALTOB200_CUDA_CHECK(cudaMemsetAsync(p->grad_weight, 0, p->cols * (w_f32 ? 4 : 2), st));
+    return ALTOB200_OK;
+  }
+  if (p->grad_out == nullptr || p->stream == nullptr || p->weight == nullptr || p->grad_in == nullptr || p->ld_grad < p->cols ||
+      p->ld_stream < p->cols || (p->grad_stream != nullptr && p->ld_grad_stream < p->cols) ||
+      (p->grad_weight != nullptr && work == nullptr))
+    return ALTOB200_EINVAL_SHAPE;
+  if (!aligned16(work)) return ALTOB200_EINVAL_ALIGN;
+  if (p->rows >= (1ll << 31) - 128) return ALTOB200_ELIMIT;
+  const NormShape s = norm_shape_for(p->cols, p->dtype, norm_backward_vec(p));
+  const int blocks = norm_blocks_backward(s, p->rows);
+  NormGradArgs a;
+  a.dy = p->grad_out; a.r = p->stream; a.ds = p->grad_stream; a.w = p->weight; a.dr = p->grad_in;
+  a.partial = p->grad_weight == nullptr ? nullptr : reinterpret_cast<float*>(work);
+  a.rows = p->rows; a.cols = p->cols; a.ld_dy = p->ld_grad; a.ld_r = p->ld_stream; a.ld_ds = p->ld_grad_stream;
+  a.eps = p->eps; a.inv_cols = (float)(1.0 / (double)p->cols); a.w_f32 = w_f32;
+  if (s.threads == 0) {
+    if (bf16) (void)launch_after(norm_backward_any_kernel<true>, dim3(blocks), dim3(256), 0, st, a);
+    else (void)launch_after(norm_backward_any_kernel<false>, dim3(blocks), dim3(256), 0, st, a);
+  } else {
+    const size_t smem = s.warp ? (size_t)p->cols * 4 : 0;
+#define ONE(B, W, N) (void)launch_after(norm_backward_kernel<B, W, N>, dim3(blocks), dim3(s.threads), smem, st, a)
+#define BY_NV(B, W) { if (s.nv == 1) ONE(B, W, 1); else if (s.nv == 2) ONE(B, W, 2); else ONE(B, W, 4); }
+    if (bf16) { if (s.warp) BY_NV(true, true) else BY_NV(true, false) }
+    else { if (s.warp) BY_NV(false, true) else BY_NV(false, false) }
+#undef BY_NV
+#undef ONE
+  }
+  if (p->grad_weight != nullptr)
+    (void)launch_after(norm_join_kernel, dim3((unsigned)ceil_div(p->cols, 32)), dim3(256), 0, st, (const float*)a.partial,
+                       (int64_t)blocks, p->cols, p->grad_weight, w_f32);
+  return cudaGetLastError() == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
+}

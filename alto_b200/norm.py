@@ -1,0 +1,106 @@
+"""Root-mean-square norm of token rows, with the residual's addition in front of it.
+
+    rms_norm(x, weight, eps)                      y = x / sqrt(mean(x^2) + eps) * weight
+    rms_norm(x, weight, eps, residual=res)        (y, r): r = x + res in the type of x, y the norm of r
+    rms_norm_mxfp8(...)                           y as MXFP8 codes and block scales (``convert_to_mxfp8`` of y, bit for bit)
+
+One kernel each, one read of the rows; sums are fp32 and y is rounded once.  ``rms_norm`` is differentiable in x, residual
+and weight (one pass for the rows' gradient, which x and the residual share, and a short one that joins the weight's).
+The codes of ``rms_norm_mxfp8`` go into ``mxfp8.blockwise_mxfp8_gemm`` or, in a training step, through
+``rms_norm_mxfp8_linear`` into the MXFP8 linear.
+
+The decoder blocks that the reference converts have this norm in front of their linears
+(alto/modifiers/lpt/base.py:171-192); its kernels leave it to tensor operations."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib as L
+
+__all__ = ["rms_norm", "rms_norm_mxfp8"]
+
+_FP8 = {"e4m3": (L.FMT_MXFP8_E4M3, torch.float8_e4m3fn), "e5m2": (L.FMT_MXFP8_E5M2, torch.float8_e5m2)}
+_TYPES = (torch.bfloat16, torch.float32)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[rows, cols] view (or copy) whose rows are contiguous and do not overlap."""
+    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:
+        t2 = t2.contiguous()
+    if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:      # one column or one row: strides that say nothing
+        t2 = t2.as_strided(t2.shape, (t2.shape[1], 1))
+    return t2
+
+
+def _check(name: str, x, weight, residual, eps) -> None:
+    if not x.is_cuda or not weight.is_cuda or (residual is not None and not residual.is_cuda):
+        raise RuntimeError(f"{name} runs on CUDA tensors only (no CPU fallback)")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name} expects rows in the last dimension, got {tuple(x.shape)}")
+    if x.dtype not in _TYPES or weight.dtype not in _TYPES:
+        raise TypeError(f"{name} expects bfloat16 or float32, got {x.dtype} and a weight of {weight.dtype}")
+    if weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
+        raise ValueError(f"{name} expects a weight of [{x.shape[-1]}], got {tuple(weight.shape)}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"{name} expects a residual like x ({tuple(x.shape)}, {x.dtype}), got {tuple(residual.shape)}, "
+                         f"{residual.dtype}")
+    if weight.device != x.device or (residual is not None and residual.device != x.device):
+        raise ValueError(f"{name} expects all tensors on one device")
+    if not eps >= 0.0:
+        raise ValueError(f"{name} expects eps >= 0, got {eps}")
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        x2, w = _rows(x), weight.contiguous()
+        out, stream, _ = L.rms_norm_forward(x2, w, eps, None if residual is None else _rows(residual))
+        ctx.save_for_backward(x if stream is None else stream, weight)
+        ctx.eps, ctx.shape, ctx.residual = eps, x.shape, residual is not None
+        ctx.set_materialize_grads(False)
+        out = out.view(x.shape)
+        return out if stream is None else (out, stream.view(x.shape))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out, grad_stream=None):
+        stream, weight = ctx.saved_tensors
+        if grad_out is None:      # only the stream was used
+            return grad_stream, torch.zeros_like(weight), grad_stream if ctx.residual else None, None
+        gx, gw = L.rms_norm_backward(_rows(grad_out), _rows(stream), weight.contiguous(), ctx.eps,
+                                     None if grad_stream is None else _rows(grad_stream), ctx.needs_input_grad[1])
+        gx = gx.view(ctx.shape)
+        return gx, gw, gx if ctx.residual else None, None
+
+
+@L.traced("rms_norm")
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None):
+    """Norm of the rows of x [..., cols] (bf16 or fp32; weight [cols] in either type).  With ``residual`` (like x) returns
+    (y, r), r = x + residual rounded to the type of x and y the norm of r; else y."""
+    _check("rms_norm", x, weight, residual, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        return _RMSNorm.apply(x, weight, residual, eps)
+    out, stream, _ = L.rms_norm_forward(_rows(x), weight.contiguous(), eps, None if residual is None else _rows(residual))
+    return out.view(x.shape) if stream is None else (out.view(x.shape), stream.view(x.shape))
+
+
+@L.traced("rms_norm_mxfp8")
+def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None,
+                   mxfp_format: str = "e4m3"):
+    """The norm's result as MXFP8: (codes [..., cols], scales uint8 [..., cols / 32]), and r behind them with ``residual``.
+    cols is a multiple of 32.  Codes and scales are those of ``convert_to_mxfp8(rms_norm(...))``.  Not differentiable, as
+    the quantizers are not: for evaluation and serving."""
+    _check("rms_norm_mxfp8", x, weight, residual, eps)
+    if mxfp_format not in _FP8:
+        raise ValueError(f"Unsupported FP8 format: {mxfp_format}. Supported: {sorted(_FP8)}")
+    if x.shape[-1] % 32 != 0:
+        raise ValueError(f"rms_norm_mxfp8 expects rows of a multiple of 32, got {x.shape[-1]}")
+    fmt, dtype = _FP8[mxfp_format]
+    with torch.no_grad():
+        codes, stream, scales = L.rms_norm_forward(_rows(x), weight.contiguous(), eps,
+                                                   None if residual is None else _rows(residual), fmt)
+    codes, scales = codes.view(dtype).view(x.shape), scales.view(*x.shape[:-1], x.shape[-1] // 32)
+    return (codes, scales) if stream is None else (codes, scales, stream.view(x.shape))

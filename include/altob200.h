@@ -416,6 +416,101 @@ int altob200_swiglu_backward(const void* h, const void* grad_out, int64_t rows, 
                              void* grad_h, void* stream);
 
 /*
+ * The same activation with its input kept for the backward pass as MXFP8 instead of bf16: codes [rows, 2H] and E8M0
+ * scales [rows, 2H / 32] are what altob200_quantize_rowwise (format ALTOB200_FMT_MXFP8_*, plain scales) makes of h.
+ * Forward writes out as altob200_swiglu_forward does, bit for bit, and the codes from the same read of h; backward takes
+ * the codes in the place of h, computes in fp32 and rounds once.  H a multiple of 32, grad_h contiguous [rows, 2H].
+ */
+int altob200_swiglu_keep_forward(const void* h, int64_t rows, int64_t H, int64_t ld_h, int32_t format, void* out,
+                                 void* codes, uint8_t* scales, void* stream);
+int altob200_swiglu_kept_backward(const void* codes, const uint8_t* scales, const void* grad_out, int64_t rows,
+                                  int64_t H, int32_t format, void* grad_h, void* stream);
+
+/*
+ * Root-mean-square norm of rows, optionally behind the addition of a residual:
+ *   r = T(x + residual)  (stream_out; r = x without a residual),   y = r / sqrt(mean(r^2) + eps) * weight
+ * with fp32 sums and one rounding of y.  T is `dtype`, weight [cols] has `weight_dtype`.  The decoder blocks that the
+ * reference converts (alto/modifiers/lpt/base.py:171-192) have this norm in front of their linears.
+ *   format < 0  : out is T [rows, cols]
+ *   format MXFP8: out is the codes [rows, cols] that altob200_quantize_rowwise makes of y (blocks of 32 along the row;
+ *                 cols a multiple of 32), with plain scales [rows, cols / 32] and / or the packed layout, padding zero.
+ * Row strides ld_* in elements; out and stream_out are contiguous.  Rows whose width, strides and pointers allow 16-byte
+ * vectors are read once, others element by element and twice.
+ */
+typedef struct altob200_rms_norm_args {
+  int64_t rows, cols, ld_x, ld_residual;
+  const void* x;
+  const void* residual; /* or NULL */
+  const void* weight;
+  void* out;
+  void* stream_out;     /* with a residual only */
+  uint8_t* scale_plain;
+  uint8_t* scale_packed;
+  float eps;
+  int32_t dtype, weight_dtype, format;
+} altob200_rms_norm_args;
+int altob200_rms_norm_forward(const altob200_rms_norm_args* p, void* stream);
+
+/*
+ * Its gradient.  With xhat = stream / sqrt(mean(stream^2) + eps) (stream: r of the forward pass):
+ *   grad_in     = T(grad_stream + (g w - xhat mean(g w xhat)) / sqrt(mean(stream^2) + eps))   of x and of the residual
+ *   grad_weight = sum over rows of g xhat, in weight_dtype
+ * g = grad_out; grad_stream (the gradient of stream_out) and grad_weight may be NULL.  grad_in is contiguous.  `work`:
+ * altob200_rms_norm_backward_work_bytes(p) bytes, 16-byte aligned, not shared by calls that may overlap; the order of all
+ * sums is fixed.
+ */
+typedef struct altob200_rms_norm_grad_args {
+  int64_t rows, cols, ld_grad, ld_stream, ld_grad_stream;
+  const void* grad_out;
+  const void* stream;
+  const void* grad_stream;
+  const void* weight;
+  void* grad_in;
+  void* grad_weight;
+  float eps;
+  int32_t dtype, weight_dtype;
+} altob200_rms_norm_grad_args;
+int64_t altob200_rms_norm_backward_work_bytes(const altob200_rms_norm_grad_args* p);
+int altob200_rms_norm_backward(const altob200_rms_norm_grad_args* p, void* work, void* stream);
+
+/*
+ * Routing of tokens to experts (the step in front of the token dispatcher, alto/modifiers/lpt/base.py:194-201).
+ * Scores are the softmax or the sigmoid of a token's logits [experts] (bf16 or fp32, row stride ld).  The top_k experts
+ * with the largest key = score + bias are chosen, largest first, the lowest index first among equals; without a bias, and
+ * unless groups are judged by two scores, the order is the logits' own.  Keys are compared as if they had 64 bits.
+ * num_groups > 1: only experts of the groups_kept groups (runs of experts / num_groups) with the largest sum of their
+ * group_top (1 or 2) best keys.  weights = scale * score, divided by the sum of the chosen scores with `renormalize`;
+ * a token whose chosen scores are all zero (all logits -inf) gets zero weights and zero gradient.  A NaN counts as the
+ * largest.  experts <= 512, top_k <= 16, num_groups <= 32.
+ */
+typedef struct altob200_route_params {
+  int32_t dtype, experts, top_k, sigmoid, num_groups, groups_kept, group_top, renormalize;
+  float scale;
+} altob200_route_params;
+int altob200_route_forward(const altob200_route_params* p, const void* logits, int64_t tokens, int64_t ld,
+                           const float* bias, int32_t* ids, float* weights, void* stream);
+/* Gradient of the weights with respect to the logits; the choice itself and the bias have none.  grad_logits
+ * [tokens, experts] contiguous in the logits' type; entries of ids outside [0, experts) contribute nothing. */
+int altob200_route_backward(const altob200_route_params* p, const void* logits, int64_t tokens, int64_t ld,
+                            const int32_t* ids, const float* grad_weights, void* grad_logits, void* stream);
+
+/*
+ * Row plan of the token buffer that the grouped GEMMs read: the routed slots (t k + j) sorted by expert, in their order
+ * within an expert, every expert's run padded to a multiple of `align` rows (an expert without slots gets `align` rows;
+ * alto/kernels/fp4/fp4_common/grouped_utils.py:81-94 fixes the runs).  ids [tokens * k], int32 or int64 (ids_bits);
+ *   token    [rows]        token that a row holds, -1: padding
+ *   position [rows]        routed slot that a row holds, -1: padding
+ *   slot     [tokens * k]  row of a routed slot; -1 for an id outside [0, experts) or a row past `rows`
+ *   offs     [experts]     ends of the padded runs,  counts [experts]  rows of the runs without padding
+ * `work`: altob200_expert_plan_work_bytes(..) bytes, 4-byte aligned, not shared by calls that may overlap.
+ * experts <= 1024.
+ */
+int64_t altob200_expert_plan_work_bytes(int64_t slots, int32_t experts);
+int altob200_expert_plan(const void* ids, int32_t ids_bits, int64_t tokens, int32_t k, int32_t experts, int32_t align,
+                         int64_t rows, int32_t* token, int32_t* position, int32_t* slot, int32_t* offs, int32_t* counts,
+                         void* work, void* stream);
+
+/*
  * Block-scaled GEMM on tcgen05:  D[m, n] = alpha * sum_k A[m, k] * B[n, k]
  * with A and B both stored reduction-axis-contiguous ("NT"), packed scales, fp32
  * accumulation in tensor memory.  Replaces blockwise_mxfp4_gemm
