@@ -633,8 +633,8 @@ def rms_norm_forward(x2: torch.Tensor, weight: torch.Tensor, eps: float, residua
     """(out, stream, scales): x2 [rows, cols] with unit column stride, rows of any stride that do not overlap; ``stream`` is
     None without a residual, ``scales`` without an 8-bit format (plain, or the packed layout)."""
     rows, cols = x2.shape
-    out = torch.empty(rows, cols, dtype=x2.dtype if fmt < 0 else torch.uint8, device=x2.device)
-    stream = None if residual2 is None else torch.empty(rows, cols, dtype=x2.dtype, device=x2.device)
+    out = torch.empty_like(x2, dtype=None if fmt < 0 else torch.uint8, memory_format=torch.contiguous_format)
+    stream = None if residual2 is None else torch.empty_like(x2, memory_format=torch.contiguous_format)
     scales = None
     a = RmsNormArgs(rows, cols, x2.stride(0), 0, x2.data_ptr(), None, weight.data_ptr(), out.data_ptr(), None, None, None,
                     eps, _dt(x2.dtype), _dt(weight.dtype), fmt)
@@ -656,8 +656,8 @@ def rms_norm_backward(grad2: torch.Tensor, stream2: torch.Tensor, weight: torch.
                       grad_stream2: Optional[torch.Tensor], need_weight: bool):
     """(grad of the rows, grad of the weight or None); operands as in ``rms_norm_forward``."""
     rows, cols = stream2.shape
-    grad_in = torch.empty(rows, cols, dtype=stream2.dtype, device=stream2.device)
-    grad_w = torch.empty(cols, dtype=weight.dtype, device=stream2.device) if need_weight else None
+    grad_in = torch.empty_like(stream2, memory_format=torch.contiguous_format)
+    grad_w = torch.empty_like(weight) if need_weight else None
     a = RmsNormGradArgs(rows, cols, grad2.stride(0), stream2.stride(0), 0, grad2.data_ptr(), stream2.data_ptr(), None,
                         weight.data_ptr(), grad_in.data_ptr(), _ptr(grad_w), eps, _dt(stream2.dtype), _dt(weight.dtype))
     if grad_stream2 is not None:

@@ -76,6 +76,17 @@ __device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) {
   return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(f));
 }
 
+// e^x = 2^hi 2^lo for |x| <= 126, hi the rounded product with log2 e and lo what the rounding (and the constant's) left of
+// it, so the result is off by the two steps of ex2 and of two products at every x.  One special-function instruction and
+// five others.  inf beyond 2^128, 0 below 2^-126.
+__device__ __forceinline__ float fast_exp(float x) {
+  const float hi = __fmul_rn(x, 1.44269502162933349609375f);                                           // fp32(log2 e)
+  const float lo = __fmaf_rn(x, 1.92596299e-8f, __fmaf_rn(x, 1.44269502162933349609375f, -hi));
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
+  return __fmul_rn(e, __fmaf_rn(lo, 0.693147182464599609375f, 1.0f));
+}
+
 // ---------------------------------------------------------------------------------------
 // packed scale layout (tiles of 128 rows x 4 scale columns, 512 bytes each)
 // ---------------------------------------------------------------------------------------

@@ -8,6 +8,8 @@
 //
 // The choice is made as if keys had 64 bits.  Keys are computed in fp32; where two that a decision separates are nearer
 // than fp32 can tell (and not equal because their inputs are), the token is done again in double.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace altob200 {
@@ -20,9 +22,15 @@ struct RouteArgs {
   int64_t tokens, ld;
   int32_t experts, k, sigmoid, groups, kept, group_top, renorm;
   float scale;
+  int32_t computed;          // keys are scores (and bias), not the logits
+  int32_t checked;           // keys in fp32 words do not settle every decision
+  int32_t per;               // experts a lane holds
+  int32_t lanes_per_group;   // that hold a group, a power of two; 0: groups are not made of whole lanes so
+  int32_t scratch;           // doubles of shared memory a warp has
+  float score_room;          // how far two scores are off together, relative
 };
 
-static constexpr int ROUTE_MAX_K = 16, ROUTE_MAX_E = 512, ROUTE_MAX_GROUPS = 32;
+static constexpr int ROUTE_MAX_K = 16, ROUTE_MAX_E = 512, ROUTE_MAX_GROUPS = 32;   // a choice and its successor fit a warp
 static constexpr unsigned FULL = 0xFFFFFFFFu;
 
 template <bool BF16>
@@ -32,11 +40,8 @@ __device__ __forceinline__ float logit_at(const void* p, int64_t i) {
 }
 
 // Unsigned words in the order of the floats; a NaN above everything, 0 below everything.
-__device__ __forceinline__ uint32_t ordered(float v) {
-  const uint32_t b = f2u(v);
-  if (v != v) return 0xFFFFFFFFu;
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
+__device__ __forceinline__ uint32_t ordered_bits(uint32_t b) { return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u); }
+__device__ __forceinline__ uint32_t ordered(float v) { return v != v ? 0xFFFFFFFFu : ordered_bits(f2u(v)); }
 __device__ __forceinline__ uint64_t ordered(double v) {
   const uint64_t b = (uint64_t)__double_as_longlong(v);
   if (v != v) return ~0ull;
@@ -53,147 +58,272 @@ __device__ __forceinline__ F warp_add(F v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   return v;
 }
-__device__ __forceinline__ uint32_t warp_max_key(uint32_t v) { return __reduce_max_sync(FULL, v); }
+__device__ __forceinline__ float from_ordered(uint32_t w) { return u2f(w >> 31 ? w & 0x7FFFFFFFu : ~w); }
+
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t v) {
   const uint32_t hi = __reduce_max_sync(FULL, (uint32_t)(v >> 32));
   const uint32_t lo = __reduce_max_sync(FULL, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
   return ((uint64_t)hi << 32) | lo;
 }
-template <class F>
-struct KeyWord;
-template <>
-struct KeyWord<float> { using U = uint32_t; };
-template <>
-struct KeyWord<double> { using U = uint64_t; };
 
-template <class F>
-__device__ __forceinline__ F exp_of(F v);
-template <>
-__device__ __forceinline__ float exp_of<float>(float v) { return expf(v); }
-template <>
-__device__ __forceinline__ double exp_of<double>(double v) { return exp(v); }
-
-// One token by one warp, lane l holding experts l, l + 32, ...  Lane i < k returns the i-th choice in *chosen.  `keys`
-// is the warp's own shared memory (padded: see at()).  Returns whether every decision is certain; F = double always is.
-template <class F, bool BF16, int V>
-__device__ bool choose(const RouteArgs& a, int64_t row, const float* l, const float* b, bool computed, F* keys, int* chosen) {
-  using U = typename KeyWord<F>::U;
-  constexpr bool FP32 = sizeof(F) == 4;
-  const int lane = threadIdx.x & 31, E = a.experts;
-  F key[V];
-  bool sure = true;
-  if (computed) {
-    F m = 0, z = 1;
-    if (!a.sigmoid) {
-      float top = -INFINITY;
+// The choice of one token by one warp in double: what the fp32 form hands over because two keys are too near.  Lane l looks
+// after experts l, l + 32, ...; `keys` is the warp's shared memory, [experts].  Lane i < k returns the i-th choice.
+template <bool BF16>
+__device__ __forceinline__ int choose_in_double(const RouteArgs& a, int64_t row, double* keys) {
+  const int lane = threadIdx.x & 31, E = a.experts, size = E / a.groups;
+  double m = -INFINITY, z = 0.0;
+  if (a.computed && !a.sigmoid) {
+    for (int e = lane; e < E; e += 32) m = fmax(m, (double)logit_at<BF16>(a.logits, row + e));
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (lane + 32 * j < E) top = fmaxf(top, l[j]);
-      m = (F)warp_max(top);
-      z = 0;
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (lane + 32 * j < E) z += exp_of<F>((F)l[j] - m);
-      z = warp_add(z);
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const F s = a.sigmoid ? (F)1 / ((F)1 + exp_of<F>(-(F)l[j])) : exp_of<F>((F)l[j] - m) / z;
-      key[j] = a.bias != nullptr ? s + (F)b[j] : s;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) key[j] = (F)l[j];
+    for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(FULL, m, o));
+    for (int e = lane; e < E; e += 32) z += exp((double)logit_at<BF16>(a.logits, row + e) - m);
+    z = warp_add(z);
   }
+  __syncwarp();
+  for (int e = lane; e < E; e += 32) {
+    const double l = logit_at<BF16>(a.logits, row + e), s = !a.computed ? l : a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
+    keys[e] = a.bias != nullptr ? s + (double)__ldg(a.bias + e) : s;
+  }
+  __syncwarp();
   uint32_t allowed = FULL;   // bit g: group g
-  int size = E;
   if (a.groups > 1) {
-    size = E / a.groups;
-    const auto at = [&](int e) { return e + e / size; };   // a word between groups: their lanes read different banks
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = lane + 32 * j;
-      if (e < E) keys[at(e)] = key[j];
-    }
-    __syncwarp();
-    F best = -INFINITY, second = -INFINITY;
-    bool nan = false;
-    if (lane < a.groups) {
-      for (int i = 0; i < size; ++i) {
-        const F v = keys[lane * (size + 1) + i];
-        nan = nan || v != v;
-        if (v > best) {
-          second = best;
-          best = v;
-        } else if (v > second) {
-          second = v;
-        }
-      }
-    }
-    F of_group = a.group_top == 2 && size > 1 ? best + second : best;
-    if (nan) of_group = NAN;
-    const U word = lane < a.groups ? ordered(of_group) : (U)0;
+    uint64_t best = 0, second = 0;
+    int every = 1;             // lanes that look after a group
+    while (every * 2 * a.groups <= 32) every *= 2;
+    const int group = lane / every;
+    const auto meet = [&](uint64_t b2, uint64_t s2) {
+      const uint64_t low = best < b2 ? best : b2, high = second > s2 ? second : s2;
+      second = low > high ? low : high;
+      best = best > b2 ? best : b2;
+    };
+    if (group < a.groups)
+      for (int i = lane & (every - 1); i < size; i += every) meet(ordered(keys[group * size + i]), 0ull);
+    for (int o = 1; o < every; o <<= 1) meet(__shfl_xor_sync(FULL, best, o), __shfl_xor_sync(FULL, second, o));
+    const auto value = [](uint64_t w) { return __longlong_as_double((long long)(w >> 63 ? w & ~(1ull << 63) : ~w)); };
+    const uint64_t word = group >= a.groups ? 0 : a.group_top == 2 && size > 1 ? ordered(value(best) + value(second)) : best;
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
-      const U other = __shfl_sync(FULL, word, g);
-      rank += other > word || (other == word && g < lane) ? 1 : 0;
+      const uint64_t other = __shfl_sync(FULL, word, g * every);
+      rank += other > word || (other == word && g < group) ? 1 : 0;
     }
-    allowed = __ballot_sync(FULL, lane < a.groups && rank < a.kept);
-    if (FP32 && computed && a.kept < a.groups) {
-      // the last group that is kept against the first that is not
-      const unsigned last = __ballot_sync(FULL, lane < a.groups && rank == a.kept - 1);
-      const unsigned first = __ballot_sync(FULL, lane < a.groups && rank == a.kept);
-      const F u = __shfl_sync(FULL, of_group, __ffs(last) - 1), v = __shfl_sync(FULL, of_group, __ffs(first) - 1);
-      if (u - v <= (F)1.6e-5f + (F)5e-7f * (F)fabsf((float)u)) sure = false;
-    }
+    allowed = 0u;
+    for (int g = 0; g < a.groups; ++g) allowed |= (uint32_t)__shfl_sync(FULL, rank < a.kept ? 1 : 0, g * every) << g;
   }
-  U word[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int e = lane + 32 * j;
-    word[j] = e < E && ((allowed >> (a.groups > 1 ? (e / size) & 31 : 0)) & 1u) ? ordered(key[j]) : (U)0;
-  }
-  // the next one after the last is looked at too, where there is one
-  const int left = (a.groups > 1 ? a.kept * size : E), picks = left > a.k ? a.k + 1 : a.k;
   int mine = 0;
-  U mine_word = 0;
-  for (int i = 0; i < picks; ++i) {
-    U top = word[0];
-    int where = lane;
-#pragma unroll
-    for (int j = 1; j < V; ++j)
-      if (word[j] > top) {
-        top = word[j];
-        where = lane + 32 * j;
+  uint64_t last = ~0ull;     // the previous choice: what comes next is smaller, or equal at a higher index
+  int last_e = -1;
+  for (int i = 0; i < a.k; ++i) {
+    uint64_t top = 0;
+    int where = 0x7FFFFFFF;
+    for (int e = lane; e < E; e += 32) {
+      const uint64_t w = (allowed >> (a.groups > 1 ? e / size : 0)) & 1u ? ordered(keys[e]) : 0ull;
+      if ((w < last || (w == last && e > last_e)) && w > top) {
+        top = w;
+        where = e;
       }
-    const U best = warp_max_key(top);
-    const int e = (int)__reduce_min_sync(FULL, top == best ? (uint32_t)where : 0x7FFFFFFFu);
+    }
+    last = warp_max_key(top);
+    last_e = (int)__reduce_min_sync(FULL, top == last ? (uint32_t)where : 0x7FFFFFFFu);
+    if (lane == i) mine = last_e;
+  }
+  return mine;
+}
+
+// Descending order of N registers from LO on (Batcher's odd-even merge sort).
+__device__ __forceinline__ void exchange(uint32_t& u, uint32_t& v) {
+  const uint32_t big = max(u, v);
+  v = min(u, v);
+  u = big;
+}
+template <int LO, int N, int R>
+__device__ __forceinline__ void merge_words(uint32_t* w) {
+  if constexpr (2 * R < N) {
+    merge_words<LO, N, 2 * R>(w);
+    merge_words<LO + R, N, 2 * R>(w);
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (lane + 32 * j == e) word[j] = (U)0;
+    for (int i = LO + R; i + R < LO + N; i += 2 * R) exchange(w[i], w[i + R]);
+  } else {
+    exchange(w[LO], w[LO + R]);
+  }
+}
+template <int LO, int N>
+__device__ __forceinline__ void sort_words(uint32_t* w) {
+  if constexpr (N > 1) {
+    sort_words<LO, N / 2>(w);
+    sort_words<LO + N / 2, N / 2>(w);
+    merge_words<LO, N, 1>(w);
+  }
+}
+
+// The choice of one token by one warp in fp32; lane l holds the a.per experts from l * a.per on.  Lane i < k returns the i-th
+// choice and its logit.  *sure: every decision holds in exact arithmetic too.
+//
+// A key is held as an ordered word whose lowest bits are V - 1 - j: each lane sorts its V words once, a choice is then the
+// largest of the lanes' first words, and its lane moves its list up.  Words are compared across lanes without those bits
+// and the lowest lane is taken, so equal keys come out by expert.  The bits that j takes are missing from every
+// comparison (none of a bf16 logit's), which `room` allows for below.
+template <bool BF16, int V, bool WHOLE>
+__device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const float* l, const float* b, uint32_t* words,
+                                      float* logit, bool* sure) {
+  constexpr uint32_t LOW = V - 1;
+  // two keys that differ by less may be in the other order: what is cut off, and half a step of each sum
+  constexpr float CUT = (V - 1) * 1.1920929e-7f + 1.2e-7f;
+  const int lane = threadIdx.x & 31, per = WHOLE ? V : a.per;
+  uint32_t word[V];
+  *sure = true;
+  if (a.computed) {
+    float p[V], r = 1.0f;
+    if (a.sigmoid) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p[j]) : "f"(1.0f + fast_exp(fminf(fmaxf(-l[j], -126.0f), 126.0f))));
+        if (l[j] != l[j]) p[j] = l[j];
+      }
+    } else {
+      float m = l[0], z = 0.0f;
+#pragma unroll
+      for (int j = 1; j < V; ++j) m = fmaxf(m, l[j]);
+      m = warp_max(m);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = l[j] - m;
+        p[j] = d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f;
+        z += p[j];
+      }
+      r = 1.0f / warp_add(z);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) word[j] = ordered_bits(f2u(p[j] * r + b[j]));   // arithmetic's NaN is above everything
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) word[j] = ordered(l[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    word[j] = WHOLE || (j < per && lane * per + j < a.experts) ? (word[j] & ~LOW) | (LOW - (uint32_t)j) : 0u;
+  int left = a.experts;
+  if (a.groups > 1) {
+    // a group's two best: by the lanes that hold it, or, where groups do not consist of a power of two of whole lanes,
+    // by one lane from shared memory
+    const int size = a.experts / a.groups, every = a.lanes_per_group > 0 ? a.lanes_per_group : 1, mine = lane / every;
+    uint32_t best = 0u, second = 0u;
+    if (a.lanes_per_group > 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        second = max(second, min(best, word[j]));
+        best = max(best, word[j]);
+      }
+      for (int o = 1; o < every; o <<= 1) {
+        const uint32_t b2 = __shfl_xor_sync(FULL, best, o), s2 = __shfl_xor_sync(FULL, second, o);
+        second = max(max(second, s2), min(best, b2));
+        best = max(best, b2);
+      }
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < per && lane * per + j < a.experts) words[lane * per + j + (lane * per + j) / size] = word[j];
+      __syncwarp();
+      if (mine < a.groups)
+        for (int i = 0; i < size; ++i) {
+          const uint32_t w = words[mine * (size + 1) + i];   // a word between groups: their lanes read different banks
+          second = max(second, min(best, w));
+          best = max(best, w);
+        }
+    }
+    const float of_group = a.group_top == 2 && size > 1 ? from_ordered(best) + from_ordered(second) : from_ordered(best);
+    // the kept groups one by one, the lowest among equals; then, if asked, the first that is not kept
+    uint32_t rest = mine >= a.groups ? 0u : a.group_top == 2 ? ordered(of_group) : best & ~LOW, kept = 0u;
+    int last = 0;
+    for (int i = 0; i < a.kept; ++i) {
+      const uint32_t top = __reduce_max_sync(FULL, rest);
+      last = __ffs(__ballot_sync(FULL, rest == top)) - 1;
+      kept |= 1u << last;
+      if (mine * every == last) rest = 0u;
+    }
+    if (a.checked) {
+      const uint32_t top = __reduce_max_sync(FULL, rest);
+      const int next = __ffs(__ballot_sync(FULL, rest == top)) - 1;
+      const float u = __shfl_sync(FULL, of_group, last), v = __shfl_sync(FULL, of_group, next);
+      const float one = fabsf(from_ordered(__shfl_sync(FULL, best, last)));   // of the two keys, which may cancel
+      if (u - v <= 2.0f * (a.score_room + CUT * fmaxf(one, fabsf(u)))) *sure = false;
+    }
+    left = a.kept * size;
+    if (a.lanes_per_group > 0) {
+      const bool in = (kept >> (mine * every)) & 1u;
+#pragma unroll
+      for (int j = 0; j < V; ++j) word[j] = in ? word[j] : 0u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (!((kept >> (((lane * per + j) / size) & 31)) & 1u)) word[j] = 0u;
+    }
+  }
+  sort_words<0, V>(word);
+  // the next one after the last is looked at too, where there is one
+  const int picks = a.checked && left > a.k ? a.k + 1 : a.k;
+  int mine = 0;
+  uint32_t mine_word = 0u;
+  for (int i = 0; i < picks; ++i) {
+    const uint32_t best = __reduce_max_sync(FULL, word[0] & ~LOW);
+    const int owner = __ffs(__ballot_sync(FULL, (word[0] & ~LOW) == best)) - 1;
+    const uint32_t taken = V > 1 ? __shfl_sync(FULL, word[0], owner) : best;
+    const bool up = lane == owner;
+#pragma unroll
+    for (int j = 0; j + 1 < V; ++j) word[j] = up ? word[j + 1] : word[j];
+    word[V - 1] = up ? 0u : word[V - 1];
     if (lane == i) {
-      mine = e;
-      mine_word = best;
+      mine = owner * per + (int)(LOW - (taken & LOW));
+      mine_word = taken;
     }
   }
-  *chosen = mine;
-  if constexpr (FP32) {
-    if (computed) {
-      // neighbours in the order whose keys fp32 cannot tell apart, unless their inputs are the same.  A score is off by
-      // at most 7e-6 of itself (the rounding of l - m before the exponential, up to 88 * 2^-24, is the most of it), the
-      // sum with the bias by half a step.
-      const bool on = lane < picks;
-      const float my_l = on ? logit_at<BF16>(a.logits, row + mine) : 0.0f, my_b = on && a.bias != nullptr ? __ldg(a.bias + mine) : 0.0f;
-      const float my_key = u2f(mine_word >> 31 ? mine_word & 0x7FFFFFFFu : ~mine_word);
-      const float next_l = __shfl_down_sync(FULL, my_l, 1), next_b = __shfl_down_sync(FULL, my_b, 1);
-      const float next_key = __shfl_down_sync(FULL, my_key, 1);
-      const float room = 1.6e-5f * fmaxf(my_key - my_b, next_key - next_b) + 5e-7f * fabsf(my_key);
-      const bool close = lane + 1 < picks && my_key - next_key <= room && !(my_l == next_l && my_b == next_b);
-      if (__any_sync(FULL, close)) sure = false;
+  const bool on = lane < picks;
+  const float my_l = on ? logit_at<BF16>(a.logits, row + mine) : 0.0f;
+  *logit = my_l;
+  if (a.checked) {
+    // Neighbours in the order whose keys fp32 cannot tell apart, unless their inputs are the same.  A softmax is off by at
+    // most 7e-6 of itself (the rounding of l - m before the exponential, up to 88 * 2^-24, is the most of it), a sigmoid by
+    // 6e-7.
+    const float my_b = on && a.bias != nullptr ? __ldg(a.bias + mine) : 0.0f, my_key = from_ordered(mine_word);
+    const float next_l = __shfl_down_sync(FULL, my_l, 1), next_b = __shfl_down_sync(FULL, my_b, 1);
+    const float next_key = __shfl_down_sync(FULL, my_key, 1);
+    const float room = a.score_room * fmaxf(my_key - my_b, next_key - next_b) + CUT * fmaxf(fabsf(my_key), fabsf(next_key));
+    if (__any_sync(FULL, lane + 1 < picks && my_key - next_key <= room && !(my_l == next_l && my_b == next_b))) *sure = false;
+  }
+  return mine;
+}
+
+// A lane's V consecutive logits from p on, aligned to a vector of them.
+template <bool BF16, int V>
+__device__ __forceinline__ void load_logits(const void* logits, int64_t at, float* l) {
+  constexpr int BYTES = V * (BF16 ? 2 : 4), WORDS = BYTES / 4;
+  if constexpr (BYTES < 4) {
+    l[0] = logit_at<BF16>(logits, at);
+  } else {
+    const char* p = reinterpret_cast<const char*>(logits) + at * (BF16 ? 2 : 4);
+    uint32_t w[WORDS];
+    if constexpr (BYTES == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else if constexpr (BYTES == 8) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x; w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int q = 0; q < WORDS / 4; ++q) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + q);
+        w[4 * q] = v.x; w[4 * q + 1] = v.y; w[4 * q + 2] = v.z; w[4 * q + 3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < WORDS; ++q) {
+      if constexpr (BF16) {
+        l[2 * q] = bf16lo_to_f32(w[q]);
+        l[2 * q + 1] = bf16hi_to_f32(w[q]);
+      } else {
+        l[q] = u2f(w[q]);
+      }
     }
   }
-  return sure;
 }
 
 // Weights of the chosen, on lanes i < k (l: the chosen logit).  `m`, `z`: maximum and sum of exponentials
@@ -203,65 +333,97 @@ __device__ __forceinline__ float chosen_weight(bool on, float l, int sigmoid, in
   *total = 1.0f;
   if (sigmoid) {
     // e^(l - c) / (1 + e^l) with c = min(0, the largest chosen logit): in range for any logits
-    const float top = warp_max(on ? l : -INFINITY);
-    const float c = renorm && top < 0.0f ? (top == -INFINITY ? 0.0f : top) : 0.0f;
-    const float s = !on ? 0.0f : l > 0.0f ? 1.0f / (1.0f + expf(-l)) : expf(l - c) / (1.0f + expf(l));
+    float c = 0.0f;
+    if (renorm) {
+      c = fminf(warp_max(on ? l : -INFINITY), 0.0f);
+      if (c == -INFINITY) c = 0.0f;
+    }
+    const float num = l > 0.0f ? 1.0f : fast_exp(fmaxf(l - c, -126.0f)), den = 1.0f + fast_exp(fmaxf(-fabsf(l), -126.0f));
+    const float s = !on ? 0.0f : l != l ? l : __fdividef(num, den);
     if (!renorm) return s;
     *total = warp_add(s);
-    return *total == 0.0f ? 0.0f : s / *total;
+    return *total == 0.0f ? 0.0f : __fdividef(s, *total);
   }
-  if (!renorm) return on && m != -INFINITY ? expf(l - m) / z : 0.0f;
+  if (!renorm) {
+    const float d = l - m;
+    return on && m != -INFINITY ? __fdividef(d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f, z) : 0.0f;
+  }
   const float top = warp_max(on ? l : -INFINITY);
   if (top == -INFINITY && !__any_sync(FULL, on && l != l)) return 0.0f;
-  const float s = on ? expf(l - top) : 0.0f;
+  const float d = l - top, s = !on ? 0.0f : d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f;
   *total = warp_add(s);
-  return s / *total;
+  return __fdividef(s, *total);
 }
 
-template <bool BF16, int V>
+// Weights of a token whose choice is made: lane i < k holds the i-th chosen expert and its logit.
+template <int V>
+__device__ __forceinline__ void write_choice(const RouteArgs& a, int64_t t, const float* l, int chosen, float mine) {
+  const int lane = threadIdx.x & 31;
+  const bool on = lane < a.k;
+  float m = 0.0f, z = 1.0f, total;
+  if (!a.sigmoid && !a.renorm) {
+    m = l[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) m = fmaxf(m, l[j]);
+    m = warp_max(m);
+    z = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = l[j] - m;   // -inf for experts that are not there; m = -inf is seen to by chosen_weight
+      z += d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f;
+    }
+    z = warp_add(z);
+  }
+  float w = chosen_weight(on, mine, a.sigmoid, a.renorm, m, z, &total);
+  if (a.bias != nullptr && !a.sigmoid) {   // a NaN that is not among the chosen makes every score one all the same
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) nan = nan || l[j] != l[j];
+    if (__any_sync(FULL, nan)) w = NAN;
+  }
+  if (on) {
+    a.ids[t * a.k + lane] = chosen;
+    a.weights[t * a.k + lane] = w * a.scale;
+  }
+}
+
+// A warp takes 32 tokens at most (the launch sees to it), so that those whose choice is not certain in fp32 are bits of a
+// word; they are done in double behind the others, by a loop that the registers of the first do not have to make room for.
+template <bool BF16, int V, bool WHOLE>
 __global__ void __launch_bounds__(256) route_forward_kernel(RouteArgs a) {
   extern __shared__ double route_smem[];
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
-  double* const scratch = route_smem + (threadIdx.x >> 5) * (a.experts + a.groups);
-  const bool computed = a.bias != nullptr || a.group_top > 1;
-  float b[V] = {};
-  if (a.bias != nullptr)
+  double* const scratch = route_smem + (threadIdx.x >> 5) * a.scratch;
+  const int per = WHOLE ? V : a.per;
+  float b[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (lane + 32 * j < a.experts) b[j] = __ldg(a.bias + lane + 32 * j);
-  for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < a.tokens; t += (int64_t)gridDim.x * 8) {
+  for (int j = 0; j < V; ++j) b[j] = a.bias != nullptr && j < per && lane * per + j < a.experts ? __ldg(a.bias + lane * per + j) : 0.0f;
+  const auto load = [&](int64_t row, float* l) {
+    if constexpr (WHOLE) {
+      load_logits<BF16, V>(a.logits, row + lane * V, l);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) l[j] = j < per && lane * per + j < a.experts ? logit_at<BF16>(a.logits, row + lane * per + j) : -INFINITY;
+    }
+  };
+  const int64_t first = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), step = (int64_t)gridDim.x * 8;
+  uint32_t again = 0u, bit = 1u;
+  for (int64_t t = first; t < a.tokens; t += step, bit <<= 1) {
+    float l[V], mine;
+    load(t * a.ld, l);
+    bool sure;
+    const int chosen = choose<BF16, V, WHOLE>(a, t * a.ld, l, b, reinterpret_cast<uint32_t*>(scratch), &mine, &sure);
+    if (sure) write_choice<V>(a, t, l, chosen, mine);
+    else again |= bit;
+  }
+  while (again != 0u) {
+    const int64_t t = first + (__ffs(again) - 1) * step;
+    again &= again - 1u;
+    const int chosen = choose_in_double<BF16>(a, t * a.ld, scratch);
     float l[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) l[j] = lane + 32 * j < a.experts ? logit_at<BF16>(a.logits, t * a.ld + lane + 32 * j) : -INFINITY;
-    int chosen;
-    if (!choose<float, BF16, V>(a, t * a.ld, l, b, computed, reinterpret_cast<float*>(scratch), &chosen))
-      choose<double, BF16, V>(a, t * a.ld, l, b, computed, scratch, &chosen);
-    const bool on = lane < a.k;
-    const float mine = on ? logit_at<BF16>(a.logits, t * a.ld + chosen) : 0.0f;
-    float m = 0.0f, z = 1.0f, total;
-    if (!a.sigmoid && !a.renorm) {
-      m = l[0];
-#pragma unroll
-      for (int j = 1; j < V; ++j) m = fmaxf(m, l[j]);
-      m = warp_max(m);
-      z = 0.0f;
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (lane + 32 * j < a.experts) z += expf(l[j] - m);
-      z = warp_add(z);
-    }
-    float w = chosen_weight(on, mine, a.sigmoid, a.renorm, m, z, &total);
-    if (a.bias != nullptr && !a.sigmoid) {   // a NaN that is not among the chosen makes every score one all the same
-      bool nan = false;
-#pragma unroll
-      for (int j = 0; j < V; ++j) nan = nan || l[j] != l[j];
-      if (__any_sync(FULL, nan)) w = NAN;
-    }
-    if (on) {
-      a.ids[t * a.k + lane] = chosen;
-      a.weights[t * a.k + lane] = w * a.scale;
-    }
+    load(t * a.ld, l);
+    write_choice<V>(a, t, l, chosen, lane < a.k ? logit_at<BF16>(a.logits, t * a.ld + chosen) : 0.0f);
   }
 }
 
@@ -273,6 +435,7 @@ struct RouteGradArgs {
   int64_t tokens, ld;
   int32_t experts, k, sigmoid, renorm;
   float scale;
+  int32_t vector;        // rows of grad_logits allow 16-byte stores
 };
 
 //   softmax              dl_e = scale p_e (g_e [chosen] - sum g p)       with p over all experts, or over the chosen when
@@ -315,24 +478,21 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteGradArgs a) {
       sum = warp_add(on ? g * w : 0.0f);
       d = a.scale * w * (g - sum);
     }
-    float out[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = dense && m != -INFINITY ? -a.scale * sum * (expf(all[j] - m) / z) : 0.0f;
-    for (int i = 0; i < a.k; ++i) {
-      const int e = __shfl_sync(FULL, id, i);
-      const float v = __shfl_sync(FULL, d, i);
+    // the row of zeros (or of the terms that every expert has), and over it, once the warp has written that, the chosen
+    using T = typename std::conditional<BF16, __nv_bfloat16, float>::type;
+    T* const out = reinterpret_cast<T*>(a.grad_logits) + t * a.experts;
+    if (dense) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (lane + 32 * j == e) out[j] = v;
+        if (lane + 32 * j < a.experts) out[lane + 32 * j] = (T)(m != -INFINITY ? -a.scale * sum * (expf(all[j] - m) / z) : 0.0f);
+    } else if (a.vector) {
+      for (int c = lane; c < a.experts * (int)sizeof(T) / 16; c += 32) reinterpret_cast<uint4*>(out)[c] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int e = lane; e < a.experts; e += 32) out[e] = (T)0.0f;
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = lane + 32 * j;
-      if (e < a.experts) {
-        if constexpr (BF16) reinterpret_cast<__nv_bfloat16*>(a.grad_logits)[t * a.experts + e] = __float2bfloat16_rn(out[j]);
-        else reinterpret_cast<float*>(a.grad_logits)[t * a.experts + e] = out[j];
-      }
-    }
+    __syncwarp();
+    if (on) out[id] = (T)d;
+    __syncwarp();
   }
 }
 
@@ -525,11 +685,27 @@ extern "C" int altob200_route_forward(const altob200_route_params* p, const void
   if (p->groups_kept == p->num_groups) a.groups = a.kept = 1;
   a.renorm = p->renormalize; a.scale = p->scale;
   const int E = p->experts;
-  const size_t smem = a.groups > 1 ? (size_t)8 * (E + a.groups) * 8 : 0;
+  const bool bf16 = p->dtype == ALTOB200_DT_BF16;
+  a.computed = bias != nullptr || a.group_top > 1;
+  a.checked = a.computed || !bf16;
+  a.score_room = !a.computed ? 0.0f : a.sigmoid ? 1.3e-6f : 1.5e-5f;
+  a.per = (E + 31) / 32;
+  const int size = E / a.groups, lanes = size % a.per == 0 ? size / a.per : 0;
+  a.lanes_per_group = lanes > 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+  // a lane's logits as vectors: as many as the kernel has room for, in rows aligned to them
+  const int bytes = a.per * (bf16 ? 2 : 4), width = bytes < 16 ? bytes : 16;
+  const bool whole = E % 32 == 0 && (a.per & (a.per - 1)) == 0 && (reinterpret_cast<uintptr_t>(logits) % width) == 0 &&
+                     (ld * (bf16 ? 2 : 4)) % width == 0;
+  a.scratch = a.checked || a.groups > 1 ? (E > 64 ? E : 64) : 0;   // keys in double, or E words and 32 between groups
+  const size_t smem = (size_t)8 * a.scratch * 8;
   int64_t blocks = ceil_div(tokens, 8);
-  if (blocks > 148 * 8) blocks = 148 * 8;
-#define RUN(B, V) (void)launch_after(route_forward_kernel<B, V>, dim3((unsigned)blocks), dim3(256), smem, (cudaStream_t)stream, a)
-  if (p->dtype == ALTOB200_DT_BF16) ROUTE_BY_V(RUN, true);
+  if (blocks > 148 * 4) blocks = 148 * 4;
+  if (blocks < ceil_div(tokens, 8 * 32)) blocks = ceil_div(tokens, 8 * 32);
+  if (blocks >= (1ll << 31)) return ALTOB200_ELIMIT;
+#define RUN(B, V)                                                                                                           \
+  (void)launch_after(whole ? route_forward_kernel<B, V, true> : route_forward_kernel<B, V, false>, dim3((unsigned)blocks), \
+                     dim3(256), smem, (cudaStream_t)stream, a)
+  if (bf16) ROUTE_BY_V(RUN, true);
   else ROUTE_BY_V(RUN, false);
 #undef RUN
   return cudaGetLastError() == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
@@ -546,6 +722,7 @@ extern "C" int altob200_route_backward(const altob200_route_params* p, const voi
   RouteGradArgs a;
   a.logits = logits; a.ids = ids; a.grad = grad_weights; a.grad_logits = grad_logits; a.tokens = tokens; a.ld = ld;
   a.experts = p->experts; a.k = p->top_k; a.sigmoid = p->sigmoid; a.renorm = p->renormalize; a.scale = p->scale;
+  a.vector = (reinterpret_cast<uintptr_t>(grad_logits) & 15) == 0 && (p->experts * (p->dtype == ALTOB200_DT_BF16 ? 2 : 4)) % 16 == 0;
   const int E = p->experts;
   int64_t blocks = ceil_div(tokens, 8);
   if (blocks > 148 * 8) blocks = 148 * 8;

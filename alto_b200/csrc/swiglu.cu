@@ -97,19 +97,12 @@ static int swiglu_launch(const void* h, const void* go, int64_t rows, int64_t H,
 // 74 % busy with 290 instructions for eight columns of both halves, DRAM 5.7 TB/s; backward 252, DRAM at the copy rate.
 // With expf and divisions 396 and 460; forward without the loads ahead 310.
 // ---------------------------------------------------------------------------------------
-// 16 / (1 + e^-g).  e^-g = 2^hi 2^lo with hi the rounded product and lo what the rounding left of it (and of the constant),
-// so the exponential is off by the steps of ex2 and two products at every g.  Two special-function instructions and eight
-// others, where the library's expf and a division take about 20.  The factor 16 keeps the reciprocal of 1 + e^88.7 above
-// the least normal number; a sixteenth of a bf16 number is exact.  Outside of +-126, where the result is 16 or 0, g is cut; a
-// NaN comes back with the product that every caller forms with g.
+// 16 / (1 + e^-g), off by the steps of the exponential and of the reciprocal.  The factor 16 keeps the reciprocal of
+// 1 + e^88.7 above the least normal number; a sixteenth of a bf16 number is exact.  Outside of +-126, where the result is 16
+// or 0, g is cut; a NaN comes back with the product that every caller forms with g.
 __device__ __forceinline__ float sigmoid16(float g) {
-  const float x = fminf(fmaxf(g, -126.0f), 126.0f);
-  const float hi = __fmul_rn(x, -1.44269502162933349609375f);                                          // fp32(log2 e)
-  const float lo = __fmaf_rn(x, -1.92596299e-8f, __fmaf_rn(x, -1.44269502162933349609375f, -hi));
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
-  e = __fmul_rn(e, __fmaf_rn(lo, 0.693147182464599609375f, 1.0f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmaf_rn(e, 0.0625f, 0.0625f)));
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmaf_rn(fast_exp(-fminf(fmaxf(g, -126.0f), 126.0f)), 0.0625f, 0.0625f)));
   return r;
 }
 

@@ -27,15 +27,23 @@ _TYPES = (torch.bfloat16, torch.float32)
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[rows, cols] view (or copy) whose rows are contiguous and do not overlap."""
-    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:
-        t2 = t2.contiguous()
-    if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:      # one column or one row: strides that say nothing
-        t2 = t2.as_strided(t2.shape, (t2.shape[1], 1))
-    return t2
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    elif t.is_contiguous() and t.shape[0] > 1 and t.shape[1] > 1:      # the usual case, with the fewest questions
+        return t
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:      # one column or one row: strides that say nothing
+        t = t.as_strided(t.shape, (t.shape[1], 1))
+    return t
 
 
 def _check(name: str, x, weight, residual, eps) -> None:
+    # one pass over what is usual; what is not is told apart below
+    if (x.is_cuda and x.dtype in _TYPES and weight.dtype in _TYPES and weight.shape == x.shape[-1:] and weight.device == x.device
+            and eps >= 0.0 and x.dim() > 0 and x.shape[-1] > 0
+            and (residual is None or (residual.shape == x.shape and residual.dtype is x.dtype and residual.device == x.device))):
+        return
     if not x.is_cuda or not weight.is_cuda or (residual is not None and not residual.is_cuda):
         raise RuntimeError(f"{name} runs on CUDA tensors only (no CPU fallback)")
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -49,31 +57,43 @@ def _check(name: str, x, weight, residual, eps) -> None:
                          f"{residual.dtype}")
     if weight.device != x.device or (residual is not None and residual.device != x.device):
         raise ValueError(f"{name} expects all tensors on one device")
-    if not eps >= 0.0:
-        raise ValueError(f"{name} expects eps >= 0, got {eps}")
+    raise ValueError(f"{name} expects eps >= 0, got {eps}")
+
+
+def _forward(x, weight, residual, eps):
+    """(out, stream) in the shape of x."""
+    two = x.dim() == 2
+    out, stream, _ = L.rms_norm_forward(_rows(x), weight if weight.is_contiguous() else weight.contiguous(), eps,
+                                        None if residual is None else _rows(residual))
+    if two:
+        return out, stream
+    return out.view(x.shape), None if stream is None else stream.view(x.shape)
 
 
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        x2, w = _rows(x), weight.contiguous()
-        out, stream, _ = L.rms_norm_forward(x2, w, eps, None if residual is None else _rows(residual))
-        ctx.save_for_backward(x if stream is None else stream, weight)
-        ctx.eps, ctx.shape, ctx.residual = eps, x.shape, residual is not None
+        out, stream = _forward(x, weight, residual, eps)
         ctx.set_materialize_grads(False)
-        out = out.view(x.shape)
-        return out if stream is None else (out, stream.view(x.shape))
+        ctx.eps = eps
+        if stream is None:
+            ctx.save_for_backward(x, weight)
+            return out
+        ctx.save_for_backward(stream, weight)
+        return out, stream
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out, grad_stream=None):
         stream, weight = ctx.saved_tensors
+        need_x, need_w, need_res, _ = ctx.needs_input_grad
         if grad_out is None:      # only the stream was used
-            return grad_stream, torch.zeros_like(weight), grad_stream if ctx.residual else None, None
-        gx, gw = L.rms_norm_backward(_rows(grad_out), _rows(stream), weight.contiguous(), ctx.eps,
-                                     None if grad_stream is None else _rows(grad_stream), ctx.needs_input_grad[1])
-        gx = gx.view(ctx.shape)
-        return gx, gw, gx if ctx.residual else None, None
+            return grad_stream, torch.zeros_like(weight) if need_w else None, grad_stream if need_res else None, None
+        gx, gw = L.rms_norm_backward(_rows(grad_out), _rows(stream), weight if weight.is_contiguous() else weight.contiguous(),
+                                     ctx.eps, None if grad_stream is None else _rows(grad_stream), need_w)
+        if stream.dim() != 2:
+            gx = gx.view(stream.shape)
+        return gx, gw, gx if need_res else None, None
 
 
 @L.traced("rms_norm")
@@ -81,10 +101,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual:
     """Norm of the rows of x [..., cols] (bf16 or fp32; weight [cols] in either type).  With ``residual`` (like x) returns
     (y, r), r = x + residual rounded to the type of x and y the norm of r; else y."""
     _check("rms_norm", x, weight, residual, eps)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+    if (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
         return _RMSNorm.apply(x, weight, residual, eps)
-    out, stream, _ = L.rms_norm_forward(_rows(x), weight.contiguous(), eps, None if residual is None else _rows(residual))
-    return out.view(x.shape) if stream is None else (out.view(x.shape), stream.view(x.shape))
+    out, stream = _forward(x, weight, residual, eps)
+    return out if stream is None else (out, stream)
 
 
 @L.traced("rms_norm_mxfp8")

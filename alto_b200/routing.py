@@ -43,12 +43,15 @@ class _Route(torch.autograd.Function):
         ids, weights = ids.view(shape), weights.view(shape)
         ctx.save_for_backward(logits, ids)
         ctx.params = params
+        ctx.set_materialize_grads(False)      # no zeros in the place of a gradient of ids
         ctx.mark_non_differentiable(ids)
         return ids, weights
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, _, grad):
+        if grad is None:
+            return None, None, None
         logits, ids = ctx.saved_tensors
         g = L.route_backward(_rows(logits), ctx.params, ids, grad.contiguous())
         return g.view(logits.shape), None, None
