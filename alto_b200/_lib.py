@@ -344,6 +344,17 @@ def on_device_of(fn):
     return inner
 
 
+def once_differentiable(fn):
+    """Decorator of an autograd function's ``backward``: torch's of the same name where a graph of the gradient is asked
+    for, nothing in front of it otherwise (its own wrapper costs a small backward pass a tenth of its time)."""
+    twice = torch.autograd.function.once_differentiable(fn)
+
+    @functools.wraps(fn)
+    def backward(ctx, *grads):
+        return twice(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+    return backward
+
+
 def packed_scale_bytes(rows: int, ncols: int) -> int:
     # altob200_packed_scale_bytes: tiles of 128 rows x 4 columns
     return (rows + 127) // 128 * ((ncols + 3) // 4) * 512
@@ -627,27 +638,34 @@ def pack_scales(scales: torch.Tensor, rows: int, block: int) -> torch.Tensor:
     return out
 
 
+_DT_OF = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
+_ROWS = torch.contiguous_format
+
+
 @on_device_of
 def rms_norm_forward(x2: torch.Tensor, weight: torch.Tensor, eps: float, residual2: Optional[torch.Tensor] = None,
                      fmt: int = -1, packed: bool = False):
     """(out, stream, scales): x2 [rows, cols] with unit column stride, rows of any stride that do not overlap; ``stream`` is
     None without a residual, ``scales`` without an 8-bit format (plain, or the packed layout)."""
     rows, cols = x2.shape
-    out = torch.empty_like(x2, dtype=None if fmt < 0 else torch.uint8, memory_format=torch.contiguous_format)
-    stream = None if residual2 is None else torch.empty_like(x2, memory_format=torch.contiguous_format)
-    scales = None
+    scales = stream = None
+    if fmt < 0:
+        out = torch.empty_like(x2, memory_format=_ROWS)
+    else:
+        out = torch.empty_like(x2, dtype=torch.uint8, memory_format=_ROWS)
     a = RmsNormArgs(rows, cols, x2.stride(0), 0, x2.data_ptr(), None, weight.data_ptr(), out.data_ptr(), None, None, None,
-                    eps, _dt(x2.dtype), _dt(weight.dtype), fmt)
+                    eps, _DT_OF[x2.dtype], _DT_OF[weight.dtype], fmt)
     if residual2 is not None:
+        stream = torch.empty_like(x2, memory_format=_ROWS)
         a.ld_residual, a.residual, a.stream_out = residual2.stride(0), residual2.data_ptr(), stream.data_ptr()
     if fmt >= 0:
         if packed:
             scales = torch.empty(packed_scale_bytes(rows, cols // 32), dtype=torch.uint8, device=x2.device)
             a.scale_packed = scales.data_ptr()
         else:
-            scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x2.device)
+            scales = torch.empty((rows, cols // 32), dtype=torch.uint8, device=x2.device)
             a.scale_plain = scales.data_ptr()
-    _check(lib().altob200_rms_norm_forward(C.byref(a), _stream()), "altob200_rms_norm_forward")
+    _check((_lib or lib()).altob200_rms_norm_forward(a, _stream()), "altob200_rms_norm_forward")
     return out, stream, scales
 
 
@@ -656,36 +674,38 @@ def rms_norm_backward(grad2: torch.Tensor, stream2: torch.Tensor, weight: torch.
                       grad_stream2: Optional[torch.Tensor], need_weight: bool):
     """(grad of the rows, grad of the weight or None); operands as in ``rms_norm_forward``."""
     rows, cols = stream2.shape
-    grad_in = torch.empty_like(stream2, memory_format=torch.contiguous_format)
-    grad_w = torch.empty_like(weight) if need_weight else None
+    grad_in = torch.empty_like(stream2, memory_format=_ROWS)
+    grad_w = work = None
     a = RmsNormGradArgs(rows, cols, grad2.stride(0), stream2.stride(0), 0, grad2.data_ptr(), stream2.data_ptr(), None,
-                        weight.data_ptr(), grad_in.data_ptr(), _ptr(grad_w), eps, _dt(stream2.dtype), _dt(weight.dtype))
+                        weight.data_ptr(), grad_in.data_ptr(), None, eps, _DT_OF[stream2.dtype], _DT_OF[weight.dtype])
     if grad_stream2 is not None:
         a.ld_grad_stream, a.grad_stream = grad_stream2.stride(0), grad_stream2.data_ptr()
-    work = None
-    if need_weight and rows > 0:
-        work = torch.empty(lib().altob200_rms_norm_backward_work_bytes(C.byref(a)), dtype=torch.uint8, device=stream2.device)
-    _check(lib().altob200_rms_norm_backward(C.byref(a), _ptr(work), _stream()), "altob200_rms_norm_backward")
+    handle = _lib or lib()
+    if need_weight:
+        grad_w = torch.empty_like(weight)
+        a.grad_weight = grad_w.data_ptr()
+        if rows > 0:
+            work = torch.empty(handle.altob200_rms_norm_backward_work_bytes(a), dtype=torch.uint8, device=stream2.device)
+    _check(handle.altob200_rms_norm_backward(a, None if work is None else work.data_ptr(), _stream()), "altob200_rms_norm_backward")
     return grad_in, grad_w
 
 
 @on_device_of
 def route_forward(logits2: torch.Tensor, p: RouteParams, bias: Optional[torch.Tensor]):
     """(ids int32 [tokens, k], weights fp32 [tokens, k]) of logits [tokens, experts] with unit column stride."""
-    tokens = logits2.shape[0]
-    ids = torch.empty(tokens, p.top_k, dtype=torch.int32, device=logits2.device)
-    weights = torch.empty(tokens, p.top_k, dtype=torch.float32, device=logits2.device)
-    _check(lib().altob200_route_forward(C.byref(p), logits2.data_ptr(), tokens, logits2.stride(0), _ptr(bias), ids.data_ptr(),
-                                        weights.data_ptr(), _stream()), "altob200_route_forward")
+    tokens, dev = logits2.shape[0], logits2.device
+    ids = torch.empty((tokens, p.top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((tokens, p.top_k), dtype=torch.float32, device=dev)
+    _check((_lib or lib()).altob200_route_forward(p, logits2.data_ptr(), tokens, logits2.stride(0), _ptr(bias), ids.data_ptr(),
+                                                  weights.data_ptr(), _stream()), "altob200_route_forward")
     return ids, weights
 
 
 @on_device_of
 def route_backward(logits2: torch.Tensor, p: RouteParams, ids: torch.Tensor, grad: torch.Tensor) -> torch.Tensor:
-    tokens, experts = logits2.shape
-    out = torch.empty(tokens, experts, dtype=logits2.dtype, device=logits2.device)
-    _check(lib().altob200_route_backward(C.byref(p), logits2.data_ptr(), tokens, logits2.stride(0), ids.data_ptr(),
-                                         grad.data_ptr(), out.data_ptr(), _stream()), "altob200_route_backward")
+    out = torch.empty_like(logits2, memory_format=_ROWS)
+    _check((_lib or lib()).altob200_route_backward(p, logits2.data_ptr(), logits2.shape[0], logits2.stride(0), ids.data_ptr(),
+                                                   grad.data_ptr(), out.data_ptr(), _stream()), "altob200_route_backward")
     return out
 
 
@@ -693,8 +713,11 @@ def route_backward(logits2: torch.Tensor, p: RouteParams, ids: torch.Tensor, gra
 def expert_plan(ids: torch.Tensor, tokens: int, k: int, experts: int, align: int, rows: int):
     """(token [rows], position [rows], slot [tokens k], offs [experts], counts [experts]), all int32; ids contiguous."""
     n, dev = tokens * k, ids.device
-    token, position, slot, offs, counts = (torch.empty(m, dtype=torch.int32, device=dev)
-                                           for m in (rows, rows, n, experts, experts))
+    token = torch.empty(rows, dtype=torch.int32, device=dev)
+    position = torch.empty_like(token)
+    slot = torch.empty(n, dtype=torch.int32, device=dev)
+    offs = torch.empty(experts, dtype=torch.int32, device=dev)
+    counts = torch.empty_like(offs)
     nbytes = lib().altob200_expert_plan_work_bytes(n, experts)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _check(lib().altob200_expert_plan(ids.data_ptr(), ids.element_size() * 8, tokens, k, experts, align, rows, token.data_ptr(),
@@ -767,11 +790,11 @@ def swiglu_backward(h: torch.Tensor, grad_out: torch.Tensor) -> torch.Tensor:
 @on_device_of
 def swiglu_keep_forward(h: torch.Tensor, fmt: int):
     """(out [rows, H], codes uint8 [rows, 2H], scales uint8 [rows, 2H / 32]) of a contiguous bf16 h [rows, 2H]."""
-    rows, two_h = h.shape
-    out = torch.empty(rows, two_h // 2, dtype=h.dtype, device=h.device)
-    codes = torch.empty(rows, two_h, dtype=torch.uint8, device=h.device)
-    scales = torch.empty(rows, two_h // 32, dtype=torch.uint8, device=h.device)
-    _check(lib().altob200_swiglu_keep_forward(h.data_ptr(), rows, two_h // 2, h.stride(0), fmt, out.data_ptr(),
+    (rows, two_h), dev = h.shape, h.device
+    out = torch.empty((rows, two_h // 2), dtype=torch.bfloat16, device=dev)
+    codes = torch.empty_like(h, dtype=torch.uint8)
+    scales = torch.empty((rows, two_h // 32), dtype=torch.uint8, device=dev)
+    _check((_lib or lib()).altob200_swiglu_keep_forward(h.data_ptr(), rows, two_h // 2, h.stride(0), fmt, out.data_ptr(),
                                               codes.data_ptr(), scales.data_ptr(), _stream()), "altob200_swiglu_keep_forward")
     return out, codes, scales
 
@@ -779,8 +802,8 @@ def swiglu_keep_forward(h: torch.Tensor, fmt: int):
 @on_device_of
 def swiglu_kept_backward(codes: torch.Tensor, scales: torch.Tensor, grad_out: torch.Tensor, fmt: int) -> torch.Tensor:
     rows, two_h = codes.shape
-    grad_h = torch.empty(rows, two_h, dtype=torch.bfloat16, device=codes.device)
-    _check(lib().altob200_swiglu_kept_backward(codes.data_ptr(), scales.data_ptr(), grad_out.data_ptr(), rows, two_h // 2, fmt,
+    grad_h = torch.empty_like(codes, dtype=torch.bfloat16)
+    _check((_lib or lib()).altob200_swiglu_kept_backward(codes.data_ptr(), scales.data_ptr(), grad_out.data_ptr(), rows, two_h // 2, fmt,
                                                grad_h.data_ptr(), _stream()), "altob200_swiglu_kept_backward")
     return grad_h
 

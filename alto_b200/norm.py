@@ -83,7 +83,7 @@ class _RMSNorm(torch.autograd.Function):
         return out, stream
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.once_differentiable
     def backward(ctx, grad_out, grad_stream=None):
         stream, weight = ctx.saved_tensors
         need_x, need_w, need_res, _ = ctx.needs_input_grad
@@ -119,8 +119,10 @@ def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, res
     if x.shape[-1] % 32 != 0:
         raise ValueError(f"rms_norm_mxfp8 expects rows of a multiple of 32, got {x.shape[-1]}")
     fmt, dtype = _FP8[mxfp_format]
-    with torch.no_grad():
-        codes, stream, scales = L.rms_norm_forward(_rows(x), weight.contiguous(), eps,
-                                                   None if residual is None else _rows(residual), fmt)
-    codes, scales = codes.view(dtype).view(x.shape), scales.view(*x.shape[:-1], x.shape[-1] // 32)
-    return (codes, scales) if stream is None else (codes, scales, stream.view(x.shape))
+    codes, stream, scales = L.rms_norm_forward(_rows(x), weight if weight.is_contiguous() else weight.contiguous(), eps,
+                                               None if residual is None else _rows(residual), fmt)
+    codes = codes.view(dtype)
+    if x.dim() != 2:
+        codes, scales = codes.view(x.shape), scales.view(*x.shape[:-1], x.shape[-1] // 32)
+        stream = None if stream is None else stream.view(x.shape)
+    return (codes, scales) if stream is None else (codes, scales, stream)

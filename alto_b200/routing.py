@@ -34,13 +34,30 @@ class ExpertPlan(NamedTuple):
     counts: torch.Tensor
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    elif t.is_contiguous() and t.shape[0] > 1 and t.shape[1] > 1:      # the usual case, with the fewest questions
+        return t
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:      # one expert or one token: strides that say nothing
+        t = t.as_strided(t.shape, (t.shape[1], 1))
+    return t
+
+
+def _forward(logits, params, bias):
+    ids, weights = L.route_forward(_rows(logits), params, bias)
+    if logits.dim() == 2:
+        return ids, weights
+    shape = (*logits.shape[:-1], params.top_k)
+    return ids.view(shape), weights.view(shape)
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, params, bias):
-        l2 = _rows(logits)
-        ids, weights = L.route_forward(l2, params, bias)
-        shape = (*logits.shape[:-1], params.top_k)
-        ids, weights = ids.view(shape), weights.view(shape)
+        ids, weights = _forward(logits, params, bias)
         ctx.save_for_backward(logits, ids)
         ctx.params = params
         ctx.set_materialize_grads(False)      # no zeros in the place of a gradient of ids
@@ -48,22 +65,13 @@ class _Route(torch.autograd.Function):
         return ids, weights
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @L.once_differentiable
     def backward(ctx, _, grad):
         if grad is None:
             return None, None, None
         logits, ids = ctx.saved_tensors
-        g = L.route_backward(_rows(logits), ctx.params, ids, grad.contiguous())
-        return g.view(logits.shape), None, None
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:
-        t2 = t2.contiguous()
-    if t2.stride(1) != 1 or t2.stride(0) < t2.shape[1]:      # one expert or one token: strides that say nothing
-        t2 = t2.as_strided(t2.shape, (t2.shape[1], 1))
-    return t2
+        g = L.route_backward(_rows(logits), ctx.params, ids, grad if grad.is_contiguous() else grad.contiguous())
+        return (g if logits.dim() == 2 else g.view(logits.shape)), None, None
 
 
 @L.traced("route_experts")
@@ -103,11 +111,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
                            1 if renormalize else 0, scale)
     if logits.requires_grad and torch.is_grad_enabled():
         return _Route.apply(logits, params, bias)
-    ids, weights = L.route_forward(_rows(logits), params, bias)
-    if logits.dim() == 2:
-        return ids, weights
-    shape = (*logits.shape[:-1], top_k)
-    return ids.view(shape), weights.view(shape)
+    return _forward(logits, params, bias)
 
 
 @L.traced("expert_plan")

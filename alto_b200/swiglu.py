@@ -43,10 +43,10 @@ class _SwiGLUKept(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, grad_out):
         codes, scales = ctx.saved_tensors
-        return _lib.swiglu_kept_backward(codes, scales, grad_out.contiguous(), ctx.fmt), None
+        return _lib.swiglu_kept_backward(codes, scales, grad_out if grad_out.is_contiguous() else grad_out.contiguous(), ctx.fmt), None
 
 
 def swiglu(h: torch.Tensor, checkpoint: Optional[str] = None) -> torch.Tensor:
@@ -66,4 +66,4 @@ def swiglu(h: torch.Tensor, checkpoint: Optional[str] = None) -> torch.Tensor:
         raise RuntimeError("swiglu runs on CUDA tensors only (no CPU fallback)")
     if not (h.requires_grad and torch.is_grad_enabled()):
         return _SwiGLU.apply(h.contiguous())      # nothing to keep
-    return _SwiGLUKept.apply(h.contiguous(), _KEEP[checkpoint])
+    return _SwiGLUKept.apply(h if h.is_contiguous() else h.contiguous(), _KEEP[checkpoint])

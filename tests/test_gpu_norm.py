@@ -187,6 +187,15 @@ def test_gradient_against_differences():
         assert abs(got - along) <= 1e-5 * (dx.double().norm() * v.norm() + dw.double().norm() * u.norm())
 
 
+def test_a_second_derivative_is_refused():
+    x, _, w, dy, _ = _inputs(8, 64, torch.float32, torch.float32)
+    x.requires_grad_(True)
+    dy.requires_grad_(True)
+    (dx,) = torch.autograd.grad(norm.rms_norm(x, w), x, dy, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
 def test_captured_calls_replay_on_new_contents_and_sums_keep_their_order():
     x, res, w, dy, ds = _inputs(300, 1536, torch.bfloat16, torch.float32)
     leaf = x.clone().requires_grad_(True)
