@@ -238,7 +238,8 @@ def plan_by_hand(ids, experts, align, rows):
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("tokens, k, experts, align", [(0, 2, 4, 128), (1, 1, 1, 128), (7, 3, 5, 128), (300, 4, 32, 128), (512, 4, 16, 1),
                                                        (513, 4, 16, 32), (3000, 2, 1, 128), (5000, 8, 256, 128), (2600, 10, 512, 8),
-                                                       (4099, 7, 1024, 128), (40000, 4, 33, 128)])
+                                                       (4099, 7, 1024, 128), (40000, 4, 33, 128),
+                                                       (200000, 3, 17, 128), (70000, 8, 700, 32), (4096, 1, 8, 128), (4097, 1, 8, 128)])
 def test_plan(tokens, k, experts, align, dtype):
     g = torch.Generator().manual_seed(tokens)
     ids = (torch.randn(tokens, k, generator=g).abs() * experts / 3).long().clamp_max(experts - 1).to(dtype)
