@@ -150,7 +150,7 @@ class LinearBackwardArgs(C.Structure):
 class RmsNormArgs(C.Structure):
     """``altob200_rms_norm_args`` of the header."""
     _fields_ = [(n, C.c_int64) for n in ("rows", "cols", "ld_x", "ld_residual")] + [
-        (n, C.c_void_p) for n in ("x", "residual", "weight", "out", "stream_out", "scale_plain", "scale_packed")] + [
+        (n, C.c_void_p) for n in ("x", "residual", "weight", "out", "stream_out", "normed_out", "scale_plain", "scale_packed")] + [
         ("eps", C.c_float)] + [(n, C.c_int32) for n in ("dtype", "weight_dtype", "format")]
 
 
@@ -644,9 +644,10 @@ _ROWS = torch.contiguous_format
 
 @on_device_of
 def rms_norm_forward(x2: torch.Tensor, weight: torch.Tensor, eps: float, residual2: Optional[torch.Tensor] = None,
-                     fmt: int = -1, packed: bool = False):
+                     fmt: int = -1, packed: bool = False, normed: Optional[torch.Tensor] = None):
     """(out, stream, scales): x2 [rows, cols] with unit column stride, rows of any stride that do not overlap; ``stream`` is
-    None without a residual, ``scales`` without an 8-bit format (plain, or the packed layout)."""
+    None without a residual, ``scales`` without an 8-bit format (plain, or the packed layout).  ``normed``: where the norm
+    goes in the type of x besides its codes."""
     rows, cols = x2.shape
     scales = stream = None
     if fmt < 0:
@@ -654,7 +655,7 @@ def rms_norm_forward(x2: torch.Tensor, weight: torch.Tensor, eps: float, residua
     else:
         out = torch.empty_like(x2, dtype=torch.uint8, memory_format=_ROWS)
     a = RmsNormArgs(rows, cols, x2.stride(0), 0, x2.data_ptr(), None, weight.data_ptr(), out.data_ptr(), None, None, None,
-                    eps, _DT_OF[x2.dtype], _DT_OF[weight.dtype], fmt)
+                    None, eps, _DT_OF[x2.dtype], _DT_OF[weight.dtype], fmt)
     if residual2 is not None:
         stream = torch.empty_like(x2, memory_format=_ROWS)
         a.ld_residual, a.residual, a.stream_out = residual2.stride(0), residual2.data_ptr(), stream.data_ptr()
@@ -665,6 +666,8 @@ def rms_norm_forward(x2: torch.Tensor, weight: torch.Tensor, eps: float, residua
         else:
             scales = torch.empty((rows, cols // 32), dtype=torch.uint8, device=x2.device)
             a.scale_plain = scales.data_ptr()
+    if normed is not None:
+        a.normed_out = normed.data_ptr()
     _check((_lib or lib()).altob200_rms_norm_forward(a, _stream()), "altob200_rms_norm_forward")
     return out, stream, scales
 

@@ -27,6 +27,7 @@ struct NormArgs {
   const void* w;
   void* y;              // T [rows, cols], or the codes
   void* r;              // T [rows, cols], only with res
+  void* y2;             // with codes: y as T [rows, cols] besides, or NULL
   uint8_t* scale_plain; // [rows, cols / 32] or NULL
   uint8_t* scale_packed;
   int64_t rows, cols, ld_x, ld_res;
@@ -259,6 +260,7 @@ __global__ void __launch_bounds__(LANES ? 128 : 1024) norm_forward_kernel(NormAr
     if constexpr (MX) {
 #pragma unroll
       for (int j = 0; j < V; ++j) p[j] = round_elem<BF16>(p[j]);
+      if (a.y2 != nullptr && u < units) store_unit<BF16, V>(reinterpret_cast<T*>(a.y2) + row * a.cols, u, pack_unit<BF16, V>(p));
       const uint32_t e = encode_block<BF16, V>(p, a.e5m2, reinterpret_cast<uint8_t*>(a.y) + row * a.cols + (int64_t)u * V, u < units);
       constexpr int HOLD = 32 / V;   // lanes that hold one block
       if (u < units && (u & (HOLD - 1)) == 0) {
@@ -296,6 +298,7 @@ __global__ void __launch_bounds__(256) norm_forward_any_kernel(NormArgs a) {
     const float v = stream(c) * rstd * weight_elem(a.w, c, a.w_f32);
     if constexpr (MX) {
       const float p = round_elem<BF16>(v);
+      if (a.y2 != nullptr) store_elem<BF16>(a.y2, row * a.cols + c, p);
       uint32_t m = f2u(p) & 0x7FFFFFFFu;
       m = __reduce_max_sync(0xFFFFFFFFu, m);
       const uint32_t e = BF16 ? e8m0_from_amax_bits<true>(m >> 16, a.e5m2 ? 2 : 3, a.e5m2 ? 15 : 8)
@@ -575,15 +578,15 @@ extern "C" int altob200_rms_norm_forward(const altob200_rms_norm_args* p, void* 
     return ALTOB200_EUNSUPPORTED;
   if (p->x == nullptr || p->weight == nullptr || p->out == nullptr || p->ld_x < p->cols ||
       (p->residual != nullptr && (p->stream_out == nullptr || p->ld_residual < p->cols)) ||
-      (mx && (p->cols % 32 != 0 || (p->scale_plain == nullptr && p->scale_packed == nullptr))))
+      (!mx && p->normed_out != nullptr) || (mx && (p->cols % 32 != 0 || (p->scale_plain == nullptr && p->scale_packed == nullptr))))
     return ALTOB200_EINVAL_SHAPE;
   if (p->rows >= (1ll << 31) - 128) return ALTOB200_ELIMIT;
   const int V = bf16 ? 8 : 4;
-  const bool vec = p->cols % V == 0 && p->ld_x % V == 0 && aligned16(p->x) && aligned16(p->out) && aligned16(p->weight) &&
+  const bool vec = p->cols % V == 0 && p->ld_x % V == 0 && aligned16(p->x) && aligned16(p->out) && aligned16(p->weight) && aligned16(p->normed_out) &&
                    (p->residual == nullptr || (p->ld_residual % V == 0 && aligned16(p->residual) && aligned16(p->stream_out)));
   const NormShape s = norm_shape(p->cols, vec ? V : 1, true);
   NormArgs a;
-  a.x = p->x; a.res = p->residual; a.w = p->weight; a.y = p->out; a.r = p->stream_out;
+  a.x = p->x; a.res = p->residual; a.w = p->weight; a.y = p->out; a.r = p->stream_out; a.y2 = p->normed_out;
   a.scale_plain = p->scale_plain; a.scale_packed = p->scale_packed;
   a.rows = p->rows; a.cols = p->cols; a.ld_x = p->ld_x; a.ld_res = p->ld_residual;
   a.eps = p->eps; a.inv_cols = (float)(1.0 / (double)p->cols);

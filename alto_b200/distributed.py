@@ -34,6 +34,7 @@ import torch
 import torch.distributed as dist
 
 from . import _lib as L
+from . import routing
 
 __all__ = ["allreduce_gradients", "shard_rows", "column_sharded_linear", "gathered_weight_linear",
            "gather_packed_rows", "gather_columns", "interleave_gathered_columns", "outer_scale_from_amax_bits",
@@ -460,7 +461,7 @@ class _AllToAllRows(torch.autograd.Function):
 
 
 class _DispatchState:
-    __slots__ = ("k", "tokens", "inv_order", "order", "in_splits", "out_splits", "index", "inverse", "offs")
+    __slots__ = ("k", "tokens", "inv_order", "order", "in_splits", "out_splits", "index", "inverse", "offs", "direct")
 
 
 class ExpertParallelDispatcher:
@@ -477,7 +478,9 @@ class ExpertParallelDispatcher:
     local re-sort to expert-major order with every expert's run padded to ``align`` rows (zeros).
     combine is the inverse followed by the score-weighted sum over each token's k routed rows.
     Both are differentiable.  One host synchronisation per dispatch (the split sizes of the
-    all-to-all live on the host); with a single rank the all-to-alls are skipped."""
+    all-to-all live on the host); with a single rank the all-to-alls are skipped, and on the GPU the two sorts of the
+    rows are one: tokens are gathered straight into the padded buffer by the rows of ``routing.expert_plan``, and
+    combined straight from it.  Ids outside [0, num_experts) are then slots without an expert."""
 
     def __init__(self, num_experts: int, group=None, align: int = ALIGN_SIZE_M):
         self.group = group
@@ -493,6 +496,9 @@ class ExpertParallelDispatcher:
         assert x.dim() == 2 and expert_ids.dim() == 2 and expert_ids.shape[0] == x.shape[0]
         T, k = expert_ids.shape
         dev = x.device
+        if (self.world == 1 and T * k > 0 and expert_ids.dtype in (torch.int32, torch.int64) and L.on_current_device(expert_ids)
+                and expert_ids.device == dev and self.num_experts <= routing.MAX_PLAN_EXPERTS):
+            return self._dispatch_alone(x, expert_ids)
         flat = expert_ids.reshape(-1).to(torch.int64)
         order = torch.argsort(flat, stable=True)
         inv_order = torch.empty_like(order)
@@ -507,7 +513,7 @@ class ExpertParallelDispatcher:
         both = torch.stack((send, recv)).cpu()                               # the one host synchronisation
         send_h, recv_h = both[0], both[1]
         st = _DispatchState()
-        st.k, st.tokens = k, T
+        st.k, st.tokens, st.direct = k, T, False
         st.inv_order = inv_order.to(torch.int32)
         st.order = order.to(torch.int32)
         st.in_splits = [int(v) for v in send_h.sum(1)]
@@ -524,8 +530,20 @@ class ExpertParallelDispatcher:
         x_local = _GatherRows.apply(rows, st.index, st.inverse)
         return x_local, st.offs, st
 
+    def _dispatch_alone(self, x: torch.Tensor, expert_ids: torch.Tensor):
+        T, k = expert_ids.shape
+        plan = routing.expert_plan(expert_ids, self.num_experts, self.align)
+        m_pad = int(plan.offs[-1])                                           # the one host synchronisation
+        st = _DispatchState()
+        st.k, st.tokens, st.direct = k, T, True
+        st.in_splits = st.out_splits = [T * k]
+        # row -> routed slot and back; the "receive buffer" is the routed slots in token order
+        st.index, st.order = plan.position[:m_pad], plan.position[:m_pad]
+        st.inverse, st.inv_order, st.offs = plan.slot, plan.slot, plan.offs
+        return _ReplicateSorted.apply(x, plan.token[:m_pad], plan.slot, k), st.offs, st
+
     def combine(self, y_local: torch.Tensor, state: _DispatchState, scores: Optional[torch.Tensor] = None):
-        rows = _GatherRows.apply(y_local, state.inverse, state.index)
+        rows = y_local if state.direct else _GatherRows.apply(y_local, state.inverse, state.index)
         if self.world > 1:
             rows = _AllToAllRows.apply(rows, state.in_splits, state.out_splits, self.group)
         # back to routed-row order (token-major, k minor: the inverse of the dispatch's sort), weighted by

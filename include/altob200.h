@@ -444,6 +444,7 @@ typedef struct altob200_rms_norm_args {
   const void* weight;
   void* out;
   void* stream_out;     /* with a residual only */
+  void* normed_out;     /* with codes: y as T [rows, cols] besides, or NULL */
   uint8_t* scale_plain;
   uint8_t* scale_packed;
   float eps;

@@ -27,7 +27,7 @@ def test_swiglu_refuses_unknown_formats_and_blocks_that_do_not_fit():
 
 def _norm_args(**change):
     # addresses that nothing reads: every call below is refused before a launch
-    a = L.RmsNormArgs(4, 64, 64, 0, 256, None, 256, 256, None, None, None, 1e-5, L.DT_BF16, L.DT_BF16, -1)
+    a = L.RmsNormArgs(4, 64, 64, 0, 256, None, 256, 256, None, None, None, None, 1e-5, L.DT_BF16, L.DT_BF16, -1)
     for k, v in change.items():
         setattr(a, k, v)
     return a
@@ -35,7 +35,7 @@ def _norm_args(**change):
 
 @pytest.mark.parametrize("change, status", [
     (dict(cols=0), L.E_SHAPE), (dict(rows=-1), L.E_SHAPE), (dict(ld_x=63), L.E_SHAPE), (dict(x=None), L.E_SHAPE),
-    (dict(residual=256), L.E_SHAPE), (dict(dtype=7), L.E_UNSUPPORTED), (dict(weight_dtype=2), L.E_UNSUPPORTED),
+    (dict(residual=256), L.E_SHAPE), (dict(normed_out=256), L.E_SHAPE), (dict(dtype=7), L.E_UNSUPPORTED), (dict(weight_dtype=2), L.E_UNSUPPORTED),
     (dict(format=L.FMT_NVFP4), L.E_UNSUPPORTED), (dict(format=L.FMT_MXFP8_E4M3), L.E_SHAPE),
     (dict(format=L.FMT_MXFP8_E4M3, scale_plain=256, cols=48, ld_x=64), L.E_SHAPE), (dict(rows=2 ** 31), L.E_LIMIT)])
 def test_norm_entry_point_refuses(change, status):
