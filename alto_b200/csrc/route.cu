@@ -47,15 +47,16 @@ __device__ __forceinline__ uint64_t ordered(double v) {
   if (v != v) return ~0ull;
   return (b >> 63) ? ~b : (b | (1ull << 63));
 }
+template <int LANES = 32>
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
   return v;
 }
-template <class F>
+template <class F, int LANES = 32>
 __device__ __forceinline__ F warp_add(F v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   return v;
 }
 __device__ __forceinline__ float from_ordered(uint32_t w) { return u2f(w >> 31 ? w & 0x7FFFFFFFu : ~w); }
@@ -329,29 +330,30 @@ __device__ __forceinline__ void load_logits(const void* logits, int64_t at, floa
 // Weights of the chosen, on lanes i < k (l: the chosen logit).  `m`, `z`: maximum and sum of exponentials
 // over all experts, used by the softmax that is not renormalised.  Ratios are formed from the chosen alone, so that they
 // hold however small the scores are; a token whose chosen scores are all zero gets zero weights.
+template <int LANES = 32>
 __device__ __forceinline__ float chosen_weight(bool on, float l, int sigmoid, int renorm, float m, float z, float* total) {
   *total = 1.0f;
   if (sigmoid) {
     // e^(l - c) / (1 + e^l) with c = min(0, the largest chosen logit): in range for any logits
     float c = 0.0f;
     if (renorm) {
-      c = fminf(warp_max(on ? l : -INFINITY), 0.0f);
+      c = fminf(warp_max<LANES>(on ? l : -INFINITY), 0.0f);
       if (c == -INFINITY) c = 0.0f;
     }
     const float num = l > 0.0f ? 1.0f : fast_exp(fmaxf(l - c, -126.0f)), den = 1.0f + fast_exp(fmaxf(-fabsf(l), -126.0f));
     const float s = !on ? 0.0f : l != l ? l : __fdividef(num, den);
     if (!renorm) return s;
-    *total = warp_add(s);
+    *total = warp_add<float, LANES>(s);
     return *total == 0.0f ? 0.0f : __fdividef(s, *total);
   }
   if (!renorm) {
     const float d = l - m;
     return on && m != -INFINITY ? __fdividef(d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f, z) : 0.0f;
   }
-  const float top = warp_max(on ? l : -INFINITY);
-  if (top == -INFINITY && !__any_sync(FULL, on && l != l)) return 0.0f;
+  const float top = warp_max<LANES>(on ? l : -INFINITY);
   const float d = l - top, s = !on ? 0.0f : d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f;
-  *total = warp_add(s);
+  *total = warp_add<float, LANES>(s);   // a NaN where top = -inf, and where there is one
+  if (top == -INFINITY && !(l != l)) return 0.0f;
   return __fdividef(s, *total);
 }
 
@@ -442,8 +444,47 @@ struct RouteGradArgs {
 //                                                                        renormalised (then zero for the others)
 //   sigmoid              dl_i = scale s_i (1 - s_i) g_i
 //   sigmoid, renormalised dl_i = scale q_i (1 - s_i) (g_i - sum g q)     q = s / sum s
+//
+// Where only the chosen have a gradient (all but the first): 16 lanes a token write its row of zeros, and over it, once
+// they have all written, the k values.  65536 x 256 fp32: 67 MB of zeros, 10 us at the copy rate.
+template <bool BF16>
+__global__ void __launch_bounds__(256) route_backward_chosen_kernel(RouteGradArgs a) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, float>::type;
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 15;
+  const int64_t step = (int64_t)gridDim.x * 16;
+  // both halves of a warp go round together (shuffles); one behind the last token does nothing
+  const int64_t mine = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), warp_first = mine & ~1ll;
+  for (int64_t lead = warp_first, t = mine; lead < a.tokens; lead += step, t += step) {
+    const bool live = t < a.tokens;
+    T* const out = reinterpret_cast<T*>(a.grad_logits) + t * a.experts;
+    int id = live && lane < a.k ? __ldg(a.ids + t * a.k + lane) : -1;
+    if (id >= a.experts) id = -1;
+    const bool on = id >= 0;
+    const float g = on ? __ldg(a.grad + t * a.k + lane) : 0.0f;
+    const float l = on ? logit_at<BF16>(a.logits, t * a.ld + id) : 0.0f;
+    if (live) {
+      if (a.vector) {
+        for (int c = lane; c < a.experts * (int)sizeof(T) / 16; c += 16) reinterpret_cast<uint4*>(out)[c] = make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        for (int e = lane; e < a.experts; e += 16) out[e] = (T)0.0f;
+      }
+    }
+    float total;
+    const float w = chosen_weight<16>(on, l, a.sigmoid, a.renorm, 0.0f, 1.0f, &total);
+    const float sum = a.renorm ? warp_add<float, 16>(on ? g * w : 0.0f) : 0.0f;
+    const float rest = a.sigmoid ? 1.0f / (1.0f + expf(l)) : 1.0f;   // 1 - s
+    const float d = a.scale * w * rest * (g - sum);
+    __syncwarp();
+    if (on) out[id] = (T)d;
+    __syncwarp();
+  }
+}
+
+// The softmax over all experts: every expert has a gradient.
 template <bool BF16, int V>
 __global__ void __launch_bounds__(256) route_backward_kernel(RouteGradArgs a) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, float>::type;
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
   for (int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); t < a.tokens; t += (int64_t)gridDim.x * 8) {
@@ -452,46 +493,29 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteGradArgs a) {
     if (id >= a.experts) id = -1;
     const bool on = id >= 0;
     const float l = on ? logit_at<BF16>(a.logits, row + id) : 0.0f, g = on ? __ldg(a.grad + t * a.k + lane) : 0.0f;
-    float m = 0.0f, z = 1.0f, total, all[V] = {};
-    const bool dense = !a.sigmoid && !a.renorm;
-    if (dense) {
-      m = -INFINITY;
+    float m = -INFINITY, z = 0.0f, total, all[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        all[j] = lane + 32 * j < a.experts ? logit_at<BF16>(a.logits, row + lane + 32 * j) : -INFINITY;
-        m = fmaxf(m, all[j]);
-      }
-      m = warp_max(m);
-      z = 0.0f;
+    for (int j = 0; j < V; ++j) {
+      all[j] = lane + 32 * j < a.experts ? logit_at<BF16>(a.logits, row + lane + 32 * j) : -INFINITY;
+      m = fmaxf(m, all[j]);
+    }
+    m = warp_max(m);
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (lane + 32 * j < a.experts) z += expf(all[j] - m);
-      z = warp_add(z);
+    for (int j = 0; j < V; ++j) {
+      const float d = all[j] - m;   // experts that are not there are -inf; m = -inf is seen to below
+      all[j] = d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f;
+      z += all[j];
     }
-    const float w = chosen_weight(on, l, a.sigmoid, a.renorm, m, z, &total);
-    float sum = 0.0f, d;
-    if (a.sigmoid) {
-      const float rest = 1.0f / (1.0f + expf(l));   // 1 - s
-      if (a.renorm) sum = warp_add(on ? g * w : 0.0f);
-      d = a.scale * w * rest * (g - sum);
-    } else {
-      sum = warp_add(on ? g * w : 0.0f);
-      d = a.scale * w * (g - sum);
-    }
-    // the row of zeros (or of the terms that every expert has), and over it, once the warp has written that, the chosen
-    using T = typename std::conditional<BF16, __nv_bfloat16, float>::type;
+    z = warp_add(z);
+    const float w = chosen_weight(on, l, 0, 0, m, z, &total);
+    const float sum = warp_add(on ? g * w : 0.0f), of_all = m != -INFINITY ? -a.scale * sum / z : 0.0f;
+    // the terms that every expert has, and over them, once the warp has written those, the chosen
     T* const out = reinterpret_cast<T*>(a.grad_logits) + t * a.experts;
-    if (dense) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (lane + 32 * j < a.experts) out[lane + 32 * j] = (T)(m != -INFINITY ? -a.scale * sum * (expf(all[j] - m) / z) : 0.0f);
-    } else if (a.vector) {
-      for (int c = lane; c < a.experts * (int)sizeof(T) / 16; c += 32) reinterpret_cast<uint4*>(out)[c] = make_uint4(0u, 0u, 0u, 0u);
-    } else {
-      for (int e = lane; e < a.experts; e += 32) out[e] = (T)0.0f;
-    }
+    for (int j = 0; j < V; ++j)
+      if (lane + 32 * j < a.experts) out[lane + 32 * j] = (T)(m != -INFINITY ? of_all * all[j] : 0.0f);
     __syncwarp();
-    if (on) out[id] = (T)d;
+    if (on) out[id] = (T)(a.scale * w * (g - sum));
     __syncwarp();
   }
 }
@@ -775,6 +799,13 @@ extern "C" int altob200_route_backward(const altob200_route_params* p, const voi
   a.experts = p->experts; a.k = p->top_k; a.sigmoid = p->sigmoid; a.renorm = p->renormalize; a.scale = p->scale;
   a.vector = (reinterpret_cast<uintptr_t>(grad_logits) & 15) == 0 && (p->experts * (p->dtype == ALTOB200_DT_BF16 ? 2 : 4)) % 16 == 0;
   const int E = p->experts;
+  if (a.sigmoid || a.renorm) {
+    int64_t blocks = ceil_div(tokens, 16);
+    if (blocks > 148 * 16) blocks = 148 * 16;
+    (void)launch_after(p->dtype == ALTOB200_DT_BF16 ? route_backward_chosen_kernel<true> : route_backward_chosen_kernel<false>,
+                       dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, a);
+    return cudaGetLastError() == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
+  }
   int64_t blocks = ceil_div(tokens, 8);
   if (blocks > 148 * 8) blocks = 148 * 8;
 #define RUN(B, V) (void)launch_after(route_backward_kernel<B, V>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, a)
