@@ -198,6 +198,7 @@ class _RMSNormMXFP8Linear(torch.autograd.Function):
 
 
 @L.traced("rms_norm_mxfp8_linear")
+@L.on_device_of
 def rms_norm_mxfp8_linear(x: torch.Tensor, norm_weight: torch.Tensor, weights: Union[torch.Tensor, Sequence[torch.Tensor]],
                           eps: float = 1e-5, residual: Optional[torch.Tensor] = None, fp8_variant: str = "e4m3",
                           use_2dblock_w: bool = False):

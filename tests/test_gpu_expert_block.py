@@ -98,6 +98,22 @@ def test_frozen_and_unused_parts_of_linears_behind_a_norm():
         norm.rms_norm_mxfp8_linear(x, nw, w.float())
 
 
+def test_converted_weights_behind_a_norm():
+    from alto_b200.lpt import LowPrecisionTrainingModifier
+    lin = torch.nn.Linear(128, 64, bias=False).cuda().bfloat16()
+    plain = lin.weight.detach().clone().requires_grad_(True)
+    model = torch.nn.Sequential(lin)
+    LowPrecisionTrainingModifier(scheme="mxfp8_e4m3", targets="Linear").convert(model)
+    x, nw, dy = _randn(64, 128, seed=1), _randn(128, seed=2, mean=1.0), _randn(64, 64, seed=3)
+    y = norm.rms_norm_mxfp8_linear(x, nw, lin.weight)
+    y.backward(dy)
+    want = norm.rms_norm_mxfp8_linear(x, nw, plain)
+    want.backward(dy)
+    assert torch.equal(y.detach(), want.detach()) and torch.equal(torch.as_tensor(lin.weight.grad), plain.grad)
+    with torch.no_grad():
+        assert torch.equal(norm.rms_norm_mxfp8_linear(x, nw, lin.weight), want.detach())
+
+
 def test_codes_of_the_norm_feed_the_block_scaled_product():
     x, res, nw, w = _randn(70, 256, seed=1), _randn(70, 256, seed=2), _randn(256, seed=3, mean=1.0), _randn(96, 256, seed=4, std=0.05)
     wc, ws = mxfp8.convert_to_mxfp8(w)
