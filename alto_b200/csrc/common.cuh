@@ -76,6 +76,13 @@ __device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) {
   return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(f));
 }
 
+// Two floats as a word of bf16 (lo in the low half), each rounded to nearest even: one instruction.
+__device__ __forceinline__ uint32_t pack_bf16_rn(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // e^x = 2^hi 2^lo for |x| <= 126, hi the rounded product with log2 e and lo what the rounding (and the constant's) left of
 // it, so the result is off by the two steps of ex2 and of two products at every x.  One special-function instruction and
 // five others.  inf beyond 2^128, 0 below 2^-126.
@@ -85,6 +92,17 @@ __device__ __forceinline__ float fast_exp(float x) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
   return __fmul_rn(e, __fmaf_rn(lo, 0.693147182464599609375f, 1.0f));
+}
+
+// The same for two numbers, two to an instruction but for the exponentials.
+__device__ __forceinline__ float2 fast_exp2x(float2 x) {
+  const float2 up = make_float2(1.44269502162933349609375f, 1.44269502162933349609375f);
+  const float2 hi = __fmul2_rn(x, up);
+  const float2 lo = __ffma2_rn(x, make_float2(1.92596299e-8f, 1.92596299e-8f), __ffma2_rn(x, up, make_float2(-hi.x, -hi.y)));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(hi.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(hi.y));
+  return __fmul2_rn(e, __ffma2_rn(lo, make_float2(0.693147182464599609375f, 0.693147182464599609375f), make_float2(1.0f, 1.0f)));
 }
 
 // ---------------------------------------------------------------------------------------

@@ -61,8 +61,7 @@ __device__ __forceinline__ void unpack_vec(const uint4& w, float* v) {
 template <bool BF16>
 __device__ __forceinline__ uint4 pack_vec(const float* v) {
   if constexpr (BF16) {
-    return make_uint4(f32_to_bf16_bits(v[0]) | (f32_to_bf16_bits(v[1]) << 16), f32_to_bf16_bits(v[2]) | (f32_to_bf16_bits(v[3]) << 16),
-                      f32_to_bf16_bits(v[4]) | (f32_to_bf16_bits(v[5]) << 16), f32_to_bf16_bits(v[6]) | (f32_to_bf16_bits(v[7]) << 16));
+    return make_uint4(pack_bf16_rn(v[0], v[1]), pack_bf16_rn(v[2], v[3]), pack_bf16_rn(v[4], v[5]), pack_bf16_rn(v[6], v[7]));
   } else {
     return make_uint4(f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3]));
   }

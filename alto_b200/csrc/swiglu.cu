@@ -93,9 +93,9 @@ static int swiglu_launch(const void* h, const void* go, int64_t rows, int64_t H,
 //   grad_h[r, c] = bf16( go u s (1 + g (1 - s)) ),  grad_h[r, H + c] = bf16( go g s )
 // in fp32 with one rounding: the tensor-op form's intermediate roundings are of an h that no longer exists here.
 //
-// 69632 x 2880 (floor 247 us a direction: 8.06 and 8.06 bytes a column at the copy rate): forward 282 us, its issue slots
-// 74 % busy with 290 instructions for eight columns of both halves, DRAM 5.7 TB/s; backward 252, DRAM at the copy rate.
-// With expf and divisions 396 and 460; forward without the loads ahead 310.
+// 69632 x 2880 (floor 247 us a direction: 8.06 and 8.06 bytes a column at the copy rate): forward 270 us, bound by
+// instructions; backward 252, the copy rate.  With expf and divisions 396 and 460; forward without the loads ahead 278, with
+// one number to an instruction 282 (290 instructions for eight columns of both halves, issue slots 74 % busy).
 // ---------------------------------------------------------------------------------------
 // 16 / (1 + e^-g), off by the steps of the exponential and of the reciprocal.  The factor 16 keeps the reciprocal of
 // 1 + e^88.7 above the least normal number; a sixteenth of a bf16 number is exact.  Outside of +-126, where the result is 16
@@ -104,6 +104,19 @@ __device__ __forceinline__ float sigmoid16(float g) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmaf_rn(fast_exp(-fminf(fmaxf(g, -126.0f), 126.0f)), 0.0625f, 0.0625f)));
   return r;
+}
+// Two at once, for the direction that has no more instructions to spare (in the other their pairs of registers cost more
+// warps than they save: 258 us for 252).
+__device__ __forceinline__ float2 sigmoid16(float2 g) {
+  const float2 e = fast_exp2x(make_float2(-fminf(fmaxf(g.x, -126.0f), 126.0f), -fminf(fmaxf(g.y, -126.0f), 126.0f)));
+  const float2 d = __ffma2_rn(e, make_float2(0.0625f, 0.0625f), make_float2(0.0625f, 0.0625f));
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  return r;
+}
+__device__ __forceinline__ uint4 pack8_rn(const float v[8]) {
+  return make_uint4(pack_bf16_rn(v[0], v[1]), pack_bf16_rn(v[2], v[3]), pack_bf16_rn(v[4], v[5]), pack_bf16_rn(v[6], v[7]));
 }
 
 // Scale byte of a block from the largest magnitude (bf16 bits), and eight of its elements (two to a word) as codes.
@@ -185,8 +198,15 @@ __global__ void __launch_bounds__(256) swiglu_keep_kernel(const uint4* __restric
     const uint32_t eg = e8m0_from_amax_bits<true>(m & 0xFFFFu, E5M2 ? 2 : 3, E5M2 ? 15 : 8);
     const uint32_t eu = e8m0_from_amax_bits<true>(m >> 16, E5M2 ? 2 : 3, E5M2 ? 15 : 8);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = __fmul_rn(round_bf16(__fmul_rn(__fmul_rn(g[j], 0.0625f), sigmoid16(g[j]))), u[j]);
-    out[at.r * hv + at.c] = pack8(o);
+    for (int j = 0; j < 8; j += 2) {
+      const float2 two = make_float2(g[j], g[j + 1]);
+      const float2 silu = __fmul2_rn(__fmul2_rn(two, make_float2(0.0625f, 0.0625f)), sigmoid16(two));
+      const uint32_t w = pack_bf16_rn(silu.x, silu.y);
+      const float2 p = __fmul2_rn(make_float2(bf16lo_to_f32(w), bf16hi_to_f32(w)), make_float2(u[j], u[j + 1]));
+      o[j] = p.x;
+      o[j + 1] = p.y;
+    }
+    out[at.r * hv + at.c] = pack8_rn(o);
     codes[at.r * 2 * hv + at.c] = encode8_mxfp8<E5M2>(g, eg);
     codes[at.r * 2 * hv + hv + at.c] = encode8_mxfp8<E5M2>(u, eu);
     if ((threadIdx.x & 3) == 0) {
@@ -229,13 +249,13 @@ __global__ void __launch_bounds__(256) swiglu_kept_backward_kernel(const uint2* 
       g[j] = __fmul_rn(ds, __fmaf_rn(gs, __fsub_rn(1.0f, s), s));   // go u (s + g s (1 - s))
       u[j] = __fmul_rn(d[j], gs);
     }
-    out[at.r * 2 * hv + at.c] = pack8(g);
-    out[at.r * 2 * hv + hv + at.c] = pack8(u);
+    out[at.r * 2 * hv + at.c] = pack8_rn(g);
+    out[at.r * 2 * hv + hv + at.c] = pack8_rn(u);
   }
 }
 
 // Backward gains from more and shorter walks (69632 x 2880: 284 us with 16 a SM, 252
-// with 64), forward, whose walks start with loads that nothing covers, does not (282 with 4 to 64).
+// with 64), forward, whose walks start with loads that nothing covers, does not.
 static unsigned swiglu_blocks(int64_t rows, int64_t H, int per_sm) {
   const int64_t blocks = ceil_div(rows * (H / 8), 256);
   return (unsigned)(blocks > 148 * per_sm ? 148 * per_sm : blocks);
