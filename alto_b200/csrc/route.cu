@@ -82,7 +82,7 @@ __device__ __forceinline__ int choose_in_double(const RouteArgs& a, int64_t row,
   }
   __syncwarp();
   for (int e = lane; e < E; e += 32) {
-    const double l = logit_at<BF16>(a.logits, row + e), s = !a.computed ? l : a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
+    const double l = logit_at<BF16>(a.logits, row + e), s = !a.computed ? l + 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - m) / z;
     keys[e] = a.bias != nullptr ? s + (double)__ldg(a.bias + e) : s;
   }
   __syncwarp();
@@ -197,7 +197,7 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
     for (int j = 0; j < V; ++j) word[j] = ordered_bits(f2u(p[j] * r + b[j]));   // arithmetic's NaN is above everything
   } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) word[j] = ordered(l[j]);
+    for (int j = 0; j < V; ++j) word[j] = ordered(l[j] + 0.0f);   // -0 is 0
   }
 #pragma unroll
   for (int j = 0; j < V; ++j)

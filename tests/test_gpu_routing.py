@@ -117,6 +117,13 @@ def test_equal_and_nearly_equal_keys(score):
     for bias in (None, zero):
         _check(logits, 7, score=score, bias=bias)
         _check(logits, 7, score=score, bias=bias, num_groups=6, groups_kept=3, group_top=2)
+    # zeros of both signs are one number
+    signed = torch.where(torch.rand(300, 48, generator=torch.Generator().manual_seed(5)) < 0.5, 0.0, -0.0)
+    signed[:, 40:] = -1.0
+    for l in (signed.cuda(), signed.cuda().bfloat16()):
+        for bias in (None, zero):
+            _check(l, 7, score=score, bias=bias)
+            _check(l, 7, score=score, bias=bias, num_groups=6, groups_kept=3, group_top=1)
     # neighbours one step of fp32 apart, whose scores fp32 does not tell apart
     g = torch.Generator().manual_seed(1)
     base = torch.tensor([4.0, 1.0, -6.0, -30.0])[torch.randint(0, 4, (600, 1), generator=g)]
