@@ -195,83 +195,100 @@ __device__ __forceinline__ void zero_packed_padding(const NormArgs& a, int64_t r
   for (int64_t c = first + thread; c < tiles * 4; c += threads) a.scale_packed[packed_scale_offset(row, c, tiles)] = 0;
 }
 
-// One row per LANES lanes of a warp, or (LANES = 0) per CTA; NV units of V elements a thread.  With codes as fast as without
-// although it writes less: the turnover of CTAs, not the copy rate, sets the pace (8192 x 4096: 45 us; 42 without any
-// 8-bit store).  CTAs that walk over rows with the next one's loads ahead, as in the backward pass, are slower (47 us for
-// 43, with codes 52), and so are scale bytes put together to words (46).
-template <bool BF16, bool MX, int LANES, int NV, int V>
+// One row per LANES lanes of a warp, or (LANES = 0) ROWS rows per CTA; NV units of V elements a thread and row.  With codes as
+// fast as without although it writes less: the turnover of CTAs sets the pace, so two rows share one (8192 x 4096: 43 us,
+// with codes 43; one row a CTA 44 and 46).  CTAs that walk over rows with the next one's loads ahead, as in the backward
+// pass, are slower (47, with codes 52), and scale bytes put together to words no faster.
+template <bool BF16, bool MX, int LANES, int NV, int V, int ROWS = 1>
 __global__ void __launch_bounds__(LANES ? 128 : 1024) norm_forward_kernel(NormArgs a) {
   using T = typename NormType<BF16>::T;
   using U = typename Held<V>::U;
   constexpr bool WARP = LANES != 0;
-  __shared__ float part[32];
+  __shared__ float part[ROWS][32];
   grid_dependency_wait();
   const int threads = WARP ? LANES : blockDim.x, t = WARP ? (threadIdx.x & (LANES - 1)) : threadIdx.x;
-  const int64_t row = WARP ? ((int64_t)blockIdx.x * 128 + threadIdx.x) / LANES : blockIdx.x;
-  if (MX && a.scale_packed != nullptr && row < ((a.rows + 127) & ~127ll)) zero_packed_padding(a, row, t, threads);
-  if (!WARP && row >= a.rows) return;
-  // lanes behind the last row go along with nothing
-  const int units = row < a.rows ? (int)(a.cols / V) : 0;
-  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
-  U raw[NV];
+  const int64_t first = WARP ? ((int64_t)blockIdx.x * 128 + threadIdx.x) / LANES : (int64_t)blockIdx.x * ROWS;
+  if (MX && a.scale_packed != nullptr) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int u = t + i * threads;
-    raw[i] = u < units ? load_unit<BF16, V>(x, u) : no_unit<V>();
+    for (int k = 0; k < ROWS; ++k)
+      if (first + k < ((a.rows + 127) & ~127ll)) zero_packed_padding(a, first + k, t, threads);
   }
-  if (a.res != nullptr) {
-    const T* res = reinterpret_cast<const T*>(a.res) + row * a.ld_res;
-    T* r = reinterpret_cast<T*>(a.r) + row * a.cols;
-    U add[NV];
+  if (!WARP && first >= a.rows) return;
+  U raw[ROWS][NV], add[ROWS][NV];
+  // threads behind the last row go along with nothing
+  const auto units_of = [&](int k) { return first + k < a.rows ? (int)(a.cols / V) : 0; };
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const T* x = reinterpret_cast<const T*>(a.x) + (first + k) * a.ld_x;
+    const T* res = reinterpret_cast<const T*>(a.res) + (first + k) * a.ld_res;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int u = t + i * threads;
-      add[i] = u < units ? load_unit<BF16, V>(res, u) : no_unit<V>();
+      const bool on = u < units_of(k);
+      raw[k][i] = on ? load_unit<BF16, V>(x, u) : no_unit<V>();
+      if (a.res != nullptr) add[k][i] = on ? load_unit<BF16, V>(res, u) : no_unit<V>();
     }
+  }
+  float ss[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    ss[k] = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int u = t + i * threads;
-      float p[V], q[V];
-      unpack_unit<BF16, V>(raw[i], p);
-      unpack_unit<BF16, V>(add[i], q);
+      float p[V];
+      unpack_unit<BF16, V>(raw[k][i], p);
+      if (a.res != nullptr) {
+        const int u = t + i * threads;
+        float q[V];
+        unpack_unit<BF16, V>(add[k][i], q);
 #pragma unroll
-      for (int j = 0; j < V; ++j) p[j] = __fadd_rn(p[j], q[j]);
-      raw[i] = pack_unit<BF16, V>(p);
-      if (u < units) store_unit<BF16, V>(r, u, raw[i]);
-    }
-  }
-  float ss = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float p[V];
-    unpack_unit<BF16, V>(raw[i], p);
-#pragma unroll
-    for (int j = 0; j < V; ++j) ss = __fmaf_rn(p[j], p[j], ss);
-  }
-  if constexpr (WARP) ss = warp_sum<LANES>(ss);
-  else ss = block_sum(ss, part);
-  const float rstd = rsqrtf(__fmaf_rn(ss, a.inv_cols, a.eps));
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int u = t + i * threads;
-    float p[V], w[V] = {};
-    unpack_unit<BF16, V>(raw[i], p);
-    if (u < units) load_weights<V>(a.w, (int64_t)u * V, a.w_f32, w);
-#pragma unroll
-    for (int j = 0; j < V; ++j) p[j] = p[j] * rstd * w[j];
-    if constexpr (MX) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) p[j] = round_elem<BF16>(p[j]);
-      if (a.y2 != nullptr && u < units) store_unit<BF16, V>(reinterpret_cast<T*>(a.y2) + row * a.cols, u, pack_unit<BF16, V>(p));
-      const uint32_t e = encode_block<BF16, V>(p, a.e5m2, reinterpret_cast<uint8_t*>(a.y) + row * a.cols + (int64_t)u * V, u < units);
-      constexpr int HOLD = 32 / V;   // lanes that hold one block
-      if (u < units && (u & (HOLD - 1)) == 0) {
-        const int64_t nkb = a.cols >> 5, kb = u / HOLD;
-        if (a.scale_plain != nullptr) a.scale_plain[row * nkb + kb] = (uint8_t)e;
-        if (a.scale_packed != nullptr) a.scale_packed[packed_scale_offset(row, kb, (nkb + 3) >> 2)] = (uint8_t)e;
+        for (int j = 0; j < V; ++j) p[j] = __fadd_rn(p[j], q[j]);
+        raw[k][i] = pack_unit<BF16, V>(p);
+        if (u < units_of(k)) store_unit<BF16, V>(reinterpret_cast<T*>(a.r) + (first + k) * a.cols, u, raw[k][i]);
+        unpack_unit<BF16, V>(raw[k][i], p);
       }
-    } else if (u < units) {
-      store_unit<BF16, V>(reinterpret_cast<T*>(a.y) + row * a.cols, u, pack_unit<BF16, V>(p));
+#pragma unroll
+      for (int j = 0; j < V; ++j) ss[k] = __fmaf_rn(p[j], p[j], ss[k]);
+    }
+    ss[k] = warp_sum<WARP ? LANES : 32>(ss[k]);
+  }
+  if constexpr (!WARP) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      if (lane == 0) part[k][warp] = ss[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) ss[k] = warp_sum(lane < warps ? part[k][lane] : 0.0f);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int u = t + i * threads;
+    float w[V] = {};
+    if (u < (int)(a.cols / V)) load_weights<V>(a.w, (int64_t)u * V, a.w_f32, w);
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      const int64_t row = first + k;
+      const bool on = u < units_of(k);
+      const float rstd = rsqrtf(__fmaf_rn(ss[k], a.inv_cols, a.eps));
+      float p[V];
+      unpack_unit<BF16, V>(raw[k][i], p);
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[j] = p[j] * rstd * w[j];
+      if constexpr (MX) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) p[j] = round_elem<BF16>(p[j]);
+        if (a.y2 != nullptr && on) store_unit<BF16, V>(reinterpret_cast<T*>(a.y2) + row * a.cols, u, pack_unit<BF16, V>(p));
+        const uint32_t e = encode_block<BF16, V>(p, a.e5m2, reinterpret_cast<uint8_t*>(a.y) + row * a.cols + (int64_t)u * V, on);
+        constexpr int HOLD = 32 / V;   // lanes that hold one block
+        if (on && (u & (HOLD - 1)) == 0) {
+          const int64_t nkb = a.cols >> 5, kb = u / HOLD;
+          if (a.scale_plain != nullptr) a.scale_plain[row * nkb + kb] = (uint8_t)e;
+          if (a.scale_packed != nullptr) a.scale_packed[packed_scale_offset(row, kb, (nkb + 3) >> 2)] = (uint8_t)e;
+        }
+      } else if (on) {
+        store_unit<BF16, V>(reinterpret_cast<T*>(a.y) + row * a.cols, u, pack_unit<BF16, V>(p));
+      }
     }
   }
 }
@@ -547,7 +564,8 @@ static NormShape norm_shape(int64_t cols, int vec, bool forward) {
   if (vec > 1) {
     const int64_t units = cols / vec;
     if (units <= 32) return {units <= 8 ? 8 : units <= 16 ? 16 : 32, 128, 1, vec};
-    const int nv = units <= 1024 ? 1 : units <= 2048 ? 2 : 4;
+    // forward: two vectors a thread rather than CTAs of more than 512 (4096 x 8192 bf16 with codes 55 us in two rows a CTA)
+    const int nv = units <= (forward ? 512 : 1024) ? 1 : units <= 2048 ? 2 : 4;
     if (units <= 4096) return {0, (int)(ceil_div(ceil_div(units, nv), 32) * 32), nv, vec};
     return {0, 0, 0, 0};
   }
@@ -602,7 +620,10 @@ extern "C" int altob200_rms_norm_forward(const altob200_rms_norm_args* p, void* 
     else { if (mx) ANY(false, true); else ANY(false, false); }
 #undef ANY
   } else {
-    const dim3 grid((unsigned)(s.lanes ? ceil_div(all_rows, 128 / s.lanes) : all_rows)), block(s.threads);
+    // two rows a CTA as soon as there are more rows than CTAs at a time (4096 columns: 148 rows 2.1 us one by one, 2.4 in
+    // pairs; 2400 rows 12.9 and 11.1, 8192 rows 48 and 43, with codes 52 and 43)
+    const bool two = s.lanes == 0 && s.nv == 1 && s.v > 1 && all_rows > 148 * 4;
+    const dim3 grid((unsigned)(s.lanes ? ceil_div(all_rows, 128 / s.lanes) : two ? ceil_div(all_rows, 2) : all_rows)), block(s.threads);
 #define ONE(B, M, L, N, V) (void)launch_after(norm_forward_kernel<B, M, L, N, V>, grid, block, 0, st, a)
 #define BY_SHAPE(B, M, V)                             \
   do {                                                \
@@ -613,6 +634,7 @@ extern "C" int altob200_rms_norm_forward(const altob200_rms_norm_args* p, void* 
     } else if (s.lanes == 8) ONE(B, M, 8, 1, V);      \
     else if (s.lanes == 16) ONE(B, M, 16, 1, V);      \
     else if (s.lanes == 32) ONE(B, M, 32, 1, V);      \
+    else if (two) (void)launch_after(norm_forward_kernel<B, M, 0, 1, V, 2>, grid, block, 0, st, a); \
     else if (s.nv == 1) ONE(B, M, 0, 1, V);           \
     else if (s.nv == 2) ONE(B, M, 0, 2, V);           \
     else ONE(B, M, 0, 4, V);                          \
