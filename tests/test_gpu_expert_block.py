@@ -50,7 +50,8 @@ def test_dispatch_leaves_out_slots_without_an_expert():
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("fmt, two_d", [("e4m3", False), ("e5m2", True)])
-@pytest.mark.parametrize("rows, k, outs", [(96, 128, (64,)), (160, 288, (96, 32)), (64, 1024, (256, 128))])
+@pytest.mark.parametrize("rows, k, outs", [(96, 128, (64,)), (160, 288, (96, 32)), (64, 1024, (256, 128)),
+                                           (608, 288, (32,)), (672, 64, (32, 64))])
 def test_linears_behind_a_norm(rows, k, outs, fmt, two_d, dtype):
     x, res, nw = _randn(rows, k, seed=1, dtype=dtype), _randn(rows, k, seed=2, dtype=dtype), _randn(k, seed=3, std=0.2, mean=1.0, dtype=dtype)
     ws = [_randn(n, k, seed=10 + i, std=0.05, dtype=dtype) for i, n in enumerate(outs)]

@@ -58,7 +58,7 @@ def _check_backward(dx, dw, r, w, dy, ds, eps=EPS):
 
 SIZES = [(1, 1), (3, 7), (5, 32), (1, 64), (130, 96), (7, 264), (33, 1000), (64, 1024), (9, 1032), (65, 2880), (31, 4096), (3, 8200),
          (2, 16384), (2, 32768), (2, 40000), (700, 512), (0, 64), (1001, 128), (77, 56), (13, 200), (1300, 255), (21, 3001),
-         (6, 8191), (3, 9001)]
+         (6, 8191), (3, 9001), (1001, 264), (603, 4096)]
 
 
 @pytest.mark.parametrize("dtype, wdtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32),
@@ -113,7 +113,7 @@ def test_leading_dimensions_transposed_and_broadcast_rows():
 @pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows, cols", [(1, 32), (3, 64), (130, 96), (17, 1024), (33, 2880), (8, 4096), (2, 16384), (2, 33024), (0, 64), (301, 128),
-                                        (4, 8192)])
+                                        (4, 8192), (1001, 288), (603, 2880)])
 def test_mxfp8_result_is_the_quantised_norm(rows, cols, dtype, fmt):
     x, res, w, _, _ = _inputs(rows, cols, dtype, dtype)
     if rows > 1:      # rows of zeros, of infinities and NaN, of magnitudes at both ends
