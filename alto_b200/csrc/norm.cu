@@ -11,7 +11,7 @@
 // Both directions are HBM streams: forward reads x (and the residual) and writes y (and r), backward reads dy, r (and
 // d_stream) and writes dr.  rstd is not kept: backward reads r anyway, and one more sum costs less than the launch-time
 // allocation of a vector.  bf16 8192 x 4096 with residual (floor 41 us a direction at the copy rate): forward 42 us, backward
-// 48 and 3 to join dw; without loads ahead 68 and 5.  32768 x 4096 (floor 164): 167 and 183 + 4.
+// 48 and 3 to join dw; without loads ahead 68 and 5.  32768 x 4096 (floor 164): 153 and 183 + 4.
 //
 // A row is held in registers: 16-byte vectors of it per thread (lane-adjacent, so that four (bf16) or eight (fp32)
 // neighbouring lanes hold a block of 32) or, where width, strides or pointers rule those out, single elements.  8 to 32
