@@ -39,9 +39,8 @@ __device__ __forceinline__ float logit_at(const void* p, int64_t i) {
   else return __ldg(reinterpret_cast<const float*>(p) + i);
 }
 
-// Unsigned words in the order of the floats; a NaN above everything, 0 below everything.
+// Unsigned words in the order of the floats; a (positive) NaN above everything, 0 below everything.
 __device__ __forceinline__ uint32_t ordered_bits(uint32_t b) { return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u); }
-__device__ __forceinline__ uint32_t ordered(float v) { return v != v ? 0xFFFFFFFFu : ordered_bits(f2u(v)); }
 __device__ __forceinline__ uint64_t ordered(double v) {
   const uint64_t b = (uint64_t)__double_as_longlong(v);
   if (v != v) return ~0ull;
@@ -156,6 +155,40 @@ __device__ __forceinline__ void sort_words(uint32_t* w) {
   }
 }
 
+// Keys of a lane's experts in fp32 (the logits, or scores and bias), and the largest score that the token can have.  Every
+// key comes out of an addition, whose NaN is the positive one: its bits are above everything.
+template <int V>
+__device__ __forceinline__ float keys_of(const RouteArgs& a, const float* l, const float* b, float* key) {
+  if (!a.computed) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = l[j] + 0.0f;   // -0 is 0
+    return 0.0f;
+  }
+  float r = 1.0f;
+  if (a.sigmoid) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(key[j]) : "f"(1.0f + fast_exp(fminf(fmaxf(-l[j], -126.0f), 126.0f))));
+      if (l[j] != l[j]) key[j] = l[j];
+    }
+  } else {
+    float m = l[0], z = 0.0f;
+#pragma unroll
+    for (int j = 1; j < V; ++j) m = fmaxf(m, l[j]);
+    m = warp_max(m);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = l[j] - m;
+      key[j] = d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f;
+      z += key[j];
+    }
+    r = 1.0f / warp_add(z);
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) key[j] = key[j] * r + b[j];
+  return r;
+}
+
 // The choice of one token by one warp in fp32; lane l holds the a.per experts from l * a.per on.  Lane i < k returns the i-th
 // choice and its logit.  *sure: every decision holds in exact arithmetic too.
 //
@@ -172,37 +205,18 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
   const int lane = threadIdx.x & 31, per = WHOLE ? V : a.per;
   uint32_t word[V];
   *sure = true;
-  if (a.computed) {
-    float p[V], r = 1.0f;
-    if (a.sigmoid) {
+  float most;
+  {
+    float key[V];
+    most = keys_of<V>(a, l, b, key);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p[j]) : "f"(1.0f + fast_exp(fminf(fmaxf(-l[j], -126.0f), 126.0f))));
-        if (l[j] != l[j]) p[j] = l[j];
-      }
-    } else {
-      float m = l[0], z = 0.0f;
-#pragma unroll
-      for (int j = 1; j < V; ++j) m = fmaxf(m, l[j]);
-      m = warp_max(m);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = l[j] - m;
-        p[j] = d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f;
-        z += p[j];
-      }
-      r = 1.0f / warp_add(z);
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) word[j] = ordered_bits(f2u(p[j] * r + b[j]));   // arithmetic's NaN is above everything
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) word[j] = ordered(l[j] + 0.0f);   // -0 is 0
+    for (int j = 0; j < V; ++j) word[j] = ordered_bits(f2u(key[j]));
   }
 #pragma unroll
   for (int j = 0; j < V; ++j)
     word[j] = WHOLE || (j < per && lane * per + j < a.experts) ? (word[j] & ~LOW) | (LOW - (uint32_t)j) : 0u;
   int left = a.experts;
+  uint32_t kept = 1u;   // bit g (times the lanes of a group): group g
   if (a.groups > 1) {
     // a group's two best: by the lanes that hold it, or, where groups do not consist of a power of two of whole lanes,
     // by one lane from shared memory
@@ -234,7 +248,8 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
     }
     const float of_group = a.group_top == 2 && size > 1 ? from_ordered(best) + from_ordered(second) : from_ordered(best);
     // the kept groups one by one, the lowest among equals; then, if asked, the first that is not kept
-    uint32_t rest = mine >= a.groups ? 0u : a.group_top == 2 ? ordered(of_group) : best & ~LOW, kept = 0u;
+    uint32_t rest = mine >= a.groups ? 0u : a.group_top == 2 ? ordered_bits(f2u(of_group)) : best & ~LOW;
+    kept = 0u;
     int last = 0;
     for (int i = 0; i < a.kept; ++i) {
       const uint32_t top = __reduce_max_sync(FULL, rest);
@@ -246,8 +261,10 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
       const uint32_t top = __reduce_max_sync(FULL, rest);
       const int next = __ffs(__ballot_sync(FULL, rest == top)) - 1;
       const float u = __shfl_sync(FULL, of_group, last), v = __shfl_sync(FULL, of_group, next);
-      const float one = fabsf(from_ordered(__shfl_sync(FULL, best, last)));   // of the two keys, which may cancel
-      if (u - v <= 2.0f * (a.score_room + CUT * fmaxf(one, fabsf(u)))) *sure = false;
+      // the largest of the (finite) keys in any group's sum, which may cancel there
+      const float large = a.group_top == 2 && size > 1 ? fmaxf(fabsf(from_ordered(best)), fabsf(from_ordered(second))) : fabsf(of_group);
+      const float both = u2f(__reduce_max_sync(FULL, mine < a.groups && large < INFINITY ? f2u(large) : 0u));
+      if (u - v <= 2.0f * (a.score_room + CUT * both)) *sure = false;
     }
     left = a.kept * size;
     if (a.lanes_per_group > 0) {
@@ -288,8 +305,35 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
     const float my_b = on && a.bias != nullptr ? __ldg(a.bias + mine) : 0.0f, my_key = from_ordered(mine_word);
     const float next_l = __shfl_down_sync(FULL, my_l, 1), next_b = __shfl_down_sync(FULL, my_b, 1);
     const float next_key = __shfl_down_sync(FULL, my_key, 1);
-    const float room = a.score_room * fmaxf(my_key - my_b, next_key - next_b) + CUT * fmaxf(fabsf(my_key), fabsf(next_key));
-    if (__any_sync(FULL, lane + 1 < picks && my_key - next_key <= room && !(my_l == next_l && my_b == next_b))) *sure = false;
+    const float cut = CUT * fmaxf(fabsf(my_key), fabsf(next_key)), gap = my_key - next_key;
+    const float room = a.score_room * fmaxf(my_key - my_b, next_key - next_b) + cut;
+    if (__any_sync(FULL, lane + 1 < a.k && gap <= room && !(my_l == next_l && my_b == next_b))) *sure = false;
+    // The last choice against everything that is left: all of it is below the next one, but with a bias any of it may have
+    // a larger score, and error, than that.
+    const bool far = gap > (a.bias != nullptr ? a.score_room * most + cut : room);
+    if (*sure && picks > a.k && !__shfl_sync(FULL, far, a.k - 1)) {
+      const float last_l = __shfl_sync(FULL, my_l, a.k - 1), last_b = __shfl_sync(FULL, my_b, a.k - 1);
+      const float last_key = __shfl_sync(FULL, my_key, a.k - 1);
+      const float low = last_key - a.score_room * (last_key - last_b) - CUT * fabsf(last_key);
+      float key[V];
+      keys_of<V>(a, l, b, key);
+      bool over = false;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int e = lane * per + j;
+        bool out = (WHOLE || (j < per && e < a.experts)) && !(l[j] == last_l && b[j] == last_b);
+        if (a.groups > 1) {
+          const int at = a.lanes_per_group > 0 ? lane / a.lanes_per_group * a.lanes_per_group : e / (a.experts / a.groups);
+          out = out && ((kept >> (at & 31)) & 1u);
+        }
+        for (int i = 0; i < a.k; ++i) {
+          const int taken = __shfl_sync(FULL, mine, i);   // by every lane
+          out = out && taken != e;
+        }
+        over = over || (out && key[j] + a.score_room * (key[j] - b[j]) + CUT * fabsf(key[j]) >= low);
+      }
+      if (__any_sync(FULL, over)) *sure = false;
+    }
   }
   return mine;
 }

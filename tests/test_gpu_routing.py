@@ -138,6 +138,38 @@ def test_equal_and_nearly_equal_keys(score):
     _check(l, 8, score=score, bias=(0.75 - s + wobble).float(), num_groups=8, groups_kept=4, group_top=2)
 
 
+@pytest.mark.parametrize("k", [1, 3])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_large_score_under_a_negative_bias(score, k):
+    # the error of expert 7's key is that of a score near 1, far above its neighbours': it passes them in steps of 1e-9
+    g = torch.Generator().manual_seed(3)
+    rows, experts = 3000, 64
+    l = torch.randn(rows, experts, generator=g) * 0.01 - 7.0
+    l[:, 7] = (3.0 if score == "softmax" else 2.0) + torch.arange(rows) * 2.0 ** -22
+    l = l.cuda()
+    s = torch.softmax(l.double(), -1) if score == "softmax" else torch.sigmoid(l.double())
+    bias = torch.zeros(experts, device="cuda")
+    middle = s[:, [e for e in range(experts) if e != 7]].topk(k, -1).values[:, -1].mean()
+    for shift in (-3e-4, -2e-5, 0.0, 2e-5):
+        bias[7] = (middle - s[rows // 2, 7] + shift).float()
+        _check(l, k, score=score, bias=bias)
+        _check(l, k, score=score, bias=bias, num_groups=8, groups_kept=7, group_top=1)
+
+
+def test_a_choice_that_ends_among_equals():
+    # the last choice and its successor are the same number; behind them one a step above or below it
+    g = torch.Generator().manual_seed(4)
+    l = torch.randn(2000, 64, generator=g) - 3.0
+    at = torch.stack([torch.randperm(64, generator=g)[:4] for _ in range(2000)])
+    l.scatter_(1, at[:, :3], 1.0)
+    step = torch.tensor([1.0 + 2.0 ** -23, 1.0 - 2.0 ** -24])[torch.randint(0, 2, (2000,), generator=g)]
+    l.scatter_(1, at[:, 3:], step.unsqueeze(1))
+    for k in (1, 2, 3):
+        _check(l.cuda(), k)
+        _check(l.cuda(), k, bias=torch.zeros(64, device="cuda"))
+        _check(l.cuda(), k, score="sigmoid", bias=torch.full((64,), 0.25, device="cuda"))
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_masked_experts_and_tokens(score, renormalize):
