@@ -11,7 +11,7 @@
 // Both directions are HBM streams: forward reads x (and the residual) and writes y (and r), backward reads dy, r (and
 // d_stream) and writes dr.  rstd is not kept: backward reads r anyway, and one more sum costs less than the launch-time
 // allocation of a vector.  bf16 8192 x 4096 with residual (floor 41 us a direction at the copy rate): forward 42 us, backward
-// 48 and 3 to join dw; without loads ahead 68 and 5.  32768 x 4096 (floor 164): 153 and 183 + 4.
+// 47 and 3 to join dw; without loads ahead 68 and 5.  32768 x 4096 (floor 164): 153 and 182 + 4.
 //
 // A row is held in registers: 16-byte vectors of it per thread (lane-adjacent, so that four (bf16) or eight (fp32)
 // neighbouring lanes hold a block of 32) or, where width, strides or pointers rule those out, single elements.  8 to 32
@@ -152,34 +152,48 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return warp_sum(lane < warps ? part[lane] : 0.0f);
 }
 
-// Codes of V values of one block of 32 that neighbouring lanes hold: amax over the lanes, scale, encode.
-template <bool BF16, int V>
-__device__ __forceinline__ uint32_t encode_block(const float* v, int e5m2, uint8_t* to, bool store) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < V; ++j) m = max(m, f2u(v[j]) & 0x7FFFFFFFu);
+// Codes of V values of one block of 32 that neighbouring lanes hold (already in the type of x): amax over the lanes, scale,
+// encode.  Returns the scale byte.
+template <bool BF16, int V, bool E5M2>
+__device__ __forceinline__ uint32_t encode_block(const typename Held<V>::U& unit, uint8_t* to, bool store) {
+  uint32_t m;   // largest magnitude, as bits of the type
+  if constexpr (V == 8) {
+    const uint32_t keep = 0x7FFF7FFFu;
+    const uint32_t two = __vmaxu2(__vmaxu2(unit.x & keep, unit.y & keep), __vmaxu2(unit.z & keep, unit.w & keep));
+    m = max(two >> 16, two & 0xFFFFu);
+  } else if constexpr (V == 4) {
+    m = max(max(unit.x & 0x7FFFFFFFu, unit.y & 0x7FFFFFFFu), max(unit.z & 0x7FFFFFFFu, unit.w & 0x7FFFFFFFu));
+  } else {
+    m = BF16 ? (f2u(unit) & 0x7FFFFFFFu) >> 16 : f2u(unit) & 0x7FFFFFFFu;
+  }
   if constexpr (V == 1) {
     m = __reduce_max_sync(0xFFFFFFFFu, m);
   } else {
 #pragma unroll
     for (int o = 1; o < 32 / V; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
   }
-  const uint32_t e = BF16 ? e8m0_from_amax_bits<true>(m >> 16, e5m2 ? 2 : 3, e5m2 ? 15 : 8)
-                          : e8m0_from_amax_bits<false>(m, e5m2 ? 2 : 3, e5m2 ? 15 : 8);
-  const float q = u2f(e << 23), rq = u2f((254u - e) << 23);
+  const uint32_t e = e8m0_from_amax_bits<BF16>(m, E5M2 ? 2 : 3, E5M2 ? 15 : 8);
   float s[V < 2 ? 2 : V];
   s[1] = 0.0f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) s[j] = e <= 253u ? __fmul_rn(v[j], rq) : __fdiv_rn(v[j], q);
+  unpack_unit<BF16, V>(unit, s);
+  // 1 / 2^(e - 127): the formats' largest exponents keep e at 247 or below, for any bits of m
+  const float r = u2f((254u - e) << 23);
   if constexpr (V == 1) {
-    const uint32_t code = e5m2 ? fp8x2_rtn_hw<true>(s[0], 0.0f) : fp8x2_rtn_hw<false>(s[0], 0.0f);
-    if (store) *to = (uint8_t)code;
+    s[0] *= r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 p = __fmul2_rn(make_float2(s[j], s[j + 1]), make_float2(r, r));
+      s[j] = p.x;
+      s[j + 1] = p.y;
+    }
+  }
+  if constexpr (V == 1) {
+    if (store) *to = (uint8_t)fp8x2_rtn_hw<E5M2>(s[0], 0.0f);
   } else {
     uint32_t code[V / 4];
 #pragma unroll
-    for (int j = 0; j < V; j += 4)
-      code[j / 4] = e5m2 ? (fp8x2_rtn_hw<true>(s[j], s[j + 1]) | (fp8x2_rtn_hw<true>(s[j + 2], s[j + 3]) << 16))
-                         : (fp8x2_rtn_hw<false>(s[j], s[j + 1]) | (fp8x2_rtn_hw<false>(s[j + 2], s[j + 3]) << 16));
+    for (int j = 0; j < V; j += 4) code[j / 4] = fp8x2_rtn_hw<E5M2>(s[j], s[j + 1]) | (fp8x2_rtn_hw<E5M2>(s[j + 2], s[j + 3]) << 16);
     if (store) {
       if constexpr (V == 8) *reinterpret_cast<uint2*>(to) = make_uint2(code[0], code[1]);
       else *reinterpret_cast<uint32_t*>(to) = code[0];
@@ -195,15 +209,19 @@ __device__ __forceinline__ void zero_packed_padding(const NormArgs& a, int64_t r
   for (int64_t c = first + thread; c < tiles * 4; c += threads) a.scale_packed[packed_scale_offset(row, c, tiles)] = 0;
 }
 
-// One row per LANES lanes of a warp, or (LANES = 0) ROWS rows per CTA; NV units of V elements a thread and row.  With codes as
-// fast as without although it writes less: the turnover of CTAs sets the pace, so two rows share one (8192 x 4096: 43 us,
-// with codes 43; one row a CTA 44 and 46).  CTAs that walk over rows with the next one's loads ahead, as in the backward
-// pass, are slower (47, with codes 52), and scale bytes put together to words no faster.
-template <bool BF16, bool MX, int LANES, int NV, int V, int ROWS = 1>
-__global__ void __launch_bounds__(LANES ? 128 : 1024) norm_forward_kernel(NormArgs a) {
+// One row per LANES lanes of a warp, or (LANES = 0) ROWS rows per CTA; NV units of V elements a thread and row.  FMT: 0 for
+// the type of x, 1 e4m3, 2 e5m2.
+//
+// One row a CTA is bound by the turnover of CTAs, so two share one (8192 x 4096: 42 us, with codes 41; one by one 44 and
+// 46), and with codes by instructions (issue slots 78 %), so elements go in pairs, maxima are taken of the packed words and
+// scales are multiplied (with one element to an instruction and quotients 43).  The bounds keep three CTAs of 512 threads
+// or two of 1024 on an SM: at 45 registers codes took 56 us.  CTAs that walk over rows with the next one's loads ahead, as in
+// the backward pass, are slower (47, with codes 52), and scale bytes put together to words no faster.
+template <bool BF16, int FMT, int LANES, int NV, int V, int ROWS = 1>
+__global__ void __launch_bounds__(LANES ? 128 : ROWS > 1 ? 512 : 1024, LANES || NV > 2 ? 1 : ROWS > 1 ? 3 : 2) norm_forward_kernel(NormArgs a) {
   using T = typename NormType<BF16>::T;
   using U = typename Held<V>::U;
-  constexpr bool WARP = LANES != 0;
+  constexpr bool WARP = LANES != 0, MX = FMT != 0;
   __shared__ float part[ROWS][32];
   grid_dependency_wait();
   const int threads = WARP ? LANES : blockDim.x, t = WARP ? (threadIdx.x & (LANES - 1)) : threadIdx.x;
@@ -241,14 +259,28 @@ __global__ void __launch_bounds__(LANES ? 128 : 1024) norm_forward_kernel(NormAr
         const int u = t + i * threads;
         float q[V];
         unpack_unit<BF16, V>(add[k][i], q);
+        if constexpr (V == 1) {
+          p[0] = __fadd_rn(p[0], q[0]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = __fadd_rn(p[j], q[j]);
+          for (int j = 0; j < V; j += 2) {
+            const float2 n = __fadd2_rn(make_float2(p[j], p[j + 1]), make_float2(q[j], q[j + 1]));
+            p[j] = n.x;
+            p[j + 1] = n.y;
+          }
+        }
         raw[k][i] = pack_unit<BF16, V>(p);
         if (u < units_of(k)) store_unit<BF16, V>(reinterpret_cast<T*>(a.r) + (first + k) * a.cols, u, raw[k][i]);
         unpack_unit<BF16, V>(raw[k][i], p);
       }
+      if constexpr (V == 1) {
+        ss[k] = __fmaf_rn(p[0], p[0], ss[k]);
+      } else {
+        float2 two = make_float2(ss[k], 0.0f);
 #pragma unroll
-      for (int j = 0; j < V; ++j) ss[k] = __fmaf_rn(p[j], p[j], ss[k]);
+        for (int j = 0; j < V; j += 2) two = __ffma2_rn(make_float2(p[j], p[j + 1]), make_float2(p[j], p[j + 1]), two);
+        ss[k] = two.x + two.y;
+      }
     }
     ss[k] = warp_sum<WARP ? LANES : 32>(ss[k]);
   }
@@ -273,13 +305,20 @@ __global__ void __launch_bounds__(LANES ? 128 : 1024) norm_forward_kernel(NormAr
       const float rstd = rsqrtf(__fmaf_rn(ss[k], a.inv_cols, a.eps));
       float p[V];
       unpack_unit<BF16, V>(raw[k][i], p);
+      if constexpr (V == 1) {
+        p[0] = p[0] * rstd * w[0];
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) p[j] = p[j] * rstd * w[j];
+        for (int j = 0; j < V; j += 2) {
+          const float2 n = __fmul2_rn(__fmul2_rn(make_float2(p[j], p[j + 1]), make_float2(rstd, rstd)), make_float2(w[j], w[j + 1]));
+          p[j] = n.x;
+          p[j + 1] = n.y;
+        }
+      }
+      const U y = pack_unit<BF16, V>(p);
       if constexpr (MX) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = round_elem<BF16>(p[j]);
-        if (a.y2 != nullptr && on) store_unit<BF16, V>(reinterpret_cast<T*>(a.y2) + row * a.cols, u, pack_unit<BF16, V>(p));
-        const uint32_t e = encode_block<BF16, V>(p, a.e5m2, reinterpret_cast<uint8_t*>(a.y) + row * a.cols + (int64_t)u * V, on);
+        if (a.y2 != nullptr && on) store_unit<BF16, V>(reinterpret_cast<T*>(a.y2) + row * a.cols, u, y);
+        const uint32_t e = encode_block<BF16, V, FMT == 2>(y, reinterpret_cast<uint8_t*>(a.y) + row * a.cols + (int64_t)u * V, on);
         constexpr int HOLD = 32 / V;   // lanes that hold one block
         if (on && (u & (HOLD - 1)) == 0) {
           const int64_t nkb = a.cols >> 5, kb = u / HOLD;
@@ -287,7 +326,7 @@ __global__ void __launch_bounds__(LANES ? 128 : 1024) norm_forward_kernel(NormAr
           if (a.scale_packed != nullptr) a.scale_packed[packed_scale_offset(row, kb, (nkb + 3) >> 2)] = (uint8_t)e;
         }
       } else if (on) {
-        store_unit<BF16, V>(reinterpret_cast<T*>(a.y) + row * a.cols, u, pack_unit<BF16, V>(p));
+        store_unit<BF16, V>(reinterpret_cast<T*>(a.y) + row * a.cols, u, y);
       }
     }
   }
@@ -322,7 +361,7 @@ __global__ void __launch_bounds__(256) norm_forward_any_kernel(NormArgs a) {
       m = __reduce_max_sync(0xFFFFFFFFu, m);
       const uint32_t e = BF16 ? e8m0_from_amax_bits<true>(m >> 16, a.e5m2 ? 2 : 3, a.e5m2 ? 15 : 8)
                               : e8m0_from_amax_bits<false>(m, a.e5m2 ? 2 : 3, a.e5m2 ? 15 : 8);
-      const float s = e <= 253u ? __fmul_rn(p, u2f((254u - e) << 23)) : __fdiv_rn(p, u2f(e << 23));
+      const float s = __fmul_rn(p, u2f((254u - e) << 23));
       reinterpret_cast<uint8_t*>(a.y)[row * a.cols + c] =
           (uint8_t)(a.e5m2 ? fp8x2_rtn_hw<true>(s, 0.0f) : fp8x2_rtn_hw<false>(s, 0.0f));
       if ((threadIdx.x & 31) == 0) {
@@ -430,10 +469,22 @@ __global__ void __launch_bounds__(LANES ? 128 : 1024) norm_backward_kernel(NormG
       unpack_unit<BF16, V>(g[i], gv);
       unpack_unit<BF16, V>(x[i], xv);
       if (u < units) weights(i, u, w);
+      if constexpr (V == 1 || NV > 1) {   // pairs cost registers that more units do not leave
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        ss = __fmaf_rn(xv[j], xv[j], ss);
-        dot = __fmaf_rn(gv[j] * w[j], xv[j], dot);
+        for (int j = 0; j < V; ++j) {
+          ss = __fmaf_rn(xv[j], xv[j], ss);
+          dot = __fmaf_rn(gv[j] * w[j], xv[j], dot);
+        }
+      } else {
+        float2 s2 = make_float2(ss, 0.0f), d2 = make_float2(dot, 0.0f);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const float2 xx = make_float2(xv[j], xv[j + 1]);
+          s2 = __ffma2_rn(xx, xx, s2);
+          d2 = __ffma2_rn(__fmul2_rn(make_float2(gv[j], gv[j + 1]), make_float2(w[j], w[j + 1])), xx, d2);
+        }
+        ss = s2.x + s2.y;
+        dot = d2.x + d2.y;
       }
     }
     if constexpr (WARP) {
@@ -456,10 +507,25 @@ __global__ void __launch_bounds__(LANES ? 128 : 1024) norm_backward_kernel(NormG
         unpack_unit<BF16, V>(x[i], xv);
         unpack_unit<BF16, V>(ds[i], d);
         weights(i, u, w);
+        if constexpr (V == 1 || NV > 1) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          acc[i][j] = __fmaf_rn(gv[j], xv[j] * rstd, acc[i][j]);
-          d[j] = __fmaf_rn(rstd, __fmaf_rn(-xv[j], along, gv[j] * w[j]), d[j]);
+          for (int j = 0; j < V; ++j) {
+            acc[i][j] = __fmaf_rn(gv[j], xv[j] * rstd, acc[i][j]);
+            d[j] = __fmaf_rn(rstd, __fmaf_rn(-xv[j], along, gv[j] * w[j]), d[j]);
+          }
+        } else {
+          const float2 rr = make_float2(rstd, rstd), back = make_float2(-along, -along);
+#pragma unroll
+          for (int j = 0; j < V; j += 2) {
+            const float2 gg = make_float2(gv[j], gv[j + 1]), xx = make_float2(xv[j], xv[j + 1]);
+            const float2 sum = __ffma2_rn(gg, __fmul2_rn(xx, rr), make_float2(acc[i][j], acc[i][j + 1]));
+            acc[i][j] = sum.x;
+            acc[i][j + 1] = sum.y;
+            const float2 gw = __fmul2_rn(gg, make_float2(w[j], w[j + 1]));
+            const float2 to = __ffma2_rn(rr, __ffma2_rn(xx, back, gw), make_float2(d[j], d[j + 1]));
+            d[j] = to.x;
+            d[j + 1] = to.y;
+          }
         }
         store_unit<BF16, V>(reinterpret_cast<T*>(a.dr) + row * a.cols, u, pack_unit<BF16, V>(d));
       }
@@ -639,8 +705,8 @@ extern "C" int altob200_rms_norm_forward(const altob200_rms_norm_args* p, void* 
     else if (s.nv == 2) ONE(B, M, 0, 2, V);           \
     else ONE(B, M, 0, 4, V);                          \
   } while (0)
-    if (bf16) { if (mx) BY_SHAPE(true, true, 8); else BY_SHAPE(true, false, 8); }
-    else { if (mx) BY_SHAPE(false, true, 4); else BY_SHAPE(false, false, 4); }
+    if (bf16) { if (!mx) BY_SHAPE(true, 0, 8); else if (!a.e5m2) BY_SHAPE(true, 1, 8); else BY_SHAPE(true, 2, 8); }
+    else { if (!mx) BY_SHAPE(false, 0, 4); else if (!a.e5m2) BY_SHAPE(false, 1, 4); else BY_SHAPE(false, 2, 4); }
 #undef BY_SHAPE
 #undef ONE
   }

@@ -388,17 +388,17 @@ __device__ __forceinline__ float chosen_weight(bool on, float l, int sigmoid, in
     const float s = !on ? 0.0f : l != l ? l : __fdividef(num, den);
     if (!renorm) return s;
     *total = warp_add<float, LANES>(s);
-    return *total == 0.0f ? 0.0f : __fdividef(s, *total);
+    return *total == 0.0f ? 0.0f : __fdiv_rn(s, *total);   // a choice of one has weight 1, and no gradient
   }
   if (!renorm) {
     const float d = l - m;
-    return on && m != -INFINITY ? __fdividef(d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f, z) : 0.0f;
+    return on && m != -INFINITY ? __fdiv_rn(d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f, z) : 0.0f;
   }
   const float top = warp_max<LANES>(on ? l : -INFINITY);
   const float d = l - top, s = !on ? 0.0f : d >= -126.0f ? fast_exp(d) : d != d ? d : 0.0f;
   *total = warp_add<float, LANES>(s);   // a NaN where top = -inf, and where there is one
   if (top == -INFINITY && !(l != l)) return 0.0f;
-  return __fdividef(s, *total);
+  return __fdiv_rn(s, *total);
 }
 
 // Weights of a token whose choice is made: lane i < k holds the i-th chosen expert and its logit.

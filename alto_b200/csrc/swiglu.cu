@@ -93,7 +93,7 @@ static int swiglu_launch(const void* h, const void* go, int64_t rows, int64_t H,
 //   grad_h[r, c] = bf16( go u s (1 + g (1 - s)) ),  grad_h[r, H + c] = bf16( go g s )
 // in fp32 with one rounding: the tensor-op form's intermediate roundings are of an h that no longer exists here.
 //
-// 69632 x 2880 (floor 247 us a direction: 8.06 and 8.06 bytes a column at the copy rate): forward 270 us, bound by
+// 69632 x 2880 (floor 247 us a direction: 8.06 and 8.06 bytes a column at the copy rate): forward 272 us, bound by
 // instructions; backward 252, the copy rate.  With expf and divisions 396 and 460; forward without the loads ahead 278, with
 // one number to an instruction 282 (290 instructions for eight columns of both halves, issue slots 74 % busy).
 // ---------------------------------------------------------------------------------------
@@ -123,17 +123,13 @@ __device__ __forceinline__ uint4 pack8_rn(const float v[8]) {
 template <bool E5M2>
 __device__ __forceinline__ uint2 encode8_mxfp8(const float v[8], uint32_t e) {
   float s[8];
-  if (e <= 253u) {
-    const float r = u2f((254u - e) << 23);
+  // 1 / 2^(e - 127): the formats' largest exponents keep e at 247 or below, for any bits of the maximum
+  const float r = u2f((254u - e) << 23);
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float2 p = __fmul2_rn(make_float2(v[j], v[j + 1]), make_float2(r, r));
-      s[j] = p.x;
-      s[j + 1] = p.y;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = __fdiv_rn(v[j], u2f(e << 23));
+  for (int j = 0; j < 8; j += 2) {
+    const float2 p = __fmul2_rn(make_float2(v[j], v[j + 1]), make_float2(r, r));
+    s[j] = p.x;
+    s[j + 1] = p.y;
   }
   uint32_t w[2];
 #pragma unroll

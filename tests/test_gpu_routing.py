@@ -138,6 +138,17 @@ def test_equal_and_nearly_equal_keys(score):
     _check(l, 8, score=score, bias=(0.75 - s + wobble).float(), num_groups=8, groups_kept=4, group_top=2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_choice_of_one_has_its_whole_weight_and_no_gradient(score, dtype):
+    for experts, renormalize in ((40, True), (256, True), (1, True)) + (((1, False),) if score == "softmax" else ()):
+        leaf = _logits(500, experts, dtype, std=4.0).requires_grad_(True)
+        _, weights = routing.route_experts(leaf, 1, score=score, renormalize=renormalize, scale=2.5)
+        assert (weights == 2.5).all()
+        (dl,) = torch.autograd.grad(weights, leaf, _logits(500, 1, torch.float32, 6))
+        assert (dl == 0).all()
+
+
 @pytest.mark.parametrize("k", [1, 3])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_a_large_score_under_a_negative_bias(score, k):
