@@ -429,7 +429,8 @@ int altob200_swiglu_kept_backward(const void* codes, const uint8_t* scales, cons
 /*
  * Root-mean-square norm of rows, optionally behind the addition of a residual:
  *   r = T(x + residual)  (stream_out; r = x without a residual),   y = r / sqrt(mean(r^2) + eps) * weight
- * with fp32 sums and one rounding of y.  T is `dtype`, weight [cols] has `weight_dtype`.  The decoder blocks that the
+ * with fp32 sums and one rounding of y (a row whose squares sum up to infinity in fp32 gives zeros, NaN where it is
+ * infinite).  T is `dtype`, weight [cols] has `weight_dtype`.  The decoder blocks that the
  * reference converts (alto/modifiers/lpt/base.py:171-192) have this norm in front of their linears.
  *   format < 0  : out is T [rows, cols]
  *   format MXFP8: out is the codes [rows, cols] that altob200_quantize_rowwise makes of y (blocks of 32 along the row;
