@@ -59,6 +59,9 @@ __device__ __forceinline__ F warp_add(F v) {
   return v;
 }
 __device__ __forceinline__ float from_ordered(uint32_t w) { return u2f(w >> 31 ? w & 0x7FFFFFFFu : ~w); }
+// The key of a word whose LOW bits hold something else: the key itself or up to LOW steps below it.
+template <uint32_t LOW>
+__device__ __forceinline__ float key_of_word(uint32_t w) { return from_ordered(w & ~LOW); }
 
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t v) {
   const uint32_t hi = __reduce_max_sync(FULL, (uint32_t)(v >> 32));
@@ -195,12 +198,13 @@ __device__ __forceinline__ float keys_of(const RouteArgs& a, const float* l, con
 // A key is held as an ordered word whose lowest bits are V - 1 - j: each lane sorts its V words once, a choice is then the
 // largest of the lanes' first words, and its lane moves its list up.  Words are compared across lanes without those bits
 // and the lowest lane is taken, so equal keys come out by expert.  The bits that j takes are missing from every
-// comparison (none of a bf16 logit's), which `room` allows for below.
+// comparison (none of a bf16 logit's), which `room` allows for below; they are zero again in every key that a margin is taken
+// of (with j left in them two keys could move by V - 1 steps each, in opposite directions).
 template <bool BF16, int V, bool WHOLE>
 __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const float* l, const float* b, uint32_t* words,
                                       float* logit, bool* sure) {
   constexpr uint32_t LOW = V - 1;
-  // two keys that differ by less may be in the other order: what is cut off, and half a step of each sum
+  // two keys that differ by less may be in the other order: what is cut off the lower one, and half a step of each sum
   constexpr float CUT = (V - 1) * 1.1920929e-7f + 1.2e-7f;
   const int lane = threadIdx.x & 31, per = WHOLE ? V : a.per;
   uint32_t word[V];
@@ -302,7 +306,7 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
     // Neighbours in the order whose keys fp32 cannot tell apart, unless their inputs are the same.  A softmax is off by at
     // most 7e-6 of itself (the rounding of l - m before the exponential, up to 88 * 2^-24, is the most of it), a sigmoid by
     // 6e-7.
-    const float my_b = on && a.bias != nullptr ? __ldg(a.bias + mine) : 0.0f, my_key = from_ordered(mine_word);
+    const float my_b = on && a.bias != nullptr ? __ldg(a.bias + mine) : 0.0f, my_key = key_of_word<LOW>(mine_word);
     const float next_l = __shfl_down_sync(FULL, my_l, 1), next_b = __shfl_down_sync(FULL, my_b, 1);
     const float next_key = __shfl_down_sync(FULL, my_key, 1);
     const float cut = CUT * fmaxf(fabsf(my_key), fabsf(next_key)), gap = my_key - next_key;
