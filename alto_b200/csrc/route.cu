@@ -59,9 +59,12 @@ __device__ __forceinline__ F warp_add(F v) {
   return v;
 }
 __device__ __forceinline__ float from_ordered(uint32_t w) { return u2f(w >> 31 ? w & 0x7FFFFFFFu : ~w); }
-// The key of a word whose LOW bits hold something else: the key itself or up to LOW steps below it.
+// The key of a word whose LOW bits hold something else: the key itself or up to LOW steps below it.  -inf is the one number
+// whose own low bits are ones; without them its word would be a NaN's.
 template <uint32_t LOW>
-__device__ __forceinline__ float key_of_word(uint32_t w) { return from_ordered(w & ~LOW); }
+__device__ __forceinline__ float key_of_word(uint32_t w) {
+  return (w | LOW) == 0x007FFFFFu ? -INFINITY : from_ordered(w & ~LOW);
+}
 
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t v) {
   const uint32_t hi = __reduce_max_sync(FULL, (uint32_t)(v >> 32));
@@ -250,7 +253,8 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
           best = max(best, w);
         }
     }
-    const float of_group = a.group_top == 2 && size > 1 ? from_ordered(best) + from_ordered(second) : from_ordered(best);
+    const bool two = a.group_top == 2 && size > 1;
+    const float first = key_of_word<LOW>(best), other = two ? key_of_word<LOW>(second) : 0.0f, of_group = first + other;
     // the kept groups one by one, the lowest among equals; then, if asked, the first that is not kept
     uint32_t rest = mine >= a.groups ? 0u : a.group_top == 2 ? ordered_bits(f2u(of_group)) : best & ~LOW;
     kept = 0u;
@@ -266,9 +270,9 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
       const int next = __ffs(__ballot_sync(FULL, rest == top)) - 1;
       const float u = __shfl_sync(FULL, of_group, last), v = __shfl_sync(FULL, of_group, next);
       // the largest of the (finite) keys in any group's sum, which may cancel there
-      const float large = a.group_top == 2 && size > 1 ? fmaxf(fabsf(from_ordered(best)), fabsf(from_ordered(second))) : fabsf(of_group);
+      const float large = fmaxf(fabsf(first), fabsf(other));
       const float both = u2f(__reduce_max_sync(FULL, mine < a.groups && large < INFINITY ? f2u(large) : 0u));
-      if (u - v <= 2.0f * (a.score_room + CUT * both)) *sure = false;
+      if (!(u - v > 2.0f * (a.score_room + CUT * both))) *sure = false;   // also where both are infinite, or one a NaN
     }
     left = a.kept * size;
     if (a.lanes_per_group > 0) {
