@@ -255,24 +255,24 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
     }
     const bool two = a.group_top == 2 && size > 1;
     const float first = key_of_word<LOW>(best), other = two ? key_of_word<LOW>(second) : 0.0f, of_group = first + other;
-    // the kept groups one by one, the lowest among equals; then, if asked, the first that is not kept
+    // the kept groups one by one, the lowest among equals
     uint32_t rest = mine >= a.groups ? 0u : a.group_top == 2 ? ordered_bits(f2u(of_group)) : best & ~LOW;
     kept = 0u;
-    int last = 0;
     for (int i = 0; i < a.kept; ++i) {
       const uint32_t top = __reduce_max_sync(FULL, rest);
-      last = __ffs(__ballot_sync(FULL, rest == top)) - 1;
+      const int last = __ffs(__ballot_sync(FULL, rest == top)) - 1;
       kept |= 1u << last;
       if (mine * every == last) rest = 0u;
     }
     if (a.checked) {
-      const uint32_t top = __reduce_max_sync(FULL, rest);
-      const int next = __ffs(__ballot_sync(FULL, rest == top)) - 1;
-      const float u = __shfl_sync(FULL, of_group, last), v = __shfl_sync(FULL, of_group, next);
-      // the largest of the (finite) keys in any group's sum, which may cancel there
-      const float large = fmaxf(fabsf(first), fabsf(other));
-      const float both = u2f(__reduce_max_sync(FULL, mine < a.groups && large < INFINITY ? f2u(large) : 0u));
-      if (!(u - v > 2.0f * (a.score_room + CUT * both))) *sure = false;   // also where both are infinite, or one a NaN
+      // Each group's own margin (half a step of the sum and one of the margin's own sum on top of CUT), so that a group far
+      // below the decision, as one masked by a large negative bias is, widens nobody else's: every kept sum as low as it
+      // can be is above every other as high as it can be.  Infinities have no margin; equal ones are not told apart here.
+      const float margin = fabsf(of_group) < INFINITY ? a.score_room * most + (CUT + 2.4e-7f) * (fabsf(first) + fabsf(other)) : 0.0f;
+      const bool in = (kept >> (mine * every)) & 1u;
+      const uint32_t low = __reduce_min_sync(FULL, mine < a.groups && in ? ordered_bits(f2u(of_group - margin)) : FULL);
+      const uint32_t high = __reduce_max_sync(FULL, mine < a.groups && !in ? ordered_bits(f2u(of_group + margin)) : 0u);
+      if (low <= high) *sure = false;
     }
     left = a.kept * size;
     if (a.lanes_per_group > 0) {
