@@ -429,7 +429,7 @@ __device__ __forceinline__ void write_choice(const RouteArgs& a, int64_t t, cons
     z = warp_add(z);
   }
   float w = chosen_weight(on, mine, a.sigmoid, a.renorm, m, z, &total);
-  if (a.bias != nullptr && !a.sigmoid) {   // a NaN that is not among the chosen makes every score one all the same
+  if (a.computed && !a.sigmoid) {   // a NaN that is not among the chosen makes every score one all the same
     bool nan = false;
 #pragma unroll
     for (int j = 0; j < V; ++j) nan = nan || l[j] != l[j];
