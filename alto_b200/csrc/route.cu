@@ -209,6 +209,7 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
   constexpr uint32_t LOW = V - 1;
   // two keys that differ by less may be in the other order: what is cut off the lower one, and half a step of each sum
   constexpr float CUT = (V - 1) * 1.1920929e-7f + 1.2e-7f;
+  constexpr float TINY = 2.4e-38f;   // two scores below the least normal number, which are zero here
   const int lane = threadIdx.x & 31, per = WHOLE ? V : a.per;
   uint32_t word[V];
   *sure = true;
@@ -268,7 +269,7 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
       // Each group's own margin (half a step of the sum and one of the margin's own sum on top of CUT), so that a group far
       // below the decision, as one masked by a large negative bias is, widens nobody else's: every kept sum as low as it
       // can be is above every other as high as it can be.  Infinities have no margin; equal ones are not told apart here.
-      const float margin = fabsf(of_group) < INFINITY ? a.score_room * most + (CUT + 2.4e-7f) * (fabsf(first) + fabsf(other)) : 0.0f;
+      const float margin = fabsf(of_group) < INFINITY ? a.score_room * most + (CUT + 2.4e-7f) * (fabsf(first) + fabsf(other)) + TINY : 0.0f;
       const bool in = (kept >> (mine * every)) & 1u;
       const uint32_t low = __reduce_min_sync(FULL, mine < a.groups && in ? ordered_bits(f2u(of_group - margin)) : FULL);
       const uint32_t high = __reduce_max_sync(FULL, mine < a.groups && !in ? ordered_bits(f2u(of_group + margin)) : 0u);
@@ -313,7 +314,7 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
     const float my_b = on && a.bias != nullptr ? __ldg(a.bias + mine) : 0.0f, my_key = key_of_word<LOW>(mine_word);
     const float next_l = __shfl_down_sync(FULL, my_l, 1), next_b = __shfl_down_sync(FULL, my_b, 1);
     const float next_key = __shfl_down_sync(FULL, my_key, 1);
-    const float cut = CUT * fmaxf(fabsf(my_key), fabsf(next_key)), gap = my_key - next_key;
+    const float cut = CUT * fmaxf(fabsf(my_key), fabsf(next_key)) + TINY, gap = my_key - next_key;
     const float room = a.score_room * fmaxf(my_key - my_b, next_key - next_b) + cut;
     if (__any_sync(FULL, lane + 1 < a.k && gap <= room && !(my_l == next_l && my_b == next_b))) *sure = false;
     // The last choice against everything that is left: all of it is below the next one, but with a bias any of it may have
@@ -322,7 +323,7 @@ __device__ __forceinline__ int choose(const RouteArgs& a, int64_t row, const flo
     if (*sure && picks > a.k && !__shfl_sync(FULL, far, a.k - 1)) {
       const float last_l = __shfl_sync(FULL, my_l, a.k - 1), last_b = __shfl_sync(FULL, my_b, a.k - 1);
       const float last_key = __shfl_sync(FULL, my_key, a.k - 1);
-      const float low = last_key - a.score_room * (last_key - last_b) - CUT * fabsf(last_key);
+      const float low = last_key - a.score_room * (last_key - last_b) - CUT * fabsf(last_key) - TINY;
       float key[V];
       keys_of<V>(a, l, b, key);
       bool over = false;

@@ -47,3 +47,20 @@ def test_many_near_keys(experts):
     for k in (1, 8, 16):
         ids, _ = routing.route_experts(l.cuda(), k, score="sigmoid", bias=bias.cuda())
         assert torch.equal(ids.cpu().long(), order[:, :k])
+
+
+def test_scores_below_the_least_normal_number():
+    # a score that fp32 flushes to zero beside a bias of its own size
+    l = torch.full((400, 64), -200.0)
+    bias = torch.zeros(64)
+    l[:, 9] = -90.0 + torch.rand(400, generator=torch.Generator().manual_seed(0)) * 4      # scores of 8e-40 to 4.5e-38
+    bias[9], bias[40] = 1.2e-38, 1.4e-38
+    key = torch.sigmoid(l.double()) + bias.double()
+    order = torch.sort(key, dim=-1, descending=True, stable=True).indices
+    assert set(order[:, 0].tolist()) == {9, 40}
+    for k in (1, 2):
+        ids, _ = routing.route_experts(l.cuda(), k, score="sigmoid", bias=bias.cuda())
+        assert torch.equal(ids.cpu().long(), order[:, :k])
+    for top in (1, 2):
+        ids, _ = routing.route_experts(l.cuda(), 1, score="sigmoid", bias=bias.cuda(), num_groups=8, groups_kept=1, group_top=top)
+        assert torch.equal(ids.cpu().long(), order[:, :1])
