@@ -797,7 +797,7 @@ def swiglu_keep_forward(h: torch.Tensor, fmt: int):
     out = torch.empty((rows, two_h // 2), dtype=torch.bfloat16, device=dev)
     codes = torch.empty_like(h, dtype=torch.uint8)
     scales = torch.empty((rows, two_h // 32), dtype=torch.uint8, device=dev)
-    _check((_lib or lib()).altob200_swiglu_keep_forward(h.data_ptr(), rows, two_h // 2, h.stride(0), fmt, out.data_ptr(),
+    _check((_lib or lib()).altob200_swiglu_keep_forward(h.data_ptr(), rows, two_h // 2, two_h, fmt, out.data_ptr(),
                                               codes.data_ptr(), scales.data_ptr(), _stream()), "altob200_swiglu_keep_forward")
     return out, codes, scales
 

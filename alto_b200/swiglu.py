@@ -22,22 +22,30 @@ __all__ = ["swiglu"]
 _KEEP = {"e4m3": _lib.FMT_MXFP8_E4M3, "e5m2": _lib.FMT_MXFP8_E5M2}
 
 
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous rows from a 16-byte boundary, as the kernels' vectors need them."""
+    if not t.is_contiguous():
+        return t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _SwiGLU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h):
+        h = _packed(h)
         ctx.save_for_backward(h)
         return _lib.swiglu_forward(h)
 
     @staticmethod
     def backward(ctx, grad_out):
         (h,) = ctx.saved_tensors
-        return _lib.swiglu_backward(h, grad_out.contiguous())
+        return _lib.swiglu_backward(h, _packed(grad_out))
 
 
 class _SwiGLUKept(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, fmt):
-        out, codes, scales = _lib.swiglu_keep_forward(h, fmt)
+        out, codes, scales = _lib.swiglu_keep_forward(_packed(h), fmt)
         ctx.save_for_backward(codes, scales)
         ctx.fmt = fmt
         return out
@@ -46,7 +54,7 @@ class _SwiGLUKept(torch.autograd.Function):
     @_lib.once_differentiable
     def backward(ctx, grad_out):
         codes, scales = ctx.saved_tensors
-        return _lib.swiglu_kept_backward(codes, scales, grad_out if grad_out.is_contiguous() else grad_out.contiguous(), ctx.fmt), None
+        return _lib.swiglu_kept_backward(codes, scales, _packed(grad_out), ctx.fmt), None
 
 
 def swiglu(h: torch.Tensor, checkpoint: Optional[str] = None) -> torch.Tensor:
@@ -57,7 +65,7 @@ def swiglu(h: torch.Tensor, checkpoint: Optional[str] = None) -> torch.Tensor:
     if h.dtype != torch.bfloat16:
         raise TypeError(f"swiglu expects bfloat16, got {h.dtype}")
     if checkpoint is None:
-        return _SwiGLU.apply(h.contiguous())
+        return _SwiGLU.apply(h)
     if checkpoint not in _KEEP:
         raise ValueError(f"unsupported checkpoint format {checkpoint!r}; supported: {sorted(_KEEP)}")
     if h.shape[1] % 64 != 0:
@@ -65,5 +73,5 @@ def swiglu(h: torch.Tensor, checkpoint: Optional[str] = None) -> torch.Tensor:
     if not h.is_cuda:
         raise RuntimeError("swiglu runs on CUDA tensors only (no CPU fallback)")
     if not (h.requires_grad and torch.is_grad_enabled()):
-        return _SwiGLU.apply(h.contiguous())      # nothing to keep
-    return _SwiGLUKept.apply(h if h.is_contiguous() else h.contiguous(), _KEEP[checkpoint])
+        return _SwiGLU.apply(h)      # nothing to keep
+    return _SwiGLUKept.apply(h, _KEEP[checkpoint])
