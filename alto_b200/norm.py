@@ -197,8 +197,12 @@ class _RMSNormMXFP8Linear(torch.autograd.Function):
         return (gx if need_x else None, gw, gx if need_res else None, None, None, None, *dws)
 
 
-@L.traced("rms_norm_mxfp8_linear")
 @L.on_device_of
+def _linears(x, norm_weight, residual, eps, fmt, use_2dblock_w, weights):
+    return _RMSNormMXFP8Linear.apply(x, norm_weight, residual, eps, fmt, use_2dblock_w, *weights)
+
+
+@L.traced("rms_norm_mxfp8_linear")
 def rms_norm_mxfp8_linear(x: torch.Tensor, norm_weight: torch.Tensor, weights: Union[torch.Tensor, Sequence[torch.Tensor]],
                           eps: float = 1e-5, residual: Optional[torch.Tensor] = None, fp8_variant: str = "e4m3",
                           use_2dblock_w: bool = False):
@@ -222,7 +226,7 @@ def rms_norm_mxfp8_linear(x: torch.Tensor, norm_weight: torch.Tensor, weights: U
         residual = None if residual is None else residual.detach()
         weights = tuple(w.detach() if type(w) is torch.nn.Parameter or type(w) is torch.Tensor else
                         unwrap_weight_wrapper(w).detach() for w in weights)
-    got = _RMSNormMXFP8Linear.apply(x, norm_weight, residual, eps, _FP8[fp8_variant][0], bool(use_2dblock_w), *weights)
+    got = _linears(x, norm_weight, residual, eps, _FP8[fp8_variant][0], bool(use_2dblock_w), weights)
     if not many and residual is None:
         return got[0]
     return got
