@@ -16,6 +16,7 @@ from pathlib import Path
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libaltob200.so"
@@ -342,6 +343,12 @@ def on_device_of(fn):
         with torch.cuda.device(t.device):
             return fn(t, *args, **kwargs)
     return inner
+
+
+def forward_mode() -> bool:
+    """Whether tensors may carry tangents: then a call goes through its autograd function, which refuses them, even where
+    nothing requires a gradient."""
+    return forward_ad._current_level >= 0
 
 
 def once_differentiable(fn):

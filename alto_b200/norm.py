@@ -103,7 +103,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual:
     """Norm of the rows of x [..., cols] (bf16 or fp32; weight [cols] in either type).  With ``residual`` (like x) returns
     (y, r), r = x + residual rounded to the type of x and y the norm of r; else y."""
     _check("rms_norm", x, weight, residual, eps)
-    if (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
+    if ((x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)) and torch.is_grad_enabled()
+            or L.forward_mode()):
         return _RMSNorm.apply(x, weight, residual, eps)
     out, stream = _forward(x, weight, residual, eps)
     return out if stream is None else (out, stream)
@@ -221,7 +222,7 @@ def rms_norm_mxfp8_linear(x: torch.Tensor, norm_weight: torch.Tensor, weights: U
         raise ValueError(f"Unsupported FP8 variant: {fp8_variant}. Supported: {sorted(_FP8)}")
     if not weights or any(w.device != x.device for w in weights):
         raise ValueError("rms_norm_mxfp8_linear expects weights on the device of x")
-    if not torch.is_grad_enabled():      # an evaluation pass: its parameters still say that they require gradients
+    if not torch.is_grad_enabled() and not L.forward_mode():      # an evaluation pass: its parameters still say that they require gradients
         x, norm_weight = x.detach(), norm_weight.detach()
         residual = None if residual is None else residual.detach()
         weights = tuple(w.detach() if type(w) is torch.nn.Parameter or type(w) is torch.Tensor else

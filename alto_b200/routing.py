@@ -109,7 +109,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
         bias = bias.detach().float().contiguous()
     params = L.RouteParams(L._dt(logits.dtype), experts, top_k, _SCORES[score], num_groups, groups_kept, group_top,
                            1 if renormalize else 0, scale)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if logits.requires_grad and torch.is_grad_enabled() or L.forward_mode():
         return _Route.apply(logits, params, bias)
     return _forward(logits, params, bias)
 
