@@ -165,7 +165,7 @@ extern "C" int altob200_gather_rows(const void* src, int64_t src_rows, int64_t r
                                     int64_t out_rows, void* dst, void* stream) {
   using namespace altob200;
   if (out_rows == 0) return ALTOB200_OK;
-  if (src == nullptr || dst == nullptr || index == nullptr || src_rows < 0 || out_rows < 0 || row_bytes <= 0)
+  if ((src == nullptr && src_rows != 0) || dst == nullptr || index == nullptr || src_rows < 0 || out_rows < 0 || row_bytes <= 0)
     return ALTOB200_EINVAL_SHAPE;
   if (row_bytes % 16 != 0 || (reinterpret_cast<uintptr_t>(src) & 15) || (reinterpret_cast<uintptr_t>(dst) & 15))
     return ALTOB200_EINVAL_ALIGN;
@@ -180,7 +180,7 @@ extern "C" int altob200_combine_rows(const void* rows, int64_t n_rows, int64_t r
                                      const void* scores, int64_t tokens, int32_t k, void* out, void* stream) {
   using namespace altob200;
   if (tokens == 0) return ALTOB200_OK;
-  if (rows == nullptr || out == nullptr || index == nullptr || n_rows < 0 || tokens < 0 || k <= 0 || row_bytes <= 0)
+  if ((rows == nullptr && n_rows != 0) || out == nullptr || index == nullptr || n_rows < 0 || tokens < 0 || k <= 0 || row_bytes <= 0)
     return ALTOB200_EINVAL_SHAPE;
   if (row_bytes % 16 != 0 || (reinterpret_cast<uintptr_t>(rows) & 15) || (reinterpret_cast<uintptr_t>(out) & 15))
     return ALTOB200_EINVAL_ALIGN;
@@ -197,7 +197,7 @@ extern "C" int altob200_spread_rows(const void* grad_out, int64_t tokens, int32_
                                     void* stream) {
   using namespace altob200;
   if (n_rows == 0) return ALTOB200_OK;
-  if (grad_out == nullptr || grad_rows == nullptr || position == nullptr || n_rows < 0 || tokens < 0 || k <= 0 ||
+  if ((grad_out == nullptr && tokens != 0) || grad_rows == nullptr || position == nullptr || n_rows < 0 || tokens < 0 || k <= 0 ||
       row_bytes <= 0)
     return ALTOB200_EINVAL_SHAPE;
   if (row_bytes % 16 != 0 || (reinterpret_cast<uintptr_t>(grad_out) & 15) || (reinterpret_cast<uintptr_t>(grad_rows) & 15))

@@ -379,7 +379,7 @@ int altob200_pack_scales(const uint8_t* scales, int64_t row_stride, int64_t col_
  * -1), and the inverse.  The reference leaves this to its TorchTitan fork's token dispatcher
  * (call sites alto/modifiers/lpt/base.py:194-201, alto/kernels/dispatch/tensor.py:224-263); the
  * grouped kernels fix the result's form (alto/kernels/fp4/fp4_common/grouped_utils.py:81-94).
- * `index` is device int32 [out_rows]; entries outside [0, src_rows) give zero rows.
+ * `index` is device int32 [out_rows]; entries outside [0, src_rows) give zero rows (src may be NULL without rows).
  */
 int altob200_gather_rows(const void* src, int64_t src_rows, int64_t row_bytes, const int32_t* index,
                          int64_t out_rows, void* dst, void* stream);
@@ -394,7 +394,7 @@ int altob200_gather_rows(const void* src, int64_t src_rows, int64_t row_bytes, c
  * altob200_spread_rows is its gradient with respect to the rows:
  *   grad_rows[r] = bf16( grad_out[position[r] / k] * scores[position[r]] ),  zero rows where position[r] < 0,
  * with position: device int32 [n_rows], the routed slot t k + j that row r feeds.
- * row_bytes a multiple of 16, pointers 16-byte aligned.
+ * row_bytes a multiple of 16, pointers 16-byte aligned; rows (grad_out) may be NULL where n_rows (tokens) is 0.
  */
 int altob200_combine_rows(const void* rows, int64_t n_rows, int64_t row_bytes, const int32_t* index,
                           const void* scores, int64_t tokens, int32_t k, void* out, void* stream);
