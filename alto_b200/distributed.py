@@ -480,7 +480,10 @@ class ExpertParallelDispatcher:
     Both are differentiable.  One host synchronisation per dispatch (the split sizes of the
     all-to-all live on the host); with a single rank the all-to-alls are skipped, and on the GPU the two sorts of the
     rows are one: tokens are gathered straight into the padded buffer by the rows of ``routing.expert_plan``, and
-    combined straight from it.  Ids outside [0, num_experts) are then slots without an expert."""
+    combined straight from it.
+
+    An id outside [0, num_experts) is a slot without an expert, on any number of ranks: nothing is sent for it and it adds
+    nothing to its token."""
 
     def __init__(self, num_experts: int, group=None, align: int = ALIGN_SIZE_M):
         self.group = group
@@ -500,10 +503,11 @@ class ExpertParallelDispatcher:
                 and expert_ids.device == dev and self.num_experts <= routing.MAX_PLAN_EXPERTS):
             return self._dispatch_alone(x, expert_ids)
         flat = expert_ids.reshape(-1).to(torch.int64)
+        flat = torch.where((flat < 0) | (flat >= self.num_experts), self.num_experts, flat)      # no expert: behind the others
         order = torch.argsort(flat, stable=True)
         inv_order = torch.empty_like(order)
         inv_order[order] = torch.arange(order.numel(), device=dev)
-        counts = torch.bincount(flat, minlength=self.num_experts)            # rows per global expert
+        counts = torch.bincount(flat, minlength=self.num_experts + 1)[:self.num_experts]         # rows per global expert
         send = counts.view(self.world, self.local_experts)
         if self.world > 1:
             recv = torch.empty_like(send)
@@ -514,10 +518,14 @@ class ExpertParallelDispatcher:
         send_h, recv_h = both[0], both[1]
         st = _DispatchState()
         st.k, st.tokens, st.direct = k, T, False
-        st.inv_order = inv_order.to(torch.int32)
-        st.order = order.to(torch.int32)
         st.in_splits = [int(v) for v in send_h.sum(1)]
         st.out_splits = [int(v) for v in recv_h.sum(1)]
+        routed = sum(st.in_splits)
+        if routed < order.numel():      # slots without an expert have no row
+            inv_order = torch.where(inv_order < routed, inv_order, -1)
+            order = order[:routed]
+        st.inv_order = inv_order.to(torch.int32)
+        st.order = order.to(torch.int32)
         # The row plan is built on the GPU from the device copy of the counts; the host copy only
         # sizes its buffers (and the all-to-all), so the host is free to run ahead again at once.
         per_expert = recv_h.sum(0)
