@@ -296,6 +296,24 @@ def lib():
     return _lib
 
 
+_autograd_module = None
+
+
+def autograd():
+    """The module of autograd functions (``csrc/autograd.cpp``), bound to this library's entry points."""
+    global _autograd_module
+    if _autograd_module is None:
+        handle = lib()
+        try:
+            from . import _autograd as module
+        except ImportError as e:
+            raise RuntimeError("alto_b200/_autograd.so is missing or was built for another torch: run `python -m alto_b200.build`") from e
+        module.bind(*(C.cast(f, C.c_void_p).value for f in (handle.altob200_rms_norm_forward, handle.altob200_rms_norm_backward_work_bytes,
+                                                            handle.altob200_rms_norm_backward)))
+        _autograd_module = module
+    return _autograd_module
+
+
 def status_string(status: int) -> str:
     return lib().altob200_status_string(int(status)).decode()
 

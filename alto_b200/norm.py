@@ -62,52 +62,13 @@ def _check(name: str, x, weight, residual, eps) -> None:
     raise ValueError(f"{name} expects eps >= 0, got {eps}")
 
 
-def _forward(x, weight, residual, eps):
-    """(out, stream) in the shape of x."""
-    two = x.dim() == 2
-    out, stream, _ = L.rms_norm_forward(_rows(x), weight if weight.is_contiguous() else weight.contiguous(), eps,
-                                        None if residual is None else _rows(residual))
-    if two:
-        return out, stream
-    return out.view(x.shape), None if stream is None else stream.view(x.shape)
-
-
-class _RMSNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        out, stream = _forward(x, weight, residual, eps)
-        ctx.set_materialize_grads(False)
-        ctx.eps = eps
-        if stream is None:
-            ctx.save_for_backward(x, weight)
-            return out
-        ctx.save_for_backward(stream, weight)
-        return out, stream
-
-    @staticmethod
-    @L.once_differentiable
-    def backward(ctx, grad_out, grad_stream=None):
-        stream, weight = ctx.saved_tensors
-        need_x, need_w, need_res, _ = ctx.needs_input_grad
-        if grad_out is None:      # only the stream was used
-            return grad_stream, torch.zeros_like(weight) if need_w else None, grad_stream if need_res else None, None
-        gx, gw = L.rms_norm_backward(_rows(grad_out), _rows(stream), weight if weight.is_contiguous() else weight.contiguous(),
-                                     ctx.eps, None if grad_stream is None else _rows(grad_stream), need_w)
-        if stream.dim() != 2:
-            gx = gx.view(stream.shape)
-        return gx, gw, gx if need_res else None, None
-
-
 @L.traced("rms_norm")
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: Optional[torch.Tensor] = None):
     """Norm of the rows of x [..., cols] (bf16 or fp32; weight [cols] in either type).  With ``residual`` (like x) returns
     (y, r), r = x + residual rounded to the type of x and y the norm of r; else y."""
     _check("rms_norm", x, weight, residual, eps)
-    if ((x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)) and torch.is_grad_enabled()
-            or L.forward_mode()):
-        return _RMSNorm.apply(x, weight, residual, eps)
-    out, stream = _forward(x, weight, residual, eps)
-    return out if stream is None else (out, stream)
+    host = L._autograd_module or L.autograd()
+    return host.rms_norm(x, weight, eps) if residual is None else host.rms_norm_residual(x, weight, residual, eps)
 
 
 @L.traced("rms_norm_mxfp8")
