@@ -94,7 +94,8 @@ def rms_norm_mxfp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, res
 
 class _RMSNormMXFP8Linear(torch.autograd.Function):
     """The norm and the MXFP8 linears behind it.  Forward writes the operand of the forward products straight from the
-    norm; what is kept is the stream and the codes of the backward products, no bf16 norm."""
+    norm; what is kept is the stream and the codes of the backward products, no bf16 norm.  Results have two dimensions: views
+    made in here could not be written to."""
 
     @staticmethod
     def forward(ctx, x, norm_weight, residual, eps, fmt, use_2dblock_w, *weights):
@@ -117,13 +118,13 @@ class _RMSNormMXFP8Linear(torch.autograd.Function):
             w2 = w if isinstance(w, E.PrequantizedWeight) else E.as_2d_rows(w.detach())
             w_k, w_t = E.weight_operands(w2, fmt, use_2dblock_w=use_2dblock_w, use_outer_scale=False,
                                          want_t=need_y)
-            outs.append(E.gemm(x_k, w_k, x.dtype).view(*x.shape[:-1], w.shape[0]))
+            outs.append(E.gemm(x_k, w_k, x.dtype))
             saved += [None, None] if w_t is None else [w_t.codes, w_t.scales]
-        ctx.save_for_backward(x if stream is None else stream.view(x.shape), norm_weight, *([None, None] if x_m is None else
-                                                                                        [x_m.codes, x_m.scales]), *saved)
-        ctx.dims, ctx.eps, ctx.fmt, ctx.outs = (M, K), eps, fmt, [w.shape[0] for w in weights]
+        ctx.save_for_backward(x if stream is None else stream, norm_weight,
+                              *([None, None] if x_m is None else [x_m.codes, x_m.scales]), *saved)
+        ctx.dims, ctx.shape, ctx.eps, ctx.fmt, ctx.outs = (M, K), x.shape, eps, fmt, [w.shape[0] for w in weights]
         ctx.set_materialize_grads(False)
-        return tuple(outs) if stream is None else (*outs, stream.view(x.shape))
+        return tuple(outs) if stream is None else (*outs, stream)
 
     @staticmethod
     @L.once_differentiable
@@ -153,9 +154,9 @@ class _RMSNormMXFP8Linear(torch.autograd.Function):
         if dy is not None:
             gx, gw = L.rms_norm_backward(dy, _rows(stream), norm_weight.contiguous(), ctx.eps,
                                          None if grad_stream is None else _rows(grad_stream), need_nw)
-            gx = gx.view(stream.shape)
         elif need_nw:
             gw = torch.zeros_like(norm_weight)
+        gx = None if gx is None else gx.reshape(ctx.shape)
         return (gx if need_x else None, gw, gx if need_res else None, None, None, None, *dws)
 
 
@@ -189,6 +190,8 @@ def rms_norm_mxfp8_linear(x: torch.Tensor, norm_weight: torch.Tensor, weights: U
         weights = tuple(w.detach() if type(w) is torch.nn.Parameter or type(w) is torch.Tensor else
                         unwrap_weight_wrapper(w).detach() for w in weights)
     got = _linears(x, norm_weight, residual, eps, _FP8[fp8_variant][0], bool(use_2dblock_w), weights)
+    if x.dim() != 2:
+        got = tuple(t.view(*x.shape[:-1], t.shape[1]) for t in got)
     if not many and residual is None:
         return got[0]
     return got

@@ -32,3 +32,21 @@ def test_routing(shape):
     # either gradient q (g - sum g q) 3 is off by at most 4 2^-18 of q (|g| + sum |g| q) 3, whose factor of q is at most 6 numel
     atol = 2 * 4 * 2.0 ** -18 * 6 * weights.numel()
     assert ids.shape == weights.shape == shape[:-1] + (4,) and ((g - want).abs() <= atol).all()
+
+
+@pytest.mark.parametrize("shape", [(64, 128), (2, 32, 128)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_linears_behind_a_norm(shape, residual):
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(shape, generator=g, device="cuda").bfloat16().requires_grad_(True)
+    w, nw = torch.randn(96, 128, generator=g, device="cuda").bfloat16().requires_grad_(True), torch.ones(128, device="cuda").bfloat16()
+    res = x.detach().clone().requires_grad_(True) if residual else None
+    up = torch.randn(*shape[:-1], 96, generator=g, device="cuda").bfloat16()
+    results = []
+    for in_place in (True, False):
+        got = norm.rms_norm_mxfp8_linear(x, nw, [w, w], residual=res)
+        assert len(got) == (3 if residual else 2) and all(t.shape[:-1] == x.shape[:-1] for t in got)
+        q = got[0].mul_(2) if in_place else got[0] * 2
+        loss = (q * up).sum() + (got[1] * up).sum() + (got[2].sum() if residual else 0)
+        results.append(torch.autograd.grad(loss, (x, w, res) if residual else (x, w)))
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and results[0][0].shape == x.shape
