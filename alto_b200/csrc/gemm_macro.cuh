@@ -142,8 +142,7 @@ __device__ __forceinline__ MacroTile decode_macro_tile(const MacroGemmArgs& marg
   m.chunk0 = 0;
   int64_t bytes = args.k_bytes;
   if (args.k_offs != nullptr) {
-    const int64_t k0 = e > 0 ? __ldg(args.k_offs + e - 1) : 0;
-    const int64_t k1 = __ldg(args.k_offs + e);
+    const int64_t k0 = k_range_start(args, e), k1 = k_range_end(args, e);
     bytes = (k1 - k0) / 2;
     t.skip = bytes <= 0;
     t.k_stages = (int)((bytes + STAGE_K_BYTES - 1) / STAGE_K_BYTES);

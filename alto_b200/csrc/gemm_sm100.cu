@@ -517,6 +517,18 @@ __device__ __forceinline__ TileCoord tile_coord(const GemmArgs& args, uint32_t t
   return t;
 }
 
+// Ends of the K ranges are device memory that no host has seen, such as a row plan's whose buffer was given too few rows:
+// they are cut off at the operands' K, and a range starts on a whole scale tile, so that no copy leaves the operands or
+// starts off a 16-byte boundary whatever is in them.
+__device__ __forceinline__ int64_t k_range_end(const GemmArgs& args, uint32_t e) {
+  const int64_t k = __ldg(args.k_offs + e);
+  return k < 0 ? 0 : k < args.K ? k : args.K;
+}
+__device__ __forceinline__ int64_t k_range_start(const GemmArgs& args, uint32_t e) {
+  const int64_t k = e > 0 ? k_range_end(args, e - 1) : 0;
+  return k == args.K ? k : k & ~127ll;
+}
+
 template <int KIND, int BN>
 __device__ __forceinline__ TileInfo decode_tile(const GemmArgs& args, int tile, int k_stages_dense) {
   TileInfo t;
@@ -534,8 +546,7 @@ __device__ __forceinline__ TileInfo decode_tile(const GemmArgs& args, int tile, 
   t.skip = false;
   if (args.k_offs != nullptr) {
     constexpr int EPB = Kind<KIND>::ELEMS_PER_BYTE;
-    const int64_t k0 = e > 0 ? __ldg(args.k_offs + e - 1) : 0;
-    const int64_t k1 = __ldg(args.k_offs + e);
+    const int64_t k0 = k_range_start(args, e), k1 = k_range_end(args, e);
     const int64_t bytes = (k1 - k0) / EPB;
     t.skip = bytes <= 0;
     t.k_stages = (int)((bytes + STAGE_K_BYTES - 1) / STAGE_K_BYTES);

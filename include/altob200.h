@@ -576,7 +576,7 @@ int altob200_grouped_gemm_blockscaled(int32_t format_a, int32_t format_b, int64_
  * A[m, k] * B[n, k], for e in [0, num_experts) (k_offs[-1] = 0).  A and B are the
  * axis-0 quantised gradient and activation ([N_out, tokens] and [K_in, tokens], token
  * axis contiguous); `k_offs` (device int32, cumulative, every entry a multiple of 128)
- * gives each expert's token range; experts with an empty range receive zeros.  Replaces
+ * gives each expert's token range, cut off at K; experts with an empty range receive zeros.  Replaces
  * mxfp4_grouped_gemm_backward_weights (alto/kernels/fp4/mxfp4/mxfp_grouped_gemm/cg_backward.py:501)
  * and the per-expert loop of the NVFP4 path
  * (alto/kernels/fp4/nvfp4/nvfp_grouped_gemm/cg_backward.py:126-141).
