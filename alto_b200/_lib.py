@@ -719,12 +719,13 @@ def rms_norm_backward(grad2: torch.Tensor, stream2: torch.Tensor, weight: torch.
 
 
 @on_device_of
-def route_forward(logits2: torch.Tensor, p: RouteParams, bias: Optional[torch.Tensor], lead: Sequence[int]):
-    """(ids int32 [*lead, k], weights fp32 [*lead, k]) of logits [tokens, experts] with unit column stride, tokens the product
-    of ``lead`` (no views: a caller of an autograd function may not write to those)."""
+def route_forward(logits2: torch.Tensor, p: RouteParams, bias: Optional[torch.Tensor], lead: Optional[Sequence[int]] = None):
+    """(ids int32 [tokens, k], weights fp32 [tokens, k]) of logits [tokens, experts] with unit column stride; ``lead``: dimensions
+    in the place of tokens (made so, not as a view: a caller of an autograd function may not write to those)."""
     tokens, dev = logits2.shape[0], logits2.device
-    ids = torch.empty((*lead, p.top_k), dtype=torch.int32, device=dev)
-    weights = torch.empty((*lead, p.top_k), dtype=torch.float32, device=dev)
+    shape = (tokens, p.top_k) if lead is None else (*lead, p.top_k)
+    ids = torch.empty(shape, dtype=torch.int32, device=dev)
+    weights = torch.empty(shape, dtype=torch.float32, device=dev)
     _check((_lib or lib()).altob200_route_forward(p, logits2.data_ptr(), tokens, logits2.stride(0), _ptr(bias), ids.data_ptr(),
                                                   weights.data_ptr(), _stream()), "altob200_route_forward")
     return ids, weights

@@ -46,10 +46,14 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _forward(logits, params, bias):
+    return L.route_forward(_rows(logits), params, bias, None if logits.dim() == 2 else logits.shape[:-1])
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, params, bias):
-        ids, weights = L.route_forward(_rows(logits), params, bias, logits.shape[:-1])
+        ids, weights = _forward(logits, params, bias)
         ctx.save_for_backward(logits, ids)
         ctx.params = params
         ctx.set_materialize_grads(False)      # no zeros in the place of a gradient of ids
@@ -103,7 +107,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
                            1 if renormalize else 0, scale)
     if logits.requires_grad and torch.is_grad_enabled() or L.forward_mode():
         return _Route.apply(logits, params, bias)
-    return L.route_forward(_rows(logits), params, bias, logits.shape[:-1])
+    return _forward(logits, params, bias)
 
 
 @L.traced("expert_plan")
