@@ -95,3 +95,16 @@ def test_a_refused_call_raises_the_package_error():
     with pytest.raises(L.Altob200Error, match="altob200_rms_norm_forward") as e:
         norm.rms_norm(x, x[0])
     assert e.value.status == L.E_LIMIT
+
+
+def test_one_tensor_as_rows_and_residual():
+    x, w = torch.randn(8, 64, device="cuda", requires_grad=True), torch.ones(64, device="cuda")
+    copy = x.detach().clone().requires_grad_(True)
+    up = torch.randn(8, 64, device="cuda")
+    (once,) = torch.autograd.grad(norm.rms_norm(x, w, residual=copy)[0], x, up)
+    (twice,) = torch.autograd.grad(norm.rms_norm(x, w, residual=x)[0], x, up)
+    assert torch.equal(twice, once * 2)
+    x.grad = None
+    norm.rms_norm(x, w, residual=x)[0].backward(up)
+    norm.rms_norm(x, w, residual=copy)[0].backward(up)
+    assert torch.allclose(x.grad, once * 3, rtol=2.0 ** -22) and torch.equal(copy.grad, once)
