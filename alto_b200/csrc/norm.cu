@@ -10,8 +10,9 @@
 //
 // Both directions are HBM streams: forward reads x (and the residual) and writes y (and r), backward reads dy, r (and
 // d_stream) and writes dr.  rstd is not kept: backward reads r anyway, and one more sum costs less than the launch-time
-// allocation of a vector.  bf16 8192 x 4096 with residual (floor 41 us a direction at the copy rate): forward 42 us, backward
-// 47 and 3 to join dw; without loads ahead 68 and 5.  32768 x 4096 (floor 164): 153 and 182 + 4.
+// allocation of a vector.  bf16 8192 x 4096 with residual (41 us a direction at the measured copy rate, a reference and no
+// floor: streams that read more than they write run a little above it): forward 42 us, backward 43 and 4 to join dw;
+// without loads ahead 68 and 5.  32768 x 4096 (164): 157 and 161 + 4.
 //
 // A row is held in registers: 16-byte vectors of it per thread (lane-adjacent, so that four (bf16) or eight (fp32)
 // neighbouring lanes hold a block of 32) or, where width, strides or pointers rule those out, single elements.  8 to 32
@@ -212,8 +213,8 @@ __device__ __forceinline__ void zero_packed_padding(const NormArgs& a, int64_t r
 // One row per LANES lanes of a warp, or (LANES = 0) ROWS rows per CTA; NV units of V elements a thread and row.  FMT: 0 for
 // the type of x, 1 e4m3, 2 e5m2.
 //
-// One row a CTA is bound by the turnover of CTAs, so two share one (8192 x 4096: 42 us, with codes 41; one by one 44 and
-// 46), and with codes by instructions (issue slots 78 %), so elements go in pairs, maxima are taken of the packed words and
+// One row a CTA is bound by the turnover of CTAs, so two share one (8192 x 4096: 42 us, with codes 41; one by one 47 and
+// 49), and with codes by instructions (issue slots 78 %), so elements go in pairs, maxima are taken of the packed words and
 // scales are multiplied (with one element to an instruction and quotients 43).  The bounds keep three CTAs of 512 threads
 // or two of 1024 on an SM: at 45 registers codes took 56 us.  CTAs that walk over rows with the next one's loads ahead, as in
 // the backward pass, are slower (47, with codes 52), and scale bytes put together to words no faster.
@@ -643,7 +644,9 @@ static NormShape norm_shape(int64_t cols, int vec, bool forward) {
   return {0, 0, 0, 0};
 }
 
-// CTAs of a backward pass: what the SMs hold at 64 registers a thread, and no more than there are rows for.
+// CTAs of a backward pass, no more than there are rows for.  A CTA a row: what the SMs hold at 64 registers a thread.  A few
+// lanes a row: eight a SM, of which five to seven fit at a time (72 to 95 registers), so that the last run in a second,
+// emptier round: 262144 x 128 bf16 54 us where the bytes take 41.
 static int norm_blocks_backward(const NormShape& s, int64_t rows) {
   if (s.threads == 0) return (int)(rows < 148 * 4 ? rows : 148 * 4);
   const int64_t all = s.lanes ? ceil_div(rows, 128 / s.lanes) : rows;
@@ -687,7 +690,7 @@ extern "C" int altob200_rms_norm_forward(const altob200_rms_norm_args* p, void* 
 #undef ANY
   } else {
     // two rows a CTA as soon as there are more rows than CTAs at a time (4096 columns: 148 rows 2.1 us one by one, 2.4 in
-    // pairs; 2400 rows 12.9 and 11.1, 8192 rows 48 and 43, with codes 52 and 43)
+    // pairs; 2400 rows 10.3 and 9.4, 8192 rows 47 and 42, with codes 49 and 41)
     const bool two = s.lanes == 0 && s.nv == 1 && s.v > 1 && all_rows > 148 * 4;
     const dim3 grid((unsigned)(s.lanes ? ceil_div(all_rows, 128 / s.lanes) : two ? ceil_div(all_rows, 2) : all_rows)), block(s.threads);
 #define ONE(B, M, L, N, V) (void)launch_after(norm_forward_kernel<B, M, L, N, V>, grid, block, 0, st, a)

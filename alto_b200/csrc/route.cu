@@ -581,8 +581,8 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteGradArgs a) {
 // slots, and a slot's row is start + parts before + warps before + lanes of the same expert before (match.any).  Integers
 // only, so no order changes the result.  One part needs no counting launch; more than PLAN_DIRECT parts get a launch in
 // between that sums over parts, so that the work stays linear.  What bounds it is latency, dependent round
-// trips to L2 and shared memory, and two launches: 65 536 slots over 32 experts 2.2 + 6.7 us, 262 144 over 256 2.8 + 12.8
-// (28 us with the host's five allocations and two launches; tensor operations 285 and 295).
+// trips to L2 and shared memory, and two launches: 65 536 slots over 32 experts 8.0 us in a stream, 262 144 over 256 14.0
+// (20 us a call with the host's five allocations and two launches; tensor operations 290 and 297).
 // ---------------------------------------------------------------------------------------
 struct PlanArgs {
   const void* ids;       // [slots] int32 or int64

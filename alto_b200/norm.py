@@ -171,7 +171,9 @@ def rms_norm_mxfp8_linear(x: torch.Tensor, norm_weight: torch.Tensor, weights: U
                           use_2dblock_w: bool = False):
     """The norm of x (behind the residual's addition) through one MXFP8 linear or several that read the same norm (query, key
     and value; gate and up): what ``_to_mxfp8_then_scaled_mm(rms_norm(x, norm_weight, eps, residual), w, fp8_variant,
-    False, False, use_2dblock_w)`` computes for each, bit for bit, without a bf16 norm between them or kept.
+    False, False, use_2dblock_w)`` computes for each, bit for bit.  The forward products read codes that the norm writes; where a
+    weight requires a gradient the norm is written in the type of x too, for the quantizer of that gradient's operand, and
+    not kept.
 
     ``weights``: one [N, K] or a sequence of them.  Returns the outputs in their order (one tensor for one weight), and r
     behind them with ``residual``.  Differentiable in x, residual, norm_weight and weights; gradients that several linears send

@@ -118,7 +118,8 @@ def expert_plan(expert_ids: torch.Tensor, num_experts: int, align: int = ALIGN_S
     ``expert_ids``: int32 or int64 [..., k]; a number outside [0, num_experts) is a slot without an expert.  ``rows``:
     rows of the buffer; by default what holds every run however the tokens are routed,
     ``(tokens * k + num_experts * align) // align * align``, so that nothing waits for the counts.  Slots whose row does not
-    fit into ``rows`` are dropped.  At most 1024 experts."""
+    fit into ``rows`` are dropped (``offs`` are the runs' ends all the same; the grouped GEMMs cut them off at the buffer's
+    end).  For the grouped GEMMs ``align`` is a multiple of 128.  At most 1024 experts."""
     if not expert_ids.is_cuda:
         raise RuntimeError("expert_plan runs on CUDA tensors only (no CPU fallback)")
     if expert_ids.dtype not in (torch.int32, torch.int64) or expert_ids.dim() < 1:

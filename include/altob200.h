@@ -436,7 +436,8 @@ int altob200_swiglu_kept_backward(const void* codes, const uint8_t* scales, cons
  *   format MXFP8: out is the codes [rows, cols] that altob200_quantize_rowwise makes of y (blocks of 32 along the row;
  *                 cols a multiple of 32), with plain scales [rows, cols / 32] and / or the packed layout, padding zero.
  * Row strides ld_* in elements; out and stream_out are contiguous.  Rows whose width, strides and pointers allow 16-byte
- * vectors are read once, others element by element and twice.
+ * vectors are held in registers and read once up to 4096 vectors, others element by element up to 16384 of them (8192 in
+ * the gradient below); wider rows are read element by element and twice.
  */
 typedef struct altob200_rms_norm_args {
   int64_t rows, cols, ld_x, ld_residual;
