@@ -214,7 +214,7 @@ __device__ __forceinline__ void zero_packed_padding(const NormArgs& a, int64_t r
 // the type of x, 1 e4m3, 2 e5m2.
 //
 // One row a CTA is bound by the turnover of CTAs, so two share one (8192 x 4096: 42 us, with codes 41; one by one 47 and
-// 49), and with codes by instructions (issue slots 78 %), so elements go in pairs, maxima are taken of the packed words and
+// 49), and with codes by instructions (issue slots 72 %), so elements go in pairs, maxima are taken of the packed words and
 // scales are multiplied (with one element to an instruction and quotients 43).  The bounds keep three CTAs of 512 threads
 // or two of 1024 on an SM: at 45 registers codes took 56 us.  CTAs that walk over rows with the next one's loads ahead, as in
 // the backward pass, are slower (47, with codes 52), and scale bytes put together to words no faster.

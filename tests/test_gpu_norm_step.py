@@ -108,3 +108,38 @@ def test_one_tensor_as_rows_and_residual():
     norm.rms_norm(x, w, residual=x)[0].backward(up)
     norm.rms_norm(x, w, residual=copy)[0].backward(up)
     assert torch.allclose(x.grad, once * 3, rtol=2.0 ** -22) and torch.equal(copy.grad, once)
+
+
+def test_inference_mode_and_hooks_around_saved_tensors():
+    x, w = torch.randn(4, 8, 64, device="cuda"), torch.ones(64, device="cuda")
+    want = norm.rms_norm(x, w, residual=x)
+    with torch.inference_mode():
+        got = norm.rms_norm(x, w, residual=x)
+        inside = norm.rms_norm(got[1], w)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(inside, norm.rms_norm(want[1], w))
+    leaf, seen = x.clone().requires_grad_(True), []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.shape) or t.cpu(), lambda t: t.cuda()):
+        y = norm.rms_norm(leaf, w)
+    (g,) = torch.autograd.grad(y, leaf, x)
+    leaf2 = x.clone().requires_grad_(True)
+    assert len(seen) == 2 and torch.equal(g, torch.autograd.grad(norm.rms_norm(leaf2, w), leaf2, x)[0])
+
+
+def test_steps_from_several_threads():
+    import threading
+    x, w, up = torch.randn(200, 512, device="cuda"), torch.ones(512, device="cuda"), torch.randn(200, 512, device="cuda")
+
+    def step():
+        leaf, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        return torch.autograd.grad(norm.rms_norm(leaf, wl), (leaf, wl), up)
+    want, got = step(), {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got[i] = step()
+        torch.cuda.synchronize()
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert len(got) == 4 and all(torch.equal(a, b) for g in got.values() for a, b in zip(g, want))
