@@ -75,6 +75,10 @@ EXPORTED_SYMBOLS = (
     "altob200_gemm_mxfp4_two_level",
     "altob200_grouped_gemm_mxfp4_two_level",
     "altob200_grouped_gemm_wgrad_mxfp4_two_level",
+    "altob200_fp8_block_quantize",
+    "altob200_fp8_block_quantize_squares",
+    "altob200_fp8_block_dequantize",
+    "altob200_fp8_block_gemm",
     "altob200_set_wait_limit_ns",
     "altob200_selftest_wait_timeout",
 )
@@ -166,6 +170,26 @@ class RouteParams(C.Structure):
     """``altob200_route_params`` of the header."""
     _fields_ = [(n, C.c_int32) for n in ("dtype", "experts", "top_k", "sigmoid", "num_groups", "groups_kept", "group_top",
                                          "renormalize")] + [("scale", C.c_float)]
+
+
+class Fp8BlockScale(C.Structure):
+    """``altob200_fp8_block_scale`` of the header."""
+    _fields_ = [("scales", C.c_void_p)] + [(n, C.c_int64) for n in ("row_stride", "chunk_stride", "expert_stride")] + [
+        (n, C.c_int32) for n in ("row_shift", "chunk_shift")]
+
+
+class Fp8BlockQuantArgs(C.Structure):
+    """``altob200_fp8_block_quant_args`` of the header."""
+    _fields_ = [("x", C.c_void_p)] + [(n, C.c_int64) for n in ("rows", "cols", "ld")] + [
+        (n, C.c_void_p) for n in ("offs", "row_codes", "row_scales", "col_codes", "col_scales")] + [("ld_col", C.c_int64)] + [
+        (n, C.c_int32) for n in ("dtype", "format", "experts")]
+
+
+class Fp8BlockGemmArgs(C.Structure):
+    """``altob200_fp8_block_gemm_args`` of the header."""
+    _fields_ = [(n, C.c_int64) for n in ("M", "N", "K", "lda", "ldd", "k_rows")] + [("a", C.c_void_p), ("b", C.c_void_p),
+                ("sa", Fp8BlockScale), ("sb", Fp8BlockScale), ("offs", C.c_void_p), ("d", C.c_void_p)] + [
+        (n, C.c_int32) for n in ("mode", "experts", "format", "a_dtype", "out_dtype")]
 
 
 class Altob200Error(RuntimeError):
@@ -273,6 +297,14 @@ def _declare_more(lib):
         f = getattr(lib, name)
         f.restype = C.c_int
         f.argtypes = [i64, i64, i64, i32, vp, vp, ms, vp, vp, ms, vp, C.c_float, i32, vp, i64, vp]
+    lib.altob200_fp8_block_quantize.restype = C.c_int
+    lib.altob200_fp8_block_quantize.argtypes = [C.POINTER(Fp8BlockQuantArgs), vp]
+    lib.altob200_fp8_block_quantize_squares.restype = C.c_int
+    lib.altob200_fp8_block_quantize_squares.argtypes = [vp, i32, i32, i64, i64, i64, i64, i64, vp, vp, vp, vp]
+    lib.altob200_fp8_block_dequantize.restype = C.c_int
+    lib.altob200_fp8_block_dequantize.argtypes = [vp, i32, i64, i64, C.POINTER(Fp8BlockScale), i32, vp, vp]
+    lib.altob200_fp8_block_gemm.restype = C.c_int
+    lib.altob200_fp8_block_gemm.argtypes = [C.POINTER(Fp8BlockGemmArgs), vp]
     lib.altob200_set_wait_limit_ns.restype = C.c_int
     lib.altob200_set_wait_limit_ns.argtypes = [C.c_uint64]
     lib.altob200_selftest_wait_timeout.restype = C.c_int
@@ -836,6 +868,58 @@ def swiglu_kept_backward(codes: torch.Tensor, scales: torch.Tensor, grad_out: to
     _check((_lib or lib()).altob200_swiglu_kept_backward(codes.data_ptr(), scales.data_ptr(), grad_out.data_ptr(), rows, two_h // 2, fmt,
                                                grad_h.data_ptr(), _stream()), "altob200_swiglu_kept_backward")
     return grad_h
+
+
+@on_device_of
+def fp8_block_quantize(x2: torch.Tensor, fmt: int, rows: bool, cols: bool, offs: Optional[torch.Tensor] = None):
+    """((codes [R, C], scales [C / 128, R]) or None, (codes [C, padded], scales [padded / 128, C]) or None) of x2 [R, C], blocks
+    along its rows and along its columns; ``offs``: ends of the experts' rows, where blocks of rows begin anew."""
+    (R, n), dev = x2.shape, x2.device
+    a = Fp8BlockQuantArgs(x2.data_ptr(), R, n, x2.stride(0) if R > 1 else n, _ptr(offs), None, None, None, None, 0, _DT_OF[x2.dtype], fmt,
+                          0 if offs is None else offs.numel())
+    by_row = by_col = None
+    if rows:
+        by_row = (torch.empty((R, n), dtype=torch.uint8, device=dev), torch.empty(((n + 127) // 128, R), dtype=torch.float32, device=dev))
+        a.row_codes, a.row_scales = by_row[0].data_ptr(), by_row[1].data_ptr()
+    if cols:
+        blocks = (R + 127) // 128 if offs is None else R // 128 + offs.numel()
+        by_col = (torch.empty((n, blocks * 128), dtype=torch.uint8, device=dev), torch.empty((blocks, n), dtype=torch.float32, device=dev))
+        a.col_codes, a.col_scales, a.ld_col = by_col[0].data_ptr(), by_col[1].data_ptr(), blocks * 128
+    if R > 0:
+        _check((_lib or lib()).altob200_fp8_block_quantize(a, _stream()), "altob200_fp8_block_quantize")
+    return by_row, by_col
+
+
+@on_device_of
+def fp8_block_quantize_squares(w3: torch.Tensor, fmt: int, plain: bool, transposed: bool):
+    """(codes [B, R, C] or None, codes [B, C, R] or None, scales [B, R / 128, C / 128]) of matrices [B, R, C]."""
+    (nb, R, n), dev = w3.shape, w3.device
+    codes = torch.empty((nb, R, n), dtype=torch.uint8, device=dev) if plain else None
+    codes_t = torch.empty((nb, n, R), dtype=torch.uint8, device=dev) if transposed else None
+    scales = torch.empty((nb, (R + 127) // 128, (n + 127) // 128), dtype=torch.float32, device=dev)
+    _check((_lib or lib()).altob200_fp8_block_quantize_squares(w3.data_ptr(), _DT_OF[w3.dtype], fmt, nb, R, n, w3.stride(1), w3.stride(0),
+                                                               _ptr(codes), _ptr(codes_t), scales.data_ptr(), _stream()),
+           "altob200_fp8_block_quantize_squares")
+    return codes, codes_t, scales
+
+
+@on_device_of
+def fp8_block_dequantize(codes2: torch.Tensor, fmt: int, scales: torch.Tensor, row_stride: int, col_stride: int, row_shift: int,
+                         col_shift: int, out: torch.Tensor) -> None:
+    s = Fp8BlockScale(scales.data_ptr(), row_stride, col_stride, 0, row_shift, col_shift)
+    _check((_lib or lib()).altob200_fp8_block_dequantize(codes2.data_ptr(), fmt, codes2.shape[0], codes2.shape[1], s, _dt(out.dtype),
+                                                         out.data_ptr(), _stream()), "altob200_fp8_block_dequantize")
+
+
+@on_device_of
+def fp8_block_gemm(a: torch.Tensor, sa: Optional[Fp8BlockScale], b: torch.Tensor, sb: Fp8BlockScale, out: torch.Tensor, fmt: int,
+                   dims, mode: int = 0, offs: Optional[torch.Tensor] = None, k_rows: int = 0) -> None:
+    """``altob200_fp8_block_gemm``: a [M, K] codes, or numbers where ``sa`` is None; ``dims`` = (M, N, K)."""
+    M, N, K = dims
+    g = Fp8BlockGemmArgs(M, N, K, a.stride(0) if M > 1 else K, N, k_rows, a.data_ptr(), b.data_ptr(), sa or Fp8BlockScale(), sb, _ptr(offs),
+                         out.data_ptr(), mode, 0 if offs is None else offs.numel(), fmt, _DT_OF[a.dtype] if sa is None else -1,
+                         _DT_OF[out.dtype])
+    _check((_lib or lib()).altob200_fp8_block_gemm(g, _stream()), "altob200_fp8_block_gemm")
 
 
 def gemm_blockscaled(fmt_a, fmt_b, M, N, K, a_codes, a_scales, b_codes, b_scales, out, alpha_a=None,

@@ -28,7 +28,7 @@ from . import _lib as L
 from . import _linear as E
 from . import dge
 from .hadamard import HadamardFactory, HadamardTransform
-from .nvfp4 import _check_scale_format, unwrap_weight_wrapper
+from .nvfp4 import _check_scale_format, outside_of_grad_mode, unwrap_weight_wrapper
 
 ALIGN_SIZE_M = 128
 
@@ -227,6 +227,16 @@ def _quantize_then_mxfp8_scaled_grouped_mm(A, B, offs, *, use_2dblock_x: bool = 
         raise NotImplementedError("MXFP8 stochastic rounding exists only as gfx950 instructions in the reference")
     return GroupedLinearFunction.apply(A, B.transpose(-2, -1), offs, _FP8[fwd_format], _FP8[bwd_grad_format],
                                        use_2dblock_x, use_2dblock_w, False, False, None)
+
+
+@L.traced("fp8_block_grouped_linear_training")
+def _quantize_then_fp8_block_scaled_grouped_mm(A, B, offs, *, fp8_variant: str = "e4m3") -> torch.Tensor:
+    """A [M, K], B [E, K, N] in FP8 with one fp32 scale for each block of 128 (``fp8_block``).  Unlike the functions above this
+    one takes any number of rows an expert: no padding, ``offs`` [E] are the ends of the runs as they are.  Rows from
+    offs[-1] on give zeros, and a zero gradient."""
+    from . import fp8_block
+    A, B = outside_of_grad_mode(A, B)
+    return fp8_block._grouped(A, B, offs, fp8_variant)
 
 
 # ---------------------------------------------------------------------------------------------

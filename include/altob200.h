@@ -656,6 +656,80 @@ int altob200_grouped_gemm_wgrad_mxfp4_two_level(int64_t M, int64_t N, int64_t K,
                                                 int64_t ldd, void* stream);
 
 /*
+ * FP8 with one fp32 scale for each block of 128 (1 x 128 of an operand along the reduced dimension, or squares of
+ * 128 x 128).  A block's scale is max(|largest|, 1e-12) / top, top = 448 (E4M3) or 57344 (E5M2), its codes are the quotients
+ * by the scale, rounded to nearest; both quotients are correctly rounded fp32.  A last block is as short as the operand.
+ * `format` is ALTOB200_FMT_MXFP8_E4M3 or _E5M2 for the elements' type.  The reference's tree has the format in a
+ * part that its recipes do not reach (alto/kernels/blockwise_fp8/blockwise_linear.py, blockwise_quantization.py).
+ *
+ * Where the scale of element (row r, reduced index k) lies:
+ *   scales[expert * expert_stride + (r >> row_shift) * row_stride + (k >> chunk_shift) * chunk_stride]
+ * with row_shift 0 (a scale per row) or 7 (squares); chunk_shift is 7 (0: only in altob200_fp8_block_dequantize, for
+ * blocks along the rows).
+ */
+typedef struct altob200_fp8_block_scale {
+  const float* scales;
+  int64_t row_stride, chunk_stride, expert_stride;
+  int32_t row_shift, chunk_shift;
+} altob200_fp8_block_scale;
+
+/*
+ * Quantizer of a matrix x [rows, cols] (rows `ld` elements apart), along its rows, along its columns or both from one read:
+ *   row_codes [rows, cols], row_scales [ceil(cols / 128), rows]           blocks of 128 columns
+ *   col_codes [cols, ld_col], col_scales [ld_col / 128, cols]             blocks of 128 rows, codes transposed
+ * (a pair of null pointers: not wanted).  `offs` (device, may be NULL): ends of the experts' rows; blocks of rows then begin
+ * at every expert's first row, an expert's ceil(rows / 128) blocks behind those of the experts in front of it, and rows behind
+ * the last expert are left out.  Codes of a block's missing rows are zero.  cols is a multiple of 16, ld_col one of 128 and
+ * at least 128 blocks, blocks = ceil(rows / 128), or rows / 128 + experts with `offs` (blocks that no expert has are not
+ * written).  x and its rows begin on 16 bytes.
+ */
+typedef struct altob200_fp8_block_quant_args {
+  const void* x;
+  int64_t rows, cols, ld;
+  const int32_t* offs;
+  void* row_codes;
+  float* row_scales;
+  void* col_codes;
+  float* col_scales;
+  int64_t ld_col;
+  int32_t dtype, format, experts;
+} altob200_fp8_block_quant_args;
+int altob200_fp8_block_quantize(const altob200_fp8_block_quant_args* args, void* stream);
+
+/*
+ * Squares of 128 x 128 of `matrices` matrices [rows, cols]: codes [matrices][rows, cols] and / or transposed
+ * [matrices][cols, rows], scales [matrices][ceil(rows / 128), ceil(cols / 128)].  rows and cols are multiples of 16.
+ */
+int altob200_fp8_block_quantize_squares(const void* x, int32_t dtype, int32_t format, int64_t matrices, int64_t rows, int64_t cols,
+                                        int64_t ld, int64_t matrix_stride, void* codes, void* codes_t, float* scales, void* stream);
+
+/* Values of codes [rows, cols] (cols a multiple of 8), code times scale, rounded once to the output's type. */
+int altob200_fp8_block_dequantize(const void* codes, int32_t format, int64_t rows, int64_t cols, const altob200_fp8_block_scale* scale,
+                                  int32_t out_dtype, void* out, void* stream);
+
+/*
+ * D[m, n] = sum over blocks c of 128 along K of sa[m, c] sb[n, c] (sum over k in c of A[m, k] B[n, k]), sums in fp32.
+ *   mode 0  A [M, K], B [N, K]
+ *   mode 1  rows of A belong to experts, `offs` (device): their ends; B [experts][N, K].  Any number of rows an expert; rows
+ *           behind the last expert give zeros.
+ *   mode 2  the reduced dimension belongs to experts: A [M, K], B [N, K] with K = ld_col of altob200_fp8_block_quantize with
+ *           the same `offs` over `k_rows` rows, D [experts][M, N]
+ * a_dtype: -1, A is codes; ALTOB200_DT_BF16 / _F32, A is numbers with rows `lda` elements apart, which the kernel quantises
+ * along its rows (modes 0 and 1, few rows an expert).  N and K are multiples of 16; codes lie without gaps; everything begins on
+ * 16 bytes.
+ */
+typedef struct altob200_fp8_block_gemm_args {
+  int64_t M, N, K, lda, ldd, k_rows;
+  const void* a;
+  const void* b;
+  altob200_fp8_block_scale sa, sb;
+  const int32_t* offs;
+  void* d;
+  int32_t mode, experts, format, a_dtype, out_dtype;
+} altob200_fp8_block_gemm_args;
+int altob200_fp8_block_gemm(const altob200_fp8_block_gemm_args* args, void* stream);
+
+/*
  * Failure detection of the GEMM kernels.  Every mbarrier wait inside them is bounded by a wall-clock
  * limit (default 4 s); a wait that runs out records {kernel, block, site} in the status word that
  * altob200_status_read returns, and the kernel leaves through its normal teardown.
