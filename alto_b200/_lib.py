@@ -79,6 +79,9 @@ EXPORTED_SYMBOLS = (
     "altob200_fp8_block_quantize_squares",
     "altob200_fp8_block_dequantize",
     "altob200_fp8_block_gemm",
+    "altob200_grad_norm_work_bytes",
+    "altob200_grad_norm",
+    "altob200_clip_grads",
     "altob200_set_wait_limit_ns",
     "altob200_selftest_wait_timeout",
 )
@@ -190,6 +193,11 @@ class Fp8BlockGemmArgs(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("M", "N", "K", "lda", "ldd", "k_rows")] + [("a", C.c_void_p), ("b", C.c_void_p),
                 ("sa", Fp8BlockScale), ("sb", Fp8BlockScale), ("offs", C.c_void_p), ("d", C.c_void_p)] + [
         (n, C.c_int32) for n in ("mode", "experts", "format", "a_dtype", "out_dtype")]
+
+
+class GradList(C.Structure):
+    """``altob200_grad_list`` of the header."""
+    _fields_ = [(n, C.c_void_p) for n in ("grads", "outs", "sizes", "dtypes")] + [("count", C.c_int64)]
 
 
 class Altob200Error(RuntimeError):
@@ -305,6 +313,12 @@ def _declare_more(lib):
     lib.altob200_fp8_block_dequantize.argtypes = [vp, i32, i64, i64, C.POINTER(Fp8BlockScale), i32, vp, vp]
     lib.altob200_fp8_block_gemm.restype = C.c_int
     lib.altob200_fp8_block_gemm.argtypes = [C.POINTER(Fp8BlockGemmArgs), vp]
+    lib.altob200_grad_norm_work_bytes.restype = i64
+    lib.altob200_grad_norm_work_bytes.argtypes = [i64]
+    lib.altob200_grad_norm.restype = C.c_int
+    lib.altob200_grad_norm.argtypes = [C.POINTER(GradList), i32, vp, vp, vp, vp]
+    lib.altob200_clip_grads.restype = C.c_int
+    lib.altob200_clip_grads.argtypes = [C.POINTER(GradList), i32, C.c_double, vp, vp, vp, vp]
     lib.altob200_set_wait_limit_ns.restype = C.c_int
     lib.altob200_set_wait_limit_ns.argtypes = [C.c_uint64]
     lib.altob200_selftest_wait_timeout.restype = C.c_int
@@ -341,7 +355,8 @@ def autograd():
         except ImportError as e:
             raise RuntimeError("alto_b200/_autograd.so is missing or was built for another torch: run `python -m alto_b200.build`") from e
         module.bind(*(C.cast(f, C.c_void_p).value for f in (handle.altob200_rms_norm_forward, handle.altob200_rms_norm_backward_work_bytes,
-                                                            handle.altob200_rms_norm_backward)))
+                                                            handle.altob200_rms_norm_backward, handle.altob200_grad_norm_work_bytes,
+                                                            handle.altob200_grad_norm, handle.altob200_clip_grads)))
         _autograd_module = module
     return _autograd_module
 

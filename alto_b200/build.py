@@ -18,7 +18,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libaltob200.so"
 AUTOGRAD_PATH = PKG_DIR / "_autograd.so"
 HEADER = PKG_DIR.parent / "include" / "altob200.h"
-SOURCES = ["quant.cu", "macro_scale.cu", "rht_dense.cu", "rows.cu", "swiglu.cu", "norm.cu", "route.cu", "dge.cu", "deosc.cu", "fp8_block.cu",
+SOURCES = ["quant.cu", "macro_scale.cu", "rht_dense.cu", "rows.cu", "swiglu.cu", "norm.cu", "route.cu", "dge.cu", "deosc.cu", "fp8_block.cu", "grad_norm.cu",
            "gemm_sm100.cu", "linear.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -15,6 +15,8 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
+#include <utility>
+#include <vector>
 
 #include "altob200.h"
 
@@ -29,6 +31,9 @@ struct Entries {
   decltype(&altob200_rms_norm_forward) forward;
   decltype(&altob200_rms_norm_backward_work_bytes) work_bytes;
   decltype(&altob200_rms_norm_backward) backward;
+  decltype(&altob200_grad_norm_work_bytes) norm_work_bytes;
+  decltype(&altob200_grad_norm) grad_norm;
+  decltype(&altob200_clip_grads) clip_grads;
 } entry = {};
 
 // The package's own error, as a refused call of the other operators raises it.
@@ -153,13 +158,86 @@ class Norm : public torch::autograd::Function<Norm> {
   }
 };
 
+// A list of tensors as the entry points take it.  A tensor whose elements are not neighbours in memory goes through a copy
+// (and back, where it is written).
+struct GradList {
+  std::vector<const void*> grads;
+  std::vector<void*> outs;
+  std::vector<int64_t> sizes;
+  std::vector<int32_t> dtypes;
+  std::vector<Tensor> hold;
+  std::vector<std::pair<Tensor, Tensor>> back;      // (copy, where it belongs)
+  altob200_grad_list list = {};
+
+  static bool same_layout(const Tensor& a, const Tensor& b) {
+    return a.is_non_overlapping_and_dense() && (a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()));
+  }
+  GradList(const std::vector<Tensor>& in, const std::vector<Tensor>& out, bool writes) {
+    const size_t n = in.size();
+    grads.reserve(n), sizes.reserve(n), dtypes.reserve(n);
+    if (writes) outs.reserve(n);
+    for (size_t i = 0; i < n; ++i) {
+      const Tensor* g = &in[i];
+      if (!g->is_non_overlapping_and_dense()) g = &hold.emplace_back(g->contiguous());
+      Tensor kept = *g;      // (hold may move)
+      grads.push_back(kept.data_ptr());
+      sizes.push_back(kept.numel());
+      dtypes.push_back(dtype_of(kept));
+      if (!writes) continue;
+      const Tensor& o = out.empty() ? in[i] : out[i];
+      if (o.is_same(kept) || same_layout(o, kept)) {
+        outs.push_back(o.data_ptr());
+      } else {
+        back.emplace_back(at::empty_like(kept), o);
+        outs.push_back(back.back().first.data_ptr());
+      }
+    }
+    list = {grads.data(), writes ? outs.data() : nullptr, sizes.data(), dtypes.data(), (int64_t)n};
+  }
+  void finish() {
+    for (auto& b : back) b.second.copy_(b.first);
+  }
+};
+
+// (total fp64, norm fp32) of the tensors together
+std::pair<Tensor, Tensor> grad_norm(const std::vector<Tensor>& grads, bool inf) {
+  const at::AutoGradMode no_graph(false);
+  const c10::cuda::CUDAGuard device(grads.at(0).device());
+  GradList l(grads, {}, false);
+  const auto options = grads[0].options();
+  Tensor total = at::empty({}, options.dtype(at::kDouble)), norm = at::empty({}, options.dtype(at::kFloat));
+  Tensor work = at::empty({entry.norm_work_bytes(l.list.count)}, options.dtype(at::kByte));
+  check(entry.grad_norm(&l.list, inf, work.data_ptr(), (double*)total.data_ptr(), (float*)norm.data_ptr(),
+                        c10::cuda::getCurrentCUDAStream().stream()), "altob200_grad_norm");
+  return {total, norm};
+}
+
+Tensor clip_grads(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs, double max_norm, bool inf, const std::optional<Tensor>& total) {
+  const at::AutoGradMode no_graph(false);
+  const c10::cuda::CUDAGuard device(grads.at(0).device());
+  GradList l(grads, outs, true);
+  const auto options = grads[0].options();
+  Tensor norm = at::empty({}, options.dtype(at::kFloat)), work;
+  if (!total.has_value()) work = at::empty({entry.norm_work_bytes(l.list.count)}, options.dtype(at::kByte));
+  check(entry.clip_grads(&l.list, inf, max_norm, total.has_value() ? (const double*)total->data_ptr() : nullptr,
+                         work.defined() ? work.data_ptr() : nullptr, (float*)norm.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()),
+        "altob200_clip_grads");
+  l.finish();
+  return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
-  m.def("bind", [](uintptr_t forward, uintptr_t work_bytes, uintptr_t backward) {
+  m.def("bind", [](uintptr_t forward, uintptr_t work_bytes, uintptr_t backward, uintptr_t norm_work_bytes, uintptr_t grad_norm,
+                   uintptr_t clip_grads) {
     entry = {reinterpret_cast<decltype(entry.forward)>(forward), reinterpret_cast<decltype(entry.work_bytes)>(work_bytes),
-             reinterpret_cast<decltype(entry.backward)>(backward)};
+             reinterpret_cast<decltype(entry.backward)>(backward), reinterpret_cast<decltype(entry.norm_work_bytes)>(norm_work_bytes),
+             reinterpret_cast<decltype(entry.grad_norm)>(grad_norm), reinterpret_cast<decltype(entry.clip_grads)>(clip_grads)};
   });
+  // lists as alto_b200/grad_clip.py has checked them
+  m.def("grad_norm", &grad_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("clip_grads", &clip_grads, pybind11::call_guard<pybind11::gil_scoped_release>());
   // operands as alto_b200/norm.py has checked them
   m.def("rms_norm", [](const Tensor& x, const Tensor& weight, double eps) { return Norm::apply(x, weight, std::optional<Tensor>(), eps)[0]; },
         pybind11::call_guard<pybind11::gil_scoped_release>());

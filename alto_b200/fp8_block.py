@@ -383,6 +383,8 @@ def _linear(a, b, fp8_variant):
 @L.traced("fp8_block_linear_training")
 def _to_fp8_block_then_scaled_mm(a: torch.Tensor, b: torch.Tensor, fp8_variant: str = "e4m3") -> torch.Tensor:
     """a b^T of a training step: a [..., K], b [N, K] (bf16 or fp32, a wrapped weight too), differentiable in both."""
+    if not a.is_cuda:
+        raise RuntimeError("FP8BlockLinearFunction runs on CUDA tensors only (no CPU fallback)")
     a, b = outside_of_grad_mode(a, b)
     return _linear(a, b, fp8_variant)
 

@@ -1,0 +1,125 @@
+"""Norm of all gradients together, and clipping by it: the step between the backward pass (or
+``distributed.allreduce_gradients``) and the optimizer.
+
+    grad_norm(tensors, norm_type)                             norm of the tensors as one vector
+    clip_grad_norm_(parameters, max_norm, ...)                torch.nn.utils' function of the same name, gradients in place
+    clip_grads(grads, max_norm, ..., out=...)                 the same for a list of tensors, in place or into others
+
+    norm = sqrt(sum g^2), or max |g|          g <- g * min(1, max_norm / (norm + 1e-6))
+
+Two launches for a thousand tensors, whatever their types (bf16, fp32), sizes and alignments; the host is not waited for.
+Squares are summed in fp32 over 32 numbers and in fp64 beyond, in an order that does not change from call to call.
+
+The reference's trainer clips with torch's function between its optimizer hooks (alto/components/optimizer.py)."""
+from __future__ import annotations
+
+import math
+from typing import Iterable, Optional, Sequence, Union
+
+import torch
+
+from . import _lib as L
+
+__all__ = ["grad_norm", "clip_grad_norm_", "clip_grads"]
+
+_TYPES = (torch.bfloat16, torch.float32)
+
+
+def _kind(norm_type) -> bool:
+    """Whether the norm is the largest magnitude."""
+    p = float(norm_type)
+    if p == 2.0:
+        return False
+    if p == math.inf:
+        return True
+    raise ValueError(f"the norms are 2 and inf, got {norm_type}")
+
+
+def _check(name: str, tensors: Sequence[torch.Tensor]) -> None:
+    device = tensors[0].device
+    for t in tensors:
+        if t.dtype in _TYPES and t.device == device and t.is_cuda and t.layout is torch.strided:
+            continue
+        if t.layout is not torch.strided:
+            raise ValueError(f"{name} expects dense tensors, got {t.layout}")
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} runs on CUDA tensors only (no CPU fallback)")
+        if t.dtype not in _TYPES:
+            raise TypeError(f"{name} expects bfloat16 or float32, got {t.dtype}")
+        raise ValueError(f"{name} expects all tensors on one device")
+
+
+def _local(t: torch.Tensor) -> torch.Tensor:
+    return t.to_local() if hasattr(t, "to_local") else t
+
+
+def _reduced(total: torch.Tensor, inf: bool, group) -> torch.Tensor:
+    dist = torch.distributed
+    dist.all_reduce(total, op=dist.ReduceOp.MAX if inf else dist.ReduceOp.SUM, group=group)
+    return total
+
+
+def _world(group) -> int:
+    dist = torch.distributed
+    return dist.get_world_size(group) if group is not None and dist.is_initialized() else 1
+
+
+@L.traced("grad_norm")
+def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0, group=None) -> torch.Tensor:
+    """fp32 scalar: the 2-norm (or the largest magnitude, ``norm_type`` inf) of all tensors together.  ``group``: over the ranks of
+    it, each of which holds a part."""
+    inf = _kind(norm_type)
+    tensors = [_local(t) for t in tensors]
+    if not tensors:
+        if _world(group) > 1:
+            raise ValueError("grad_norm over ranks expects a tensor on each")
+        return torch.zeros(())
+    _check("grad_norm", tensors)
+    total, norm = (L._autograd_module or L.autograd()).grad_norm(tensors, inf)
+    if _world(group) > 1:
+        total = _reduced(total, inf, group)
+        norm = (total if inf else total.sqrt()).float()
+    return norm
+
+
+@L.traced("clip_grads")
+def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None,
+               group=None, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Scales the tensors to a common norm of at most ``max_norm``, in place or into ``out`` (tensors of the same shapes and types
+    that do not overlap them); returns the norm before, an fp32 scalar.  Where nothing is clipped, tensors scaled in place are not written.
+    ``group``: the norm is taken over its ranks.  ``error_if_nonfinite`` waits for the norm and raises before anything is
+    scaled."""
+    inf, max_norm = _kind(norm_type), float(max_norm)
+    grads = [_local(g) for g in grads]
+    if not grads:
+        if _world(group) > 1:
+            raise ValueError("clip_grads over ranks expects a tensor on each")
+        return torch.zeros(())
+    _check("clip_grads", grads)
+    outs = []
+    if out is not None:
+        outs = [_local(o) for o in out]
+        if len(outs) != len(grads) or any(o.shape != g.shape or o.dtype != g.dtype for o, g in zip(outs, grads)):
+            raise ValueError("clip_grads expects out like grads: as many tensors, of their shapes and types")
+        _check("clip_grads", outs)
+        if outs[0].device != grads[0].device:
+            raise ValueError("clip_grads expects all tensors on one device")
+    host = L._autograd_module or L.autograd()
+    total = None
+    if error_if_nonfinite or _world(group) > 1:
+        total, _ = host.grad_norm(grads, inf)
+        if _world(group) > 1:
+            total = _reduced(total, inf, group)
+        if error_if_nonfinite and not math.isfinite(float(total)):
+            raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is non-finite, so it cannot "
+                               "be clipped. To disable this error and scale the gradients by the non-finite norm anyway, set "
+                               "`error_if_nonfinite=False`")
+    return host.clip_grads(grads, outs, max_norm, inf, total)
+
+
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False, group=None) -> torch.Tensor:
+    """``clip_grads`` of the gradients that the parameters have (sharded ones by their local part, with ``group``)."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    return clip_grads([p.grad for p in parameters if p.grad is not None], max_norm, norm_type, None, group, error_if_nonfinite)

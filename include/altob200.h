@@ -730,6 +730,34 @@ typedef struct altob200_fp8_block_gemm_args {
 int altob200_fp8_block_gemm(const altob200_fp8_block_gemm_args* args, void* stream);
 
 /*
+ * Many tensors taken as one vector: its norm, and the tensors scaled to a largest norm.  The arrays of the list are HOST memory,
+ * read before the call returns; `outs` NULL: in place.  Elements of a tensor are neighbours in memory, at any alignment of
+ * their type.  Beside the optimizer hooks of the reference's trainer (alto/components/optimizer.py), which clips by torch's
+ * function.
+ */
+typedef struct altob200_grad_list {
+  const void* const* grads;
+  void* const* outs;
+  const int64_t* sizes;
+  const int32_t* dtypes; /* ALTOB200_DT_* */
+  int64_t count;
+} altob200_grad_list;
+/* Bytes of work space for a list of `count` tensors (8-byte aligned, not shared by calls that may overlap). */
+int64_t altob200_grad_norm_work_bytes(int64_t count);
+/*
+ * total = sum of squares, or the largest magnitude where norm_inf; norm = its root, or itself (each may be NULL).  Squares are
+ * summed in fp32 over 32 numbers and in fp64 beyond; the same list gives the same bits.  A NaN gives a NaN.
+ */
+int altob200_grad_norm(const altob200_grad_list* list, int32_t norm_inf, void* work, double* total, float* norm, void* stream);
+/*
+ * out = g * min(1, max_norm / (norm + 1e-6)), the factor rounded to fp32 and the product to the type.  `total` (device, may be
+ * NULL): the sum or maximum over more than this list (a sum over ranks); NULL: the list's own, with `work`.  Tensors
+ * scaled in place are not written where the factor is 1.
+ */
+int altob200_clip_grads(const altob200_grad_list* list, int32_t norm_inf, double max_norm, const double* total, void* work, float* norm,
+                        void* stream);
+
+/*
  * Failure detection of the GEMM kernels.  Every mbarrier wait inside them is bounded by a wall-clock
  * limit (default 4 s); a wait that runs out records {kernel, block, site} in the status word that
  * altob200_status_read returns, and the kernel leaves through its normal teardown.

@@ -1,0 +1,143 @@
+"""Norm of many tensors and clipping by it, against 64 bits."""
+import math
+
+import pytest
+import torch
+
+from alto_b200 import grad_clip as GC
+
+pytestmark = pytest.mark.gpu
+
+
+def tensors(sizes, dtypes, seed=0, std=1e-2, gap=0):
+    """Views of one buffer per type, one behind the other (``gap``: elements between them)."""
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    for i, n in enumerate(sizes):
+        t = dtypes[i % len(dtypes)]
+        out.append((torch.randn(n + gap, generator=g) * std).to(t).cuda()[gap:])
+    return out
+
+
+def exact_norm(ts, inf):
+    if inf:
+        return max([float(t.double().abs().max()) for t in ts if t.numel()] or [0.0])
+    return math.sqrt(math.fsum(float(t.double().square().sum()) for t in ts))
+
+
+def factor(norm, most):
+    return min(1.0, most / (norm + 1e-6))
+
+
+SIZES = [[1], [7, 8, 9], [0, 3, 0], [4096 * 8, 4096 * 8 + 1, 33, 65536 * 8 - 1], [1000003], list(range(1, 400)), [5] * 2500]
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("inf", [False, True])
+@pytest.mark.parametrize("dtypes", [[BF], [F32], [BF, F32]], ids=str)
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{s[-1]}")
+@pytest.mark.parametrize("gap", [0, 1])
+def test_norm_and_clipping(sizes, dtypes, inf, gap):
+    ts = tensors(sizes, dtypes, len(sizes), gap=gap)
+    before = [t.clone() for t in ts]
+    kind = math.inf if inf else 2.0
+    exact = exact_norm(ts, inf)
+    # the root and its rounding to fp32: 2^-24 each; fp32 sums of at most 32 squares, 33 roundings of 2^-24 of the square, half of it
+    # in the root
+    near = exact * (33 / 2 + 2) * 2.0 ** -24
+    assert abs(float(GC.grad_norm(ts, kind)) - exact) <= near
+    most = exact * 0.37
+    into = [torch.full_like(t, 7.0) for t in ts]
+    norm = GC.clip_grads(ts, most, kind, out=into)
+    assert norm.dtype == F32 and norm.dim() == 0 and abs(float(norm) - exact) <= near
+    f = factor(exact, most)
+    for t, b, o in zip(ts, before, into):
+        assert torch.equal(t, b)                    # only out is written
+        want = b.double() * f
+        # norm, factor and product rounded to fp32 steps, then to the type
+        bound = want.abs() * ((33 / 2 + 6) * 2.0 ** -24 + (2.0 ** -8 if t.dtype == BF else 2.0 ** -24)) + 2.0 ** -133
+        assert bool(((o.double() - want).abs() <= bound).all())
+    again = GC.clip_grads(ts, most, kind)           # in place: the same bits
+    assert torch.equal(again, norm) and all(torch.equal(t, o) for t, o in zip(ts, into))
+    held = [t.clone() for t in ts]
+    GC.clip_grads(ts, exact * 4, kind)              # nothing to clip
+    assert all(torch.equal(t, b) for t, b in zip(ts, held))
+    copied = [torch.full_like(t, 7.0) for t in ts]
+    GC.clip_grads(ts, exact * 4, kind, out=copied)
+    assert all(torch.equal(t, b) for t, b in zip(copied, held))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("std", [1e30, 1e-30, 1e-38, 0.0])
+def test_far_from_one(std, dtype):
+    ts = [t.to(dtype) for t in tensors([70001, 13], [F32], 3, std)]
+    exact = exact_norm(ts, False)
+    got = float(GC.grad_norm(ts))
+    assert abs(got - exact) <= exact * (33 / 2 + 2) * 2.0 ** -24
+    mixed = tensors([5000], [F32], 4, 1e-3) + ts
+    exact = exact_norm(mixed, False)
+    assert abs(float(GC.grad_norm(mixed)) - exact) <= exact * (33 / 2 + 2) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+@pytest.mark.parametrize("where", [0, 3, 50000, 70000])
+def test_not_finite(where, kind, bad):
+    for dtype in (BF, F32):
+        ts = tensors([11, 70001], [dtype])
+        ts[1][where] = bad
+        norm = float(GC.grad_norm(ts, kind))
+        assert math.isnan(norm) if math.isnan(bad) else norm == math.inf
+        before = [t.clone() for t in ts]
+        with pytest.raises(RuntimeError, match="non-finite"):
+            GC.clip_grads(ts, 1.0, kind, error_if_nonfinite=True)
+        assert all(torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0)) for a, b in zip(ts, before))
+        GC.clip_grads(ts, 1.0, kind)
+        want = torch.nn.utils.clip_grads_with_norm_
+        ps = [torch.nn.Parameter(b.clone()) for b in before]
+        for p, b in zip(ps, before):
+            p.grad = b.clone()
+        want(ps, 1.0, torch.tensor(norm, device="cuda"))
+        assert all(torch.equal(a.isnan(), p.grad.isnan()) and torch.equal(a.nan_to_num(5.0), p.grad.nan_to_num(5.0)) for a, p in zip(ts, ps))
+
+
+def test_parameters_and_layouts():
+    g = torch.Generator().manual_seed(1)
+    ps = [torch.nn.Parameter(torch.randn(s, generator=g).cuda()) for s in ((64, 48), (5,), (7, 9, 11), (3, 1))]
+    grads = [torch.randn(48, 64, generator=g).cuda().t(), torch.randn(10, generator=g).cuda()[::2], torch.randn(7, 9, 22, generator=g).cuda()[..., ::2],
+             None]
+    for p, q in zip(ps, grads):
+        p.grad = q
+    before = [q.clone() for q in grads[:3]]
+    exact = exact_norm(before, False)
+    norm = GC.clip_grad_norm_(ps, 0.5)
+    assert abs(float(norm) - exact) <= exact * 19 * 2.0 ** -24
+    f = factor(exact, 0.5)
+    for p, b in zip(ps, before):
+        assert bool(((p.grad.double() - b.double() * f).abs() <= b.double().abs() * f * 25 * 2.0 ** -24).all())
+    assert float(GC.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3).cuda())], 1.0)) == 0.0
+    p = torch.nn.Parameter(torch.zeros(4).cuda())
+    p.grad = torch.full((4,), 3.0, device="cuda")
+    assert float(GC.clip_grad_norm_(p, 3.0)) == 6.0
+    assert bool(((p.grad - 1.5).abs() < 1e-5).all())
+    out = [torch.zeros(48, 64).cuda().t(), torch.zeros(64, 48).cuda()]      # other strides than the gradients'
+    src = [grads[0], grads[0]]
+    GC.clip_grads(src, 1e9, out=out)
+    assert torch.equal(out[0], src[0]) and torch.equal(out[1], src[0])
+
+
+def test_captured_and_replayed():
+    ts = tensors([70001, 5, 3000], [BF, F32])
+    into = [torch.empty_like(t) for t in ts]
+    GC.clip_grads(ts, 1.0, out=into)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = GC.clip_grads(ts, 0.1, out=into)
+    for k in range(3):
+        for t in ts:
+            t.mul_(1.5)
+        graph.replay()
+        want = [torch.empty_like(t) for t in ts]
+        n = GC.clip_grads(ts, 0.1, out=want)
+        assert torch.equal(n, norm) and all(torch.equal(a, b) for a, b in zip(into, want))
