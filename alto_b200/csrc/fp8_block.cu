@@ -565,6 +565,11 @@ int altob200_fp8_block_gemm(const altob200_fp8_block_gemm_args* a, void* stream)
   if (a->d == nullptr || (a->K > 0 && (a->a == nullptr || a->b == nullptr || a->sb.scales == nullptr || (!numbers && a->sa.scales == nullptr))))
     return ALTOB200_EINVAL_SHAPE;
   cudaStream_t st = (cudaStream_t)stream;
+  const int64_t per_run = a->mode == 1 ? ceil_div(a->M, a->experts) : a->M;
+  if (per_run > 64 || a->mode == 2) {
+    const int rc = fp8_block_gemm_tiles(a, st);
+    if (rc != ALTOB200_EUNSUPPORTED) return rc;
+  }
   Fp8bRows q;
   q.M = a->M; q.N = a->N; q.K = a->K;
   q.a = a->a; q.lda = a->lda; q.b = (const uint8_t*)a->b;
@@ -577,10 +582,9 @@ int altob200_fp8_block_gemm(const altob200_fp8_block_gemm_args* a, void* stream)
   q.out_bf16 = a->out_dtype == ALTOB200_DT_BF16;
   q.d = a->d; q.ldd = a->ldd;
   const bool e5 = a->format == ALTOB200_FMT_MXFP8_E5M2;
-  const int64_t per_expert = a->mode == 1 ? ceil_div(a->M, a->experts) : a->M;
   const bool wide = ceil_div(a->N, 32) * (a->mode == 0 ? 1 : a->experts) >= 2 * sms();
-  const int tokens = !numbers ? 32 : per_expert <= 8 ? 8 : 16;
-  int64_t y = ceil_div(per_expert, tokens);
+  const int tokens = !numbers ? 32 : per_run <= 8 ? 8 : 16;
+  int64_t y = ceil_div(per_run, tokens);
   if (y > 65535) y = 65535;
   const dim3 grid((unsigned)ceil_div(a->N, wide ? 32 : 16), (unsigned)y, (unsigned)(a->mode == 1 ? a->experts + 1 : q.experts));
   cudaError_t rc;

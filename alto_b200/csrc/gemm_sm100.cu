@@ -1402,6 +1402,7 @@ gemm_blockscaled_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const _
 }
 
 #include "gemm_macro.cuh"
+#include "gemm_fp8_block.cuh"
 
 // ---------------------------------------------------------------------------------------
 // self-test of the bounded waits: every form on barriers that are complete and on one that nobody arrives on
@@ -1879,6 +1880,83 @@ static int gemm_macro_common(int64_t M, int64_t N, int64_t K, int32_t num_expert
   cudaStream_t st = (cudaStream_t)stream;
   if (!b_uniform) return launch_gemm_macro<128, false>(ta, tb, td, m, grid, st);
   return BN == 128 ? launch_gemm_macro<128, true>(ta, tb, td, m, grid, st) : launch_gemm_macro<192, true>(ta, tb, td, m, grid, st);
+}
+
+// Products in FP8 with one fp32 scale for each block of 128; EUNSUPPORTED: not for this kernel (fp8_block.cu has the other).
+template <bool OUT_BF16, bool B_ROWS>
+static int launch_fp8_block(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td, const F8Args& args, int64_t tiles,
+                            cudaStream_t st) {
+  using C = CfgF8;
+  static std::atomic<int> clusters_of[MAX_DEVICES];  // 0 = not asked yet, < 0 = the device cannot run the kernel
+  auto kernel = gemm_fp8_block_kernel<OUT_BF16, B_ROWS>;
+  const int dev = current_device();
+  int max_clusters = dev >= 0 ? clusters_of[dev].load(std::memory_order_relaxed) : 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see launch_after()
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.blockDim = dim3(C::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  if (max_clusters == 0) {
+    cudaFuncAttributes fa;
+    ALTOB200_CUDA_CHECK(cudaFuncGetAttributes(&fa, kernel));
+    ALTOB200_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+    cfg.gridDim = dim3(2 * (unsigned)sm_count_gemm(), 1, 1);
+    int n = 0;
+    // (the fold warps wait for registers that a launch with fewer would not have)
+    if (fa.numRegs < C::REGS_LAUNCH || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      max_clusters = -1;
+    } else {
+      max_clusters = n;
+    }
+    if (dev >= 0) clusters_of[dev].store(max_clusters, std::memory_order_relaxed);
+  }
+  if (max_clusters < 0) return ALTOB200_EUNSUPPORTED;
+  const int64_t clusters = tiles < max_clusters ? tiles : max_clusters;
+  cfg.gridDim = dim3((unsigned)(2 * clusters), 1, 1);
+  return cudaLaunchKernelEx(&cfg, kernel, ta, tb, td, args) == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
+}
+
+int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st) {
+  const bool b_rows = a->sb.row_shift == 0;
+  if (a->a_dtype != -1 || a->K <= 0) return ALTOB200_EUNSUPPORTED;
+  if (b_rows && (a->sb.row_stride != 1 || a->sb.chunk_stride % 4 != 0 || a->mode == 1 || (reinterpret_cast<uintptr_t>(a->sb.scales) & 15)))
+    return ALTOB200_EUNSUPPORTED;
+  const int64_t runs = a->mode == 0 ? 0 : a->experts, units = ceil_div(a->M, 256) + (a->mode == 1 ? runs + 1 : 0);
+  if (a->mode != 0 && (runs + 2 > CfgF8::MAX_RUNS || units > CfgF8::MAX_UNITS)) return ALTOB200_EUNSUPPORTED;
+  const int64_t tiles_n = ceil_div(a->N, CfgF8::BN), tiles = units * tiles_n * (a->mode == 2 ? runs : 1);
+  const int64_t b_rows_total = a->N * (a->mode == 1 ? runs : 1);
+  if (tiles >= (1ll << 31) || b_rows_total >= (1ll << 31)) return ALTOB200_EUNSUPPORTED;
+  CUtensorMap ta, tb, td;
+  int rc = make_tmap(&ta, a->a, a->M, a->K, BM);
+  if (rc != ALTOB200_OK) return rc;
+  rc = make_tmap(&tb, a->b, b_rows_total, a->K, CfgF8::BN / 2);
+  if (rc != ALTOB200_OK) return rc;
+  const bool obf = a->out_dtype == ALTOB200_DT_BF16;
+  rc = make_tmap_out(&td, a->d, a->mode == 2 ? runs : 1, a->M, a->N, a->ldd, obf, 128);
+  if (rc != ALTOB200_OK) return rc;
+  F8Args g;
+  g.M = a->M; g.N = a->N; g.K = a->K;
+  g.sa = a->sa.scales; g.sa_row = a->sa.row_stride; g.sa_chunk = a->sa.chunk_stride; g.sa_shift = a->sa.row_shift;
+  g.sb = a->sb.scales; g.sb_row = a->sb.row_stride; g.sb_chunk = a->sb.chunk_stride; g.sb_expert = a->mode == 1 ? a->sb.expert_stride : 0;
+  g.offs = a->offs; g.mode = a->mode; g.experts = a->mode == 0 ? 1 : a->experts; g.k_rows = a->k_rows;
+  g.d = a->d; g.ldd = a->ldd;
+  g.tiles_n = (int)tiles_n;
+  g.group_m = 4;
+  const uint32_t f = a->format == ALTOB200_FMT_MXFP8_E5M2 ? 1u : 0u;
+  // fp32 sums [4, 6), formats of A and B [7, 10) and [10, 13), n / 8 [17, 23), m / 16 [24, 29)
+  g.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)(CfgF8::BN >> 3) << 17) | ((uint32_t)(2 * BM >> 4) << 24);
+  g.wait_ns = wait_limit_ns();
+  if (obf) return b_rows ? launch_fp8_block<true, true>(ta, tb, td, g, tiles, st) : launch_fp8_block<true, false>(ta, tb, td, g, tiles, st);
+  return b_rows ? launch_fp8_block<false, true>(ta, tb, td, g, tiles, st) : launch_fp8_block<false, false>(ta, tb, td, g, tiles, st);
 }
 
 }  // namespace altob200
