@@ -1932,13 +1932,19 @@ int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st)
     return ALTOB200_EUNSUPPORTED;
   const int64_t runs = a->mode == 0 ? 0 : a->experts, units = ceil_div(a->M, 256) + (a->mode == 1 ? runs + 1 : 0);
   if (a->mode != 0 && (runs + 2 > CfgF8::MAX_RUNS || units > CfgF8::MAX_UNITS)) return ALTOB200_EUNSUPPORTED;
+  // places of the scales fit in 31 bits
+  const int64_t chunks = ceil_div(a->K, 128), last_a = ((a->M - 1) >> a->sa.row_shift) * a->sa.row_stride + chunks * a->sa.chunk_stride;
+  const int64_t last_b = (a->mode == 1 ? runs * a->sb.expert_stride : 0) + ((a->N - 1) >> 7) * a->sb.row_stride + chunks * a->sb.chunk_stride;
+  if (a->sa.row_stride < 0 || a->sa.chunk_stride < 0 || a->sb.row_stride < 0 || a->sb.chunk_stride < 0 || a->sb.expert_stride < 0 ||
+      last_a >= (1ll << 31) || (!b_rows && last_b >= (1ll << 31)))
+    return ALTOB200_EUNSUPPORTED;
   const int64_t tiles_n = ceil_div(a->N, CfgF8::BN), tiles = units * tiles_n * (a->mode == 2 ? runs : 1);
   const int64_t b_rows_total = a->N * (a->mode == 1 ? runs : 1);
   if (tiles >= (1ll << 31) || b_rows_total >= (1ll << 31)) return ALTOB200_EUNSUPPORTED;
   CUtensorMap ta, tb, td;
   int rc = make_tmap(&ta, a->a, a->M, a->K, BM);
   if (rc != ALTOB200_OK) return rc;
-  rc = make_tmap(&tb, a->b, b_rows_total, a->K, CfgF8::BN / 2);
+  rc = make_tmap(&tb, a->b, b_rows_total, a->K, CfgF8::BN / 4);
   if (rc != ALTOB200_OK) return rc;
   const bool obf = a->out_dtype == ALTOB200_DT_BF16;
   rc = make_tmap_out(&td, a->d, a->mode == 2 ? runs : 1, a->M, a->N, a->ldd, obf, 128);
@@ -1953,7 +1959,7 @@ int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st)
   g.group_m = 4;
   const uint32_t f = a->format == ALTOB200_FMT_MXFP8_E5M2 ? 1u : 0u;
   // fp32 sums [4, 6), formats of A and B [7, 10) and [10, 13), n / 8 [17, 23), m / 16 [24, 29)
-  g.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)(CfgF8::BN >> 3) << 17) | ((uint32_t)(2 * BM >> 4) << 24);
+  g.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)((CfgF8::BN / 2) >> 3) << 17) | ((uint32_t)(2 * BM >> 4) << 24);
   g.wait_ns = wait_limit_ns();
   if (obf) return b_rows ? launch_fp8_block<true, true>(ta, tb, td, g, tiles, st) : launch_fp8_block<true, false>(ta, tb, td, g, tiles, st);
   return b_rows ? launch_fp8_block<false, true>(ta, tb, td, g, tiles, st) : launch_fp8_block<false, false>(ta, tb, td, g, tiles, st);
