@@ -26,11 +26,26 @@ struct Fp8bQuant {
 };
 enum { FP8B_ROWS = 1, FP8B_COLS = 2, FP8B_SQUARES = 4 };
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// Maxima of two non-negative bf16 a word, by their bits (a NaN is above an infinity).
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// 8 x 8 numbers of a thread, and maxima of their magnitudes in a form that packs: two to a word from bf16, whose bits order
+// them, or one fp32 a word.
 template <class T>
 struct Fp8bTile;
 template <>
 struct Fp8bTile<__nv_bfloat16> {
   static constexpr bool BF16 = true;
+  static constexpr int WORDS = 4;      // of eight maxima
   uint4 v[8];
   __device__ __forceinline__ void load(int i, const void* base, int64_t at) { v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + at)); }
   __device__ __forceinline__ void zero(int i) { v[i] = make_uint4(0, 0, 0, 0); }
@@ -38,10 +53,36 @@ struct Fp8bTile<__nv_bfloat16> {
     const uint32_t w = (&v[i].x)[j >> 1];
     return (j & 1) ? bf16hi_to_f32(w) : bf16lo_to_f32(w);
   }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return max_halves(a, b); }
+  // words of eight rows' maxima over this thread's columns, of eight columns' over its rows
+  __device__ __forceinline__ void maxima(uint32_t (&rows)[4], uint32_t (&cols)[4], bool want_rows, bool want_cols) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) rows[j] = cols[j] = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m = 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w = (&v[i].x)[j] & 0x7FFF7FFFu;
+        if (want_rows) m = max_halves(m, w);
+        if (want_cols) cols[j] = max_halves(cols[j], w);
+      }
+      if (want_rows) {      // both halves in one, rows 2 k and 2 k + 1 a word
+        m = max_halves(m, __byte_perm(m, 0, 0x1032));
+        rows[i >> 1] = (i & 1) ? __byte_perm(rows[i >> 1], m, 0x5410) : m;
+      }
+    }
+  }
+  static __device__ __forceinline__ float value(uint32_t w, int half) { return half ? bf16hi_to_f32(w) : bf16lo_to_f32(w); }
+  static __device__ __forceinline__ float whole(const uint32_t (&w)[4]) {
+    const uint32_t m = max_halves(max_halves(w[0], w[1]), max_halves(w[2], w[3]));
+    return max_nan(bf16lo_to_f32(m), bf16hi_to_f32(m));
+  }
 };
 template <>
 struct Fp8bTile<float> {
   static constexpr bool BF16 = false;
+  static constexpr int WORDS = 8;
   float4 v[8][2];
   __device__ __forceinline__ void load(int i, const void* base, int64_t at) {
     const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
@@ -50,12 +91,66 @@ struct Fp8bTile<float> {
   }
   __device__ __forceinline__ void zero(int i) { v[i][0] = v[i][1] = make_float4(0, 0, 0, 0); }
   __device__ __forceinline__ float get(int i, int j) const { return (&v[i][j >> 2].x)[j & 3]; }
+  static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return a > b ? a : b; }      // magnitudes' bits
+  __device__ __forceinline__ void maxima(uint32_t (&rows)[8], uint32_t (&cols)[8], bool want_rows, bool want_cols) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) rows[j] = cols[j] = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (want_rows) {
+        float m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) m = absmax3_nan(m, get(i, j), get(i, j + 1));
+        rows[i] = f2u(m) & 0x7FFFFFFFu;
+      }
+    }
+    if (want_cols)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) m = absmax3_nan(m, get(i, j), get(i + 1, j));
+        cols[j] = f2u(m) & 0x7FFFFFFFu;
+      }
+  }
+  static __device__ __forceinline__ float value(uint32_t w, int) { return u2f(w); }
+  static __device__ __forceinline__ float whole(const uint32_t (&w)[8]) {
+    float m = u2f(w[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = max_nan(m, u2f(w[i]));
+    return m;
+  }
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
+// x / s of two numbers of one block in packed arithmetic (the roundings of div_bf16_num and div_f32_num).
+template <bool BF16>
+__device__ __forceinline__ float2 fp8b_quotients(float a, float b, float s, float r) {
+  const float2 x = make_float2(a, b), s2 = make_float2(s, s), n2 = make_float2(-r, -r), m2 = make_float2(-a, -b);
+  float2 y = __fmul2_rn(x, make_float2(r, r));
+  if (!BF16) y = __ffma2_rn(n2, __ffma2_rn(y, s2, m2), y);
+  return __ffma2_rn(n2, __ffma2_rn(y, s2, m2), y);
+}
+// The codes of four numbers of one block as a word.
+template <bool BF16, bool E5M2>
+__device__ __forceinline__ uint32_t fp8b_word(float a, float b, float c, float d, float2 f, bool fast) {
+  float2 p, q;
+  if (fast) {
+    p = fp8b_quotients<BF16>(a, b, f.x, f.y);
+    q = fp8b_quotients<BF16>(c, d, f.x, f.y);
+  } else {
+    p = make_float2(__fdiv_rn(a, f.x), __fdiv_rn(b, f.x));
+    q = make_float2(__fdiv_rn(c, f.x), __fdiv_rn(d, f.x));
+  }
+  uint32_t w;
+  if (E5M2)
+    asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e5m2x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e5m2x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(w) : "f"(p.x), "f"(p.y), "f"(q.x), "f"(q.y));
+  else
+    asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(w) : "f"(p.x), "f"(p.y), "f"(q.x), "f"(q.y));
+  return w;
 }
 
 // Four words whose bytes are four rows -> four words whose bytes are four columns.
@@ -98,77 +193,69 @@ __global__ void __launch_bounds__(256) fp8b_quantize_kernel(const Fp8bQuant q) {
     else t.zero(i);
   }
   // largest magnitudes
-  float rm[8], cm[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) rm[i] = cm[i] = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = fabsf(t.get(i, j));
-      if (R || S) rm[i] = max_nan(rm[i], a);
-      if (C) cm[j] = max_nan(cm[j], a);
-    }
+  using Tile = Fp8bTile<T>;
+  constexpr int W = Tile::WORDS;
+  uint32_t rm[W], cm[W];
+  t.maxima(rm, cm, R || S, C);
   if (S) {
-    float m = rm[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) m = max_nan(m, rm[i]);
+    float m = Tile::whole(rm);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
     if (lane == 0) whole[warp] = m;
   }
   if (R) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < W; ++i)
 #pragma unroll
-      for (int d = 1; d < 8; d <<= 1) rm[i] = max_nan(rm[i], __shfl_xor_sync(0xFFFFFFFFu, rm[i], d));
+      for (int d = 1; d < 8; d <<= 1) rm[i] = Tile::most(rm[i], __shfl_xor_sync(0xFFFFFFFFu, rm[i], d));
     if ((lane & 7) == 0)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) row_max[warp >> 2][r_in + i] = rm[i];
+      for (int i = 0; i < 8; ++i) row_max[warp >> 2][r_in + i] = Tile::value(rm[i * W / 8], i & 1);
   }
   if (C) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < W; ++j)
 #pragma unroll
-      for (int d = 8; d < 32; d <<= 1) cm[j] = max_nan(cm[j], __shfl_xor_sync(0xFFFFFFFFu, cm[j], d));
+      for (int d = 8; d < 32; d <<= 1) cm[j] = Tile::most(cm[j], __shfl_xor_sync(0xFFFFFFFFu, cm[j], d));
     if (lane < 8)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) col_max[warp & 3][c_in + j] = cm[j];
+      for (int j = 0; j < 8; ++j) col_max[warp & 3][c_in + j] = Tile::value(cm[j * W / 8], j & 1);
   }
   __syncthreads();
+  // scales, a thread each; whether the reciprocal form serves them all
+  bool fast = true;
   if (S) {
     if (threadIdx.x == 0) {
       float m = whole[0];
       for (int w = 1; w < 8; ++w) m = max_nan(m, whole[w]);
       const float s = fp8b_scale<E5M2>(m);
       row_f[0] = make_float2(s, __frcp_rn(s));
+      fast = div_fast_ok(s);
       q.row_scales[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = s;
     }
   } else if (threadIdx.x < 128) {
     if (R) {
       const float s = fp8b_scale<E5M2>(max_nan(row_max[0][threadIdx.x], row_max[1][threadIdx.x]));
       row_f[threadIdx.x] = make_float2(s, __frcp_rn(s));
+      fast = div_fast_ok(s);
       if (row0 + (int)threadIdx.x < row_end) q.row_scales[(int64_t)blockIdx.x * q.rows + row0 + threadIdx.x] = s;
     }
   } else if (C) {
     const int c = (int)threadIdx.x - 128;
     const float s = fp8b_scale<E5M2>(max_nan(max_nan(col_max[0][c], col_max[1][c]), max_nan(col_max[2][c], col_max[3][c])));
     col_f[c] = make_float2(s, __frcp_rn(s));
+    fast = div_fast_ok(s);
     if (col0 + c < q.cols) q.col_scales[chunk * q.cols + col0 + c] = s;
   }
-  __syncthreads();
+  fast = __syncthreads_and(fast);
   if (col >= q.cols) return;
   if (R || S) {
     uint2 words[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 f = row_f[S ? 0 : r_in + i];
-      const bool fast = div_fast_ok(f.x);
-      uint32_t p[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        p[j] = fp8x2_rtn_hw<E5M2>(fp8b_quotient<BF16>(t.get(i, 2 * j), f.x, f.y, fast), fp8b_quotient<BF16>(t.get(i, 2 * j + 1), f.x, f.y, fast));
-      words[i] = make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
+      words[i].x = fp8b_word<BF16, E5M2>(t.get(i, 0), t.get(i, 1), t.get(i, 2), t.get(i, 3), f, fast);
+      words[i].y = fp8b_word<BF16, E5M2>(t.get(i, 4), t.get(i, 5), t.get(i, 6), t.get(i, 7), f, fast);
       const int64_t r = (int64_t)row0 + r_in + i;
       if (q.row_codes != nullptr && r < row_end)
         *reinterpret_cast<uint2*>(q.row_codes + ((S ? (int64_t)blockIdx.z * q.rows : 0) + r) * q.cols + col) = words[i];
@@ -189,21 +276,14 @@ __global__ void __launch_bounds__(256) fp8b_quantize_kernel(const Fp8bQuant q) {
     }
   }
   if (C) {
-    uint32_t lo[8], hi[8];      // per column: codes of rows 0-3 and 4-7
+    uint8_t* const out = q.col_codes + col * q.ld_col + chunk * 128 + r_in;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float2 f = col_f[c_in + j];
-      const bool fast = div_fast_ok(f.x);
-      uint32_t p[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        p[i] = fp8x2_rtn_hw<E5M2>(fp8b_quotient<BF16>(t.get(2 * i, j), f.x, f.y, fast), fp8b_quotient<BF16>(t.get(2 * i + 1, j), f.x, f.y, fast));
-      lo[j] = p[0] | (p[1] << 16);
-      hi[j] = p[2] | (p[3] << 16);
+      *reinterpret_cast<uint2*>(out + j * q.ld_col) =
+          make_uint2(fp8b_word<BF16, E5M2>(t.get(0, j), t.get(1, j), t.get(2, j), t.get(3, j), f, fast),
+                     fp8b_word<BF16, E5M2>(t.get(4, j), t.get(5, j), t.get(6, j), t.get(7, j), f, fast));
     }
-    uint8_t* const out = q.col_codes + col * q.ld_col + chunk * 128 + r_in;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) *reinterpret_cast<uint2*>(out + j * q.ld_col) = make_uint2(lo[j], hi[j]);
   }
 }
 
