@@ -122,37 +122,6 @@ struct Fp8bTile<float> {
   }
 };
 
-// x / s of two numbers of one block in packed arithmetic (the roundings of div_bf16_num and div_f32_num).
-template <bool BF16>
-__device__ __forceinline__ float2 fp8b_quotients(float a, float b, float s, float r) {
-  const float2 x = make_float2(a, b), s2 = make_float2(s, s), n2 = make_float2(-r, -r), m2 = make_float2(-a, -b);
-  float2 y = __fmul2_rn(x, make_float2(r, r));
-  if (!BF16) y = __ffma2_rn(n2, __ffma2_rn(y, s2, m2), y);
-  return __ffma2_rn(n2, __ffma2_rn(y, s2, m2), y);
-}
-// The codes of four numbers of one block as a word.
-template <bool BF16, bool E5M2>
-__device__ __forceinline__ uint32_t fp8b_word(float a, float b, float c, float d, float2 f, bool fast) {
-  float2 p, q;
-  if (fast) {
-    p = fp8b_quotients<BF16>(a, b, f.x, f.y);
-    q = fp8b_quotients<BF16>(c, d, f.x, f.y);
-  } else {
-    p = make_float2(__fdiv_rn(a, f.x), __fdiv_rn(b, f.x));
-    q = make_float2(__fdiv_rn(c, f.x), __fdiv_rn(d, f.x));
-  }
-  uint32_t w;
-  if (E5M2)
-    asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e5m2x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e5m2x2.f32 hi, %4, %3;\n\t"
-        "mov.b32 %0, {lo, hi};\n\t}"
-        : "=r"(w) : "f"(p.x), "f"(p.y), "f"(q.x), "f"(q.y));
-  else
-    asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
-        "mov.b32 %0, {lo, hi};\n\t}"
-        : "=r"(w) : "f"(p.x), "f"(p.y), "f"(q.x), "f"(q.y));
-  return w;
-}
-
 // Four words whose bytes are four rows -> four words whose bytes are four columns.
 __device__ __forceinline__ void transpose4(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
   const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab1 = __byte_perm(a, b, 0x7362);
@@ -163,11 +132,54 @@ __device__ __forceinline__ void transpose4(uint32_t& a, uint32_t& b, uint32_t& c
   d = __byte_perm(ab1, cd1, 0x7632);
 }
 
+// The codes of a thread's 8 x 8 numbers, along their rows and / or columns, and where they go.
+template <class T, int WHAT, bool E5M2>
+__device__ __forceinline__ void fp8b_emit(const Fp8bQuant& q, const Fp8bTile<T>& t, const float2* row_f, const float2* col_f, int row0, int row_end,
+                                          int r_in, int c_in, int64_t col, int64_t chunk) {
+  constexpr bool BF16 = Fp8bTile<T>::BF16;
+  constexpr bool R = (WHAT & FP8B_ROWS) != 0, C = (WHAT & FP8B_COLS) != 0, S = (WHAT & FP8B_SQUARES) != 0;
+  if (R || S) {
+    uint2 words[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = row_f[S ? 0 : r_in + i];
+      words[i].x = fp8b_word<BF16, E5M2>(t.get(i, 0), t.get(i, 1), t.get(i, 2), t.get(i, 3), f);
+      words[i].y = fp8b_word<BF16, E5M2>(t.get(i, 4), t.get(i, 5), t.get(i, 6), t.get(i, 7), f);
+      const int64_t r = (int64_t)row0 + r_in + i;
+      if (q.row_codes != nullptr && r < row_end)
+        *reinterpret_cast<uint2*>(q.row_codes + ((S ? (int64_t)blockIdx.z * q.rows : 0) + r) * q.cols + col) = words[i];
+    }
+    if (S && q.col_codes != nullptr) {
+      // (rows are a multiple of 16, so that a thread's eight are inside or outside together)
+      if (row0 + r_in < row_end) {
+        uint8_t* const out = q.col_codes + ((int64_t)blockIdx.z * q.cols + col) * q.ld_col + row0 + r_in;
+        transpose4(words[0].x, words[1].x, words[2].x, words[3].x);
+        transpose4(words[0].y, words[1].y, words[2].y, words[3].y);
+        transpose4(words[4].x, words[5].x, words[6].x, words[7].x);
+        transpose4(words[4].y, words[5].y, words[6].y, words[7].y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint2*>(out + j * q.ld_col) =
+              j < 4 ? make_uint2(words[j].x, words[j + 4].x) : make_uint2(words[j - 4].y, words[j].y);
+      }
+    }
+  }
+  if (C) {
+    uint8_t* const out = q.col_codes + col * q.ld_col + chunk * 128 + r_in;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 f = col_f[c_in + j];
+      *reinterpret_cast<uint2*>(out + j * q.ld_col) =
+          make_uint2(fp8b_word<BF16, E5M2>(t.get(0, j), t.get(1, j), t.get(2, j), t.get(3, j), f),
+                     fp8b_word<BF16, E5M2>(t.get(4, j), t.get(5, j), t.get(6, j), t.get(7, j), f));
+    }
+  }
+}
+
 // A tile of 128 rows x 128 columns a CTA (256 threads), 8 x 8 numbers a thread, a warp 32 rows x 64 columns: a row's part of a
 // warp is 128 bytes of bf16, a column's 32 bytes of codes.
 template <class T, int WHAT, bool E5M2>
-__global__ void __launch_bounds__(256) fp8b_quantize_kernel(const Fp8bQuant q) {
-  constexpr bool BF16 = Fp8bTile<T>::BF16;
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? (WHAT == (FP8B_ROWS | FP8B_COLS) ? 3 : 4) : 2) fp8b_quantize_kernel(const Fp8bQuant q) {
   constexpr bool R = (WHAT & FP8B_ROWS) != 0, C = (WHAT & FP8B_COLS) != 0, S = (WHAT & FP8B_SQUARES) != 0;
   __shared__ float row_max[2][128], col_max[4][128], whole[8];
   __shared__ float2 row_f[128], col_f[128];      // scale and its reciprocal
@@ -222,67 +234,84 @@ __global__ void __launch_bounds__(256) fp8b_quantize_kernel(const Fp8bQuant q) {
       for (int j = 0; j < 8; ++j) col_max[warp & 3][c_in + j] = Tile::value(cm[j * W / 8], j & 1);
   }
   __syncthreads();
-  // scales, a thread each; whether the reciprocal form serves them all
-  bool fast = true;
+  // scales, a thread each
   if (S) {
     if (threadIdx.x == 0) {
       float m = whole[0];
       for (int w = 1; w < 8; ++w) m = max_nan(m, whole[w]);
       const float s = fp8b_scale<E5M2>(m);
-      row_f[0] = make_float2(s, __frcp_rn(s));
-      fast = div_fast_ok(s);
+      row_f[0] = fp8b_divisor(s);
       q.row_scales[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = s;
     }
   } else if (threadIdx.x < 128) {
     if (R) {
       const float s = fp8b_scale<E5M2>(max_nan(row_max[0][threadIdx.x], row_max[1][threadIdx.x]));
-      row_f[threadIdx.x] = make_float2(s, __frcp_rn(s));
-      fast = div_fast_ok(s);
+      row_f[threadIdx.x] = fp8b_divisor(s);
       if (row0 + (int)threadIdx.x < row_end) q.row_scales[(int64_t)blockIdx.x * q.rows + row0 + threadIdx.x] = s;
     }
   } else if (C) {
     const int c = (int)threadIdx.x - 128;
     const float s = fp8b_scale<E5M2>(max_nan(max_nan(col_max[0][c], col_max[1][c]), max_nan(col_max[2][c], col_max[3][c])));
-    col_f[c] = make_float2(s, __frcp_rn(s));
-    fast = div_fast_ok(s);
+    col_f[c] = fp8b_divisor(s);
     if (col0 + c < q.cols) q.col_scales[chunk * q.cols + col0 + c] = s;
   }
-  fast = __syncthreads_and(fast);
+  __syncthreads();
   if (col >= q.cols) return;
-  if (R || S) {
-    uint2 words[8];
+  fp8b_emit<T, WHAT, E5M2>(q, t, row_f, col_f, row0, row_end, r_in, c_in, col, chunk);
+}
+
+// Rows alone: eight lanes a block of 128, sixteen numbers a lane, no shared memory; a warp four rows, two blocks of each.
+template <class T, bool E5M2>
+__global__ void __launch_bounds__(256) fp8b_quantize_rows_kernel(const Fp8bQuant q) {
+  constexpr bool BF16 = sizeof(T) == 2;
+  constexpr int U = 2;
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t col0 = (int64_t)blockIdx.x * (128 * U) + (lane & 7) * 16;
+  for (int64_t at = blockIdx.y; at * 32 < q.rows; at += gridDim.y) {
+    const int64_t row = at * 32 + (threadIdx.x >> 5) * 4 + (lane >> 3);
+    const T* const x = static_cast<const T*>(q.x) + row * q.ld + col0;
+    float v[U][16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 f = row_f[S ? 0 : r_in + i];
-      words[i].x = fp8b_word<BF16, E5M2>(t.get(i, 0), t.get(i, 1), t.get(i, 2), t.get(i, 3), f, fast);
-      words[i].y = fp8b_word<BF16, E5M2>(t.get(i, 4), t.get(i, 5), t.get(i, 6), t.get(i, 7), f, fast);
-      const int64_t r = (int64_t)row0 + r_in + i;
-      if (q.row_codes != nullptr && r < row_end)
-        *reinterpret_cast<uint2*>(q.row_codes + ((S ? (int64_t)blockIdx.z * q.rows : 0) + r) * q.cols + col) = words[i];
-    }
-    if (S && q.col_codes != nullptr) {
-      // (rows are a multiple of 16, so that a thread's eight are inside or outside together)
-      if (row0 + r_in < row_end) {
-        uint8_t* const out = q.col_codes + ((int64_t)blockIdx.z * q.cols + col) * q.ld_col + row0 + r_in;
-        transpose4(words[0].x, words[1].x, words[2].x, words[3].x);
-        transpose4(words[0].y, words[1].y, words[2].y, words[3].y);
-        transpose4(words[4].x, words[5].x, words[6].x, words[7].x);
-        transpose4(words[4].y, words[5].y, words[6].y, words[7].y);
+    for (int u = 0; u < U; ++u) {
+      const bool in = row < q.rows && col0 + 128 * u < q.cols;      // (columns come in sixteens)
+      if (BF16) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          *reinterpret_cast<uint2*>(out + j * q.ld_col) =
-              j < 4 ? make_uint2(words[j].x, words[j + 4].x) : make_uint2(words[j - 4].y, words[j].y);
+        for (int k = 0; k < 2; ++k) {
+          const uint4 w = in ? __ldg(reinterpret_cast<const uint4*>(x + 128 * u) + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[u][8 * k + 2 * j] = bf16lo_to_f32((&w.x)[j]);
+            v[u][8 * k + 2 * j + 1] = bf16hi_to_f32((&w.x)[j]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 w = in ? __ldg(reinterpret_cast<const float4*>(x + 128 * u) + k) : make_float4(0, 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[u][4 * k + j] = (&w.x)[j];
+        }
       }
     }
-  }
-  if (C) {
-    uint8_t* const out = q.col_codes + col * q.ld_col + chunk * 128 + r_in;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 f = col_f[c_in + j];
-      *reinterpret_cast<uint2*>(out + j * q.ld_col) =
-          make_uint2(fp8b_word<BF16, E5M2>(t.get(0, j), t.get(1, j), t.get(2, j), t.get(3, j), f, fast),
-                     fp8b_word<BF16, E5M2>(t.get(4, j), t.get(5, j), t.get(6, j), t.get(7, j), f, fast));
+    for (int u = 0; u < U; ++u) {
+      float m = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) m = absmax3_nan(m, v[u][j], v[u][j + 1]);
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+      const float s = fp8b_scale<E5M2>(m);
+      const float2 f = fp8b_divisor(s);
+      uint4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        (&w.x)[j] = fp8b_word<BF16, E5M2>(v[u][4 * j], v[u][4 * j + 1], v[u][4 * j + 2], v[u][4 * j + 3], f);
+      const int64_t col = col0 + 128 * u;
+      if (row < q.rows && col < q.cols) {
+        *reinterpret_cast<uint4*>(q.row_codes + row * q.cols + col) = w;
+        if ((lane & 7) == 0) q.row_scales[((int64_t)blockIdx.x * U + u) * q.rows + row] = s;
+      }
     }
   }
 }
@@ -398,15 +427,14 @@ __device__ __forceinline__ float fp8b_row_codes(const T* row, int64_t k, int64_t
   for (int j = 0; j < 16; ++j) m = absmax3_nan(m, v[2 * j], v[2 * j + 1]);
   m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
   m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-  const float s = fp8b_scale<E5M2>(m), r = __frcp_rn(s);
-  const bool fast = __all_sync(0xFFFFFFFFu, div_fast_ok(s));
+  const float s = fp8b_scale<E5M2>(m);
+  const float2 f = fp8b_divisor(s);
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float* x = v + 16 * h + 4 * j;
-      (&w[h].x)[j] = fp8x2_rtn_hw<E5M2>(fp8b_quotient<BF16>(x[0], s, r, fast), fp8b_quotient<BF16>(x[1], s, r, fast)) |
-                     (fp8x2_rtn_hw<E5M2>(fp8b_quotient<BF16>(x[2], s, r, fast), fp8b_quotient<BF16>(x[3], s, r, fast)) << 16);
+      (&w[h].x)[j] = fp8b_word<BF16, E5M2>(x[0], x[1], x[2], x[3], f);
     }
   return s;
 }
@@ -564,25 +592,31 @@ int altob200_fp8_block_quantize(const altob200_fp8_block_quant_args* a, void* st
     return ALTOB200_EINVAL_ALIGN;
   const int64_t chunks = a->offs != nullptr ? a->rows / 128 + a->experts : ceil_div(a->rows, 128);
   if (a->col_codes != nullptr && a->ld_col < chunks * 128) return ALTOB200_EINVAL_SHAPE;
-  if (a->rows >= (1ll << 30) || chunks > 65535ll * 128) return ALTOB200_ELIMIT;
+  if (a->rows >= (1ll << 30)) return ALTOB200_ELIMIT;
   if (a->rows == 0) return ALTOB200_OK;
   if (a->x == nullptr) return ALTOB200_EINVAL_SHAPE;
-  if (chunks > 65535) return ALTOB200_ELIMIT;
+  if (chunks > 65535 && a->col_codes != nullptr) return ALTOB200_ELIMIT;
   Fp8bQuant q = {a->x, a->rows, a->cols, a->ld, a->offs, a->experts, (uint8_t*)a->row_codes, a->row_scales, (uint8_t*)a->col_codes, a->ld_col,
                  a->col_scales, 0};
-  const dim3 grid((unsigned)ceil_div(a->cols, 128), (unsigned)chunks);
+  const dim3 grid((unsigned)ceil_div(a->cols, 128), (unsigned)(chunks < 65535 ? chunks : 65535));
   const bool e5 = a->format == ALTOB200_FMT_MXFP8_E5M2;
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t rc;
 #define ALTOB200_Q(T, W) \
   rc = e5 ? launch_after(fp8b_quantize_kernel<T, W, true>, grid, dim3(256), 0, st, q) : launch_after(fp8b_quantize_kernel<T, W, false>, grid, dim3(256), 0, st, q)
-  if (a->dtype == ALTOB200_DT_BF16) {
-    if (a->col_codes == nullptr) { ALTOB200_Q(__nv_bfloat16, FP8B_ROWS); }
-    else if (a->row_codes == nullptr) { ALTOB200_Q(__nv_bfloat16, FP8B_COLS); }
+  if (a->col_codes == nullptr) {
+    const int64_t groups = ceil_div(a->rows, 32);
+    const dim3 g((unsigned)ceil_div(a->cols, 256), (unsigned)(groups < 65535 ? groups : 65535));
+#define ALTOB200_QR(T) \
+  rc = e5 ? launch_after(fp8b_quantize_rows_kernel<T, true>, g, dim3(256), 0, st, q) : launch_after(fp8b_quantize_rows_kernel<T, false>, g, dim3(256), 0, st, q)
+    if (a->dtype == ALTOB200_DT_BF16) { ALTOB200_QR(__nv_bfloat16); }
+    else { ALTOB200_QR(float); }
+#undef ALTOB200_QR
+  } else if (a->dtype == ALTOB200_DT_BF16) {
+    if (a->row_codes == nullptr) { ALTOB200_Q(__nv_bfloat16, FP8B_COLS); }
     else { ALTOB200_Q(__nv_bfloat16, (FP8B_ROWS | FP8B_COLS)); }
   } else {
-    if (a->col_codes == nullptr) { ALTOB200_Q(float, FP8B_ROWS); }
-    else if (a->row_codes == nullptr) { ALTOB200_Q(float, FP8B_COLS); }
+    if (a->row_codes == nullptr) { ALTOB200_Q(float, FP8B_COLS); }
     else { ALTOB200_Q(float, (FP8B_ROWS | FP8B_COLS)); }
   }
   return rc == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;

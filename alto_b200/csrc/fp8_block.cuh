@@ -18,11 +18,34 @@ __device__ __forceinline__ float fp8b_scale(float amax) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(amax), "f"(FP8B_LEAST));
   return __fdiv_rn(a, E5M2 ? 57344.0f : 448.0f);
 }
-// x / s; r = RN(1 / s), fast: s within the range of the reciprocal forms (common.cuh)
+// What the quotients by a scale take: (s, RN(1 / s)).  The reciprocal forms of common.cuh hold for every scale there is, 2^-56 to
+// 2^120: a quotient that any code but zero stands for keeps its residual normal, and one below that may be off.  Behind an
+// infinite scale every number but the infinities and NaN has quotient zero, which (0, 0) gives.
+__device__ __forceinline__ float2 fp8b_divisor(float s) {
+  return s == __int_as_float(0x7F800000) ? make_float2(0.0f, 0.0f) : make_float2(s, __frcp_rn(s));
+}
+// x / s of two numbers in packed arithmetic (the roundings of div_bf16_num and div_f32_num)
 template <bool BF16>
-__device__ __forceinline__ float fp8b_quotient(float x, float s, float r, bool fast) {
-  if (!fast) return __fdiv_rn(x, s);
-  return BF16 ? div_bf16_num(x, s, r) : div_f32_num(x, s, r);
+__device__ __forceinline__ float2 fp8b_quotients(float a, float b, float2 f) {
+  const float2 x = make_float2(a, b), s2 = make_float2(f.x, f.x), n2 = make_float2(-f.y, -f.y), m2 = make_float2(-a, -b);
+  float2 y = __fmul2_rn(x, make_float2(f.y, f.y));
+  if (!BF16) y = __ffma2_rn(n2, __ffma2_rn(y, s2, m2), y);
+  return __ffma2_rn(n2, __ffma2_rn(y, s2, m2), y);
+}
+// The codes of four numbers of one block as a word.
+template <bool BF16, bool E5M2>
+__device__ __forceinline__ uint32_t fp8b_word(float a, float b, float c, float d, float2 f) {
+  const float2 p = fp8b_quotients<BF16>(a, b, f), q = fp8b_quotients<BF16>(c, d, f);
+  uint32_t w;
+  if (E5M2)
+    asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e5m2x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e5m2x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(w) : "f"(p.x), "f"(p.y), "f"(q.x), "f"(q.y));
+  else
+    asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(w) : "f"(p.x), "f"(p.y), "f"(q.x), "f"(q.y));
+  return w;
 }
 
 // Rows of expert e: ends are device memory that no host has seen, so they are taken as they would be in order and inside
