@@ -356,7 +356,9 @@ def autograd():
             raise RuntimeError("alto_b200/_autograd.so is missing or was built for another torch: run `python -m alto_b200.build`") from e
         module.bind(*(C.cast(f, C.c_void_p).value for f in (handle.altob200_rms_norm_forward, handle.altob200_rms_norm_backward_work_bytes,
                                                             handle.altob200_rms_norm_backward, handle.altob200_grad_norm_work_bytes,
-                                                            handle.altob200_grad_norm, handle.altob200_clip_grads)))
+                                                            handle.altob200_grad_norm, handle.altob200_clip_grads,
+                                                            handle.altob200_fp8_block_quantize, handle.altob200_fp8_block_quantize_squares,
+                                                            handle.altob200_fp8_block_gemm)))
         _autograd_module = module
     return _autograd_module
 

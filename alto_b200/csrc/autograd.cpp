@@ -14,7 +14,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <initializer_list>
 #include <optional>
+#include <string>
 #include <utility>
 #include <vector>
 
@@ -34,6 +36,9 @@ struct Entries {
   decltype(&altob200_grad_norm_work_bytes) norm_work_bytes;
   decltype(&altob200_grad_norm) grad_norm;
   decltype(&altob200_clip_grads) clip_grads;
+  decltype(&altob200_fp8_block_quantize) fp8_quantize;
+  decltype(&altob200_fp8_block_quantize_squares) fp8_squares;
+  decltype(&altob200_fp8_block_gemm) fp8_gemm;
 } entry = {};
 
 // The package's own error, as a refused call of the other operators raises it.
@@ -60,6 +65,21 @@ struct Rows {
   }
   void* p() const { return hold.data_ptr(); }
 };
+
+// Gradients in a graph of their own: a second derivative is refused when it is asked for.
+void refuse_second(std::initializer_list<Tensor*> grads, const char* of) {
+  variable_list first;
+  for (const Tensor* t : grads)
+    if (t->defined()) first.push_back(t->detach().requires_grad_(true));
+  if (first.empty()) return;
+  const auto refuse = std::make_shared<torch::autograd::DelayedError>(
+      std::string("trying to differentiate the gradient of ") + of + ", which has none", (int64_t)first.size());
+  const at::AutoGradMode again(true);
+  first = (*refuse)(std::move(first));
+  size_t i = 0;
+  for (Tensor* t : grads)
+    if (t->defined()) *t = first[i++];
+}
 
 class Norm : public torch::autograd::Function<Norm> {
  public:
@@ -142,21 +162,183 @@ class Norm : public torch::autograd::Function<Norm> {
       }
       check(entry.backward(&a, work.defined() ? work.data_ptr() : nullptr, c10::cuda::getCurrentCUDAStream().stream()),
             "altob200_rms_norm_backward");
-      if (graph) {      // a second derivative is refused when it is asked for
-        variable_list first;
-        for (const Tensor* t : {&grad_rows, &grad_weight})
-          if (t->defined()) first.push_back(t->detach().requires_grad_(true));
-        const auto refuse = std::make_shared<torch::autograd::DelayedError>(
-            "trying to differentiate the gradient of rms_norm, which has none", (int64_t)first.size());
-        const at::AutoGradMode again(true);
-        first = (*refuse)(std::move(first));
-        grad_rows = first[0];
-        if (need_weight) grad_weight = first[1];
-      }
+      if (graph) refuse_second({&grad_rows, &grad_weight}, "rms_norm");
     }
     return {grad_rows, grad_weight, residual ? grad_rows : Tensor(), Tensor()};
   }
 };
+
+// ---------------------------------------------------------------------------------------
+// FP8 with one fp32 scale for each block of 128 (alto_b200/fp8_block.py has the checks and the words)
+// ---------------------------------------------------------------------------------------
+void* stream_here() { return c10::cuda::getCurrentCUDAStream().stream(); }
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// [rows, cols] with neighbouring columns, rows that do not overlap and begin on 16 bytes: the tensor's own, or a copy's.
+Tensor fp8_rows(const Tensor& t) {
+  Tensor x = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  const bool at16 = reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 == 0;
+  if (x.stride(1) == 1 && at16 && (x.size(0) <= 1 || (x.stride(0) >= x.size(1) && x.stride(0) * x.element_size() % 16 == 0))) return x;
+  return x.clone(at::MemoryFormat::Contiguous);
+}
+Tensor fp8_packed(const Tensor& t) {
+  if (!t.is_contiguous()) return t.contiguous();
+  return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t : t.clone();
+}
+struct Coded {
+  Tensor codes, scales;
+  bool there() const { return codes.defined(); }
+};
+altob200_fp8_block_scale by_row(const Tensor& s) { return {(const float*)s.const_data_ptr(), 1, s.stride(0), 0, 0, 7}; }
+altob200_fp8_block_scale by_square(const Tensor& s, bool transposed) {
+  const int64_t r = s.stride(1), c = s.stride(2);
+  return {(const float*)s.const_data_ptr(), transposed ? c : r, transposed ? r : c, s.stride(0), 7, 7};
+}
+// x2 in blocks of its rows and / or of its columns (of 128 rows from every expert's first).
+void fp8_quantize(const Tensor& x2, int32_t fmt, const Tensor& offs, Coded* rows, Coded* cols) {
+  const int64_t R = x2.size(0), C = x2.size(1);
+  const auto bytes = x2.options().dtype(at::kByte), floats = x2.options().dtype(at::kFloat);
+  altob200_fp8_block_quant_args a = {};
+  a.x = x2.const_data_ptr();
+  a.rows = R;
+  a.cols = C;
+  a.ld = R > 1 ? x2.stride(0) : C;
+  if (offs.defined()) {
+    a.offs = (const int32_t*)offs.const_data_ptr();
+    a.experts = (int32_t)offs.numel();
+  }
+  if (rows != nullptr) {
+    *rows = {at::empty({R, C}, bytes), at::empty({blocks_of(C), R}, floats)};
+    a.row_codes = rows->codes.data_ptr();
+    a.row_scales = (float*)rows->scales.data_ptr();
+  }
+  if (cols != nullptr) {
+    const int64_t blocks = offs.defined() ? R / 128 + offs.numel() : blocks_of(R);
+    *cols = {at::empty({C, blocks * 128}, bytes), at::empty({blocks, C}, floats)};
+    a.col_codes = cols->codes.data_ptr();
+    a.col_scales = (float*)cols->scales.data_ptr();
+    a.ld_col = blocks * 128;
+  }
+  a.dtype = dtype_of(x2);
+  a.format = fmt;
+  if (R > 0 && (rows != nullptr || cols != nullptr)) check(entry.fp8_quantize(&a, stream_here()), "altob200_fp8_block_quantize");
+}
+// D = A B^T; sa without scales: a is numbers.
+void fp8_gemm(const Tensor& a, const altob200_fp8_block_scale& sa, const Tensor& b, const altob200_fp8_block_scale& sb, const Tensor& out,
+              int32_t fmt, int64_t M, int64_t N, int64_t K, int32_t mode, const Tensor& offs, int64_t k_rows) {
+  altob200_fp8_block_gemm_args g = {};
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.lda = M > 1 ? a.stride(0) : K;
+  g.ldd = N;
+  g.k_rows = k_rows;
+  g.a = a.const_data_ptr();
+  g.b = b.const_data_ptr();
+  g.sa = sa;
+  g.sb = sb;
+  if (offs.defined()) {
+    g.offs = (const int32_t*)offs.const_data_ptr();
+    g.experts = (int32_t)offs.numel();
+  }
+  g.d = out.data_ptr();
+  g.mode = mode;
+  g.format = fmt;
+  g.a_dtype = sa.scales == nullptr ? dtype_of(a) : -1;
+  g.out_dtype = dtype_of(out);
+  check(entry.fp8_gemm(&g, stream_here()), "altob200_fp8_block_gemm");
+}
+
+// The linear, dense (weight [N, K]) or by expert (weight [E, K, N], ends of the experts' rows).  `weight` is what the graph
+// knows (a wrapper, too), `data` its numbers.
+class Fp8Linear : public torch::autograd::Function<Fp8Linear> {
+ public:
+  static Variable forward(AutogradContext* ctx, const Variable& x, const Variable& weight, const Tensor& data, const std::optional<Tensor>& ends,
+                          int64_t fmt64, bool need_x, bool need_w) {
+    const c10::cuda::CUDAGuard device(x.device());
+    const int32_t fmt = (int32_t)fmt64;
+    const Tensor offs = ends.value_or(Tensor());
+    const bool grouped = offs.defined();
+    const Tensor x2 = fp8_rows(x.detach());
+    Tensor w = data;
+    // matrices as they lie in memory, [rows, cols]: of the weight N x K, or K x N
+    bool kn = false;
+    if (grouped) {
+      kn = w.stride(2) == 1 || w.stride(1) != 1;
+      w = fp8_packed(kn ? w : w.transpose(1, 2));
+    } else {
+      w = fp8_rows(w).unsqueeze(0);
+    }
+    const int64_t E = w.size(0), R = w.size(1), C = w.size(2), N = kn ? C : R, K = kn ? R : C, M = x2.size(0);
+    const auto bytes = w.options().dtype(at::kByte);
+    const bool need_plain = !kn || need_x, need_t = kn || need_x;
+    const Tensor plain = need_plain ? at::empty({E, R, C}, bytes) : Tensor(), turned = need_t ? at::empty({E, C, R}, bytes) : Tensor();
+    const Tensor scales = at::empty({E, blocks_of(R), blocks_of(C)}, w.options().dtype(at::kFloat));
+    check(entry.fp8_squares(w.const_data_ptr(), dtype_of(w), fmt, E, R, C, w.stride(1), w.stride(0), need_plain ? plain.data_ptr() : nullptr,
+                            need_t ? turned.data_ptr() : nullptr, (float*)scales.data_ptr(), stream_here()), "altob200_fp8_block_quantize_squares");
+    Coded rows, cols;
+    fp8_quantize(x2, fmt, offs, &rows, need_w ? &cols : nullptr);
+    auto shape = x.sizes().vec();
+    shape.back() = N;
+    const Tensor out = at::empty(shape, x.options());
+    fp8_gemm(rows.codes, by_row(rows.scales), kn ? turned : plain, by_square(scales, kn), out, fmt, M, N, K, grouped ? 1 : 0, offs, 0);
+    ctx->save_for_backward({cols.codes, cols.scales, need_x ? (kn ? plain : turned) : Tensor(), need_x ? scales : Tensor(), offs});
+    ctx->saved_data["dims"] = std::vector<int64_t>{M, K, N, fmt64, kn ? 1 : 0};
+    ctx->saved_data["shape"] = x.sizes().vec();
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto dims = ctx->saved_data["dims"].toIntVector();
+    const int64_t M = dims[0], K = dims[1], N = dims[2];
+    const int32_t fmt = (int32_t)dims[3];
+    const Tensor &grad = grads[0], &offs = saved[4];
+    const bool graph = at::GradMode::is_enabled(), need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), grouped = offs.defined();
+    Tensor dx, dw;
+    {
+      const at::AutoGradMode no_graph(false);
+      const c10::cuda::CUDAGuard device(grad.device());
+      const Tensor g2 = fp8_rows(grad);
+      Coded rows, cols;
+      if (need_x || need_w) fp8_quantize(g2, fmt, offs, need_x ? &rows : nullptr, need_w ? &cols : nullptr);
+      if (need_x) {
+        dx = at::empty(ctx->saved_data["shape"].toIntVector(), grad.options());
+        fp8_gemm(rows.codes, by_row(rows.scales), saved[2], by_square(saved[3], dims[4] == 0), dx, fmt, M, K, N, grouped ? 1 : 0, offs, 0);
+      }
+      if (need_w && grouped) {
+        dw = at::empty({offs.numel(), K, N}, grad.options());
+        fp8_gemm(saved[0], by_row(saved[1]), cols.codes, by_row(cols.scales), dw, fmt, K, N, cols.codes.size(1), 2, offs, M);
+      } else if (need_w) {
+        dw = M > 0 ? at::empty({N, K}, grad.options()) : at::zeros({N, K}, grad.options());
+        if (M > 0) fp8_gemm(cols.codes, by_row(cols.scales), saved[0], by_row(saved[1]), dw, fmt, N, K, cols.codes.size(1), 0, Tensor(), 0);
+      }
+    }
+    if (graph) refuse_second({&dx, &dw}, "a linear in FP8 blocks");
+    return {dx, dw, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// x times codes of weights [E or 1, N, K]; few rows an expert are quantised by the product itself.
+Tensor fp8_serve(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales, const std::optional<Tensor>& ends, int64_t fmt, int64_t few) {
+  const at::AutoGradMode no_graph(false);
+  const c10::cuda::CUDAGuard device(x.device());
+  const int64_t N = w_codes.size(-2), K = w_codes.size(-1);
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  const Tensor out = at::empty(shape, x.options()), x2 = fp8_rows(x), w = fp8_packed(w_codes), offs = ends.value_or(Tensor());
+  const Tensor s = w_scales.dim() == 3 ? w_scales : w_scales.unsqueeze(0);
+  const int64_t M = x2.size(0);
+  const int32_t mode = offs.defined() ? 1 : 0;
+  if (M <= few * (offs.defined() ? offs.numel() : 1)) {
+    fp8_gemm(x2, altob200_fp8_block_scale{}, w, by_square(s, false), out, (int32_t)fmt, M, N, K, mode, offs, 0);
+  } else {
+    Coded rows;
+    fp8_quantize(x2, (int32_t)fmt, Tensor(), &rows, nullptr);
+    fp8_gemm(rows.codes, by_row(rows.scales), w, by_square(s, false), out, (int32_t)fmt, M, N, K, mode, offs, 0);
+  }
+  return out;
+}
 
 // A list of tensors as the entry points take it.  A tensor whose elements are not neighbours in memory goes through a copy
 // (and back, where it is written).
@@ -230,11 +412,21 @@ Tensor clip_grads(const std::vector<Tensor>& grads, const std::vector<Tensor>& o
 
 PYBIND11_MODULE(_autograd, m) {
   m.def("bind", [](uintptr_t forward, uintptr_t work_bytes, uintptr_t backward, uintptr_t norm_work_bytes, uintptr_t grad_norm,
-                   uintptr_t clip_grads) {
+                   uintptr_t clip_grads, uintptr_t fp8_quantize, uintptr_t fp8_squares, uintptr_t fp8_gemm) {
     entry = {reinterpret_cast<decltype(entry.forward)>(forward), reinterpret_cast<decltype(entry.work_bytes)>(work_bytes),
              reinterpret_cast<decltype(entry.backward)>(backward), reinterpret_cast<decltype(entry.norm_work_bytes)>(norm_work_bytes),
-             reinterpret_cast<decltype(entry.grad_norm)>(grad_norm), reinterpret_cast<decltype(entry.clip_grads)>(clip_grads)};
+             reinterpret_cast<decltype(entry.grad_norm)>(grad_norm), reinterpret_cast<decltype(entry.clip_grads)>(clip_grads),
+             reinterpret_cast<decltype(entry.fp8_quantize)>(fp8_quantize), reinterpret_cast<decltype(entry.fp8_squares)>(fp8_squares),
+             reinterpret_cast<decltype(entry.fp8_gemm)>(fp8_gemm)};
   });
+  m.def("fp8_linear",
+        [](const Tensor& x, const Tensor& weight, const Tensor& data, const std::optional<Tensor>& offs, int64_t fmt) {
+          // (inside forward every input says what it said before, and the mode is off)
+          const bool graph = at::GradMode::is_enabled();
+          return Fp8Linear::apply(x, weight, data.detach(), offs, fmt, graph && x.requires_grad(), graph && weight.requires_grad());
+        },
+        pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("fp8_serve", &fp8_serve, pybind11::call_guard<pybind11::gil_scoped_release>());
   // lists as alto_b200/grad_clip.py has checked them
   m.def("grad_norm", &grad_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("clip_grads", &clip_grads, pybind11::call_guard<pybind11::gil_scoped_release>());

@@ -2,8 +2,8 @@
 
     convert_to_fp8_block / convert_from_fp8_block      codes and scales along an axis, or of squares of 128 x 128
     blockwise_fp8_gemm(a, a_s, b, b_s)                 a b^T of two quantised operands
-    _to_fp8_block_then_scaled_mm / FP8BlockLinearFunction            a training step's linear (x in blocks of a row, weights
-                                                                     in squares; the weight gradient in blocks of tokens)
+    _to_fp8_block_then_scaled_mm                       a training step's linear (x in blocks of a row, weights in squares; the
+                                                       weight gradient in blocks of tokens); its autograd function is C++
     fp8_block_linear / fp8_block_grouped_linear        serving: weights that are there as codes and scales, from one token up
 
 A block's scale is max(|largest|, 1e-12) / top (top: 448 for E4M3, 57344 for E5M2) and its codes are the quotients by it, to
@@ -20,9 +20,9 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from .nvfp4 import outside_of_grad_mode, unwrap_weight_wrapper
+from .nvfp4 import unwrap_weight_wrapper
 
-__all__ = ["convert_to_fp8_block", "convert_from_fp8_block", "blockwise_fp8_gemm", "FP8BlockLinearFunction", "fp8_block_linear",
+__all__ = ["convert_to_fp8_block", "convert_from_fp8_block", "blockwise_fp8_gemm", "fp8_block_linear",
            "fp8_block_grouped_linear"]
 
 BLOCK_SIZE = 128
@@ -189,17 +189,6 @@ def blockwise_fp8_gemm(a: torch.Tensor, a_s: torch.Tensor, b: torch.Tensor, b_s:
     return out
 
 
-def _product(x2: torch.Tensor, w8: torch.Tensor, sw: L.Fp8BlockScale, out: torch.Tensor, fmt: int, dims, offs=None) -> None:
-    """x2 (numbers) times codes of weights; few rows an expert are quantised by the product itself."""
-    M = dims[0]
-    mode = 0 if offs is None else 1
-    if M <= 16 * (1 if offs is None else offs.numel()):
-        L.fp8_block_gemm(x2, None, w8, sw, out, fmt, dims, mode, offs)
-        return
-    (codes, scales), _ = L.fp8_block_quantize(x2, fmt, True, False)
-    L.fp8_block_gemm(codes, _row_scales(scales), w8, sw, out, fmt, dims, mode, offs)
-
-
 def _check_serving(name: str, x, w_codes, w_scales, dims: int) -> None:
     if not (x.is_cuda and w_codes.is_cuda and w_scales.is_cuda):
         raise RuntimeError(f"{name} runs on CUDA tensors only (no CPU fallback)")
@@ -222,14 +211,8 @@ def _check_serving(name: str, x, w_codes, w_scales, dims: int) -> None:
         raise RuntimeError(f"{name} has no gradient: codes of weights serve evaluation")
 
 
-@L.on_device_of
-def _serve(x, w_codes, w_scales, offs):
-    N, K = w_codes.shape[-2:]
-    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-    x2, w8 = _rows(x.detach()), _packed(w_codes.detach()).view(torch.uint8)
-    s = w_scales.detach()
-    _product(x2, w8, _square_scales(s if s.dim() == 3 else s.unsqueeze(0)), out, _FMT_OF_DTYPE[w_codes.dtype], (x2.shape[0], N, K), offs)
-    return out
+#: most rows (an expert) that the product quantises itself, instead of a launch in front of it
+_FEW_ROWS = 16
 
 
 @L.traced("fp8_block_linear")
@@ -238,7 +221,7 @@ def fp8_block_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Ten
     [ceil(N / 128), ceil(K / 128)] (``convert_to_fp8_block(w, is_2d_block=True)``); the result has x's type.  x is quantised in
     the weight's format, in blocks of a row.  Not differentiable."""
     _check_serving("fp8_block_linear", x, w_codes, w_scales, 2)
-    return _serve(x, w_codes, w_scales, None)
+    return (L._autograd_module or L.autograd()).fp8_serve(x, w_codes, w_scales, None, _FMT_OF_DTYPE[w_codes.dtype], _FEW_ROWS)
 
 
 @L.traced("fp8_block_grouped_linear")
@@ -249,7 +232,8 @@ def fp8_block_grouped_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: t
     _check_serving("fp8_block_grouped_linear", x, w_codes, w_scales, 3)
     if x.dim() != 2:
         raise ValueError(f"fp8_block_grouped_linear expects rows [M, K], got {tuple(x.shape)}")
-    return _serve(x, w_codes, w_scales, _ends("fp8_block_grouped_linear", offs, w_codes.shape[0], x.device))
+    offs = _ends("fp8_block_grouped_linear", offs, w_codes.shape[0], x.device)
+    return (L._autograd_module or L.autograd()).fp8_serve(x, w_codes, w_scales, offs, _FMT_OF_DTYPE[w_codes.dtype], _FEW_ROWS)
 
 
 def _ends(name: str, offs: torch.Tensor, experts: int, device) -> torch.Tensor:
@@ -257,138 +241,47 @@ def _ends(name: str, offs: torch.Tensor, experts: int, device) -> torch.Tensor:
         raise ValueError(f"{name} expects offs as int32 [{experts}] on {device}, got {tuple(offs.shape)}, {offs.dtype} on {offs.device}")
     if experts == 0:
         raise ValueError(f"{name} expects at least one expert")
+    if offs.dtype is torch.int32 and offs.is_contiguous():
+        return offs
     return offs.to(torch.int32).contiguous()
 
 
 # ---------------------------------------------------------------------------------------------
 # training
 # ---------------------------------------------------------------------------------------------
-def _backward_products(ctx, grad, x_t, w_other, w_scale, offs):
-    """(dx, dw in the layout [experts or 1, rows of the weight that x meets ...]) - see the two functions."""
-    (M, K, N), fmt = ctx.dims, ctx.fmt
-    need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    g2 = _rows(grad)
-    by_row, by_col = L.fp8_block_quantize(g2, fmt, need_x, need_w, offs) if need_x or need_w else (None, None)
-    dx = dw = None
-    if need_x:
-        dx = torch.empty(ctx.shape, dtype=grad.dtype, device=grad.device)
-        L.fp8_block_gemm(by_row[0], _row_scales(by_row[1]), w_other, w_scale, dx, fmt, (M, K, N), 0 if offs is None else 1, offs)
-    if need_w:
-        if offs is None:
-            dw = torch.empty((N, K), dtype=grad.dtype, device=grad.device)
-            if M == 0:
-                dw.zero_()
-            else:
-                L.fp8_block_gemm(by_col[0], _row_scales(by_col[1]), x_t[0], _row_scales(x_t[1]), dw, fmt, (N, K, by_col[0].shape[1]))
-        else:
-            dw = torch.empty((offs.numel(), K, N), dtype=grad.dtype, device=grad.device)
-            L.fp8_block_gemm(x_t[0], _row_scales(x_t[1]), by_col[0], _row_scales(by_col[1]), dw, fmt, (K, N, by_col[0].shape[1]), 2, offs, M)
-    return dx, dw
+def _plain(weight: torch.Tensor) -> torch.Tensor:
+    return weight if type(weight) is torch.Tensor or type(weight) is torch.nn.Parameter else unwrap_weight_wrapper(weight)
 
 
-class FP8BlockLinearFunction(torch.autograd.Function):
-    """y = x W^T, x in blocks of a row and W [N, K] in squares; dx from the gradient in blocks of a row, dW from the gradient and
-    x in blocks of 128 tokens.  What is kept is codes: of x along its columns (where W requires a gradient), of W."""
-
-    @staticmethod
-    def forward(ctx, x, weight, fp8_variant: str = "e4m3"):
-        weight = unwrap_weight_wrapper(weight)
-        _check_format(fp8_variant)
-        if not x.is_cuda or not weight.is_cuda:
-            raise RuntimeError("FP8BlockLinearFunction runs on CUDA tensors only (no CPU fallback)")
-        if x.dtype not in _TYPES:
-            raise ValueError(f"x dtype must be float32/bfloat16, got {x.dtype}")
-        if weight.dtype != x.dtype:
-            raise ValueError(f"weight dtype ({weight.dtype}) must match x dtype ({x.dtype})")
-        if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-            raise ValueError(f"FP8BlockLinearFunction expects x [..., K] and a weight [N, K], got {tuple(x.shape)} and {tuple(weight.shape)}")
-        if weight.device != x.device:
-            raise ValueError("FP8BlockLinearFunction expects x and weight on one device")
-        N, K = weight.shape
-        if N % 16 != 0 or K % 16 != 0 or N == 0 or K == 0:
-            raise ValueError(f"FP8BlockLinearFunction expects features in multiples of 16, got in={K}, out={N}")
-        fmt = _FMT[fp8_variant]
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        x2 = _rows(x.detach())
-        M = x2.shape[0]
-        w_k, w_n, w_s = L.fp8_block_quantize_squares(_rows(weight.detach()).unsqueeze(0), fmt, True, need_x)
-        by_row, x_t = L.fp8_block_quantize(x2, fmt, True, need_w)
-        out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-        L.fp8_block_gemm(by_row[0], _row_scales(by_row[1]), w_k, _square_scales(w_s), out, fmt, (M, N, K))
-        ctx.save_for_backward(*([None, None] if x_t is None else x_t), *([None, None] if w_n is None else [w_n, w_s]))
-        ctx.dims, ctx.shape, ctx.fmt = (M, K, N), x.shape, fmt
-        return out
-
-    @staticmethod
-    @L.once_differentiable
-    def backward(ctx, grad):
-        xc, xs, w_n, w_s = ctx.saved_tensors
-        dx, dw = _backward_products(ctx, grad, (xc, xs), w_n, None if w_s is None else _square_scales(w_s, True), None)
-        return dx, dw, None
-
-
-class GroupedFP8BlockFunction(torch.autograd.Function):
-    """y[m] = x[m] B[e(m)] for B [E, K, N] and rows sorted by expert, ends in ``offs``, any number of rows an expert."""
-
-    @staticmethod
-    def forward(ctx, x, B, offs, fp8_variant: str = "e4m3"):
-        name = "_quantize_then_fp8_block_scaled_grouped_mm"
-        B = unwrap_weight_wrapper(B)
-        _check_format(fp8_variant)
-        if not x.is_cuda or not B.is_cuda:
-            raise RuntimeError(f"{name} runs on CUDA tensors only (no CPU fallback)")
-        if x.dtype not in _TYPES:
-            raise ValueError(f"A dtype must be float32/bfloat16, got {x.dtype}")
-        if B.dtype != x.dtype:
-            raise ValueError(f"B dtype ({B.dtype}) must match A dtype ({x.dtype})")
-        if x.dim() != 2 or B.dim() != 3 or B.shape[1] != x.shape[1]:
-            raise ValueError(f"{name} expects A [M, K] and B [E, K, N], got {tuple(x.shape)} and {tuple(B.shape)}")
-        if B.device != x.device:
-            raise ValueError(f"{name} expects A and B on one device")
-        experts, K, N = B.shape
-        if N % 16 != 0 or K % 16 != 0 or N == 0 or K == 0:
-            raise ValueError(f"{name} expects features in multiples of 16, got in={K}, out={N}")
-        offs = _ends(name, offs, experts, x.device)
-        fmt = _FMT[fp8_variant]
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        x2 = _rows(x.detach())
-        M = x2.shape[0]
-        b = B.detach()
-        if b.stride(2) == 1 or b.stride(1) != 1:      # [K, N] in memory
-            w_n, w_k, w_s = L.fp8_block_quantize_squares(_packed(b), fmt, need_x, True)
-            stored_t = True
-        else:                                         # [N, K]
-            w_k, w_n, w_s = L.fp8_block_quantize_squares(_packed(b.transpose(1, 2)), fmt, True, need_x)
-            stored_t = False
-        by_row, x_t = L.fp8_block_quantize(x2, fmt, True, need_w, offs)
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
-        L.fp8_block_gemm(by_row[0], _row_scales(by_row[1]), w_k, _square_scales(w_s, stored_t), out, fmt, (M, N, K), 1, offs)
-        ctx.save_for_backward(offs, *([None, None] if x_t is None else x_t), *([None, None] if w_n is None else [w_n, w_s]))
-        ctx.dims, ctx.shape, ctx.fmt, ctx.stored_t = (M, K, N), x.shape, fmt, stored_t
-        return out
-
-    @staticmethod
-    @L.once_differentiable
-    def backward(ctx, grad):
-        offs, xc, xs, w_n, w_s = ctx.saved_tensors
-        dx, dw = _backward_products(ctx, grad, (xc, xs), w_n, None if w_s is None else _square_scales(w_s, not ctx.stored_t), offs)
-        return dx, dw, None, None
-
-
-@L.on_device_of
-def _linear(a, b, fp8_variant):
-    return FP8BlockLinearFunction.apply(a, b, fp8_variant)
+def _check_training(name: str, x: torch.Tensor, w: torch.Tensor, dims: int, fp8_variant: str) -> None:
+    _check_format(fp8_variant)
+    if not x.is_cuda or not w.is_cuda:
+        raise RuntimeError(f"{name} runs on CUDA tensors only (no CPU fallback)")
+    if x.dtype not in _TYPES:
+        raise ValueError(f"A dtype must be float32/bfloat16, got {x.dtype}")
+    if w.dtype != x.dtype:
+        raise ValueError(f"weight dtype ({w.dtype}) must match the activations' ({x.dtype})")
+    if w.dim() != dims or x.dim() < 1 or (dims == 3 and x.dim() != 2) or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"{name} expects " + ("A [..., K] and B [N, K]" if dims == 2 else "A [M, K] and B [E, K, N]") +
+                         f", got {tuple(x.shape)} and {tuple(w.shape)}")
+    if w.device != x.device:
+        raise ValueError(f"{name} expects all tensors on one device")
+    if any(n % 16 != 0 or n == 0 for n in w.shape[-2:]):
+        raise ValueError(f"{name} expects features in multiples of 16, got {tuple(w.shape[-2:])}")
 
 
 @L.traced("fp8_block_linear_training")
 def _to_fp8_block_then_scaled_mm(a: torch.Tensor, b: torch.Tensor, fp8_variant: str = "e4m3") -> torch.Tensor:
-    """a b^T of a training step: a [..., K], b [N, K] (bf16 or fp32, a wrapped weight too), differentiable in both."""
-    if not a.is_cuda:
-        raise RuntimeError("FP8BlockLinearFunction runs on CUDA tensors only (no CPU fallback)")
-    a, b = outside_of_grad_mode(a, b)
-    return _linear(a, b, fp8_variant)
+    """a b^T of a training step: a [..., K], b [N, K] (bf16 or fp32, a wrapped weight too), differentiable in both.  a is quantised
+    in blocks of a row and b in squares; the gradient of a takes the upstream one in blocks of a row, that of b both in blocks
+    of 128 tokens.  What is kept is codes: of a along its columns (where b requires a gradient) and of b."""
+    w = _plain(b)
+    _check_training("_to_fp8_block_then_scaled_mm", a, w, 2, fp8_variant)
+    return (L._autograd_module or L.autograd()).fp8_linear(a, b, w, None, _FMT[fp8_variant])
 
 
-@L.on_device_of
-def _grouped(a, b, offs, fp8_variant):
-    return GroupedFP8BlockFunction.apply(a, b, offs, fp8_variant)
+def _grouped(a: torch.Tensor, b: torch.Tensor, offs: torch.Tensor, fp8_variant: str) -> torch.Tensor:
+    name = "_quantize_then_fp8_block_scaled_grouped_mm"
+    w = _plain(b)
+    _check_training(name, a, w, 3, fp8_variant)
+    return (L._autograd_module or L.autograd()).fp8_linear(a, b, w, _ends(name, offs, w.shape[0], a.device), _FMT[fp8_variant])

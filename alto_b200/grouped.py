@@ -28,7 +28,7 @@ from . import _lib as L
 from . import _linear as E
 from . import dge
 from .hadamard import HadamardFactory, HadamardTransform
-from .nvfp4 import _check_scale_format, outside_of_grad_mode, unwrap_weight_wrapper
+from .nvfp4 import _check_scale_format, unwrap_weight_wrapper
 
 ALIGN_SIZE_M = 128
 
@@ -235,9 +235,6 @@ def _quantize_then_fp8_block_scaled_grouped_mm(A, B, offs, *, fp8_variant: str =
     one takes any number of rows an expert: no padding, ``offs`` [E] are the ends of the runs as they are.  Rows from
     offs[-1] on give zeros, and a zero gradient."""
     from . import fp8_block
-    if not A.is_cuda:
-        raise RuntimeError("_quantize_then_fp8_block_scaled_grouped_mm runs on CUDA tensors only (no CPU fallback)")
-    A, B = outside_of_grad_mode(A, B)
     return fp8_block._grouped(A, B, offs, fp8_variant)
 
 
