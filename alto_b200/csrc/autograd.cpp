@@ -381,8 +381,25 @@ struct GradList {
   }
 };
 
+// Whether lists are what the entry points take: alto_b200/grad_clip.py tells what is wrong with the others (or takes the local
+// part of sharded ones).
+bool usual(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs) {
+  if (grads.empty() || (!outs.empty() && outs.size() != grads.size())) return false;
+  const auto device = grads[0].device();
+  const auto fine = [&](const Tensor& t) {
+    return t.defined() && t.is_cuda() && t.device() == device && t.layout() == at::kStrided &&
+           (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) && !t.key_set().has(c10::DispatchKey::Python);
+  };
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (!fine(grads[i])) return false;
+    if (!outs.empty() && (!fine(outs[i]) || outs[i].scalar_type() != grads[i].scalar_type() || outs[i].sizes() != grads[i].sizes())) return false;
+  }
+  return true;
+}
+
 // (total fp64, norm fp32) of the tensors together
-std::pair<Tensor, Tensor> grad_norm(const std::vector<Tensor>& grads, bool inf) {
+std::optional<std::pair<Tensor, Tensor>> grad_norm(const std::vector<Tensor>& grads, bool inf) {
+  if (!usual(grads, {})) return std::nullopt;
   const at::AutoGradMode no_graph(false);
   const c10::cuda::CUDAGuard device(grads.at(0).device());
   GradList l(grads, {}, false);
@@ -391,10 +408,11 @@ std::pair<Tensor, Tensor> grad_norm(const std::vector<Tensor>& grads, bool inf) 
   Tensor work = at::empty({entry.norm_work_bytes(l.list.count)}, options.dtype(at::kByte));
   check(entry.grad_norm(&l.list, inf, work.data_ptr(), (double*)total.data_ptr(), (float*)norm.data_ptr(),
                         c10::cuda::getCurrentCUDAStream().stream()), "altob200_grad_norm");
-  return {total, norm};
+  return std::make_pair(total, norm);
 }
 
-Tensor clip_grads(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs, double max_norm, bool inf, const std::optional<Tensor>& total) {
+std::optional<Tensor> clip_grads(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs, double max_norm, bool inf, const std::optional<Tensor>& total) {
+  if (!usual(grads, outs)) return std::nullopt;
   const at::AutoGradMode no_graph(false);
   const c10::cuda::CUDAGuard device(grads.at(0).device());
   GradList l(grads, outs, true);
@@ -427,7 +445,7 @@ PYBIND11_MODULE(_autograd, m) {
         },
         pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("fp8_serve", &fp8_serve, pybind11::call_guard<pybind11::gil_scoped_release>());
-  // lists as alto_b200/grad_clip.py has checked them
+  // None: a list that alto_b200/grad_clip.py has to look at
   m.def("grad_norm", &grad_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("clip_grads", &clip_grads, pybind11::call_guard<pybind11::gil_scoped_release>());
   // operands as alto_b200/norm.py has checked them

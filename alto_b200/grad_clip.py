@@ -19,6 +19,7 @@ from typing import Iterable, Optional, Sequence, Union
 import torch
 
 from . import _lib as L
+from .nvfp4 import unwrap_weight_wrapper
 
 __all__ = ["grad_norm", "clip_grad_norm_", "clip_grads"]
 
@@ -35,22 +36,24 @@ def _kind(norm_type) -> bool:
     raise ValueError(f"the norms are 2 and inf, got {norm_type}")
 
 
-def _check(name: str, tensors: Sequence[torch.Tensor]) -> None:
-    device = tensors[0].device
-    for t in tensors:
-        if t.dtype in _TYPES and t.device == device and t.is_cuda and t.layout is torch.strided:
-            continue
+def _refuse(name: str, tensors: Sequence[torch.Tensor], out: Sequence[torch.Tensor] = ()) -> None:
+    """Says what is wrong with a list that the kernels do not take."""
+    for t in (*tensors, *out):
         if t.layout is not torch.strided:
             raise ValueError(f"{name} expects dense tensors, got {t.layout}")
         if not t.is_cuda:
             raise RuntimeError(f"{name} runs on CUDA tensors only (no CPU fallback)")
         if t.dtype not in _TYPES:
             raise TypeError(f"{name} expects bfloat16 or float32, got {t.dtype}")
-        raise ValueError(f"{name} expects all tensors on one device")
+        if t.device != tensors[0].device:
+            raise ValueError(f"{name} expects all tensors on one device")
+    raise ValueError(f"{name} expects out like grads: as many tensors, of their shapes and types")
 
 
 def _local(t: torch.Tensor) -> torch.Tensor:
-    return t.to_local() if hasattr(t, "to_local") else t
+    """The local part of a sharded tensor, a wrapper's data."""
+    t = t.to_local() if hasattr(t, "to_local") else t
+    return unwrap_weight_wrapper(t) if hasattr(t, "_data") else t
 
 
 def _reduced(total: torch.Tensor, inf: bool, group) -> torch.Tensor:
@@ -64,57 +67,61 @@ def _world(group) -> int:
     return dist.get_world_size(group) if group is not None and dist.is_initialized() else 1
 
 
+def _norm(name: str, tensors: Sequence[torch.Tensor], inf: bool, group):
+    """(total, norm), over the ranks of ``group`` too."""
+    host = L._autograd_module or L.autograd()
+    got = host.grad_norm(tensors, inf) or host.grad_norm([_local(t) for t in tensors], inf)
+    if got is None:
+        _refuse(name, tensors)
+    total, norm = got
+    if _world(group) > 1:
+        total = _reduced(total, inf, group)
+        norm = (total if inf else total.sqrt()).float()
+    return total, norm
+
+
 @L.traced("grad_norm")
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0, group=None) -> torch.Tensor:
     """fp32 scalar: the 2-norm (or the largest magnitude, ``norm_type`` inf) of all tensors together.  ``group``: over the ranks of
     it, each of which holds a part."""
     inf = _kind(norm_type)
-    tensors = [_local(t) for t in tensors]
+    tensors = list(tensors)
     if not tensors:
         if _world(group) > 1:
             raise ValueError("grad_norm over ranks expects a tensor on each")
         return torch.zeros(())
-    _check("grad_norm", tensors)
-    total, norm = (L._autograd_module or L.autograd()).grad_norm(tensors, inf)
-    if _world(group) > 1:
-        total = _reduced(total, inf, group)
-        norm = (total if inf else total.sqrt()).float()
-    return norm
+    return _norm("grad_norm", tensors, inf, group)[1]
 
 
 @L.traced("clip_grads")
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None,
                group=None, error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the tensors to a common norm of at most ``max_norm``, in place or into ``out`` (tensors of the same shapes and types
-    that do not overlap them); returns the norm before, an fp32 scalar.  Where nothing is clipped, tensors scaled in place are not written.
-    ``group``: the norm is taken over its ranks.  ``error_if_nonfinite`` waits for the norm and raises before anything is
-    scaled."""
+    that do not overlap them); returns the norm before, an fp32 scalar.  Where nothing is clipped, tensors scaled in place are not
+    written.  ``group``: the norm is taken over its ranks.  ``error_if_nonfinite`` waits for the norm and raises before anything
+    is scaled."""
     inf, max_norm = _kind(norm_type), float(max_norm)
-    grads = [_local(g) for g in grads]
+    grads, outs = list(grads), [] if out is None else list(out)
     if not grads:
         if _world(group) > 1:
             raise ValueError("clip_grads over ranks expects a tensor on each")
         return torch.zeros(())
-    _check("clip_grads", grads)
-    outs = []
-    if out is not None:
-        outs = [_local(o) for o in out]
-        if len(outs) != len(grads) or any(o.shape != g.shape or o.dtype != g.dtype for o, g in zip(outs, grads)):
-            raise ValueError("clip_grads expects out like grads: as many tensors, of their shapes and types")
-        _check("clip_grads", outs)
-        if outs[0].device != grads[0].device:
-            raise ValueError("clip_grads expects all tensors on one device")
-    host = L._autograd_module or L.autograd()
+    if out is not None and len(outs) != len(grads):
+        raise ValueError("clip_grads expects out like grads: as many tensors, of their shapes and types")
     total = None
     if error_if_nonfinite or _world(group) > 1:
-        total, _ = host.grad_norm(grads, inf)
-        if _world(group) > 1:
-            total = _reduced(total, inf, group)
+        total, _ = _norm("clip_grads", grads, inf, group)
         if error_if_nonfinite and not math.isfinite(float(total)):
             raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is non-finite, so it cannot "
                                "be clipped. To disable this error and scale the gradients by the non-finite norm anyway, set "
                                "`error_if_nonfinite=False`")
-    return host.clip_grads(grads, outs, max_norm, inf, total)
+    host = L._autograd_module or L.autograd()
+    got = host.clip_grads(grads, outs, max_norm, inf, total)
+    if got is None:
+        got = host.clip_grads([_local(g) for g in grads], [_local(o) for o in outs], max_norm, inf, total)
+    if got is None:
+        _refuse("clip_grads", grads, outs)
+    return got
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
