@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <initializer_list>
@@ -340,8 +341,19 @@ Tensor fp8_serve(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales,
   return out;
 }
 
-// A list of tensors as the entry points take it.  A tensor whose elements are not neighbours in memory goes through a copy
-// (and back, where it is written).
+// ---------------------------------------------------------------------------------------
+// norm of many tensors and clipping by it (alto_b200/grad_clip.py)
+// ---------------------------------------------------------------------------------------
+// Where the first of the tensors is.
+std::optional<c10::Device> on_device(const pybind11::list& l) {
+  if (l.size() == 0 || !THPVariable_Check(PyList_GET_ITEM(l.ptr(), 0))) return std::nullopt;
+  const Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(l.ptr(), 0));
+  return t.is_cuda() ? std::optional<c10::Device>(t.device()) : std::nullopt;
+}
+
+// Lists of tensors as the entry points take them.  A tensor whose elements are not neighbours in memory goes through a copy
+// (and back, where it is written).  Thousands of tensors make up a call's host time, so the lists are walked once, without taking
+// references.
 struct GradList {
   std::vector<const void*> grads;
   std::vector<void*> outs;
@@ -349,79 +361,91 @@ struct GradList {
   std::vector<int32_t> dtypes;
   std::vector<Tensor> hold;
   std::vector<std::pair<Tensor, Tensor>> back;      // (copy, where it belongs)
+  Tensor first;
   altob200_grad_list list = {};
 
-  static bool same_layout(const Tensor& a, const Tensor& b) {
-    return a.is_non_overlapping_and_dense() && (a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()));
+  static const Tensor* plain(PyObject* o) {
+    if (!THPVariable_Check(o)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(o);
+    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) &&
+                   !t.key_set().has(c10::DispatchKey::Python)
+               ? &t : nullptr;
   }
-  GradList(const std::vector<Tensor>& in, const std::vector<Tensor>& out, bool writes) {
+  // False: a list that alto_b200/grad_clip.py has to look at.
+  bool take(const pybind11::list& in, const pybind11::list& out, bool writes) {
     const size_t n = in.size();
+    if (n == 0 || (out.size() != 0 && out.size() != n)) return false;
     grads.reserve(n), sizes.reserve(n), dtypes.reserve(n);
     if (writes) outs.reserve(n);
+    c10::Device device(c10::kCPU);
     for (size_t i = 0; i < n; ++i) {
-      const Tensor* g = &in[i];
-      if (!g->is_non_overlapping_and_dense()) g = &hold.emplace_back(g->contiguous());
-      Tensor kept = *g;      // (hold may move)
-      grads.push_back(kept.data_ptr());
-      sizes.push_back(kept.numel());
-      dtypes.push_back(dtype_of(kept));
-      if (!writes) continue;
-      const Tensor& o = out.empty() ? in[i] : out[i];
-      if (o.is_same(kept) || same_layout(o, kept)) {
-        outs.push_back(o.data_ptr());
+      const Tensor* g = plain(PyList_GET_ITEM(in.ptr(), (Py_ssize_t)i));
+      if (g == nullptr) return false;
+      if (i == 0) {
+        first = *g;
+        device = g->device();
+      } else if (g->device() != device) {
+        return false;
+      }
+      const Tensor* o = g;
+      if (out.size() != 0) {
+        o = plain(PyList_GET_ITEM(out.ptr(), (Py_ssize_t)i));
+        if (o == nullptr || o->device() != device || o->scalar_type() != g->scalar_type() || o->sizes() != g->sizes()) return false;
+      }
+      sizes.push_back(g->numel());
+      dtypes.push_back(dtype_of(*g));
+      if (g->is_contiguous() && o->is_contiguous()) {
+        grads.push_back(g->const_data_ptr());
+        if (writes) outs.push_back(o->mutable_data_ptr());
+        continue;
+      }
+      if (!g->is_non_overlapping_and_dense()) {
+        hold.push_back(g->contiguous());
+        grads.push_back(hold.back().const_data_ptr());
       } else {
-        back.emplace_back(at::empty_like(kept), o);
-        outs.push_back(back.back().first.data_ptr());
+        grads.push_back(g->const_data_ptr());
+      }
+      if (!writes) continue;
+      if (g->is_non_overlapping_and_dense() && o->strides() == g->strides()) {
+        outs.push_back(o->mutable_data_ptr());
+      } else {      // in the order of what is read
+        back.emplace_back(at::empty_like(g->is_non_overlapping_and_dense() ? *g : hold.back()), *o);
+        outs.push_back(back.back().first.mutable_data_ptr());
       }
     }
     list = {grads.data(), writes ? outs.data() : nullptr, sizes.data(), dtypes.data(), (int64_t)n};
+    return true;
   }
   void finish() {
     for (auto& b : back) b.second.copy_(b.first);
   }
 };
 
-// Whether lists are what the entry points take: alto_b200/grad_clip.py tells what is wrong with the others (or takes the local
-// part of sharded ones).
-bool usual(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs) {
-  if (grads.empty() || (!outs.empty() && outs.size() != grads.size())) return false;
-  const auto device = grads[0].device();
-  const auto fine = [&](const Tensor& t) {
-    return t.defined() && t.is_cuda() && t.device() == device && t.layout() == at::kStrided &&
-           (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) && !t.key_set().has(c10::DispatchKey::Python);
-  };
-  for (size_t i = 0; i < grads.size(); ++i) {
-    if (!fine(grads[i])) return false;
-    if (!outs.empty() && (!fine(outs[i]) || outs[i].scalar_type() != grads[i].scalar_type() || outs[i].sizes() != grads[i].sizes())) return false;
-  }
-  return true;
-}
-
 // (total fp64, norm fp32) of the tensors together
-std::optional<std::pair<Tensor, Tensor>> grad_norm(const std::vector<Tensor>& grads, bool inf) {
-  if (!usual(grads, {})) return std::nullopt;
+std::optional<std::pair<Tensor, Tensor>> grad_norm(const pybind11::list& grads, bool inf) {
   const at::AutoGradMode no_graph(false);
-  const c10::cuda::CUDAGuard device(grads.at(0).device());
-  GradList l(grads, {}, false);
-  const auto options = grads[0].options();
-  Tensor total = at::empty({}, options.dtype(at::kDouble)), norm = at::empty({}, options.dtype(at::kFloat));
-  Tensor work = at::empty({entry.norm_work_bytes(l.list.count)}, options.dtype(at::kByte));
-  check(entry.grad_norm(&l.list, inf, work.data_ptr(), (double*)total.data_ptr(), (float*)norm.data_ptr(),
-                        c10::cuda::getCurrentCUDAStream().stream()), "altob200_grad_norm");
+  GradList l;
+  const c10::cuda::OptionalCUDAGuard device(on_device(grads));
+  if (!l.take(grads, pybind11::list(), false)) return std::nullopt;
+  const auto options = l.first.options();
+  const Tensor total = at::empty({}, options.dtype(at::kDouble)), norm = at::empty({}, options.dtype(at::kFloat));
+  const Tensor work = at::empty({entry.norm_work_bytes(l.list.count)}, options.dtype(at::kByte));
+  check(entry.grad_norm(&l.list, inf, work.data_ptr(), (double*)total.data_ptr(), (float*)norm.data_ptr(), stream_here()), "altob200_grad_norm");
   return std::make_pair(total, norm);
 }
 
-std::optional<Tensor> clip_grads(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs, double max_norm, bool inf, const std::optional<Tensor>& total) {
-  if (!usual(grads, outs)) return std::nullopt;
+std::optional<Tensor> clip_grads(const pybind11::list& grads, const pybind11::list& outs, double max_norm, bool inf,
+                                 const std::optional<Tensor>& total) {
   const at::AutoGradMode no_graph(false);
-  const c10::cuda::CUDAGuard device(grads.at(0).device());
-  GradList l(grads, outs, true);
-  const auto options = grads[0].options();
-  Tensor norm = at::empty({}, options.dtype(at::kFloat)), work;
+  GradList l;
+  const c10::cuda::OptionalCUDAGuard device(on_device(grads));
+  if (!l.take(grads, outs, true)) return std::nullopt;
+  const auto options = l.first.options();
+  const Tensor norm = at::empty({}, options.dtype(at::kFloat));
+  Tensor work;
   if (!total.has_value()) work = at::empty({entry.norm_work_bytes(l.list.count)}, options.dtype(at::kByte));
   check(entry.clip_grads(&l.list, inf, max_norm, total.has_value() ? (const double*)total->data_ptr() : nullptr,
-                         work.defined() ? work.data_ptr() : nullptr, (float*)norm.data_ptr(), c10::cuda::getCurrentCUDAStream().stream()),
-        "altob200_clip_grads");
+                         work.defined() ? work.data_ptr() : nullptr, (float*)norm.data_ptr(), stream_here()), "altob200_clip_grads");
   l.finish();
   return norm;
 }
@@ -446,8 +470,8 @@ PYBIND11_MODULE(_autograd, m) {
         pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("fp8_serve", &fp8_serve, pybind11::call_guard<pybind11::gil_scoped_release>());
   // None: a list that alto_b200/grad_clip.py has to look at
-  m.def("grad_norm", &grad_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
-  m.def("clip_grads", &clip_grads, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("grad_norm", &grad_norm);
+  m.def("clip_grads", &clip_grads);
   // operands as alto_b200/norm.py has checked them
   m.def("rms_norm", [](const Tensor& x, const Tensor& weight, double eps) { return Norm::apply(x, weight, std::optional<Tensor>(), eps)[0]; },
         pybind11::call_guard<pybind11::gil_scoped_release>());

@@ -15,7 +15,7 @@ namespace altob200 {
 constexpr int GN_TENSORS = 1000;            // of a launch
 constexpr int GN_THREADS = 256;
 constexpr int GN_UNROLL = 4;
-constexpr int64_t GN_CHUNK = 16 * GN_THREADS;    // 16-byte vectors of a block's piece
+constexpr int64_t GN_CHUNK = 8 * GN_THREADS;    // 16-byte vectors of a block's piece
 
 struct GradTable {
   const void* g[GN_TENSORS];
@@ -252,7 +252,7 @@ static int64_t pieces_of(const void* g, int64_t n, bool f32) {
   const int64_t p = ceil_div(vectors, GN_CHUNK);
   return p < 1 ? 1 : p;
 }
-constexpr int GN_BLOCKS_PER_SM = 6;
+constexpr int GN_BLOCKS_PER_SM = 8;
 
 // Walks the list a launch at a time.  fn(table, blocks, launch's first partial) -> status
 template <class F>
