@@ -192,7 +192,7 @@ class Fp8BlockGemmArgs(C.Structure):
     """``altob200_fp8_block_gemm_args`` of the header."""
     _fields_ = [(n, C.c_int64) for n in ("M", "N", "K", "lda", "ldd", "k_rows")] + [("a", C.c_void_p), ("b", C.c_void_p),
                 ("sa", Fp8BlockScale), ("sb", Fp8BlockScale), ("offs", C.c_void_p), ("d", C.c_void_p)] + [
-        (n, C.c_int32) for n in ("mode", "experts", "format", "a_dtype", "out_dtype")]
+        (n, C.c_int32) for n in ("mode", "experts", "format", "a_dtype", "out_dtype", "b_ready")]
 
 
 class GradList(C.Structure):

@@ -54,6 +54,9 @@ static inline cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, dim3
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the kernel launched through launch_after() behind this one start already.  Called after grid_dependency_wait(), it also
+// tells that kernel that whatever came before this one is complete: it may read that before its own wait.
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------------------
 // bit casts

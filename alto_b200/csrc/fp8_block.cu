@@ -3,8 +3,9 @@
 //   fp8b_quantize_kernel   rows (blocks of 128 columns), columns (blocks of 128 rows from every expert's first one, codes
 //                          transposed) or both from one read; squares of 128 x 128 in either packing
 //   fp8b_dequantize_kernel values of codes and scales
-//   fp8b_rows_kernel       D = A B^T for few rows of A, which it may quantise itself
-// The products of many rows are in gemm_fp8_block.cuh.
+//   fp8b_rows_kernel       D = A B^T for up to eight rows of numbers, which it quantises itself, and for codes that no other
+//                          kernel takes (lists of experts or places of scales past its limits, no columns to reduce)
+// The products of few rows of codes are in gemm_fp8_stream.cuh, those of many in gemm_fp8_block.cuh.
 #include "fp8_block.cuh"
 
 namespace altob200 {
@@ -26,11 +27,6 @@ struct Fp8bQuant {
 };
 enum { FP8B_ROWS = 1, FP8B_COLS = 2, FP8B_SQUARES = 4 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 // Maxima of two non-negative bf16 a word, by their bits (a NaN is above an infinity).
 __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -266,6 +262,7 @@ __global__ void __launch_bounds__(256) fp8b_quantize_rows_kernel(const Fp8bQuant
   constexpr bool BF16 = sizeof(T) == 2;
   constexpr int U = 2;
   grid_dependency_wait();
+  grid_launch_dependents();          // (products that read their weights meanwhile: altob200_fp8_block_gemm_args.b_ready)
   const int lane = threadIdx.x & 31;
   const int64_t col0 = (int64_t)blockIdx.x * (128 * U) + (lane & 7) * 16;
   for (int64_t at = blockIdx.y; at * 32 < q.rows; at += gridDim.y) {
@@ -572,6 +569,8 @@ static bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) 
 
 // in gemm_sm100.cu: the products of many rows
 int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st);
+// and of few
+int fp8_block_gemm_stream(const altob200_fp8_block_gemm_args* a, int64_t rows_a_run, cudaStream_t st);
 
 }  // namespace altob200
 
@@ -680,10 +679,9 @@ int altob200_fp8_block_gemm(const altob200_fp8_block_gemm_args* a, void* stream)
     return ALTOB200_EINVAL_SHAPE;
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t per_run = a->mode == 1 ? ceil_div(a->M, a->experts) : a->M;
-  if (per_run > 64 || a->mode == 2) {
-    const int rc = fp8_block_gemm_tiles(a, st);
-    if (rc != ALTOB200_EUNSUPPORTED) return rc;
-  }
+  int done = a->mode == 2 || per_run > FP8B_STREAM_ROWS ? ALTOB200_EUNSUPPORTED : fp8_block_gemm_stream(a, per_run, st);
+  if (done == ALTOB200_EUNSUPPORTED && !numbers) done = fp8_block_gemm_tiles(a, st);
+  if (done != ALTOB200_EUNSUPPORTED) return done;
   Fp8bRows q;
   q.M = a->M; q.N = a->N; q.K = a->K;
   q.a = a->a; q.lda = a->lda; q.b = (const uint8_t*)a->b;
@@ -697,15 +695,15 @@ int altob200_fp8_block_gemm(const altob200_fp8_block_gemm_args* a, void* stream)
   q.d = a->d; q.ldd = a->ldd;
   const bool e5 = a->format == ALTOB200_FMT_MXFP8_E5M2;
   const bool wide = ceil_div(a->N, 32) * (a->mode == 0 ? 1 : a->experts) >= 2 * sms();
-  const int tokens = !numbers ? 32 : per_run <= 8 ? 8 : 16;
+  const int tokens = numbers ? 8 : 32;
   int64_t y = ceil_div(per_run, tokens);
   if (y > 65535) y = 65535;
   const dim3 grid((unsigned)ceil_div(a->N, wide ? 32 : 16), (unsigned)y, (unsigned)(a->mode == 1 ? a->experts + 1 : q.experts));
   cudaError_t rc;
 #define ALTOB200_R(T, J) rc = wide ? launch_rows<T, 2, J>(q, grid, e5, st) : launch_rows<T, 1, J>(q, grid, e5, st)
   if (!numbers) { ALTOB200_R(uint8_t, 4); }
-  else if (a->a_dtype == ALTOB200_DT_BF16) { if (tokens == 8) { ALTOB200_R(__nv_bfloat16, 1); } else { ALTOB200_R(__nv_bfloat16, 2); } }
-  else { if (tokens == 8) { ALTOB200_R(float, 1); } else { ALTOB200_R(float, 2); } }
+  else if (a->a_dtype == ALTOB200_DT_BF16) { ALTOB200_R(__nv_bfloat16, 1); }
+  else { ALTOB200_R(float, 1); }
 #undef ALTOB200_R
   return rc == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
 }

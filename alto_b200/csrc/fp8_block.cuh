@@ -11,12 +11,16 @@ namespace altob200 {
 
 constexpr int FP8B = 128;      // numbers of a block
 constexpr float FP8B_LEAST = 1e-12f;
+constexpr int FP8B_STREAM_ROWS = 32;      // most rows of A (of a run, on average) for gemm_fp8_stream.cuh
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 template <bool E5M2>
 __device__ __forceinline__ float fp8b_scale(float amax) {
-  float a;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(amax), "f"(FP8B_LEAST));
-  return __fdiv_rn(a, E5M2 ? 57344.0f : 448.0f);
+  return __fdiv_rn(max_nan(amax, FP8B_LEAST), E5M2 ? 57344.0f : 448.0f);
 }
 // What the quotients by a scale take: (s, RN(1 / s)).  The reciprocal forms of common.cuh hold for every scale there is, 2^-56 to
 // 2^120: a quotient that any code but zero stands for keeps its residual normal, and one below that may be off.  Behind an

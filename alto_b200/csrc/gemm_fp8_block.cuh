@@ -243,6 +243,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   uint64_t* fac_full = acc_empty + 4;             // each CTA: bytes of its own factors
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fac_full + C::FAC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* never = abort_flag + 1;           // an abort flag that nothing raises
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();        // 0 = leader
@@ -260,6 +261,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     }
     for (int f = 0; f < C::FAC; ++f) mbar_init(&fac_full[f], B_ROWS ? 2 : 1);
     *abort_flag = 0;
+    *never = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -297,7 +299,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       struct Scales {
         float a[4], b[2];
       } q[2];
-      uint32_t f_tile_at = pair, f_slot = 0;    // of the factors: next tile, slot of the next chunk
+      uint32_t f_tile_at = pair;    // of the factors: next tile
       int f_left = 0;
       int at_a[4] = {0, 0, 0, 0}, at_b[2] = {0, 0};      // (fewer than 2^31 scales)
       auto request = [&](Scales& v) {
@@ -353,7 +355,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       request(q[0]);
       request(q[1]);
       const bool elected = elect_one();
-      uint32_t s = 0, phase = 1, slot = 0, tile = pair;
+      uint32_t s = 0, phase = 1, slot = 0, tile = pair, stages = 0;
       int left = 0;
       int32_t kx = 0, ya = 0, yb = 0;
       uint32_t fac_bytes = 0;
@@ -398,6 +400,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           kx += 128;
           if (B_ROWS) sb_at += args.sb_chunk;
           --left;
+          ++stages;
           if (++slot == C::FAC) slot = 0;
           if (++s == C::STAGES) {
             s = 0;
@@ -405,7 +408,13 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           }
         }
       }
-      if (!alive) report_timeout(abort_flag, 31);
+      if (!alive) {
+        report_timeout(abort_flag, 31);
+        // the copies in flight land before the CTAs end (both wait for each other below)
+        if (leader)
+          for (uint32_t i = stages < C::STAGES ? 0 : stages - C::STAGES; i < stages; ++i)
+            (void)mbar_wait_tight(smem_u32(&full_bar[i % C::STAGES]), (i / C::STAGES) & 1u, smem_u32(const_cast<int*>(never)), limit);
+      }
     } else if (warp == 1) {
       // ------------------------------ MMA issuer (leader) ------------------------------
       if (leader) {

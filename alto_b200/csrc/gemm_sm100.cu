@@ -36,6 +36,7 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "fp8_block.cuh"
 
 namespace altob200 {
 
@@ -1403,6 +1404,7 @@ gemm_blockscaled_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const _
 
 #include "gemm_macro.cuh"
 #include "gemm_fp8_block.cuh"
+#include "gemm_fp8_stream.cuh"
 
 // ---------------------------------------------------------------------------------------
 // self-test of the bounded waits: every form on barriers that are complete and on one that nobody arrives on
@@ -1963,6 +1965,59 @@ int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st)
   g.wait_ns = wait_limit_ns();
   if (obf) return b_rows ? launch_fp8_block<true, true>(ta, tb, td, g, tiles, st) : launch_fp8_block<true, false>(ta, tb, td, g, tiles, st);
   return b_rows ? launch_fp8_block<false, true>(ta, tb, td, g, tiles, st) : launch_fp8_block<false, false>(ta, tb, td, g, tiles, st);
+}
+
+template <int NW, int J, bool E5M2>
+static int launch_fp8_stream(const CUtensorMap& ta, const CUtensorMap& tb, StreamArgs q, int64_t tiles, cudaStream_t st) {
+  using C = CfgStream;
+  auto kernel = fp8_stream_kernel<NW, J, E5M2>;
+  static std::atomic<int> attr_set[MAX_DEVICES];
+  const int rc = ensure_smem_attr(kernel, C::MOST_SMEM, attr_set);
+  if (rc != ALTOB200_OK) return rc;
+  const int beside = C::beside(NW, J, q.offs != nullptr), room = (C::MOST_SMEM - beside) / C::stage_bytes(NW, J);
+  q.stages = room < C::MOST_STAGES ? room : C::MOST_STAGES;
+  const int64_t sms = sm_count_gemm();
+  // equal shares where their number is known
+  const int64_t grid = q.offs != nullptr ? (tiles < sms ? tiles : sms) : ceil_div(tiles, ceil_div(tiles, sms));
+  const cudaError_t e = launch_after(kernel, dim3((unsigned)grid), dim3(C::THREADS), (size_t)(q.stages * C::stage_bytes(NW, J) + beside), st, ta, tb, q);
+  return e == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
+}
+
+// Products of few rows; EUNSUPPORTED: not for this kernel.
+int fp8_block_gemm_stream(const altob200_fp8_block_gemm_args* a, int64_t rows_a_run, cudaStream_t st) {
+  using C = CfgStream;
+  if (a->mode == 2 || a->K <= 0 || a->a_dtype != -1) return ALTOB200_EUNSUPPORTED;
+  const bool grouped = a->mode == 1, e5 = a->format == ALTOB200_FMT_MXFP8_E5M2;
+  const int J = rows_a_run <= 8 ? 1 : rows_a_run <= 16 ? 2 : 4;
+  const int64_t runs = grouped ? a->experts : 1, units = ceil_div(a->M, 8 * J) + (grouped ? runs + 1 : 0);
+  if (units > C::MAX_UNITS || a->N * runs >= (1ll << 31) || units * ceil_div(a->N, 16) >= (1ll << 31)) return ALTOB200_EUNSUPPORTED;
+  // tiles of 32 rows of B where they fill most SMs
+  const int64_t busy = grouped ? (a->M < runs ? a->M : runs) : units;
+  const bool wide = busy * ceil_div(a->N, 32) >= 100;
+  const int64_t tiles = units * ceil_div(a->N, wide ? 32 : 16);
+  CUtensorMap ta, tb;
+  int rc = make_tmap(&ta, a->a, a->M, a->K, 8 * J);
+  if (rc == ALTOB200_OK) rc = make_tmap(&tb, a->b, a->N * runs, a->K, wide ? 32 : 16);
+  if (rc != ALTOB200_OK) return rc;
+  StreamArgs q;
+  q.M = a->M; q.N = a->N; q.K = a->K;
+  q.a = (const uint8_t*)a->a;
+  q.sa = a->sa.scales; q.sa_row = a->sa.row_stride; q.sa_chunk = a->sa.chunk_stride; q.sa_shift = a->sa.row_shift;
+  q.sb = a->sb.scales; q.sb_row = a->sb.row_stride; q.sb_chunk = a->sb.chunk_stride; q.sb_shift = a->sb.row_shift;
+  q.sb_expert = grouped ? a->sb.expert_stride : 0;
+  q.offs = grouped ? a->offs : nullptr; q.experts = (int)runs;
+  q.out_bf16 = a->out_dtype == ALTOB200_DT_BF16;
+  q.b_ready = a->b_ready;
+  q.d = a->d; q.ldd = a->ldd;
+  q.stages = 0;
+  q.wait_ns = wait_limit_ns();
+#define ALTOB200_S3(NW, J) (e5 ? launch_fp8_stream<NW, J, true>(ta, tb, q, tiles, st) : launch_fp8_stream<NW, J, false>(ta, tb, q, tiles, st))
+#define ALTOB200_S(J) return wide ? ALTOB200_S3(2, J) : ALTOB200_S3(1, J)
+  if (J == 1) ALTOB200_S(1);
+  if (J == 2) ALTOB200_S(2);
+  ALTOB200_S(4);
+#undef ALTOB200_S
+#undef ALTOB200_S3
 }
 
 }  // namespace altob200

@@ -211,17 +211,13 @@ def _check_serving(name: str, x, w_codes, w_scales, dims: int) -> None:
         raise RuntimeError(f"{name} has no gradient: codes of weights serve evaluation")
 
 
-#: most rows (an expert) that the product quantises itself, instead of a launch in front of it
-_FEW_ROWS = 16
-
-
 @L.traced("fp8_block_linear")
 def fp8_block_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
     """x W^T for x [..., K] (bf16 or fp32) and a weight that is there as codes [N, K] and fp32 scales of its squares
     [ceil(N / 128), ceil(K / 128)] (``convert_to_fp8_block(w, is_2d_block=True)``); the result has x's type.  x is quantised in
     the weight's format, in blocks of a row.  Not differentiable."""
     _check_serving("fp8_block_linear", x, w_codes, w_scales, 2)
-    return (L._autograd_module or L.autograd()).fp8_serve(x, w_codes, w_scales, None, _FMT_OF_DTYPE[w_codes.dtype], _FEW_ROWS)
+    return (L._autograd_module or L.autograd()).fp8_serve(x, w_codes, w_scales, None, _FMT_OF_DTYPE[w_codes.dtype])
 
 
 @L.traced("fp8_block_grouped_linear")
@@ -233,7 +229,7 @@ def fp8_block_grouped_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: t
     if x.dim() != 2:
         raise ValueError(f"fp8_block_grouped_linear expects rows [M, K], got {tuple(x.shape)}")
     offs = _ends("fp8_block_grouped_linear", offs, w_codes.shape[0], x.device)
-    return (L._autograd_module or L.autograd()).fp8_serve(x, w_codes, w_scales, offs, _FMT_OF_DTYPE[w_codes.dtype], _FEW_ROWS)
+    return (L._autograd_module or L.autograd()).fp8_serve(x, w_codes, w_scales, offs, _FMT_OF_DTYPE[w_codes.dtype])
 
 
 def _ends(name: str, offs: torch.Tensor, experts: int, device) -> torch.Tensor:

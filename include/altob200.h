@@ -77,7 +77,8 @@ size_t altob200_packed_scale_bytes(int64_t rows, int64_t ncols);
  * {kernel id, block id, wait site, 0}.  Kernel 1 is a GEMM; its wait sites are, for one CTA / a CTA pair / the
  * two-level kernel: free stage 1 / 11 / 21, drained accumulator 2 / 12 / 22, operands 3 / 13 / 23, finished
  * accumulator 4 / 14 / 24, scales in tensor memory 5 / 15 / 25, landed scales 6 / 16 / 26, free scale slot 17.  Of the
- * FP8 block kernel: 31, 32, 33 and 34 (a finished accumulator and its column scales). */
+ * FP8 block kernel: 31, 32, 33 and 34 (a finished accumulator and its column scales); of the one of few rows: free stage 41,
+ * landed stage 42. */
 int altob200_status_read(void* stream, int32_t detail[4]);
 
 #define ALTOB200_CLIP_NONE 0
@@ -716,7 +717,8 @@ int altob200_fp8_block_dequantize(const void* codes, int32_t format, int64_t row
  *   mode 2  the reduced dimension belongs to experts: A [M, K], B [N, K] with K = ld_col of altob200_fp8_block_quantize with
  *           the same `offs` over `k_rows` rows, D [experts][M, N]
  * a_dtype: -1, A is codes; ALTOB200_DT_BF16 / _F32, A is numbers with rows `lda` elements apart, which the kernel quantises
- * along its rows (modes 0 and 1, few rows an expert).  N and K are multiples of 16; codes lie without gaps; everything begins on
+ * along its rows (modes 0 and 1; each eight rows of an expert read its B anew).  b_ready: not 0 where the launch in front of this one is the
+ * altob200_fp8_block_quantize of A and B, sb and offs were complete before that one; they may then be read while it runs.  N and K are multiples of 16; codes lie without gaps; everything begins on
  * 16 bytes.
  */
 typedef struct altob200_fp8_block_gemm_args {
@@ -726,7 +728,7 @@ typedef struct altob200_fp8_block_gemm_args {
   altob200_fp8_block_scale sa, sb;
   const int32_t* offs;
   void* d;
-  int32_t mode, experts, format, a_dtype, out_dtype;
+  int32_t mode, experts, format, a_dtype, out_dtype, b_ready;
 } altob200_fp8_block_gemm_args;
 int altob200_fp8_block_gemm(const altob200_fp8_block_gemm_args* args, void* stream);
 
