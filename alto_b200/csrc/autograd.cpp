@@ -417,8 +417,32 @@ struct GradList {
         outs.push_back(back.back().first.mutable_data_ptr());
       }
     }
+    if (writes) {
+      once(in, out);
+      // what autograd has kept of a tensor that changes is no longer what it was
+      for (size_t i = 0; i < n; ++i) {
+        const Tensor& o = THPVariable_Unpack(PyList_GET_ITEM((out.size() != 0 ? out : in).ptr(), (Py_ssize_t)i));
+        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+      }
+    }
     list = {grads.data(), writes ? outs.data() : nullptr, sizes.data(), dtypes.data(), (int64_t)n};
     return true;
+  }
+  // A tensor that is there twice would be scaled by two blocks at once: refused.  (A table of the addresses, at most half full.)
+  void once(const pybind11::list& in, const pybind11::list& out) const {
+    size_t room = 16;
+    while (room < 2 * sizes.size()) room *= 2;
+    std::vector<const void*> seen(room, nullptr);
+    for (size_t i = 0; i < sizes.size(); ++i) {
+      if (sizes[i] == 0) continue;
+      const void* p = THPVariable_Unpack(PyList_GET_ITEM((out.size() != 0 ? out : in).ptr(), (Py_ssize_t)i)).const_data_ptr();
+      size_t at = (reinterpret_cast<uintptr_t>(p) * 0x9E3779B97F4A7C15ull >> 20) & (room - 1);
+      while (seen[at] != nullptr) {
+        if (seen[at] == p) throw pybind11::value_error("clip_grads expects tensors that do not overlap: one is in the list twice");
+        at = (at + 1) & (room - 1);
+      }
+      seen[at] = p;
+    }
   }
   void finish() {
     for (auto& b : back) b.second.copy_(b.first);

@@ -645,6 +645,9 @@ int altob200_fp8_block_quantize_squares(const void* x, int32_t dtype, int32_t fo
 int altob200_fp8_block_dequantize(const void* codes, int32_t format, int64_t rows, int64_t cols, const altob200_fp8_block_scale* scale,
                                   int32_t out_dtype, void* out, void* stream) {
   if (rows < 0 || cols <= 0 || cols % 8 != 0 || scale == nullptr) return ALTOB200_EINVAL_SHAPE;
+  if ((format != ALTOB200_FMT_MXFP8_E4M3 && format != ALTOB200_FMT_MXFP8_E5M2) || (out_dtype != ALTOB200_DT_BF16 && out_dtype != ALTOB200_DT_F32))
+    return ALTOB200_EUNSUPPORTED;
+  if ((scale->row_shift != 0 && scale->row_shift != 7) || (scale->chunk_shift != 0 && scale->chunk_shift != 7)) return ALTOB200_EINVAL_SHAPE;
   if (rows == 0) return ALTOB200_OK;
   if (codes == nullptr || out == nullptr || scale->scales == nullptr) return ALTOB200_EINVAL_SHAPE;
   if ((reinterpret_cast<uintptr_t>(codes) & 7) || off16(out)) return ALTOB200_EINVAL_ALIGN;

@@ -20,6 +20,7 @@ import torch.utils._pytree as pytree
 from torch import nn
 from torch._prims_common import suggest_memory_format
 
+from . import fp8_block as _fp8_block
 from . import grouped as _grouped
 from . import mxfp4 as _mxfp4
 from . import mxfp8 as _mxfp8
@@ -32,17 +33,20 @@ logger = logging.getLogger("alto_b200")
 _to_mxfp4_then_scaled_mm = _mxfp4._to_mxfp4_then_scaled_mm
 _to_nvfp4_then_scaled_mm = _nvfp4._to_nvfp4_then_scaled_mm
 _to_mxfp8_then_scaled_mm = _mxfp8._to_mxfp8_then_scaled_mm
+_to_fp8_block_then_scaled_mm = _fp8_block._to_fp8_block_then_scaled_mm
 _quantize_then_mxfp_scaled_grouped_mm = _grouped._quantize_then_mxfp_scaled_grouped_mm
 _quantize_then_nvfp4_scaled_grouped_mm = _grouped._quantize_then_nvfp4_scaled_grouped_mm
 _quantize_then_mxfp8_scaled_grouped_mm = _grouped._quantize_then_mxfp8_scaled_grouped_mm
+_quantize_then_fp8_block_scaled_grouped_mm = _grouped._quantize_then_fp8_block_scaled_grouped_mm
 
 
 @dataclass(unsafe_hash=True, kw_only=True, slots=True)
 class TrainingOpConfig:
     """Quantisation recipe of one group of modules (alto/kernels/dispatch/config.py:10-54).
 
-    precision          "mxfp4" | "mxfp8_e4m3" | "mxfp8_e5m2" | "nvfp4" ("amdfp4" is AMD-only: it is
-                       accepted as a value, and refused when a GEMM is dispatched)
+    precision          "mxfp4" | "mxfp8_e4m3" | "mxfp8_e5m2" | "nvfp4" | "fp8_block_e4m3" | "fp8_block_e5m2"
+                       ("amdfp4" is AMD-only: it is accepted as a value, and refused when a GEMM is dispatched;
+                       the two with fp32 scales of blocks of 128 take use_2dblock_w alone, set)
     use_2dblock_x/_w   square blocks for activations / weights
     use_hadamard       randomised Hadamard rotation of the wgrad operands
     use_sr_grad        stochastic rounding of gradients
@@ -52,7 +56,7 @@ class TrainingOpConfig:
     use_uos            7.25 instead of 6 as the MXFP4 target maximum
     """
 
-    precision: Literal["mxfp4", "mxfp8_e4m3", "mxfp8_e5m2", "nvfp4", "amdfp4"]
+    precision: Literal["mxfp4", "mxfp8_e4m3", "mxfp8_e5m2", "nvfp4", "amdfp4", "fp8_block_e4m3", "fp8_block_e5m2"]
     use_2dblock_x: bool
     use_2dblock_w: bool
     use_hadamard: bool
@@ -439,8 +443,42 @@ class MXFP8TrainingWeightWrapperTensor(TrainingWeightWrapperBaseTensor):
         return _passthrough(func, args, kwargs)
 
 
+class FP8BlockTrainingWeightWrapperTensor(TrainingWeightWrapperBaseTensor):
+    """Routes GEMMs to the FP8 path with one fp32 scale for each block of 128: x in blocks of a row, weights in squares.  (The
+    reference has the format in a module of its own, alto/kernels/blockwise_fp8/blockwise_linear.py:161.)"""
+
+    _PRECISION_TO_FP8_VARIANT = {"fp8_block_e4m3": "e4m3", "fp8_block_e5m2": "e5m2"}
+
+    @classmethod
+    def _variant(cls, config: TrainingOpConfig) -> str:
+        assert config.precision in cls._PRECISION_TO_FP8_VARIANT, (
+            f"expected TrainingOpConfig with precision in {tuple(cls._PRECISION_TO_FP8_VARIANT)}, got {config.precision}")
+        assert config.use_2dblock_w and not config.use_2dblock_x, (
+            f"{config.precision} quantises weights in 2-D blocks and activations in blocks of a row: it needs use_2dblock_w, without "
+            "use_2dblock_x.")
+        assert not (config.use_hadamard or config.use_sr_grad or config.use_dge or config.use_uos) and \
+            config.clip_mode == "none" and config.two_level_scaling == "none", (
+                f"{config.precision} does not support Hadamard, stochastic rounding, DGE, UOS, clipping or two-level scaling options.")
+        return cls._PRECISION_TO_FP8_VARIANT[config.precision]
+
+    @classmethod
+    def __torch_function__(cls, func, types, args, kwargs={}):
+        import alto_b200.dispatch as D
+        if func.__name__ == "_grouped_mm":
+            A, B, offs = _grouped_args(cls, args, kwargs)
+            return D._quantize_then_fp8_block_scaled_grouped_mm(A, B, offs=offs, fp8_variant=cls._variant(B.config))
+        if func.__name__ in gemm_ops:
+            A, B, bias = _split_gemm_args(func, args)
+            assert not isinstance(A, cls), f"A should not be a {cls.__name__} for func {func.__name__}"
+            assert isinstance(B, cls), f"B should be a {cls.__name__} for func {func.__name__}"
+            Y = D._to_fp8_block_then_scaled_mm(A, B if func.__name__ == "linear" else B.T, fp8_variant=cls._variant(B.config))
+            return Y if bias is None else Y + bias
+        return _passthrough(func, args, kwargs)
+
+
 torch.serialization.add_safe_globals([
-    MXFP4TrainingWeightWrapperTensor, NVFP4TrainingWeightWrapperTensor, MXFP8TrainingWeightWrapperTensor])
+    MXFP4TrainingWeightWrapperTensor, NVFP4TrainingWeightWrapperTensor, MXFP8TrainingWeightWrapperTensor,
+    FP8BlockTrainingWeightWrapperTensor])
 
 
 def _get_tensor_cls_for_config(config: TrainingOpConfig) -> Type[torch.Tensor]:
@@ -450,6 +488,8 @@ def _get_tensor_cls_for_config(config: TrainingOpConfig) -> Type[torch.Tensor]:
         return MXFP8TrainingWeightWrapperTensor
     if config.precision in ("nvfp4", "amdfp4"):
         return NVFP4TrainingWeightWrapperTensor
+    if config.precision in ("fp8_block_e4m3", "fp8_block_e5m2"):
+        return FP8BlockTrainingWeightWrapperTensor
     raise ValueError(f"Unsupported training op config: {config}")
 
 

@@ -12,7 +12,7 @@ up in fp32 with both scales.  Features (in and out) are multiples of 16, tokens 
 ``grouped._quantize_then_fp8_block_scaled_grouped_mm``.
 
 The reference has this format in a part that its recipes do not reach (alto/kernels/blockwise_fp8/blockwise_linear.py:161);
-recipes name it here as the scheme "fp8_block" (``dispatch.TrainingOpConfig``, ``lpt.LowPrecisionTrainingModifier``)."""
+recipes name it here as the schemes "fp8_block_e4m3" and "fp8_block_e5m2" (``dispatch.TrainingOpConfig``, ``lpt.LowPrecisionTrainingModifier``)."""
 from __future__ import annotations
 
 from typing import Optional, Tuple

@@ -58,7 +58,11 @@ def _local(t: torch.Tensor) -> torch.Tensor:
 
 def _reduced(total: torch.Tensor, inf: bool, group) -> torch.Tensor:
     dist = torch.distributed
-    dist.all_reduce(total, op=dist.ReduceOp.MAX if inf else dist.ReduceOp.SUM, group=group)
+    if inf:      # by their bits: the largest of numbers, and a NaN above them all
+        total = total.abs()
+        dist.all_reduce(total.view(torch.int64), op=dist.ReduceOp.MAX, group=group)
+    else:
+        dist.all_reduce(total, op=dist.ReduceOp.SUM, group=group)
     return total
 
 
@@ -96,8 +100,8 @@ def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0, group=Non
 @L.traced("clip_grads")
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None,
                group=None, error_if_nonfinite: bool = False) -> torch.Tensor:
-    """Scales the tensors to a common norm of at most ``max_norm``, in place or into ``out`` (tensors of the same shapes and types
-    that do not overlap them); returns the norm before, an fp32 scalar.  Where nothing is clipped, tensors scaled in place are not
+    """Scales the tensors (which do not overlap) to a common norm of at most ``max_norm``, in place or into ``out`` (others of the same
+    shapes and types); returns the norm before, an fp32 scalar.  Where nothing is clipped, tensors scaled in place are not
     written.  ``group``: the norm is taken over its ranks.  ``error_if_nonfinite`` waits for the norm and raises before anything
     is scaled."""
     inf, max_norm = _kind(norm_type), float(max_norm)

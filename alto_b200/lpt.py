@@ -1,7 +1,8 @@
 """``LowPrecisionTrainingModifier``: the recipe-facing scheme surface.
 
 Field for field the reference's pydantic model (alto/modifiers/lpt/base.py:29-258): ``scheme``
-(one of mxfp4 / mxfp8_e4m3 / mxfp8_e5m2 / nvfp4 / amdfp4, or a dict scheme -> targets),
+(one of mxfp4 / mxfp8_e4m3 / mxfp8_e5m2 / nvfp4 / amdfp4, here also fp8_block_e4m3 / fp8_block_e5m2, or a dict
+scheme -> targets),
 ``targets``, ``ignore``, the recipe flags, ``lora_rank`` and the de-oscillation knobs, the same
 validators, ``resolved_config`` and the modifier lifecycle (convert / convert_config / initialize /
 pre_step / post_step / finalize, alto/modifiers/base.py:56-113).  ``on_convert`` wraps the
@@ -29,7 +30,7 @@ logger = logging.getLogger("alto_b200")
 
 __all__ = ["LowPrecisionTrainingModifier"]
 
-_SCHEMES = ["mxfp4", "mxfp8_e4m3", "mxfp8_e5m2", "nvfp4", "amdfp4"]
+_SCHEMES = ["mxfp4", "mxfp8_e4m3", "mxfp8_e5m2", "nvfp4", "amdfp4", "fp8_block_e4m3", "fp8_block_e5m2"]
 
 
 def _match_named_modules(model: Module, targets, ignore):
