@@ -15,9 +15,11 @@ The reference has this format in a part that its recipes do not reach (alto/kern
 recipes name it here as the schemes "fp8_block_e4m3" and "fp8_block_e5m2" (``dispatch.TrainingOpConfig``, ``lpt.LowPrecisionTrainingModifier``)."""
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from .nvfp4 import unwrap_weight_wrapper
@@ -92,7 +94,7 @@ def convert_to_fp8_block(data_hp: torch.Tensor, block_size: int = BLOCK_SIZE, fp
     if axis == -1:
         (codes, scales), _ = L.fp8_block_quantize(_rows(x), fmt, True, False)
         return codes.view(data_hp.shape).view(_CODE[fp8_format]), scales.t().reshape(*lead, M, scales.shape[0])
-    x3 = x.reshape(-1, M, N)
+    x3 = x.reshape(math.prod(lead), M, N)
     parts = [L.fp8_block_quantize(_rows(m), fmt, False, True)[1] for m in x3]
     if not parts:
         codes = torch.empty(0, N, _blocks(M) * BLOCK_SIZE, dtype=torch.uint8, device=x.device)
@@ -209,6 +211,8 @@ def _check_serving(name: str, x, w_codes, w_scales, dims: int) -> None:
         raise ValueError(f"{name} expects all tensors on one device")
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError(f"{name} has no gradient: codes of weights serve evaluation")
+    if L.forward_mode() and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, w_scales)):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 @L.traced("fp8_block_linear")

@@ -141,3 +141,63 @@ def test_captured_and_replayed():
         want = [torch.empty_like(t) for t in ts]
         n = GC.clip_grads(ts, 0.1, out=want)
         assert torch.equal(n, norm) and all(torch.equal(a, b) for a, b in zip(into, want))
+
+
+def test_a_tensor_that_is_listed_twice_and_versions():
+    t, u = tensors([70001, 5], [F32])
+    before = t.clone()
+    for bad, out in (([t, u, t], None), ([t, t.view(-1)], None), ([t, t], [u.new_empty(70001)] * 2)):
+        with pytest.raises(ValueError, match="twice"):
+            GC.clip_grads(bad, 1e-3, out=out)
+    assert torch.equal(t, before)
+    empty = t[:0]
+    GC.clip_grads([empty, empty, u], 1e-3)
+    # a graph that holds what is written says so
+    leaf = torch.randn(100, device="cuda").requires_grad_(True)
+    g = torch.randn(100, device="cuda")
+    y = leaf * g
+    GC.clip_grads([g], 1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        GC.clip_grads([torch.randn(100, device="cuda")], 1e-3)
+
+
+def test_refusals():
+    t = torch.ones(8, device="cuda")
+    for bad, kind in (([t.half()], TypeError), ([t, t.cpu()], RuntimeError), ([t.to_sparse()], ValueError), ([t.long()], TypeError)):
+        with pytest.raises(kind):
+            GC.grad_norm(bad)
+        with pytest.raises(kind):
+            GC.clip_grads(bad, 1.0)
+    for out in ([], [t, t], [t[:4]], [t.bfloat16()], [t.view(2, 4)]):
+        with pytest.raises(ValueError):
+            GC.clip_grads([t], 1.0, out=out)
+    assert bool((t == 1).all())
+
+
+@pytest.mark.parametrize("most", [0.0, 1e-30, math.inf])
+def test_extreme_limits(most):
+    ts = tensors([1000, 33], [BF, F32])
+    before = [t.clone() for t in ts]
+    norm = GC.clip_grads(ts, most)
+    if most == math.inf:
+        assert all(torch.equal(a, b) for a, b in zip(ts, before))
+    else:
+        f = most / (float(norm) + 1e-6)
+        assert all(bool(((a.double() - b.double() * f).abs() <= b.double().abs() * f * 2.0 ** -7 + 2.0 ** -133).all()) for a, b in zip(ts, before))
+
+
+def test_on_another_stream_and_two_at_once():
+    lists = [tensors([70001, 5, 300000], [BF, F32], seed=i) for i in range(2)]
+    want = [[t.clone() for t in l] for l in lists]
+    norms = [GC.clip_grads(l, 0.1) for l in want]
+    streams = [torch.cuda.Stream() for _ in lists]
+    torch.cuda.synchronize()
+    got = []
+    for s, l in zip(streams, lists):
+        with torch.cuda.stream(s):
+            got.append(GC.clip_grads(l, 0.1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, norms))
+    assert all(torch.equal(a, b) for l, w in zip(lists, want) for a, b in zip(l, w))
