@@ -365,8 +365,20 @@ struct GradList {
   std::vector<int32_t> dtypes;
   std::vector<Tensor> hold;
   std::vector<std::pair<Tensor, Tensor>> back;      // (copy, where it belongs)
+  std::vector<const Tensor*> written;
+  std::vector<const void*> seen;                    // a table of the addresses that are written, at most half full
   Tensor first;
   altob200_grad_list list = {};
+
+  // A tensor that is there twice would be scaled by two blocks at once: refused.
+  void once(const void* p) {
+    size_t at = (reinterpret_cast<uintptr_t>(p) * 0x9E3779B97F4A7C15ull >> 20) & (seen.size() - 1);
+    while (seen[at] != nullptr) {
+      if (seen[at] == p) throw pybind11::value_error("clip_grads expects tensors that do not overlap: one is in the list twice");
+      at = (at + 1) & (seen.size() - 1);
+    }
+    seen[at] = p;
+  }
 
   static const Tensor* plain(PyObject* o) {
     if (!THPVariable_Check(o)) return nullptr;
@@ -380,7 +392,12 @@ struct GradList {
     const size_t n = in.size();
     if (n == 0 || (out.size() != 0 && out.size() != n)) return false;
     grads.reserve(n), sizes.reserve(n), dtypes.reserve(n);
-    if (writes) outs.reserve(n);
+    if (writes) {
+      outs.reserve(n), written.reserve(n);
+      size_t room = 16;
+      while (room < 2 * n) room *= 2;
+      seen.assign(room, nullptr);
+    }
     c10::Device device(c10::kCPU);
     for (size_t i = 0; i < n; ++i) {
       const Tensor* g = plain(PyList_GET_ITEM(in.ptr(), (Py_ssize_t)i));
@@ -395,6 +412,10 @@ struct GradList {
       if (out.size() != 0) {
         o = plain(PyList_GET_ITEM(out.ptr(), (Py_ssize_t)i));
         if (o == nullptr || o->device() != device || o->scalar_type() != g->scalar_type() || o->sizes() != g->sizes()) return false;
+      }
+      if (writes) {
+        written.push_back(o);
+        if (g->numel() != 0) once(o->const_data_ptr());
       }
       sizes.push_back(g->numel());
       dtypes.push_back(dtype_of(*g));
@@ -417,32 +438,11 @@ struct GradList {
         outs.push_back(back.back().first.mutable_data_ptr());
       }
     }
-    if (writes) {
-      once(in, out);
-      // what autograd has kept of a tensor that changes is no longer what it was
-      for (size_t i = 0; i < n; ++i) {
-        const Tensor& o = THPVariable_Unpack(PyList_GET_ITEM((out.size() != 0 ? out : in).ptr(), (Py_ssize_t)i));
-        if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
-      }
-    }
+    // what autograd has kept of a tensor that changes is no longer what it was
+    for (const Tensor* o : written)
+      if (!o->is_inference()) o->unsafeGetTensorImpl()->bump_version();
     list = {grads.data(), writes ? outs.data() : nullptr, sizes.data(), dtypes.data(), (int64_t)n};
     return true;
-  }
-  // A tensor that is there twice would be scaled by two blocks at once: refused.  (A table of the addresses, at most half full.)
-  void once(const pybind11::list& in, const pybind11::list& out) const {
-    size_t room = 16;
-    while (room < 2 * sizes.size()) room *= 2;
-    std::vector<const void*> seen(room, nullptr);
-    for (size_t i = 0; i < sizes.size(); ++i) {
-      if (sizes[i] == 0) continue;
-      const void* p = THPVariable_Unpack(PyList_GET_ITEM((out.size() != 0 ? out : in).ptr(), (Py_ssize_t)i)).const_data_ptr();
-      size_t at = (reinterpret_cast<uintptr_t>(p) * 0x9E3779B97F4A7C15ull >> 20) & (room - 1);
-      while (seen[at] != nullptr) {
-        if (seen[at] == p) throw pybind11::value_error("clip_grads expects tensors that do not overlap: one is in the list twice");
-        at = (at + 1) & (room - 1);
-      }
-      seen[at] = p;
-    }
   }
   void finish() {
     for (auto& b : back) b.second.copy_(b.first);

@@ -682,7 +682,7 @@ int altob200_fp8_block_gemm(const altob200_fp8_block_gemm_args* a, void* stream)
     return ALTOB200_EINVAL_SHAPE;
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t per_run = a->mode == 1 ? ceil_div(a->M, a->experts) : a->M;
-  int done = a->mode == 2 || per_run > FP8B_STREAM_ROWS ? ALTOB200_EUNSUPPORTED : fp8_block_gemm_stream(a, per_run, st);
+  int done = fp8_block_gemm_stream(a, per_run, st);
   if (done == ALTOB200_EUNSUPPORTED && !numbers) done = fp8_block_gemm_tiles(a, st);
   if (done != ALTOB200_EUNSUPPORTED) return done;
   Fp8bRows q;

@@ -11,7 +11,6 @@ namespace altob200 {
 
 constexpr int FP8B = 128;      // numbers of a block
 constexpr float FP8B_LEAST = 1e-12f;
-constexpr int FP8B_STREAM_ROWS = 32;      // most rows of A (of a run, on average) for gemm_fp8_stream.cuh
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;

@@ -1,9 +1,11 @@
-// FP8 products of few rows of A (32 at most, on average over the experts): B, the weights, streams through shared memory.
+// FP8 products of few rows of A (32, on average over the experts, or what two rounds of tiles hold): B, the weights, streams
+// through shared memory.
 //
 //   D[m, n] = sum over chunks c of 128 along K of sa[m, c] * sb[n, c] * sum_{k in c} A[m, k] * B[n, k]
 //
-// Bound by the reading of B; 1 | 16 | 32 rows past 14336 x 4096 take 15.3 | 20.0 | 30.6 us (B alone: 9.0), past 4096 x 4096
-// 6.1 | 7.3 | 11, 64 rows over 32 experts of 2880 x 2880 45 (33).  33 rows and more go to gemm_fp8_block.cuh (14336 x 4096: 22).
+// Bound by the reading of B up to eight rows, beyond by the matrix instructions (some 4 cycles of an SM each): 1 | 16 | 32 rows
+// past 14336 x 4096 take 15.3 | 20.0 | 30.6 us (B alone: 9.0), 1 | 16 | 24 | 32 past 4096 x 4096 6.1 | 7.3 | 8.2 | 9.6, 64 rows
+// over 32 experts of 2880 x 2880 45 (33).
 // tcgen05 on the same stages, 128 rows of B its M side, takes 17.0 | 18.5 | 21.7 and 8.9 | 10.0 | 12 us: a tile of 128 rows of B
 // leaves 36 of 148 SMs idle at 14336 and has to be split along K below that, at 1.5 us a join.  A CTA (one an SM, a contiguous range of tiles of 16 NW rows of B) keeps its stages of eight chunks of
 // a tile in flight by TMA; a stage's chunks are shared out among eight warps, which take rows of B as the 16-row side of the
