@@ -16,6 +16,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <initializer_list>
+#include <memory>
 #include <optional>
 #include <string>
 #include <utility>
@@ -359,13 +360,13 @@ std::optional<c10::Device> on_device(const pybind11::list& l) {
 // (and back, where it is written).  Thousands of tensors make up a call's host time, so the lists are walked once, without taking
 // references.
 struct GradList {
-  std::vector<const void*> grads;
-  std::vector<void*> outs;
-  std::vector<int64_t> sizes;
-  std::vector<int32_t> dtypes;
+  std::unique_ptr<const void*[]> grads;
+  std::unique_ptr<void*[]> outs;
+  std::unique_ptr<int64_t[]> sizes;
+  std::unique_ptr<int32_t[]> dtypes;
   std::vector<Tensor> hold;
   std::vector<std::pair<Tensor, Tensor>> back;      // (copy, where it belongs)
-  std::vector<const Tensor*> written;
+  std::unique_ptr<c10::TensorImpl*[]> written;
   std::vector<const void*> seen;                    // a table of the addresses that are written, at most half full
   Tensor first;
   altob200_grad_list list = {};
@@ -380,27 +381,33 @@ struct GradList {
     seen[at] = p;
   }
 
-  static const Tensor* plain(PyObject* o) {
+  // The tensor of an object that the kernels can take, or null.  `keys`: those of the one before, which say the same of this one.
+  static const Tensor* plain(PyObject* o, c10::DispatchKeySet& keys) {
     if (!THPVariable_Check(o)) return nullptr;
     const Tensor& t = THPVariable_Unpack(o);
-    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat) &&
-                   !t.key_set().has(c10::DispatchKey::Python)
-               ? &t : nullptr;
+    if (t.key_set() != keys) {
+      if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.key_set().has(c10::DispatchKey::Python)) return nullptr;
+      keys = t.key_set();
+    }
+    return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat ? &t : nullptr;
   }
   // False: a list that alto_b200/grad_clip.py has to look at.
   bool take(const pybind11::list& in, const pybind11::list& out, bool writes) {
     const size_t n = in.size();
-    if (n == 0 || (out.size() != 0 && out.size() != n)) return false;
-    grads.reserve(n), sizes.reserve(n), dtypes.reserve(n);
+    const bool others = out.size() != 0;
+    if (n == 0 || (others && out.size() != n)) return false;
+    grads.reset(new const void*[n]), sizes.reset(new int64_t[n]), dtypes.reset(new int32_t[n]);
     if (writes) {
-      outs.reserve(n), written.reserve(n);
+      outs.reset(new void*[n]), written.reset(new c10::TensorImpl*[n]);
       size_t room = 16;
       while (room < 2 * n) room *= 2;
       seen.assign(room, nullptr);
     }
+    PyObject *const *const items = PySequence_Fast_ITEMS(in.ptr()), *const *const others_items = PySequence_Fast_ITEMS(out.ptr());
     c10::Device device(c10::kCPU);
+    c10::DispatchKeySet keys, out_keys;
     for (size_t i = 0; i < n; ++i) {
-      const Tensor* g = plain(PyList_GET_ITEM(in.ptr(), (Py_ssize_t)i));
+      const Tensor* g = plain(items[i], keys);
       if (g == nullptr) return false;
       if (i == 0) {
         first = *g;
@@ -409,39 +416,36 @@ struct GradList {
         return false;
       }
       const Tensor* o = g;
-      if (out.size() != 0) {
-        o = plain(PyList_GET_ITEM(out.ptr(), (Py_ssize_t)i));
+      if (others) {
+        o = plain(others_items[i], out_keys);
         if (o == nullptr || o->device() != device || o->scalar_type() != g->scalar_type() || o->sizes() != g->sizes()) return false;
       }
+      sizes[i] = g->numel();
+      dtypes[i] = dtype_of(*g);
       if (writes) {
-        written.push_back(o);
-        if (g->numel() != 0) once(o->const_data_ptr());
+        written[i] = o->unsafeGetTensorImpl();
+        outs[i] = o->mutable_data_ptr();
+        if (sizes[i] != 0) once(outs[i]);
       }
-      sizes.push_back(g->numel());
-      dtypes.push_back(dtype_of(*g));
       if (g->is_contiguous() && o->is_contiguous()) {
-        grads.push_back(g->const_data_ptr());
-        if (writes) outs.push_back(o->mutable_data_ptr());
+        grads[i] = g->const_data_ptr();
         continue;
       }
       if (!g->is_non_overlapping_and_dense()) {
         hold.push_back(g->contiguous());
-        grads.push_back(hold.back().const_data_ptr());
+        grads[i] = hold.back().const_data_ptr();
       } else {
-        grads.push_back(g->const_data_ptr());
+        grads[i] = g->const_data_ptr();
       }
-      if (!writes) continue;
-      if (g->is_non_overlapping_and_dense() && o->strides() == g->strides()) {
-        outs.push_back(o->mutable_data_ptr());
-      } else {      // in the order of what is read
-        back.emplace_back(at::empty_like(g->is_non_overlapping_and_dense() ? *g : hold.back()), *o);
-        outs.push_back(back.back().first.mutable_data_ptr());
-      }
+      if (!writes || (g->is_non_overlapping_and_dense() && o->strides() == g->strides())) continue;
+      // in the order of what is read
+      back.emplace_back(at::empty_like(g->is_non_overlapping_and_dense() ? *g : hold.back()), *o);
+      outs[i] = back.back().first.mutable_data_ptr();
     }
     // what autograd has kept of a tensor that changes is no longer what it was
-    for (const Tensor* o : written)
-      if (!o->is_inference()) o->unsafeGetTensorImpl()->bump_version();
-    list = {grads.data(), writes ? outs.data() : nullptr, sizes.data(), dtypes.data(), (int64_t)n};
+    for (size_t i = 0; writes && i < n; ++i)
+      if (!written[i]->is_inference()) written[i]->bump_version();
+    list = {grads.get(), outs.get(), sizes.get(), dtypes.get(), (int64_t)n};
     return true;
   }
   void finish() {

@@ -36,6 +36,10 @@ def _kind(norm_type) -> bool:
     raise ValueError(f"the norms are 2 and inf, got {norm_type}")
 
 
+def _list(tensors) -> list:
+    return tensors if type(tensors) is list else list(tensors)
+
+
 def _refuse(name: str, tensors: Sequence[torch.Tensor], out: Sequence[torch.Tensor] = ()) -> None:
     """Says what is wrong with a list that the kernels do not take."""
     for t in (*tensors, *out):
@@ -89,7 +93,7 @@ def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0, group=Non
     """fp32 scalar: the 2-norm (or the largest magnitude, ``norm_type`` inf) of all tensors together.  ``group``: over the ranks of
     it, each of which holds a part."""
     inf = _kind(norm_type)
-    tensors = list(tensors)
+    tensors = _list(tensors)
     if not tensors:
         if _world(group) > 1:
             raise ValueError("grad_norm over ranks expects a tensor on each")
@@ -105,7 +109,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     written.  ``group``: the norm is taken over its ranks.  ``error_if_nonfinite`` waits for the norm and raises before anything
     is scaled."""
     inf, max_norm = _kind(norm_type), float(max_norm)
-    grads, outs = list(grads), [] if out is None else list(out)
+    grads, outs = _list(grads), [] if out is None else _list(out)
     if not grads:
         if _world(group) > 1:
             raise ValueError("clip_grads over ranks expects a tensor on each")
