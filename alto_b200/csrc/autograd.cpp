@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <memory>
 #include <optional>
@@ -333,10 +334,12 @@ Tensor fp8_serve(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales,
   const Tensor s = w_scales.dim() == 3 ? w_scales : w_scales.unsqueeze(0);
   const int64_t M = x2.size(0);
   const int32_t mode = offs.defined() ? 1 : 0;
-  // Up to eight rows go to a product that quantises them itself, each of its blocks all of a row's numbers: N x K 512 x 512 in
-  // 1.9 us against 3.4 with a launch in front, 2880 x 2880 5.0 against 7.6, 4096 x 4096 6.8 against 7.5, 14336 x 4096 16.2
-  // against 17.0, but 4096 x 14336 18.5 against 14.8.
-  if (M <= 8 && K <= 8192) {
+  // Up to eight rows go to a product that quantises them itself, each of its blocks all of a row's numbers, where a launch in front
+  // is longer than that: N x K 512 x 512 in 1.9 us against 3.4, 4096 x 4096 6.7 against 7.9, 14336 x 4096 16.1 against 16.4, eight
+  // experts of 4096 x 1024 12.5 against 15.0, but 2048 x 8192 9.9 against 8.9, 8192 x 8192 21.7 against 16.5, 28672 x 4096 28.6
+  // against 26.8, eight experts of 4096 x 4096 31.2 against 29.8.
+  const int64_t read = (offs.defined() ? std::min(M, offs.numel()) : 1) * N * K;
+  if (M <= 8 && K <= 6144 && read <= (int64_t)1 << 26) {
     fp8_gemm(x2, altob200_fp8_block_scale{}, w, by_square(s, false), out, (int32_t)fmt, M, N, K, mode, offs, 0);
   } else {
     Coded rows;
@@ -344,6 +347,47 @@ Tensor fp8_serve(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales,
     fp8_gemm(rows.codes, by_row(rows.scales), w, by_square(s, false), out, (int32_t)fmt, M, N, K, mode, offs, 0, true);
   }
   return out;
+}
+
+// The operands of the linears, looked at here: a few attributes of Python's cost as much as a small product takes.  False: what
+// alto_b200/fp8_block.py has to look at, to say what is wrong or to take a wrapper's data.
+bool fp8_number(const Tensor& t) {
+  return t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has(c10::DispatchKey::Python) &&
+         (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat);
+}
+bool fp8_ends(const std::optional<Tensor>& offs, const Tensor& x, int64_t experts) {
+  return offs.has_value() && offs->scalar_type() == at::kInt && offs->device() == x.device() && offs->dim() == 1 && offs->size(0) == experts &&
+         offs->is_contiguous() && experts > 0;
+}
+std::optional<Tensor> fp8_try_serve(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales, const std::optional<Tensor>& offs) {
+  const int64_t dims = offs.has_value() ? 3 : 2;
+  if (!fp8_number(x) || x.dim() < 1 || (dims == 3 && x.dim() != 2) || (at::GradMode::is_enabled() && x.requires_grad())) return std::nullopt;
+  const bool e4 = w_codes.scalar_type() == at::kFloat8_e4m3fn;
+  if ((!e4 && w_codes.scalar_type() != at::kFloat8_e5m2) || w_codes.dim() != dims || w_codes.device() != x.device()) return std::nullopt;
+  const int64_t N = w_codes.size(-2), K = w_codes.size(-1);
+  if (N <= 0 || K <= 0 || N % 16 != 0 || K % 16 != 0 || x.size(-1) != K) return std::nullopt;
+  if (w_scales.scalar_type() != at::kFloat || w_scales.dim() != dims || w_scales.device() != x.device() || w_scales.size(-2) != blocks_of(N) ||
+      w_scales.size(-1) != blocks_of(K))
+    return std::nullopt;
+  if (dims == 3 && (w_scales.size(0) != w_codes.size(0) || !fp8_ends(offs, x, w_codes.size(0)))) return std::nullopt;
+  const pybind11::gil_scoped_release no_gil;
+  return fp8_serve(x, w_codes, w_scales, offs, e4 ? ALTOB200_FMT_MXFP8_E4M3 : ALTOB200_FMT_MXFP8_E5M2);
+}
+Tensor fp8_linear(const Tensor& x, const Tensor& weight, const Tensor& data, const std::optional<Tensor>& offs, int64_t fmt) {
+  // (inside forward every input says what it said before, and the mode is off)
+  const bool graph = at::GradMode::is_enabled();
+  return Fp8Linear::apply(x, weight, data.detach(), offs, fmt, graph && x.requires_grad(), graph && weight.requires_grad());
+}
+std::optional<Tensor> fp8_try_linear(const Tensor& x, const Tensor& w, const std::optional<Tensor>& offs, int64_t fmt) {
+  const int64_t dims = offs.has_value() ? 3 : 2;
+  if (!fp8_number(x) || !fp8_number(w) || x.dim() < 1 || (dims == 3 && x.dim() != 2) || w.dim() != dims || w.scalar_type() != x.scalar_type() ||
+      w.device() != x.device() || x.size(-1) != w.size(1))
+    return std::nullopt;
+  for (int64_t d = dims - 2; d < dims; ++d)
+    if (w.size(d) <= 0 || w.size(d) % 16 != 0) return std::nullopt;
+  if (dims == 3 && !fp8_ends(offs, x, w.size(0))) return std::nullopt;
+  const pybind11::gil_scoped_release no_gil;
+  return fp8_linear(x, w, w, offs, fmt);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -493,15 +537,11 @@ PYBIND11_MODULE(_autograd, m) {
              reinterpret_cast<decltype(entry.fp8_quantize)>(fp8_quantize), reinterpret_cast<decltype(entry.fp8_squares)>(fp8_squares),
              reinterpret_cast<decltype(entry.fp8_gemm)>(fp8_gemm)};
   });
-  m.def("fp8_linear",
-        [](const Tensor& x, const Tensor& weight, const Tensor& data, const std::optional<Tensor>& offs, int64_t fmt) {
-          // (inside forward every input says what it said before, and the mode is off)
-          const bool graph = at::GradMode::is_enabled();
-          return Fp8Linear::apply(x, weight, data.detach(), offs, fmt, graph && x.requires_grad(), graph && weight.requires_grad());
-        },
-        pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("fp8_linear", &fp8_linear, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("fp8_serve", &fp8_serve, pybind11::call_guard<pybind11::gil_scoped_release>());
-  // None: a list that alto_b200/grad_clip.py has to look at
+  // None: operands that alto_b200/fp8_block.py, a list that alto_b200/grad_clip.py has to look at
+  m.def("fp8_try_serve", &fp8_try_serve);
+  m.def("fp8_try_linear", &fp8_try_linear);
   m.def("grad_norm", &grad_norm);
   m.def("clip_grads", &clip_grads);
   // operands as alto_b200/norm.py has checked them

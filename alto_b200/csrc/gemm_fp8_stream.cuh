@@ -3,12 +3,14 @@
 //
 //   D[m, n] = sum over chunks c of 128 along K of sa[m, c] * sb[n, c] * sum_{k in c} A[m, k] * B[n, k]
 //
-// Bound by the reading of B up to eight rows, beyond by the matrix instructions (some 4 cycles of an SM each): 1 | 16 | 32 rows
-// past 14336 x 4096 take 15.3 | 20.0 | 30.6 us (B alone: 9.0), 1 | 16 | 24 | 32 past 4096 x 4096 6.1 | 7.3 | 8.2 | 9.6, 64 rows
-// over 32 experts of 2880 x 2880 45 (33).
+// Bound by the reading of B up to eight rows, beyond by the instructions: 1 | 16 | 32 rows past 14336 x 4096 take 14.4 | 19.2 |
+// 30.4 us (B alone: 9.0), 1 | 16 | 24 | 32 past 4096 x 4096 6.3 | 7.5 | 8.3 | 9.7, 64 rows over 32 experts of 5760 x 2880 80
+// (81 for all of them, some are empty).
 // tcgen05 on the same stages, 128 rows of B its M side, takes 17.0 | 18.5 | 21.7 and 8.9 | 10.0 | 12 us: a tile of 128 rows of B
-// leaves 36 of 148 SMs idle at 14336 and has to be split along K below that, at 1.5 us a join.  A CTA (one an SM, a contiguous range of tiles of 16 NW rows of B) keeps its stages of eight chunks of
-// a tile in flight by TMA; a stage's chunks are shared out among eight warps, which take rows of B as the 16-row side of the
+// leaves 36 of 148 SMs idle at 14336 and has to be split along K below that, at 1.5 us a join.
+//
+// A CTA (one an SM, a contiguous range of tiles of up to 16 NW rows of B) keeps its stages of eight chunks of a tile in flight
+// by TMA; a stage's chunks are shared out among eight warps, which take rows of B as the 16-row side of the
 // matrix instruction and rows of A as the 8-column side, scale a chunk's products and add them in fp32.  The warps' sums are
 // joined through shared memory in their order.  A lane's 16 bytes of a row are four instructions' operands: which of a chunk's
 // numbers meet in one instruction does not matter as long as both sides agree, so nothing is shuffled.  Codes go through the
@@ -18,7 +20,6 @@
 
 struct StreamArgs {
   int64_t M, N, K;
-  const uint8_t* a;        // codes [M, K]
   const float *sa, *sb;
   int64_t sa_row, sa_chunk, sb_row, sb_chunk, sb_expert;
   int sa_shift, sb_shift;
@@ -28,6 +29,7 @@ struct StreamArgs {
   int b_ready;             // B, its scales and `offs` were complete before the launch in front of this one
   void* d;
   int64_t ldd;
+  int rows;                // of B a tile, a multiple of 8 up to 16 NW
   int stages;
   uint64_t wait_ns;
 };
@@ -37,7 +39,7 @@ struct CfgStream {
   static constexpr int MOST_STAGES = 6;
   static constexpr int MAX_UNITS = 1024;                  // 8 J rows of A and their expert
   static constexpr int MOST_SMEM = 232448;
-  __host__ __device__ static constexpr int stage_bytes(int nw, int j) { return 8 * (16 * nw + 8 * j) * 128; }
+  __host__ __device__ static constexpr int stage_bytes(int rows, int j) { return 8 * (rows + 8 * j) * 128; }
   __host__ __device__ static constexpr int part_bytes(int nw, int j) { return 8 * 8 * j * (16 * nw + 1) * 4; }
   __host__ __device__ static constexpr int beside(int nw, int j, bool units) {
     return part_bytes(nw, j) + (units ? MAX_UNITS * 12 : 0) + 1024 /*align*/ + 256 /*barriers*/;
@@ -100,10 +102,11 @@ __device__ __forceinline__ void stream_mma(float (&c)[4], uint32_t a0, uint32_t 
 template <int NW, int J, bool E5M2>
 __global__ void __launch_bounds__(CfgStream::THREADS, 1) fp8_stream_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const StreamArgs q) {
   using C = CfgStream;
-  constexpr int ROWS = 16 * NW, STAGE = C::stage_bytes(NW, J), BOX = ROWS * 128, A_OFF = 8 * BOX, A_BOX = 8 * J * 128;
+  constexpr int A_BOX = 8 * J * 128, PITCH = 16 * NW + 1;
+  const int ROWS = q.rows, STAGE = C::stage_bytes(ROWS, J), BOX = ROWS * 128, A_OFF = 8 * BOX;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* const part = reinterpret_cast<float*>(smem + q.stages * STAGE);               // [8 warps][8 J][ROWS + 1]
+  float* const part = reinterpret_cast<float*>(smem + q.stages * STAGE);               // [8 warps][8 J][PITCH]
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + q.stages * STAGE + C::part_bytes(NW, J));
   uint64_t *const full = bars, *const empty = bars + C::MOST_STAGES;
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(bars + 2 * C::MOST_STAGES);
@@ -306,14 +309,14 @@ __global__ void __launch_bounds__(CfgStream::THREADS, 1) fp8_stream_kernel(const
       for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          part[(warp * 8 * J + 8 * j + 2 * t + (i & 1)) * (ROWS + 1) + 16 * w + g + 8 * (i >> 1)] = acc[w][j][i];
+          part[(warp * 8 * J + 8 * j + 2 * t + (i & 1)) * PITCH + 16 * w + g + 8 * (i >> 1)] = acc[w][j][i];
     if (named_barrier_or(1, 256, !alive)) break;
-    for (int i = threadIdx.x; i < 8 * J * ROWS; i += 256) {
-      const int m = i / ROWS, n = i % ROWS;
-      if (m0 + m >= u.row1 || n0 + n >= q.N) continue;
-      float v = part[m * (ROWS + 1) + n];
+    for (int i = threadIdx.x; i < 8 * J * 16 * NW; i += 256) {
+      const int m = i / (16 * NW), n = i % (16 * NW);
+      if (n >= ROWS || m0 + m >= u.row1 || n0 + n >= q.N) continue;
+      float v = part[m * PITCH + n];
 #pragma unroll
-      for (int w = 1; w < 8; ++w) v += part[(w * 8 * J + m) * (ROWS + 1) + n];
+      for (int w = 1; w < 8; ++w) v += part[(w * 8 * J + m) * PITCH + n];
       const int64_t to = (int64_t)(m0 + m) * q.ldd + n0 + n;
       if (q.out_bf16) static_cast<__nv_bfloat16*>(q.d)[to] = __float2bfloat16_rn(v);
       else static_cast<float*>(q.d)[to] = v;

@@ -1974,12 +1974,12 @@ static int launch_fp8_stream(const CUtensorMap& ta, const CUtensorMap& tb, Strea
   static std::atomic<int> attr_set[MAX_DEVICES];
   const int rc = ensure_smem_attr(kernel, C::MOST_SMEM, attr_set);
   if (rc != ALTOB200_OK) return rc;
-  const int beside = C::beside(NW, J, q.offs != nullptr), room = (C::MOST_SMEM - beside) / C::stage_bytes(NW, J);
+  const int beside = C::beside(NW, J, q.offs != nullptr), room = (C::MOST_SMEM - beside) / C::stage_bytes(q.rows, J);
   q.stages = room < C::MOST_STAGES ? room : C::MOST_STAGES;
   const int64_t sms = sm_count_gemm();
   // equal shares where their number is known
   const int64_t grid = q.offs != nullptr ? (tiles < sms ? tiles : sms) : ceil_div(tiles, ceil_div(tiles, sms));
-  const cudaError_t e = launch_after(kernel, dim3((unsigned)grid), dim3(C::THREADS), (size_t)(q.stages * C::stage_bytes(NW, J) + beside), st, ta, tb, q);
+  const cudaError_t e = launch_after(kernel, dim3((unsigned)grid), dim3(C::THREADS), (size_t)(q.stages * C::stage_bytes(q.rows, J) + beside), st, ta, tb, q);
   return e == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
 }
 
@@ -1994,17 +1994,30 @@ int fp8_block_gemm_stream(const altob200_fp8_block_gemm_args* a, int64_t rows_a_
   const int J = rows_a_run <= 8 ? 1 : rows_a_run <= 16 ? 2 : rows_a_run <= 24 ? 3 : 4;
   const int64_t runs = grouped ? a->experts : 1, units = ceil_div(a->M, 8 * J) + (grouped ? runs + 1 : 0);
   if (units > C::MAX_UNITS || a->N * runs >= (1ll << 31) || units * ceil_div(a->N, 16) >= (1ll << 31)) return ALTOB200_EUNSUPPORTED;
-  // tiles of 32 rows of B where they fill most SMs
-  const int64_t busy = grouped ? (a->M < runs ? a->M : runs) : units;
-  const bool wide = busy * ceil_div(a->N, 32) >= 100;
-  const int64_t tiles = units * ceil_div(a->N, wide ? 32 : 16);
+  // Rows of B a tile: what takes the least time by what a chunk took (ns, eight rows of A; 37% more for each eight more) and 0.3 us
+  // a tile.  14336 x 4096: 56, two tiles on each of 128 SMs, 14.4 us (32: four on 112, 15.2); 28672 x 8192: 32, 44 (56: 45).
+  // More than 32 rows of B with three groups of rows of A do not fit into registers.
+  struct Height {
+    int rows, ns;
+  };
+  static constexpr Height heights[] = {{16, 70}, {32, 100}, {48, 147}, {56, 180}, {64, 194}};
+  const int64_t busy = grouped ? (a->M < runs ? a->M : runs) : units, sms = sm_count_gemm();
+  StreamArgs q;
+  q.rows = 0;
+  double best = 0.0;
+  for (const Height& h : heights) {
+    if (J > 2 && h.rows > 32) break;
+    const double ns = (double)ceil_div(busy * ceil_div(a->N, h.rows), sms) * ((double)ceil_div(a->K, 128) * h.ns * (0.63 + 0.37 * J) + 300.0);
+    if (q.rows != 0 && ns >= best) continue;
+    q.rows = h.rows;
+    best = ns;
+  }
+  const int64_t tiles = units * ceil_div(a->N, q.rows);
   CUtensorMap ta, tb;
   int rc = make_tmap(&ta, a->a, a->M, a->K, 8 * J);
-  if (rc == ALTOB200_OK) rc = make_tmap(&tb, a->b, a->N * runs, a->K, wide ? 32 : 16);
+  if (rc == ALTOB200_OK) rc = make_tmap(&tb, a->b, a->N * runs, a->K, q.rows);
   if (rc != ALTOB200_OK) return rc;
-  StreamArgs q;
   q.M = a->M; q.N = a->N; q.K = a->K;
-  q.a = (const uint8_t*)a->a;
   q.sa = a->sa.scales; q.sa_row = a->sa.row_stride; q.sa_chunk = a->sa.chunk_stride; q.sa_shift = a->sa.row_shift;
   q.sb = a->sb.scales; q.sb_row = a->sb.row_stride; q.sb_chunk = a->sb.chunk_stride; q.sb_shift = a->sb.row_shift;
   q.sb_expert = grouped ? a->sb.expert_stride : 0;
@@ -2015,7 +2028,9 @@ int fp8_block_gemm_stream(const altob200_fp8_block_gemm_args* a, int64_t rows_a_
   q.stages = 0;
   q.wait_ns = wait_limit_ns();
 #define ALTOB200_S3(NW, J) (e5 ? launch_fp8_stream<NW, J, true>(ta, tb, q, tiles, st) : launch_fp8_stream<NW, J, false>(ta, tb, q, tiles, st))
-#define ALTOB200_S(J) return wide ? ALTOB200_S3(2, J) : ALTOB200_S3(1, J)
+#define ALTOB200_S(J) return q.rows > 16 ? ALTOB200_S3(2, J) : ALTOB200_S3(1, J)
+  if (J == 1 && q.rows > 32) return q.rows > 48 ? ALTOB200_S3(4, 1) : ALTOB200_S3(3, 1);
+  if (J == 2 && q.rows > 32) return q.rows > 48 ? ALTOB200_S3(4, 2) : ALTOB200_S3(3, 2);
   if (J == 1) ALTOB200_S(1);
   if (J == 2) ALTOB200_S(2);
   if (J == 3) ALTOB200_S(3);

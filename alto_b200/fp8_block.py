@@ -220,8 +220,13 @@ def fp8_block_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Ten
     """x W^T for x [..., K] (bf16 or fp32) and a weight that is there as codes [N, K] and fp32 scales of its squares
     [ceil(N / 128), ceil(K / 128)] (``convert_to_fp8_block(w, is_2d_block=True)``); the result has x's type.  x is quantised in
     the weight's format, in blocks of a row.  Not differentiable."""
+    host = L._autograd_module or L.autograd()
+    if not L.forward_mode():
+        y = host.fp8_try_serve(x, w_codes, w_scales, None)
+        if y is not None:
+            return y
     _check_serving("fp8_block_linear", x, w_codes, w_scales, 2)
-    return (L._autograd_module or L.autograd()).fp8_serve(x, w_codes, w_scales, None, _FMT_OF_DTYPE[w_codes.dtype])
+    return host.fp8_serve(x, w_codes, w_scales, None, _FMT_OF_DTYPE[w_codes.dtype])
 
 
 @L.traced("fp8_block_grouped_linear")
@@ -229,11 +234,16 @@ def fp8_block_grouped_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: t
     """The same for rows x [M, K] that lie sorted by expert: codes [E, N, K], scales [E, ceil(N / 128), ceil(K / 128)], ``offs``
     [E] the ends of the experts' rows (any number of rows each, none too).  Rows from offs[-1] on give zeros.  Nothing
     synchronises with the host."""
+    host = L._autograd_module or L.autograd()
+    if not L.forward_mode():
+        y = host.fp8_try_serve(x, w_codes, w_scales, offs)
+        if y is not None:
+            return y
     _check_serving("fp8_block_grouped_linear", x, w_codes, w_scales, 3)
     if x.dim() != 2:
         raise ValueError(f"fp8_block_grouped_linear expects rows [M, K], got {tuple(x.shape)}")
     offs = _ends("fp8_block_grouped_linear", offs, w_codes.shape[0], x.device)
-    return (L._autograd_module or L.autograd()).fp8_serve(x, w_codes, w_scales, offs, _FMT_OF_DTYPE[w_codes.dtype])
+    return host.fp8_serve(x, w_codes, w_scales, offs, _FMT_OF_DTYPE[w_codes.dtype])
 
 
 def _ends(name: str, offs: torch.Tensor, experts: int, device) -> torch.Tensor:
@@ -275,13 +285,23 @@ def _to_fp8_block_then_scaled_mm(a: torch.Tensor, b: torch.Tensor, fp8_variant: 
     """a b^T of a training step: a [..., K], b [N, K] (bf16 or fp32, a wrapped weight too), differentiable in both.  a is quantised
     in blocks of a row and b in squares; the gradient of a takes the upstream one in blocks of a row, that of b both in blocks
     of 128 tokens.  What is kept is codes: of a along its columns (where b requires a gradient) and of b."""
+    host = L._autograd_module or L.autograd()
+    if fp8_variant in _FMT:
+        y = host.fp8_try_linear(a, b, None, _FMT[fp8_variant])
+        if y is not None:
+            return y
     w = _plain(b)
     _check_training("_to_fp8_block_then_scaled_mm", a, w, 2, fp8_variant)
-    return (L._autograd_module or L.autograd()).fp8_linear(a, b, w, None, _FMT[fp8_variant])
+    return host.fp8_linear(a, b, w, None, _FMT[fp8_variant])
 
 
 def _grouped(a: torch.Tensor, b: torch.Tensor, offs: torch.Tensor, fp8_variant: str) -> torch.Tensor:
     name = "_quantize_then_fp8_block_scaled_grouped_mm"
+    host = L._autograd_module or L.autograd()
+    if fp8_variant in _FMT:
+        y = host.fp8_try_linear(a, b, offs, _FMT[fp8_variant])
+        if y is not None:
+            return y
     w = _plain(b)
     _check_training(name, a, w, 3, fp8_variant)
-    return (L._autograd_module or L.autograd()).fp8_linear(a, b, w, _ends(name, offs, w.shape[0], a.device), _FMT[fp8_variant])
+    return host.fp8_linear(a, b, w, _ends(name, offs, w.shape[0], a.device), _FMT[fp8_variant])
