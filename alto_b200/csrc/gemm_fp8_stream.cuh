@@ -1,5 +1,5 @@
-// FP8 products of few rows of A (32, on average over the experts, or what two rounds of tiles hold): B, the weights, streams
-// through shared memory.
+// FP8 products of few rows of A (16, or six an expert, or what two rounds of tiles hold): B, the weights, streams through
+// shared memory.
 //
 //   D[m, n] = sum over chunks c of 128 along K of sa[m, c] * sb[n, c] * sum_{k in c} A[m, k] * B[n, k]
 //

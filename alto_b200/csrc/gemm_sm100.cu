@@ -1988,9 +1988,12 @@ int fp8_block_gemm_stream(const altob200_fp8_block_gemm_args* a, int64_t rows_a_
   using C = CfgStream;
   if (a->mode == 2 || a->K <= 0 || a->a_dtype != -1) return ALTOB200_EUNSUPPORTED;
   const bool grouped = a->mode == 1, e5 = a->format == ALTOB200_FMT_MXFP8_E5M2;
-  // Up to 32 rows, and as many as two rounds of tiles of 32 x 32 hold (M x N x K 64 x 1024 x 1024 in 3.6 us, in the tiles of
-  // gemm_fp8_block.cuh 9.1; 256 x 1024 x 4096 15.5 and 19.1; 64 x 4096 x 14336 42 and 52; but 33 x 14336 x 4096 51 and 21).
-  if (rows_a_run > 32 && (grouped || ceil_div(a->M, 32) * ceil_div(a->N, 32) > 2 * sm_count_gemm())) return ALTOB200_EUNSUPPORTED;
+  // Up to 16 rows, and as many as two rounds of tiles of 32 x 32 hold: M x N x K 16 x 28672 x 8192 in 60 us, in the tiles of
+  // gemm_fp8_block.cuh 68; 64 x 1024 x 1024 3.6 and 9.1, 256 x 1024 x 4096 15.5 and 19.1, 32 x 4096 x 14336 23 and 51; but
+  // 24 x 14336 x 4096 24.3 and 24.6, 32 of them 30 and 21.  By expert, where some have twice the average and more and read their B
+  // again, up to six on average: 4 of each of 32 x 5760 x 2880 108 and 132, 8 135 and 141, 16 189 and 143; 8 of each of
+  // 8 x 14336 x 4096 121 and 106.
+  if (grouped ? rows_a_run > 6 : rows_a_run > 16 && ceil_div(a->M, 32) * ceil_div(a->N, 32) > 2 * sm_count_gemm()) return ALTOB200_EUNSUPPORTED;
   const int J = rows_a_run <= 8 ? 1 : rows_a_run <= 16 ? 2 : rows_a_run <= 24 ? 3 : 4;
   const int64_t runs = grouped ? a->experts : 1, units = ceil_div(a->M, 8 * J) + (grouped ? runs + 1 : 0);
   if (units > C::MAX_UNITS || a->N * runs >= (1ll << 31) || units * ceil_div(a->N, 16) >= (1ll << 31)) return ALTOB200_EUNSUPPORTED;
