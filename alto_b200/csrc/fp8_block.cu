@@ -173,7 +173,10 @@ __device__ __forceinline__ void fp8b_emit(const Fp8bQuant& q, const Fp8bTile<T>&
 }
 
 // A tile of 128 rows x 128 columns a CTA (256 threads), 8 x 8 numbers a thread, a warp 32 rows x 64 columns: a row's part of a
-// warp is 128 bytes of bf16, a column's 32 bytes of codes.
+// warp is 128 bytes of bf16, a column's 32 bytes of codes.  8192 x 14336 bf16: both ways 103 us (4.5 TB/s), columns 66 (5.3), squares
+// in both packings 78 (6.0).  Both ways is bound by instructions and their latency (17 an element, two quotients and their
+// encoding among them; 24 warps an SM issue on 55 % of the cycles), the others come near HBM.  Runs of experts add a search
+// of their ends a CTA and their last tiles, which are not full: 65536 x 5760 over 32 experts 366 us (321 without).
 template <class T, int WHAT, bool E5M2>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (WHAT == (FP8B_ROWS | FP8B_COLS) ? 3 : 4) : 2) fp8b_quantize_kernel(const Fp8bQuant q) {
   constexpr bool R = (WHAT & FP8B_ROWS) != 0, C = (WHAT & FP8B_COLS) != 0, S = (WHAT & FP8B_SQUARES) != 0;
@@ -257,6 +260,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (WHAT == (FP8B_ROWS | FP
 }
 
 // Rows alone: eight lanes a block of 128, sixteen numbers a lane, no shared memory; a warp four rows, two blocks of each.
+// Bound by HBM: 8192 x 14336 bf16 60 us (5.9 TB/s).
 template <class T, bool E5M2>
 __global__ void __launch_bounds__(256) fp8b_quantize_rows_kernel(const Fp8bQuant q) {
   constexpr bool BF16 = sizeof(T) == 2;
