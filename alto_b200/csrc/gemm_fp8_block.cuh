@@ -408,13 +408,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
           }
         }
       }
-      if (!alive) {
-        report_timeout(abort_flag, 31);
-        // the copies in flight land before the CTAs end (both wait for each other below)
-        if (leader)
-          for (uint32_t i = stages < C::STAGES ? 0 : stages - C::STAGES; i < stages; ++i)
-            (void)mbar_wait_tight(smem_u32(&full_bar[i % C::STAGES]), (i / C::STAGES) & 1u, smem_u32(const_cast<int*>(never)), limit);
-      }
+      if (!alive) report_timeout(abort_flag, 31);
+      // the copies in flight land before the CTAs end (both wait for each other below), whoever gave up
+      if (leader)
+        for (uint32_t i = stages < C::STAGES ? 0 : stages - C::STAGES; i < stages; ++i)
+          (void)mbar_wait_tight(smem_u32(&full_bar[i % C::STAGES]), (i / C::STAGES) & 1u, smem_u32(const_cast<int*>(never)), limit);
     } else if (warp == 1) {
       // ------------------------------ MMA issuer (leader) ------------------------------
       if (leader) {

@@ -717,9 +717,9 @@ int altob200_fp8_block_dequantize(const void* codes, int32_t format, int64_t row
  *   mode 2  the reduced dimension belongs to experts: A [M, K], B [N, K] with K = ld_col of altob200_fp8_block_quantize with
  *           the same `offs` over `k_rows` rows, D [experts][M, N]
  * a_dtype: -1, A is codes; ALTOB200_DT_BF16 / _F32, A is numbers with rows `lda` elements apart, which the kernel quantises
- * along its rows (modes 0 and 1; each eight rows of an expert read its B anew).  b_ready: not 0 where the launch in front of this one is the
- * altob200_fp8_block_quantize of A and B, sb and offs were complete before that one; they may then be read while it runs.  N and K are multiples of 16; codes lie without gaps; everything begins on
- * 16 bytes.
+ * along its rows (modes 0 and 1; each eight rows of an expert read its B anew).  b_ready: not 0 where the launch in front of
+ * this one is the altob200_fp8_block_quantize of A, and B, sb and offs were complete before that one began; they may then be
+ * read while it runs.  N and K are multiples of 16; codes lie without gaps; everything begins on 16 bytes.
  */
 typedef struct altob200_fp8_block_gemm_args {
   int64_t M, N, K, lda, ldd, k_rows;
