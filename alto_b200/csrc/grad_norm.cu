@@ -10,25 +10,31 @@
 // Squares are summed in fp32 over 32 numbers of a thread and in fp64 from there on; where those 32 leave the range in which
 // fp32 squares are exact to a step (below 2^-80, above 2^100, or not finite) they are summed again in fp64.  Every block leaves
 // one partial sum and they are joined in order: the result does not depend on timing.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace altob200 {
 
-constexpr int GN_TENSORS = 1000;            // of a launch
+// Tensors of a launch.  Short lists travel in a short table: arguments of 28 KB take the host some microseconds.
+constexpr int GN_TENSORS = 1000, GN_FEW = 128;
 constexpr int GN_THREADS = 256;
 constexpr int GN_UNROLL = 4;
 constexpr int64_t GN_CHUNK = 8 * GN_THREADS;    // 16-byte vectors of a block's piece
 
+template <int MOST>
 struct GradTable {
-  const void* g[GN_TENSORS];
-  void* out[GN_TENSORS];
-  int64_t n[GN_TENSORS];                    // elements * 2 + (1: fp32)
-  uint32_t first[GN_TENSORS + 1];           // pieces of the tensors in front
+  static constexpr int SIZE = MOST;
+  const void* g[MOST];
+  void* out[MOST];
+  int64_t n[MOST];                          // elements * 2 + (1: fp32)
+  uint32_t first[MOST + 1];                 // pieces of the tensors in front
   int count;
 };
-static_assert(sizeof(GradTable) <= 30000, "kernel arguments");
+static_assert(sizeof(GradTable<GN_TENSORS>) <= 30000, "kernel arguments");
 
-__device__ __forceinline__ int table_find(const GradTable& t, uint32_t piece) {
+template <int MOST>
+__device__ __forceinline__ int table_find(const GradTable<MOST>& t, uint32_t piece) {
   int lo = 0, hi = t.count - 1;             // the last tensor that begins at or before the piece (empty ones have none)
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -146,8 +152,8 @@ __device__ __forceinline__ void piece_sum(const void* p, int64_t n, int64_t piec
   }
 }
 
-template <bool INF>
-__global__ void __launch_bounds__(GN_THREADS) grad_norm_kernel(const __grid_constant__ GradTable t, double* parts) {
+template <bool INF, int MOST>
+__global__ void __launch_bounds__(GN_THREADS) grad_norm_kernel(const __grid_constant__ GradTable<MOST> t, double* parts) {
   __shared__ double shared[GN_THREADS / 32];
   grid_dependency_wait();
   Sum<INF> s;
@@ -224,7 +230,8 @@ __device__ __forceinline__ void piece_scale(const void* p, void* out, int64_t n,
   }
 }
 
-__global__ void __launch_bounds__(GN_THREADS) grad_scale_kernel(const __grid_constant__ GradTable t, const double* parts, int n_parts, int inf,
+template <int MOST>
+__global__ void __launch_bounds__(GN_THREADS) grad_scale_kernel(const __grid_constant__ GradTable<MOST> t, const double* parts, int n_parts, int inf,
                                                                 double max_norm, float* norm_out) {
   __shared__ double shared[GN_THREADS / 32];
   grid_dependency_wait();
@@ -257,15 +264,15 @@ static int64_t pieces_of(const void* g, int64_t n, bool f32) {
 constexpr int GN_BLOCKS_PER_SM = 8;
 
 // Walks the list a launch at a time.  fn(table, blocks, launch's first partial) -> status
-template <class F>
-static int for_each_launch(const altob200_grad_list* l, int blocks_most, F fn) {
+template <int MOST, class F>
+static int walk_launches(const altob200_grad_list* l, int blocks_most, F fn) {
   int64_t i = 0;
   int parts = 0;
   while (i < l->count) {
-    GradTable t;
+    GradTable<MOST> t;
     t.count = 0;
     int64_t pieces = 0;
-    while (i < l->count && t.count < GN_TENSORS) {
+    while (i < l->count && t.count < MOST) {
       const int64_t n = l->sizes[i];
       const bool f32 = l->dtypes[i] == ALTOB200_DT_F32;
       if (n > 0) {
@@ -288,6 +295,11 @@ static int for_each_launch(const altob200_grad_list* l, int blocks_most, F fn) {
     parts += blocks;
   }
   return ALTOB200_OK;
+}
+
+template <class F>
+static int for_each_launch(const altob200_grad_list* l, int blocks_most, F fn) {
+  return l->count <= GN_FEW ? walk_launches<GN_FEW>(l, blocks_most, fn) : walk_launches<GN_TENSORS>(l, blocks_most, fn);
 }
 
 static int check_list(const altob200_grad_list* l) {
@@ -313,9 +325,10 @@ int64_t altob200_grad_norm_work_bytes(int64_t count) {
 
 static int launch_parts(const altob200_grad_list* l, int norm_inf, double* parts, int* n_parts, cudaStream_t st) {
   *n_parts = 0;
-  return for_each_launch(l, gn_sms() * GN_BLOCKS_PER_SM, [&](const GradTable& t, int blocks, int first) {
-    const cudaError_t e = norm_inf ? launch_after(grad_norm_kernel<true>, dim3(blocks), dim3(GN_THREADS), 0, st, t, parts + first)
-                                   : launch_after(grad_norm_kernel<false>, dim3(blocks), dim3(GN_THREADS), 0, st, t, parts + first);
+  return for_each_launch(l, gn_sms() * GN_BLOCKS_PER_SM, [&](const auto& t, int blocks, int first) {
+    constexpr int MOST = std::decay_t<decltype(t)>::SIZE;
+    const cudaError_t e = norm_inf ? launch_after(grad_norm_kernel<true, MOST>, dim3(blocks), dim3(GN_THREADS), 0, st, t, parts + first)
+                                   : launch_after(grad_norm_kernel<false, MOST>, dim3(blocks), dim3(GN_THREADS), 0, st, t, parts + first);
     *n_parts = first + blocks;
     return e == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
   });
@@ -347,8 +360,9 @@ int altob200_clip_grads(const altob200_grad_list* list, int32_t norm_inf, double
     if (rc != ALTOB200_OK) return rc;
   }
   bool said = false;
-  rc = for_each_launch(list, gn_sms() * GN_BLOCKS_PER_SM, [&](const GradTable& t, int blocks, int) {
-    const cudaError_t e = launch_after(grad_scale_kernel, dim3(blocks), dim3(GN_THREADS), 0, st, t, parts, n, (int)norm_inf, max_norm,
+  rc = for_each_launch(list, gn_sms() * GN_BLOCKS_PER_SM, [&](const auto& t, int blocks, int) {
+    constexpr int MOST = std::decay_t<decltype(t)>::SIZE;
+    const cudaError_t e = launch_after(grad_scale_kernel<MOST>, dim3(blocks), dim3(GN_THREADS), 0, st, t, parts, n, (int)norm_inf, max_norm,
                                        said ? (float*)nullptr : norm);
     said = true;
     return e == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
