@@ -570,7 +570,9 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
               o[e] = pack_bf16_rn(v.x, v.y);
             } else {
               const float2 v = acc[u * (COLS / 2) + q * 2 + (e >> 1)];
-              o[e] = f2u((e & 1) ? v.y : v.x);
+              // (into registers of its own, by an addition of -0: stored from where they are, the sums would have to lie in
+              // fours, and some would spill in the loop above)
+              asm volatile("add.f32 %0, %1, 0f80000000;" : "=r"(o[e]) : "f"((e & 1) ? v.y : v.x));
             }
           }
           st_shared_v4(at + ((((uint32_t)q) ^ sw) << 4), o[0], o[1], o[2], o[3]);
