@@ -419,6 +419,31 @@ def test_results_do_not_change_from_call_to_call():
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
 
 
+def test_a_graph_that_is_used_twice_and_saved_elsewhere():
+    x, w, dy = (H.numbers(s, BF, i).cuda() for i, s in enumerate(((300, 272), (144, 272), (300, 144))))
+    b, offs = H.numbers((2 * 272, 144), BF, 5).cuda().view(2, 272, 144), torch.tensor([100, 290], device="cuda", dtype=torch.int32)
+
+    def grads(twice=False, change=False):
+        xl, wl, bl = (t.clone().requires_grad_(True) for t in (x, w, b))
+        y = FB._to_fp8_block_then_scaled_mm(xl, wl)
+        z = grouped._quantize_then_fp8_block_scaled_grouped_mm(xl, bl, offs=offs)
+        if change:                       # what is kept are codes
+            with torch.no_grad():
+                xl.zero_(), wl.zero_(), bl.zero_()
+        if twice:
+            torch.autograd.grad((y, z), (xl, wl, bl), (dy, dy), retain_graph=True)
+        return torch.autograd.grad((y, z), (xl, wl, bl), (dy, dy))
+    want = grads()
+    assert all(torch.equal(p, q) for p, q in zip(grads(twice=True), want))
+    assert all(torch.equal(p, q) for p, q in zip(grads(change=True), want))
+    with torch.autograd.graph.save_on_cpu():
+        assert all(torch.equal(p, q) for p, q in zip(grads(), want))
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        grads()
+    assert kept and all(t.dtype in (torch.uint8, torch.float32, torch.int32) for t in kept)
+
+
 # ---------------------------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------------------------

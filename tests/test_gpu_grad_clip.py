@@ -201,3 +201,17 @@ def test_on_another_stream_and_two_at_once():
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, norms))
     assert all(torch.equal(a, b) for l, w in zip(lists, want) for a, b in zip(l, w))
+
+
+def test_nothing_in_the_list_and_long_tensors():
+    empty = [torch.empty(0, device="cuda"), torch.empty(0, 5, device="cuda", dtype=BF)]
+    assert float(GC.grad_norm(empty)) == 0.0 and float(GC.clip_grads(empty, 1.0)) == 0.0 and float(GC.clip_grads(empty, 1.0, math.inf)) == 0.0
+    t = torch.zeros(2 ** 31 + 70001, device="cuda", dtype=BF)
+    u = torch.zeros(2 ** 31 + 9, device="cuda", dtype=BF)[1:]          # off 16 bytes
+    t[5], t[-3], u[2 ** 31], u[7] = 1.0, 2.0, 2.0, 4.0
+    assert float(GC.grad_norm([t, u])) == 5.0 and float(GC.grad_norm([t, u], math.inf)) == 4.0
+    assert float(GC.clip_grads([t, u], 2.5)) == 5.0
+    half = 2.5 / (5.0 + 1e-6)
+    for got, want in ((t[5], 1.0), (t[-3], 2.0), (u[2 ** 31], 2.0), (u[7], 4.0)):
+        assert abs(float(got) - want * half) <= want * half * (2.0 ** -8 + 2.0 ** -23)
+    assert int(torch.count_nonzero(t)) == 2 and int(torch.count_nonzero(u)) == 2
