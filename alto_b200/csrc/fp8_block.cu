@@ -128,6 +128,9 @@ __device__ __forceinline__ void transpose4(uint32_t& a, uint32_t& b, uint32_t& c
   d = __byte_perm(ab1, cd1, 0x7632);
 }
 
+// Threads eight rows or columns apart read without conflicts.
+__device__ __forceinline__ int fp8b_slot(int i) { return i + (i >> 3); }
+
 // The codes of a thread's 8 x 8 numbers, along their rows and / or columns, and where they go.
 template <class T, int WHAT, bool E5M2>
 __device__ __forceinline__ void fp8b_emit(const Fp8bQuant& q, const Fp8bTile<T>& t, const float2* row_f, const float2* col_f, int row0, int row_end,
@@ -138,7 +141,7 @@ __device__ __forceinline__ void fp8b_emit(const Fp8bQuant& q, const Fp8bTile<T>&
     uint2 words[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 f = row_f[S ? 0 : r_in + i];
+      const float2 f = row_f[S ? 0 : fp8b_slot(r_in + i)];
       words[i].x = fp8b_word<BF16, E5M2>(t.get(i, 0), t.get(i, 1), t.get(i, 2), t.get(i, 3), f);
       words[i].y = fp8b_word<BF16, E5M2>(t.get(i, 4), t.get(i, 5), t.get(i, 6), t.get(i, 7), f);
       const int64_t r = (int64_t)row0 + r_in + i;
@@ -164,7 +167,7 @@ __device__ __forceinline__ void fp8b_emit(const Fp8bQuant& q, const Fp8bTile<T>&
     uint8_t* const out = q.col_codes + col * q.ld_col + chunk * 128 + r_in;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float2 f = col_f[c_in + j];
+      const float2 f = col_f[fp8b_slot(c_in + j)];
       *reinterpret_cast<uint2*>(out + j * q.ld_col) =
           make_uint2(fp8b_word<BF16, E5M2>(t.get(0, j), t.get(1, j), t.get(2, j), t.get(3, j), f),
                      fp8b_word<BF16, E5M2>(t.get(4, j), t.get(5, j), t.get(6, j), t.get(7, j), f));
@@ -181,7 +184,7 @@ template <class T, int WHAT, bool E5M2>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (WHAT == (FP8B_ROWS | FP8B_COLS) ? 3 : 4) : 2) fp8b_quantize_kernel(const Fp8bQuant q) {
   constexpr bool R = (WHAT & FP8B_ROWS) != 0, C = (WHAT & FP8B_COLS) != 0, S = (WHAT & FP8B_SQUARES) != 0;
   __shared__ float row_max[2][128], col_max[4][128], whole[8];
-  __shared__ float2 row_f[128], col_f[128];      // scale and its reciprocal
+  __shared__ float2 row_f[144], col_f[144];      // scale and its reciprocal, by fp8b_slot
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   int row0 = (int)blockIdx.y * 128, row_end = (int)q.rows;
@@ -245,13 +248,13 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (WHAT == (FP8B_ROWS | FP
   } else if (threadIdx.x < 128) {
     if (R) {
       const float s = fp8b_scale<E5M2>(max_nan(row_max[0][threadIdx.x], row_max[1][threadIdx.x]));
-      row_f[threadIdx.x] = fp8b_divisor(s);
+      row_f[fp8b_slot((int)threadIdx.x)] = fp8b_divisor(s);
       if (row0 + (int)threadIdx.x < row_end) q.row_scales[(int64_t)blockIdx.x * q.rows + row0 + threadIdx.x] = s;
     }
   } else if (C) {
     const int c = (int)threadIdx.x - 128;
     const float s = fp8b_scale<E5M2>(max_nan(max_nan(col_max[0][c], col_max[1][c]), max_nan(col_max[2][c], col_max[3][c])));
-    col_f[c] = fp8b_divisor(s);
+    col_f[fp8b_slot(c)] = fp8b_divisor(s);
     if (col0 + c < q.cols) q.col_scales[chunk * q.cols + col0 + c] = s;
   }
   __syncthreads();
