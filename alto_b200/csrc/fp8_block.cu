@@ -176,10 +176,10 @@ __device__ __forceinline__ void fp8b_emit(const Fp8bQuant& q, const Fp8bTile<T>&
 }
 
 // A tile of 128 rows x 128 columns a CTA (256 threads), 8 x 8 numbers a thread, a warp 32 rows x 64 columns: a row's part of a
-// warp is 128 bytes of bf16, a column's 32 bytes of codes.  8192 x 14336 bf16: both ways 103 us (4.5 TB/s), columns 66 (5.3), squares
+// warp is 128 bytes of bf16, a column's 32 bytes of codes.  8192 x 14336 bf16: both ways 102 us (4.6 TB/s), columns 63 (5.6), squares
 // in both packings 78 (6.0).  Both ways is bound by instructions and their latency (17 an element, two quotients and their
 // encoding among them; 24 warps an SM issue on 55 % of the cycles), the others come near HBM.  Runs of experts add a search
-// of their ends a CTA and their last tiles, which are not full: 65536 x 5760 over 32 experts 366 us (321 without).
+// of their ends a CTA and their last tiles, which are not full: 65536 x 5760 over 32 experts 352 us (309 without).
 template <class T, int WHAT, bool E5M2>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (WHAT == (FP8B_ROWS | FP8B_COLS) ? 3 : 4) : 2) fp8b_quantize_kernel(const Fp8bQuant q) {
   constexpr bool R = (WHAT & FP8B_ROWS) != 0, C = (WHAT & FP8B_COLS) != 0, S = (WHAT & FP8B_SQUARES) != 0;
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? (WHAT == (FP8B_ROWS | FP
   int row0 = (int)blockIdx.y * 128, row_end = (int)q.rows;
   int64_t chunk = blockIdx.y;
   if (!S && q.offs != nullptr) {
-    const Fp8bRun run = fp8b_find(q.offs, q.experts, q.rows, (int)blockIdx.y, 128, false);
+    const Fp8bRun run = fp8b_find(q.offs, q.experts, q.rows, (int)blockIdx.y, 128);
     if (run.expert < 0) return;
     row0 = run.row0 + run.unit * 128;
     row_end = run.row1;

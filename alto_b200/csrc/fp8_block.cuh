@@ -57,30 +57,29 @@ struct Fp8bRun {
   int expert;      // -1: none
   int row0, row1;  // rows of the run
   int unit;        // of the run
-  int first;       // units of the runs in front
 };
-// The run that holds unit `at` where every run is cut into units of `size` rows, by one warp; rows behind the last run are a
-// run of expert `experts` where `behind`.  offs == nullptr: one run of all rows.
-__device__ __forceinline__ Fp8bRun fp8b_find(const int32_t* offs, int experts, int64_t rows, int at, int size, bool behind) {
-  Fp8bRun r = {-1, 0, 0, 0, 0};
-  if (offs == nullptr) {
-    if ((int64_t)at * size < rows) r = {0, 0, (int)rows, at, 0};
-    return r;
-  }
-  const int lane = threadIdx.x & 31, total = experts + (behind ? 1 : 0);
+// The run that holds unit `at` where every run is cut into units of `size` rows, by one warp.
+__device__ __forceinline__ Fp8bRun fp8b_find(const int32_t* offs, int experts, int64_t rows, int at, int size) {
+  Fp8bRun r = {-1, 0, 0, 0};
+  const int lane = threadIdx.x & 31;
   int carry_end = 0, carry_units = 0;
-  for (int e0 = 0; e0 < total; e0 += 32) {
+  for (int e0 = 0; e0 < experts; e0 += 32) {
     const int e = e0 + lane;
-    int end = e < experts ? __ldg(offs + e) : (e == experts && behind) ? (int)rows : 0;
+    int end = e < experts ? __ldg(offs + e) : 0;
     end = end < 0 ? 0 : (int64_t)end > rows ? (int)rows : end;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xFFFFFFFFu, end, d);
-      if (lane >= d && o > end) end = o;
-    }
-    if (end < carry_end) end = carry_end;
     int start = __shfl_up_sync(0xFFFFFFFFu, end, 1);
     if (lane == 0) start = carry_end;
+    if (!__all_sync(0xFFFFFFFFu, end >= start || e >= experts)) {      // not in order
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xFFFFFFFFu, end, d);
+        if (lane >= d && o > end) end = o;
+      }
+      if (end < carry_end) end = carry_end;
+      start = __shfl_up_sync(0xFFFFFFFFu, end, 1);
+      if (lane == 0) start = carry_end;
+    }
+    if (e >= experts) end = start = 0;
     const int n = (end - start + size - 1) / size;
     int sum = n;
 #pragma unroll
@@ -95,11 +94,10 @@ __device__ __forceinline__ Fp8bRun fp8b_find(const int32_t* offs, int experts, i
       r.expert = e0 + src;
       r.row0 = __shfl_sync(0xFFFFFFFFu, start, src);
       r.row1 = __shfl_sync(0xFFFFFFFFu, end, src);
-      r.first = __shfl_sync(0xFFFFFFFFu, before, src);
-      r.unit = at - r.first;
+      r.unit = at - __shfl_sync(0xFFFFFFFFu, before, src);
       return r;
     }
-    carry_end = __shfl_sync(0xFFFFFFFFu, end, 31);
+    carry_end = __shfl_sync(0xFFFFFFFFu, end, 31);      // (of no use behind the last experts)
     carry_units = __shfl_sync(0xFFFFFFFFu, before + n, 31);
   }
   return r;
