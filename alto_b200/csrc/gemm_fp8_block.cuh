@@ -27,7 +27,8 @@
 // columns in two accumulators, which the issuer waits for longer; 1180 / 1240 with the scales loaded by the fold warps (in registers, where
 // a spilled one costs more than the load); 960 / 1310 with them by cp.async; 1330 / 1080 with the factors made by the waiting
 // warp; 905 / 1230 with fold warps that look at the barriers themselves.  A column factor in the 16 x 128-bit layout (eight
-// shared-memory words a lane and 32 columns instead of 32) 2000.  A launch of one chunk a tile takes 7.8 us (2048 x 2048 bf16): some
+// shared-memory words a lane and 32 columns instead of 32) 2000.  Sixteen fold warps of 64 columns instead of eight of 128: 16 to
+// 45 % more a chunk (2048 x 2048, 0.50 us for 0.43, 0.75 for 0.57).  A launch of one chunk a tile takes 7.8 us (2048 x 2048 bf16): some
 // 0.7 to begin, 2.4 to the first chunk (most of it the fetch of instructions that no SM has yet: copies issued before the factors'
 // loads, and prefetched descriptors, took as long or longer), 2.5 for the stores and the end.
 #pragma once
