@@ -888,18 +888,17 @@ def swiglu_kept_backward(codes: torch.Tensor, scales: torch.Tensor, grad_out: to
 
 
 @on_device_of
-def fp8_block_quantize(x2: torch.Tensor, fmt: int, rows: bool, cols: bool, offs: Optional[torch.Tensor] = None):
+def fp8_block_quantize(x2: torch.Tensor, fmt: int, rows: bool, cols: bool):
     """((codes [R, C], scales [C / 128, R]) or None, (codes [C, padded], scales [padded / 128, C]) or None) of x2 [R, C], blocks
-    along its rows and along its columns; ``offs``: ends of the experts' rows, where blocks of rows begin anew."""
+    along its rows and along its columns."""
     (R, n), dev = x2.shape, x2.device
-    a = Fp8BlockQuantArgs(x2.data_ptr(), R, n, x2.stride(0) if R > 1 else n, _ptr(offs), None, None, None, None, 0, _DT_OF[x2.dtype], fmt,
-                          0 if offs is None else offs.numel())
+    a = Fp8BlockQuantArgs(x2.data_ptr(), R, n, x2.stride(0) if R > 1 else n, None, None, None, None, None, 0, _DT_OF[x2.dtype], fmt, 0)
     by_row = by_col = None
     if rows:
         by_row = (torch.empty((R, n), dtype=torch.uint8, device=dev), torch.empty(((n + 127) // 128, R), dtype=torch.float32, device=dev))
         a.row_codes, a.row_scales = by_row[0].data_ptr(), by_row[1].data_ptr()
     if cols:
-        blocks = (R + 127) // 128 if offs is None else R // 128 + offs.numel()
+        blocks = (R + 127) // 128
         by_col = (torch.empty((n, blocks * 128), dtype=torch.uint8, device=dev), torch.empty((blocks, n), dtype=torch.float32, device=dev))
         a.col_codes, a.col_scales, a.ld_col = by_col[0].data_ptr(), by_col[1].data_ptr(), blocks * 128
     if R > 0:
@@ -929,13 +928,10 @@ def fp8_block_dequantize(codes2: torch.Tensor, fmt: int, scales: torch.Tensor, r
 
 
 @on_device_of
-def fp8_block_gemm(a: torch.Tensor, sa: Optional[Fp8BlockScale], b: torch.Tensor, sb: Fp8BlockScale, out: torch.Tensor, fmt: int,
-                   dims, mode: int = 0, offs: Optional[torch.Tensor] = None, k_rows: int = 0) -> None:
-    """``altob200_fp8_block_gemm``: a [M, K] codes, or numbers where ``sa`` is None; ``dims`` = (M, N, K)."""
+def fp8_block_gemm(a: torch.Tensor, sa: Fp8BlockScale, b: torch.Tensor, sb: Fp8BlockScale, out: torch.Tensor, fmt: int, dims) -> None:
+    """``altob200_fp8_block_gemm`` of one matrix: codes a [M, K] and b [N, K]; ``dims`` = (M, N, K)."""
     M, N, K = dims
-    g = Fp8BlockGemmArgs(M, N, K, a.stride(0) if M > 1 else K, N, k_rows, a.data_ptr(), b.data_ptr(), sa or Fp8BlockScale(), sb, _ptr(offs),
-                         out.data_ptr(), mode, 0 if offs is None else offs.numel(), fmt, _DT_OF[a.dtype] if sa is None else -1,
-                         _DT_OF[out.dtype])
+    g = Fp8BlockGemmArgs(M, N, K, K, N, 0, a.data_ptr(), b.data_ptr(), sa, sb, None, out.data_ptr(), 0, 0, fmt, -1, _DT_OF[out.dtype], 0)
     _check((_lib or lib()).altob200_fp8_block_gemm(g, _stream()), "altob200_fp8_block_gemm")
 
 

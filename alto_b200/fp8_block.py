@@ -235,7 +235,7 @@ def fp8_block_grouped_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: t
     [E] the ends of the experts' rows (any number of rows each, none too).  Rows from offs[-1] on give zeros.  Nothing
     synchronises with the host."""
     host = L._autograd_module or L.autograd()
-    if not L.forward_mode():
+    if offs is not None and not L.forward_mode():
         y = host.fp8_try_serve(x, w_codes, w_scales, offs)
         if y is not None:
             return y
@@ -247,12 +247,16 @@ def fp8_block_grouped_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: t
 
 
 def _ends(name: str, offs: torch.Tensor, experts: int, device) -> torch.Tensor:
+    if not isinstance(offs, torch.Tensor):
+        raise ValueError(f"{name} expects offs as int32 [{experts}] on {device}, got {type(offs).__name__}")
     if offs.dtype not in (torch.int32, torch.int64) or offs.dim() != 1 or offs.shape[0] != experts or offs.device != device:
         raise ValueError(f"{name} expects offs as int32 [{experts}] on {device}, got {tuple(offs.shape)}, {offs.dtype} on {offs.device}")
     if experts == 0:
         raise ValueError(f"{name} expects at least one expert")
     if offs.dtype is torch.int32 and offs.is_contiguous():
         return offs
+    if offs.dtype is torch.int64:      # an end past 31 bits is past the buffer, too
+        offs = offs.clamp(-1, 2 ** 31 - 1)
     return offs.to(torch.int32).contiguous()
 
 
@@ -298,7 +302,7 @@ def _to_fp8_block_then_scaled_mm(a: torch.Tensor, b: torch.Tensor, fp8_variant: 
 def _grouped(a: torch.Tensor, b: torch.Tensor, offs: torch.Tensor, fp8_variant: str) -> torch.Tensor:
     name = "_quantize_then_fp8_block_scaled_grouped_mm"
     host = L._autograd_module or L.autograd()
-    if fp8_variant in _FMT:
+    if offs is not None and fp8_variant in _FMT:
         y = host.fp8_try_linear(a, b, offs, _FMT[fp8_variant])
         if y is not None:
             return y

@@ -43,6 +43,8 @@ def _list(tensors) -> list:
 def _refuse(name: str, tensors: Sequence[torch.Tensor], out: Sequence[torch.Tensor] = ()) -> None:
     """Says what is wrong with a list that the kernels do not take."""
     for t in (*tensors, *out):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} expects tensors, got {type(t).__name__}")
         if t.layout is not torch.strided:
             raise ValueError(f"{name} expects dense tensors, got {t.layout}")
         if not t.is_cuda:

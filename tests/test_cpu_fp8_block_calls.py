@@ -23,6 +23,13 @@ def test_host_tensors_are_refused():
             call()
 
 
+def test_what_is_not_a_tensor():
+    for bad in ([None], [1.0]):
+        for call in (lambda: GC.grad_norm(bad), lambda: GC.clip_grads(bad, 1.0)):
+            with pytest.raises(TypeError, match="expects tensors"):
+                call()
+
+
 def test_norms_and_lists():
     assert float(GC.grad_norm([])) == 0.0 and float(GC.clip_grads([], 1.0)) == 0.0
     assert float(GC.clip_grad_norm_([torch.nn.Parameter(torch.zeros(2))], 1.0)) == 0.0

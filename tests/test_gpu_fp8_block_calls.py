@@ -161,6 +161,15 @@ def test_one_gradient_alone(part):
     H.assert_within(served, *H.product_bound(H.quantize(x.cpu(), "e4m3", -1)[2], H.quantize(w.cpu(), "e4m3", None)[2], BF))
 
 
+def test_one_token_without_a_dimension_for_it():
+    x, w, dy = H.numbers((272,), BF, 1).cuda().requires_grad_(True), H.numbers((144, 272), BF, 2).cuda().requires_grad_(True), H.numbers((144,), BF, 3).cuda()
+    y = FB._to_fp8_block_then_scaled_mm(x, w)
+    got = (y, *torch.autograd.grad(y, (x, w), dy))
+    z = FB._to_fp8_block_then_scaled_mm(x[None], w)
+    want = (z, *torch.autograd.grad(z, (x, w), dy[None]))
+    assert y.shape == (144,) and all(torch.equal(a, b.view(a.shape)) for a, b in zip(got, want))
+
+
 def test_no_rows():
     w, x = torch.randn(48, 64, device="cuda", dtype=BF).requires_grad_(True), torch.zeros(0, 64, device="cuda", dtype=BF).requires_grad_(True)
     y = FB._to_fp8_block_then_scaled_mm(x, w)
@@ -235,6 +244,23 @@ def test_ends_of_sixty_four_bits_and_bad_ones():
         assert all(torch.equal(p, q) for p, q in zip(a, b))
         a, b = (run(torch.tensor(o, device="cuda", dtype=torch.int32).clamp(max=40 if o is like else 2 ** 31 - 1), 40) for o in (bad, like))
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_ends_past_thirty_one_bits_and_none():
+    x, w = H.numbers((40, 272), BF, 1).cuda(), H.numbers((2 * 144, 272), BF, 2, 0.1).cuda().view(2, 144, 272)
+    codes, scales = FB.convert_to_fp8_block(w, is_2d_block=True)
+    for ends, like in (([2 ** 32 + 5, 2 ** 40], [40, 40]), ([7, 2 ** 33], [7, 40]), ([-2 ** 40, 2 ** 32], [0, 40])):
+        a, b = torch.tensor(ends, device="cuda"), torch.tensor(like, device="cuda", dtype=torch.int32)
+        assert torch.equal(FB.fp8_block_grouped_linear(x, codes, scales, a), FB.fp8_block_grouped_linear(x, codes, scales, b))
+        assert torch.equal(grouped._quantize_then_fp8_block_scaled_grouped_mm(x, w.transpose(1, 2), offs=a),
+                           grouped._quantize_then_fp8_block_scaled_grouped_mm(x, w.transpose(1, 2), offs=b))
+    for bad in (None, [7, 40]):                 # (nor is a matrix taken for the experts' then)
+        for c, s in ((codes, scales), (codes[0], scales[0])):
+            with pytest.raises((ValueError, TypeError)):
+                FB.fp8_block_grouped_linear(x, c, s, bad)
+        for b in (w.transpose(1, 2), w[0], w[0].t()):
+            with pytest.raises((ValueError, TypeError)):
+                grouped._quantize_then_fp8_block_scaled_grouped_mm(x, b, offs=bad)
 
 
 @pytest.mark.parametrize("m", [4, 24, 300])

@@ -165,7 +165,7 @@ def test_a_tensor_that_is_listed_twice_and_versions():
 
 def test_refusals():
     t = torch.ones(8, device="cuda")
-    for bad, kind in (([t.half()], TypeError), ([t, t.cpu()], RuntimeError), ([t.to_sparse()], ValueError), ([t.long()], TypeError)):
+    for bad, kind in (([t.half()], TypeError), ([t, t.cpu()], RuntimeError), ([t.to_sparse()], ValueError), ([t.long()], TypeError), ([t, None], TypeError)):
         with pytest.raises(kind):
             GC.grad_norm(bad)
         with pytest.raises(kind):
