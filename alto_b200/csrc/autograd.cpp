@@ -1,10 +1,12 @@
-// Autograd function of the RMS norm, compiled against torch: allocation, stream, device and graph in C++ around the C ABI's
-// two entry points.
+// Autograd functions of the RMS norm and of the FP8 block linears, serving by their codes, and the walk over lists of gradients,
+// compiled against torch: allocation, stream, device and graph in C++ around the C ABI's entry points.
 //
 // A step of a few thousand rows takes 6 to 20 us of kernels; as a Python function each way it took the host 93 us (forward 27,
 // and behind each of autograd's two changes of thread a cold interpreter: 21 for a backward pass that takes 15 when warm),
 // more than a string of tensor operations that keeps no graph.  1023 x 1537 fp32: 65 us a step (98 before), tensor operations
-// 84 to 86; 8192 x 4096 bf16 with residual 90 us (117 before) for 88 of kernels.
+// 84 to 86; 8192 x 4096 bf16 with residual 90 us (117 before) for 88 of kernels.  A step of an FP8 block linear, 513 x 768 x 1040 fp32:
+// 208 us as a Python function, 95 here (47 as a captured graph; a step of one elementwise product takes 57); 24 tokens past a
+// 4096 x 4096 weight 12.3 us with the operands looked at in Python, 9.8 here.
 //
 // The library stays free of torch: its entry points come as addresses from the handle that alto_b200/_lib.py holds.
 #include <ATen/ATen.h>

@@ -367,7 +367,9 @@ __global__ void __launch_bounds__(256) fp8b_dequantize_kernel(const Fp8bDequant 
 // scaled and added in fp32, the warps' sums joined through shared memory in their order.
 // A lane's 16 bytes of a row are two instructions' operands: which of a chunk's numbers meet in one instruction does not
 // matter as long as both sides agree, so nothing is shuffled.  FUSED: A is bf16 or fp32 and a lane makes the codes of the
-// numbers that it needs, so that a token's step is one launch.
+// numbers that it needs, so that a token's step is one launch: 1 | 8 rows past 14336 x 4096 take 16.1 | 16.4 us (B alone 9.0), past
+// 4096 x 4096 6.7 (2.6), 512 x 512 1.9.  (Codes that gemm_fp8_stream.cuh takes are faster there: this instruction converts
+// both sides' 8 bits on every use.)
 struct Fp8bRows {
   int64_t M, N, K;
   const void* a;         // codes [M, K], or numbers (FUSED, lda)
