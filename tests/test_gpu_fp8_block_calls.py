@@ -432,6 +432,26 @@ def test_weights_that_were_just_written(m):
         codes.zero_()
 
 
+@pytest.mark.parametrize("m,n,k", [(8, 4096, 1024), (300, 4096, 2048), (2000, 272, 400), (2000, 1040, 4096)])
+def test_operands_that_were_just_written(m, n, k):
+    """Both operands may come from the launches in front, and go right behind."""
+    xs, ws = [torch.randn(m, k, device="cuda", dtype=BF) for _ in range(2)], [torch.randn(n, k, device="cuda", dtype=BF) for _ in range(2)]
+    dy = torch.randn(m, n, device="cuda", dtype=BF)
+
+    def step(x, w):
+        xl, wl = x.requires_grad_(True), w.requires_grad_(True)
+        y = FB._to_fp8_block_then_scaled_mm(xl, wl)
+        return (y.detach(), *torch.autograd.grad(y, (xl, wl), dy))
+    want = [step(x.clone(), w.clone()) for x, w in zip(xs, ws)]
+    for i in range(20):
+        x, w = xs[i % 2].mul(1.0), ws[i % 2].mul(1.0)
+        got = step(x, w)
+        with torch.no_grad():
+            x.zero_(), w.zero_()
+        del x, w
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i % 2]))
+
+
 def test_results_do_not_change_from_call_to_call():
     x, w, dy = torch.randn(2000, 1040, device="cuda", dtype=BF), torch.randn(784, 1040, device="cuda", dtype=BF), torch.randn(2000, 784, device="cuda", dtype=BF)
 
