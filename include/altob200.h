@@ -713,7 +713,7 @@ int altob200_fp8_block_dequantize(const void* codes, int32_t format, int64_t row
  * D[m, n] = sum over blocks c of 128 along K of sa[m, c] sb[n, c] (sum over k in c of A[m, k] B[n, k]), sums in fp32.
  *   mode 0  A [M, K], B [N, K]
  *   mode 1  rows of A belong to experts, `offs` (device): their ends; B [experts][N, K].  Any number of rows an expert; rows
- *           behind the last expert give zeros.
+ *           behind the last expert give zeros.  Ends out of order or outside the rows are taken as a running maximum cut off at M.
  *   mode 2  the reduced dimension belongs to experts: A [M, K], B [N, K] with K = ld_col of altob200_fp8_block_quantize with
  *           the same `offs` over `k_rows` rows, D [experts][M, N]
  * a_dtype: -1, A is codes; ALTOB200_DT_BF16 / _F32, A is numbers with rows `lda` elements apart, which the kernel quantises

@@ -263,6 +263,47 @@ def test_ends_past_thirty_one_bits_and_none():
                 grouped._quantize_then_fp8_block_scaled_grouped_mm(x, b, offs=bad)
 
 
+def in_order(ends, rows):
+    """The running maximum of ends that are cut off at the rows."""
+    return torch.cummax(ends.clamp(0, rows), 0)[0].to(torch.int32)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,e", [(1, 2), (5, 3), (8, 4), (8, 40), (20, 4), (24, 40), (90, 3), (8, 1500), (20, 1500), (300, 1500)])
+def test_bad_ends_in_every_product(m, e, dtype):
+    # up to eight rows, few an expert, many an expert, more experts than the lists hold
+    n, k = 48, 272
+    x, w = H.numbers((m, k), dtype, 1).cuda(), H.numbers((e * n, k), dtype, 2, 0.1).cuda().view(e, n, k)
+    dy = H.numbers((m, n), dtype, 3).cuda()
+    codes, scales = FB.convert_to_fp8_block(w, is_2d_block=True)
+
+    def run(offs):
+        xl, b = x.clone().requires_grad_(True), w.transpose(1, 2).clone().requires_grad_(True)
+        y = grouped._quantize_then_fp8_block_scaled_grouped_mm(xl, b, offs=offs)
+        return (FB.fp8_block_grouped_linear(x, codes, scales, offs), y, *torch.autograd.grad(y, (xl, b), dy))
+    g = torch.Generator().manual_seed(m * e)
+    lists = [torch.randint(-2, m + 3, (e,), generator=g) for _ in range(4)]
+    lists += [torch.full((e,), m), torch.arange(e, 0, -1) * m // e, torch.cat([torch.tensor([m]), torch.zeros(e - 1, dtype=torch.long)])]
+    for ends in lists:
+        want = run(in_order(ends, m).cuda())
+        for _ in range(3):
+            assert all(torch.equal(p, q) for p, q in zip(run(ends.to(torch.int32).cuda()), want))
+
+
+@pytest.mark.parametrize("ends", [[5, 3, 8], [8, 3, 1], [6, 2, 8], [3, -4, 2], [99, 0, 1]], ids=str)
+def test_bad_ends_of_up_to_eight_rows_against_the_formula(ends):
+    m, n, k = 8, 144, 400
+    x, w = H.numbers((m, k), F32, 1), H.numbers((3 * n, k), F32, 2, 0.1).view(3, n, k)
+    codes, scales = FB.convert_to_fp8_block(w.cuda(), is_2d_block=True)
+    got = FB.fp8_block_grouped_linear(x.cuda(), codes, scales, torch.tensor(ends, device="cuda", dtype=torch.int32))
+    a, at = H.quantize(x, "e4m3", -1)[2], 0
+    for e, end in enumerate(in_order(torch.tensor(ends), m).tolist()):
+        exact, bound = H.product_bound(a[at:end], H.quantize(w[e], "e4m3", None)[2], F32)
+        H.assert_within(got[at:end], exact, bound, f"expert {e}")
+        at = end
+    assert not bool(got[at:].any())
+
+
 @pytest.mark.parametrize("m", [4, 24, 300])
 def test_numbers_that_are_not_finite_stay_in_their_blocks(m):
     n, k = 272, 400
