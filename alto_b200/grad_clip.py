@@ -62,6 +62,34 @@ def _local(t: torch.Tensor) -> torch.Tensor:
     return unwrap_weight_wrapper(t) if hasattr(t, "_data") else t
 
 
+def _sharded(t) -> bool:
+    return hasattr(t, "placements") and hasattr(t, "device_mesh")
+
+
+def _holders(name: str, t: torch.Tensor, group) -> tuple:
+    """The process groups over whose ranks a tensor's parts lie, one behind the other: of a sharded tensor the mesh says them, and
+    ``group`` has to be of the same ranks; any other tensor is a part of ``group``'s, or whole where there is none."""
+    dist = torch.distributed
+    given = (group,) if _world(group) > 1 else ()
+    if not _sharded(t):
+        return given
+    mesh, split = t.device_mesh, []
+    for d, p in enumerate(t.placements):
+        if mesh.size(d) == 1 or p.is_replicate():
+            continue
+        if not (p.is_shard() or hasattr(p, "split_factor")):      # (a shard of a shard says no to is_shard)
+            raise ValueError(f"{name} expects gradients that are reduced over their mesh, got the placements {t.placements}")
+        split.append(d)
+    if group is None:
+        return tuple(mesh.get_group(d) for d in split)
+    here = mesh.get_coordinate()
+    ranks = mesh.mesh[tuple(slice(None) if d in split else here[d] for d in range(mesh.ndim))].flatten().tolist()
+    if sorted(ranks) != sorted(dist.get_process_group_ranks(group)):
+        raise ValueError(f"{name} over the ranks {dist.get_process_group_ranks(group)} expects tensors whose parts lie on these, got one with the "
+                         f"placements {t.placements} whose parts lie on {ranks}; without a group the norm is taken over each one's mesh")
+    return given
+
+
 def _reduced(total: torch.Tensor, inf: bool, group) -> torch.Tensor:
     dist = torch.distributed
     if inf:      # by their bits: the largest of numbers, and a NaN above them all
@@ -78,22 +106,39 @@ def _world(group) -> int:
 
 
 def _norm(name: str, tensors: Sequence[torch.Tensor], inf: bool, group):
-    """(total, norm), over the ranks of ``group`` too."""
+    """(total, norm), over the ranks of ``group`` and of the tensors' meshes too."""
     host = L._autograd_module or L.autograd()
-    got = host.grad_norm(tensors, inf) or host.grad_norm([_local(t) for t in tensors], inf)
-    if got is None:
-        _refuse(name, tensors)
-    total, norm = got
-    if _world(group) > 1:
-        total = _reduced(total, inf, group)
-        norm = (total if inf else total.sqrt()).float()
-    return total, norm
+    got = host.grad_norm(tensors, inf)
+    if got is not None:
+        total, norm = got
+        if _world(group) > 1:
+            total = _reduced(total, inf, group)
+            norm = (total if inf else total.sqrt()).float()
+        return total, norm
+    parts: dict = {}           # the groups' names -> (groups, tensors whose parts lie on them)
+    for t in tensors:
+        groups = _holders(name, t, group)
+        parts.setdefault(tuple(g.group_name for g in groups), (groups, []))[1].append(_local(t))
+    totals = []
+    for _, local in parts.values():
+        got = host.grad_norm(local, inf)
+        if got is None:
+            _refuse(name, tensors)
+        totals.append(got[0])
+    for i, (groups, _) in enumerate(parts.values()):
+        for g in groups:
+            totals[i] = _reduced(totals[i], inf, g)
+    total = totals[0]
+    if len(totals) > 1:
+        total = torch.stack(totals).amax() if inf else torch.stack(totals).sum()
+    return total, (total if inf else total.sqrt()).float()
 
 
 @L.traced("grad_norm")
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0, group=None) -> torch.Tensor:
-    """fp32 scalar: the 2-norm (or the largest magnitude, ``norm_type`` inf) of all tensors together.  ``group``: over the ranks of
-    it, each of which holds a part."""
+    """fp32 scalar: the 2-norm (or the largest magnitude, ``norm_type`` inf) of all tensors together, of DTensors as whole ones:
+    over the ranks of their meshes that they are sharded over (replicas count once).  ``group``: over the ranks of it, each of
+    which holds a part of everything; DTensors have to be sharded over just these."""
     inf = _kind(norm_type)
     tensors = _list(tensors)
     if not tensors:
@@ -108,8 +153,8 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
                group=None, error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the tensors (which do not overlap) to a common norm of at most ``max_norm``, in place or into ``out`` (others of the same
     shapes and types); returns the norm before, an fp32 scalar.  Where nothing is clipped, tensors scaled in place are not
-    written.  ``group``: the norm is taken over its ranks.  ``error_if_nonfinite`` waits for the norm and raises before anything
-    is scaled."""
+    written.  DTensors and ``group``: as ``grad_norm`` takes them; ``out`` is sharded like ``grads``, and a norm over ranks needs the call
+    on all of them.  ``error_if_nonfinite`` waits for the norm and raises before anything is scaled."""
     inf, max_norm = _kind(norm_type), float(max_norm)
     grads, outs = _list(grads), [] if out is None else _list(out)
     if not grads:
@@ -128,15 +173,23 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     host = L._autograd_module or L.autograd()
     got = host.clip_grads(grads, outs, max_norm, inf, total)
     if got is None:
+        whole = [_sharded(t) for t in (*grads, *outs)]
+        if any(whole):
+            for g, o in zip(grads, outs):
+                if _sharded(g) != _sharded(o) or (_sharded(g) and (g.placements != o.placements or g.device_mesh != o.device_mesh)):
+                    raise ValueError("clip_grads expects out like grads: as many tensors, of their shapes and types, sharded like them")
+            if total is None:
+                total, _ = _norm("clip_grads", grads, inf, group)
         got = host.clip_grads([_local(g) for g in grads], [_local(o) for o in outs], max_norm, inf, total)
-    if got is None:
-        _refuse("clip_grads", grads, outs)
+        if got is None:
+            _refuse("clip_grads", grads, outs)
+        torch.autograd.graph.increment_version([t for t in outs or grads if _sharded(t) and not t.is_inference()])
     return got
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False, group=None) -> torch.Tensor:
-    """``clip_grads`` of the gradients that the parameters have (sharded ones by their local part, with ``group``)."""
+    """``clip_grads`` of the gradients that the parameters have, DTensors among them (their norm is taken over the mesh)."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     return clip_grads([p.grad for p in parameters if p.grad is not None], max_norm, norm_type, None, group, error_if_nonfinite)

@@ -203,6 +203,32 @@ def test_on_another_stream_and_two_at_once():
     assert all(torch.equal(a, b) for l, w in zip(lists, want) for a, b in zip(l, w))
 
 
+def test_sharded_tensors_of_a_mesh_of_one():
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor, Replicate, Shard
+    dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cuda", (1,))
+        ts = tensors([70001, 5, 300000, 0], [BF, F32])
+        want = [t.clone() for t in ts]
+        norm = GC.clip_grads(want, 0.1)
+        sharded = [DTensor.from_local(t.clone(), mesh, [Shard(0) if i % 2 else Replicate()]) for i, t in enumerate(ts)]
+        into = [torch.zeros_like(t) for t in sharded]
+        for out in (into, None):
+            got = GC.clip_grads(sharded, 0.1, out=out)
+            assert type(got) is torch.Tensor and abs(float(got) - float(norm)) <= 4e-7 * float(norm)
+            # (sums of types that are apart have another order: a factor that is off by steps of fp32)
+            assert all(torch.allclose(a.to_local().double(), b.double(), rtol=2.0 ** -7 if b.dtype == BF else 1e-6, atol=0)
+                       for a, b in zip(out or sharded, want))
+        mixed = [ts[0].clone(), DTensor.from_local(ts[1].clone(), mesh, [Shard(0)])]
+        assert abs(float(GC.grad_norm(mixed, math.inf)) - exact_norm(ts[:2], True)) == 0.0
+        with pytest.raises(TypeError):
+            GC.clip_grads([DTensor.from_local(torch.ones(3, device="cuda").half(), mesh, [Shard(0)])], 1.0)
+    finally:
+        dist.destroy_process_group()
+
+
 def test_nothing_in_the_list_and_long_tensors():
     empty = [torch.empty(0, device="cuda"), torch.empty(0, 5, device="cuda", dtype=BF)]
     assert float(GC.grad_norm(empty)) == 0.0 and float(GC.clip_grads(empty, 1.0)) == 0.0 and float(GC.clip_grads(empty, 1.0, math.inf)) == 0.0
