@@ -105,14 +105,30 @@ def _world(group) -> int:
     return dist.get_world_size(group) if group is not None and dist.is_initialized() else 1
 
 
+def _over(name: str, total: Optional[torch.Tensor], inf: bool, group) -> torch.Tensor:
+    """The total over the ranks of ``group``.  A rank without tensors (None) takes part with nothing, so that the others do not wait for it,
+    and learns whether any has one."""
+    if total is None:
+        own = torch.zeros(2, dtype=torch.float64, device="cuda" if torch.cuda.is_available() else "cpu")
+    else:
+        own = torch.stack([total, torch.ones_like(total)])
+    got = _reduced(own, inf, group)
+    if total is None and float(got[1]) == 0.0:
+        raise ValueError(f"{name} over ranks expects a tensor on each, or on one of them at least: none has any")
+    return got[0]
+
+
 def _norm(name: str, tensors: Sequence[torch.Tensor], inf: bool, group):
     """(total, norm), over the ranks of ``group`` and of the tensors' meshes too."""
+    if not tensors:
+        total = _over(name, None, inf, group)
+        return total, (total if inf else total.sqrt()).float()
     host = L._autograd_module or L.autograd()
     got = host.grad_norm(tensors, inf)
     if got is not None:
         total, norm = got
         if _world(group) > 1:
-            total = _reduced(total, inf, group)
+            total = _over(name, total, inf, group)
             norm = (total if inf else total.sqrt()).float()
         return total, norm
     parts: dict = {}           # the groups' names -> (groups, tensors whose parts lie on them)
@@ -127,7 +143,7 @@ def _norm(name: str, tensors: Sequence[torch.Tensor], inf: bool, group):
         totals.append(got[0])
     for i, (groups, _) in enumerate(parts.values()):
         for g in groups:
-            totals[i] = _reduced(totals[i], inf, g)
+            totals[i] = _over(name, totals[i], inf, g) if g is group else _reduced(totals[i], inf, g)
     total = totals[0]
     if len(totals) > 1:
         total = torch.stack(totals).amax() if inf else torch.stack(totals).sum()
@@ -137,13 +153,12 @@ def _norm(name: str, tensors: Sequence[torch.Tensor], inf: bool, group):
 @L.traced("grad_norm")
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0, group=None) -> torch.Tensor:
     """fp32 scalar: the 2-norm (or the largest magnitude, ``norm_type`` inf) of all tensors together, of DTensors as whole ones:
-    over the ranks of their meshes that they are sharded over (replicas count once).  ``group``: over the ranks of it, each of
-    which holds a part of everything; DTensors have to be sharded over just these."""
+    over the ranks of their meshes that they are sharded over (replicas count once; all ranks list the same ones).  ``group``: over
+    the ranks of it, each of which holds a part of everything, or nothing (such a rank waits for the answer); DTensors have to
+    be sharded over just these."""
     inf = _kind(norm_type)
     tensors = _list(tensors)
-    if not tensors:
-        if _world(group) > 1:
-            raise ValueError("grad_norm over ranks expects a tensor on each")
+    if not tensors and _world(group) == 1:
         return torch.zeros(())
     return _norm("grad_norm", tensors, inf, group)[1]
 
@@ -157,19 +172,19 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     on all of them.  ``error_if_nonfinite`` waits for the norm and raises before anything is scaled."""
     inf, max_norm = _kind(norm_type), float(max_norm)
     grads, outs = _list(grads), [] if out is None else _list(out)
-    if not grads:
-        if _world(group) > 1:
-            raise ValueError("clip_grads over ranks expects a tensor on each")
+    if not grads and _world(group) == 1:
         return torch.zeros(())
     if out is not None and len(outs) != len(grads):
         raise ValueError("clip_grads expects out like grads: as many tensors, of their shapes and types")
     total = None
     if error_if_nonfinite or _world(group) > 1:
-        total, _ = _norm("clip_grads", grads, inf, group)
+        total, norm = _norm("clip_grads", grads, inf, group)
         if error_if_nonfinite and not math.isfinite(float(total)):
             raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is non-finite, so it cannot "
                                "be clipped. To disable this error and scale the gradients by the non-finite norm anyway, set "
                                "`error_if_nonfinite=False`")
+        if not grads:
+            return norm
     host = L._autograd_module or L.autograd()
     got = host.clip_grads(grads, outs, max_norm, inf, total)
     if got is None:

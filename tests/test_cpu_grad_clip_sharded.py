@@ -120,6 +120,35 @@ def _one_dimension(rank):
     assert torch.equal(even.full_tensor(), full[0]) and torch.equal(copies.full_tensor(), full[3])
 
 
+def _a_rank_without_tensors(rank):
+    world = dist.group.WORLD
+    for empty in (0, 1):
+        for inf in (False, True):
+            kind = math.inf if inf else 2.0
+            for value in (numbers(9, seed=1), torch.zeros(4), torch.empty(0), torch.tensor([1.0, math.nan]), torch.tensor([math.inf])):
+                ts = [] if rank == empty else [value.clone()]
+                want = exact([value], inf) if value.numel() and not value.isnan().any() else math.nan if value.numel() else 0.0
+                same = lambda got: got.dtype == torch.float32 and got.dim() == 0 and (          # noqa: E731
+                    float(got) == pytest.approx(want, rel=1e-6, nan_ok=True))
+                assert same(GC.grad_norm(ts, kind, group=world))
+                assert same(GC.clip_grads(ts, 0.5, kind, out=[t.clone() for t in ts], group=world))
+                if not math.isfinite(want):
+                    with pytest.raises(RuntimeError, match="non-finite"):
+                        GC.clip_grads(ts, 0.5, kind, group=world, error_if_nonfinite=True)
+                assert same(GC.clip_grads(ts, 0.5, kind, group=world))          # in place
+        used = torch.nn.Parameter(torch.zeros(9))
+        if rank != empty:
+            used.grad = numbers(9, seed=2)
+        want = exact([numbers(9, seed=2)], False)
+        assert abs(float(GC.clip_grad_norm_([used], 0.5, group=world)) - want) <= 1e-6 * want
+        assert (used.grad is None) == (rank == empty)
+    for call in (lambda: GC.grad_norm([], group=world), lambda: GC.clip_grads([], 1.0, group=world), lambda: GC.clip_grads([], 1.0, out=[], group=world)):
+        with pytest.raises(ValueError, match="on one of them at least"):
+            call()
+    with pytest.raises(ValueError):          # (before anything is waited for)
+        GC.clip_grads([], 1.0, out=[torch.zeros(3)], group=world)
+
+
 def _two_dimensions(rank):
     mesh = init_device_mesh("cpu", (2, 2), mesh_dim_names=("replicas", "parts"))
     full = [numbers(5, 4, seed=1), numbers(6, 7, seed=2), numbers(3, seed=3), numbers(8, 2, seed=4)]
@@ -159,6 +188,6 @@ def _sharded_model(rank):
         assert torch.allclose(q.grad.full_tensor(), p.grad * 0.5, rtol=1e-4, atol=1e-7)
 
 
-@pytest.mark.parametrize("fn,world", [(_one_dimension, 2), (_two_dimensions, 4), (_sharded_model, 4)], ids=lambda v: getattr(v, "__name__", str(v)))
+@pytest.mark.parametrize("fn,world", [(_one_dimension, 2), (_a_rank_without_tensors, 2), (_two_dimensions, 4), (_sharded_model, 4)], ids=lambda v: getattr(v, "__name__", str(v)))
 def test_sharded_gradients(fn, world):
     over_ranks(fn, world)
