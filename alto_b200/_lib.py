@@ -84,6 +84,7 @@ EXPORTED_SYMBOLS = (
     "altob200_clip_grads",
     "altob200_set_wait_limit_ns",
     "altob200_selftest_wait_timeout",
+    "altob200_selftest_drain",
 )
 
 
@@ -323,6 +324,8 @@ def _declare_more(lib):
     lib.altob200_set_wait_limit_ns.argtypes = [C.c_uint64]
     lib.altob200_selftest_wait_timeout.restype = C.c_int
     lib.altob200_selftest_wait_timeout.argtypes = [C.c_uint64, vp]
+    lib.altob200_selftest_drain.restype = C.c_int
+    lib.altob200_selftest_drain.argtypes = [vp, vp, vp]
 
 
 def lib():
@@ -1057,3 +1060,11 @@ def set_wait_limit_ns(limit_ns: int) -> None:
 def selftest_wait_timeout(limit_ns: int = 1_000_000) -> None:
     """Launches the kernel whose waits cannot be satisfied; ``status_read`` then reports the timeout."""
     _check(lib().altob200_selftest_wait_timeout(int(limit_ns), _stream()), "altob200_selftest_wait_timeout")
+
+
+def selftest_drain():
+    """(cases in which a copy had not landed, cases) of ``altob200_selftest_drain``."""
+    src = (torch.arange(14, device="cuda", dtype=torch.uint8) + 1).repeat_interleave(1024)
+    counts = torch.zeros(2, dtype=torch.int32, device="cuda")
+    _check(lib().altob200_selftest_drain(src.data_ptr(), counts.data_ptr(), _stream()), "altob200_selftest_drain")
+    return tuple(counts.tolist())

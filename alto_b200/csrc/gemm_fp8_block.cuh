@@ -69,9 +69,9 @@ struct CfgF8 {
   // column factors (a scale for every row of B, no units), or units; and runs
   static constexpr int EXTRA_BYTES = MAX_UNITS * 4 > FAC_BYTES ? MAX_UNITS * 4 : FAC_BYTES;
   static constexpr int RUN_BYTES = 16 + MAX_RUNS * 4;      // (counts in front)
-  static constexpr int NUM_BARS = 2 * STAGES + 8 + FAC;
+  static constexpr int NUM_BARS = 2 * STAGES + 8 + FAC + 1;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + EXTRA_BYTES + RUN_BYTES + ROW_FAC_BYTES + 1024 /*align*/ + 512 /*barriers*/;
-  static_assert(NUM_BARS * 8 + 32 <= 512, "barrier area");
+  static_assert(NUM_BARS * 8 + 64 <= 512, "barrier area");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
   // setmaxnreg.inc takes only what setmaxnreg.dec released of the registers at launch
   static constexpr int REGS_LAUNCH = 168, REGS_SMALL = 56, REGS_FOLD = 224;
@@ -92,6 +92,39 @@ __device__ __forceinline__ void mbar_arrive_cluster_one(uint32_t cluster_addr) {
       "@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}"
       ::"r"(cluster_addr)
       : "memory");
+}
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+// A wait for copies that are on their way when a role has given up: a millisecond at least, however short the others' limit is.
+__device__ __forceinline__ uint64_t drain_limit(uint64_t limit) { return limit > (1ull << 21) ? limit : 1ull << 21; }
+// The operand copies of a CTA pair that are on their way when a role has given up land before the CTAs end.  The leader's producer
+// issued `mine` stages, the peer's `theirs`; a stage goes out when the one STAGES before has been consumed in both, so that only the
+// last STAGES can be on their way.  A stage's bytes complete on the leader's barrier, which expects those of both: where one did
+// not issue it, the leader makes up for that.  By one warp of the leader; once a wait has run out, the later ones have waited as long.
+template <int STAGES, int STAGE_BYTES>
+__device__ __forceinline__ void drain_pair(uint64_t* full_bar, uint32_t mine, uint32_t theirs, int lane, uint32_t never, uint64_t limit) {
+  const uint32_t most = mine > theirs ? mine : theirs;
+  bool landed = true;
+  for (uint32_t i = most < STAGES ? 0 : most - STAGES; i < most && landed; ++i) {
+    uint64_t* const bar = &full_bar[i % STAGES];
+    if (lane == 0) {
+      if (i >= mine) mbar_expect_tx(bar, STAGE_BYTES);
+      else if (i >= theirs) mbar_complete_tx(bar, STAGE_BYTES);
+    }
+    __syncwarp();
+    landed = __all_sync(0xFFFFFFFFu, mbar_wait_tight(smem_u32(bar), (i / STAGES) & 1u, never, limit));
+  }
+}
+// The same of a ring of a CTA's own barriers, whose last `issued` phases were all armed.
+template <int SLOTS>
+__device__ __forceinline__ void drain_ring(uint64_t* bars, uint32_t issued, uint32_t never, uint64_t limit) {
+  bool landed = true;
+  for (uint32_t i = issued < SLOTS ? 0 : issued - SLOTS; i < issued && landed; ++i)
+    landed = __all_sync(0xFFFFFFFFu, mbar_wait_tight(smem_u32(&bars[i % SLOTS]), (i / SLOTS) & 1u, never, limit));
 }
 __device__ __forceinline__ uint32_t thread_here() {      // (not kept in a register from elsewhere)
   uint32_t v;
@@ -244,9 +277,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   uint64_t* acc_full = bars + 2 * C::STAGES;      // each CTA, by the leader's commit [chunk & 1]
   uint64_t* acc_empty = acc_full + 4;             // leader: the fold warps of both CTAs
   uint64_t* fac_full = acc_empty + 4;             // each CTA: bytes of its own factors
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fac_full + C::FAC);
+  uint64_t* mma_done = fac_full + C::FAC;         // each CTA, where a role has given up: by the leader's last commit
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* never = abort_flag + 1;           // an abort flag that nothing raises
+  volatile uint32_t* ends = reinterpret_cast<volatile uint32_t*>(never + 1);   // stages issued here; by the peer: its own, its abort flag
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();        // 0 = leader
@@ -263,6 +298,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
       mbar_init(&acc_empty[b], C::FOLD_WARPS);
     }
     for (int f = 0; f < C::FAC; ++f) mbar_init(&fac_full[f], B_ROWS ? 2 : 1);
+    mbar_init(mma_done, 1);
     *abort_flag = 0;
     *never = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -412,10 +448,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         }
       }
       if (!alive) report_timeout(abort_flag, 31);
-      // the copies in flight land before the CTAs end (both wait for each other below), whoever gave up
-      if (leader)
-        for (uint32_t i = stages < C::STAGES ? 0 : stages - C::STAGES; i < stages; ++i)
-          (void)mbar_wait_tight(smem_u32(&full_bar[i % C::STAGES]), (i / C::STAGES) & 1u, smem_u32(const_cast<int*>(never)), limit);
+      if (lane == 0) ends[0] = stages;
     } else if (warp == 1) {
       // ------------------------------ MMA issuer (leader) ------------------------------
       if (leader) {
@@ -612,7 +645,28 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
   // Neither CTA may leave while its peer can still arrive on its barriers or read its shared memory.
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t to = mapa_u32(smem_u32(const_cast<uint32_t*>(ends) + 1), rank ^ 1u);
+    st_cluster_u32(to, ends[0]);
+    st_cluster_u32(to + 4, (uint32_t)*abort_flag);
+  }
+  __syncwarp();
   cluster_sync_all();
+  if (((uint32_t)*abort_flag | ends[2]) != 0u) {
+    // A role of either CTA gave up (both know): copies and MMAs that are on their way land.  (Where none did, all have been waited for.)
+    const uint32_t never_addr = smem_u32(const_cast<int*>(never));
+    const uint64_t patience = drain_limit(limit);
+    if (warp == 0) {
+      if (B_ROWS) drain_ring<C::FAC>(fac_full, ends[0], never_addr, patience);
+      if (leader) drain_pair<C::STAGES, C::STAGE_BYTES>(full_bar, ends[0], ends[1], lane, never_addr, patience);
+    } else if (warp == 1) {
+      if (leader && elect_one()) tc_commit_pair(mma_done);
+      __syncwarp();
+      (void)mbar_wait_tight(smem_u32(mma_done), 0, never_addr, patience);
+    }
+    __syncwarp();
+    cluster_sync_all();
+  }
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");

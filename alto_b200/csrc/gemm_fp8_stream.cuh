@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(CfgStream::THREADS, 1) fp8_stream_kernel(const
     // the copies in flight land before the CTA ends, whoever gave up
     const uint32_t n = (uint32_t)q.stages;
     for (uint32_t i = loaded < n ? 0 : loaded - n; i < loaded; ++i)
-      (void)mbar_wait_tight(smem_u32(&full[i % n]), (i / n) & 1u, smem_u32(const_cast<int*>(never)), limit);
+      (void)mbar_wait_tight(smem_u32(&full[i % n]), (i / n) & 1u, smem_u32(const_cast<int*>(never)), drain_limit(limit));
     return;
   }
 

@@ -1459,6 +1459,79 @@ __global__ void __launch_bounds__(256, 1) wait_selftest_kernel(uint64_t limit_ns
 }
 
 // ---------------------------------------------------------------------------------------
+// self-test of what a CTA pair does behind a role that gave up: copies of every number of stages that the two producers can have issued
+// ---------------------------------------------------------------------------------------
+struct DrainTest {
+  static constexpr int STAGES = 4, STAGE_BYTES = 1024, SLOTS = 8, SLOT_BYTES = 256, MOST = 14;   // (MOST: of `src`, 1024 bytes of i + 1 each)
+};
+// One cluster of two warps.  counts: {cases in which a copy had not landed, cases}.
+__global__ void __launch_bounds__(32, 1) drain_selftest_kernel(const __grid_constant__ CUtensorMap map, const uint8_t* src, int* counts, uint64_t limit_ns) {
+  using C = DrainTest;
+  __shared__ __align__(1024) uint8_t stage[C::STAGES][C::STAGE_BYTES];
+  __shared__ __align__(16) uint8_t slot[C::SLOTS][C::SLOT_BYTES];
+  __shared__ uint64_t full[C::STAGES], ring[C::SLOTS];
+  __shared__ int never;
+  const int lane = threadIdx.x;
+  const bool leader = cluster_ctarank() == 0;
+  const uint64_t limit = limit_ns * 2ull;
+  if (lane == 0) never = 0;
+  const uint32_t flag = smem_u32(&never);
+  bool first = true;
+  for (int mine = 0; mine < C::MOST - C::STAGES; ++mine)
+    for (int theirs = mine < C::STAGES ? 0 : mine - C::STAGES; theirs <= mine + C::STAGES; ++theirs) {
+      const int own = leader ? mine : theirs, most = mine > theirs ? mine : theirs;
+      if (lane == 0) {
+        for (int i = 0; i < C::STAGES + C::SLOTS; ++i) {
+          uint64_t* const bar = i < C::STAGES ? &full[i] : &ring[i - C::STAGES];
+          if (!first) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+          mbar_init(bar, 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      }
+      first = false;
+      for (int i = lane; i < C::STAGES * C::STAGE_BYTES; i += 32) stage[0][i] = 0;
+      for (int i = lane; i < C::SLOTS * C::SLOT_BYTES; i += 32) slot[0][i] = 0;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      cluster_sync_all();
+      bool ok = true;
+      for (int i = 0; i < most; ++i) {
+        if (i >= C::STAGES) {      // what the stage held has been consumed in both
+          if (leader) ok = mbar_wait_tight(smem_u32(&full[i % C::STAGES]), (i / C::STAGES - 1) & 1u, flag, limit) && ok;
+          __syncwarp();
+          cluster_sync_all();
+        }
+        if (i < own && i >= C::SLOTS) ok = mbar_wait_tight(smem_u32(&ring[i % C::SLOTS]), (i / C::SLOTS - 1) & 1u, flag, limit) && ok;
+        __syncwarp();
+        if (i < own && lane == 0) {
+          if (leader) mbar_expect_tx(&full[i % C::STAGES], 2 * C::STAGE_BYTES);
+          tma_load_2d_pair(stage[i % C::STAGES], &map, 0, i * 8, mapa_u32(smem_u32(&full[i % C::STAGES]), 0));
+          mbar_expect_tx(&ring[i % C::SLOTS], C::SLOT_BYTES);
+          bulk_load(slot[i % C::SLOTS], src + i * C::STAGE_BYTES, C::SLOT_BYTES, &ring[i % C::SLOTS]);
+        }
+        __syncwarp();
+      }
+      cluster_sync_all();
+      drain_ring<C::SLOTS>(ring, (uint32_t)own, flag, limit);
+      if (leader) drain_pair<C::STAGES, C::STAGE_BYTES>(full, (uint32_t)mine, (uint32_t)theirs, lane, flag, limit);
+      __syncwarp();
+      cluster_sync_all();
+      for (int i = most < C::STAGES ? 0 : most - C::STAGES; i < most && leader; ++i) ok = mbar_complete(smem_u32(&full[i % C::STAGES]), (i / C::STAGES) & 1u) && ok;
+      for (int i = own < C::STAGES ? 0 : own - C::STAGES; i < own; ++i)
+        for (int j = lane; j < C::STAGE_BYTES; j += 32) ok = stage[i % C::STAGES][j] == i + 1 && ok;
+      for (int i = own < C::SLOTS ? 0 : own - C::SLOTS; i < own; ++i)
+        for (int j = lane; j < C::SLOT_BYTES; j += 32) ok = slot[i % C::SLOTS][j] == i + 1 && ok;
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (lane == 0) {
+        if (!ok) atomicAdd(&counts[0], 1);
+        if (leader) atomicAdd(&counts[1], 1);
+      }
+      __syncwarp();
+      cluster_sync_all();
+    }
+}
+
+// ---------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------
 static std::atomic<uint64_t> g_wait_limit_ns{WAIT_LIMIT_NS};
@@ -2116,6 +2189,25 @@ int altob200_selftest_wait_timeout(uint64_t limit_ns, void* stream) {
   if (limit_ns == 0 || limit_ns > 1000000000ull) return ALTOB200_EINVAL_SHAPE;  // at most one second
   wait_selftest_kernel<<<1, 256, 0, (cudaStream_t)stream>>>(limit_ns);
   return cudaGetLastError() == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
+}
+
+int altob200_selftest_drain(const void* src, int32_t* counts, void* stream) {
+  if (src == nullptr || counts == nullptr) return ALTOB200_EINVAL_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(src) & 15) || (reinterpret_cast<uintptr_t>(counts) & 3)) return ALTOB200_EINVAL_ALIGN;
+  CUtensorMap map;
+  const int rc = make_tmap(&map, src, DrainTest::MOST * 8, 128, 8);
+  if (rc != ALTOB200_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(32);
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, drain_selftest_kernel, map, (const uint8_t*)src, (int*)counts, (uint64_t)20000000ull) == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
 }
 
 int altob200_status_read(void* stream, int32_t detail[4]) {

@@ -778,6 +778,13 @@ int altob200_set_wait_limit_ns(uint64_t limit_ns);
  * the host-side handling of a device timeout.  No counterpart in the reference.
  */
 int altob200_selftest_wait_timeout(uint64_t limit_ns, void* stream);
+/*
+ * One small kernel, a CTA pair, that issues copies as the two producers of the FP8 block GEMM can have done when a role gives
+ * up (every lead of one over the other), and checks that the GEMM's wait for them leaves none on its way.  src (device): 14
+ * x 1024 bytes, byte i + 1 in the i-th 1024; counts (device, zeroed): {cases in which a copy had not landed, cases}.  No
+ * counterpart in the reference.
+ */
+int altob200_selftest_drain(const void* src, int32_t* counts, void* stream);
 
 #ifdef __cplusplus
 }

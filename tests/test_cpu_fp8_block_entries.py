@@ -91,6 +91,11 @@ def test_lists(pointers, sizes, dtypes, outs):
     assert L.lib().altob200_grad_norm(None, 0, P, P, P, None) < 0
 
 
+@pytest.mark.parametrize("src,counts", [(None, P), (P, None), (P + 8, P), (P, P + 2)], ids=str)
+def test_selftest_of_the_copies(src, counts):
+    assert L.lib().altob200_selftest_drain(src, counts, None) < 0
+
+
 def _norms(rank, port):
     os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
     dist.init_process_group("gloo", rank=rank, world_size=2)

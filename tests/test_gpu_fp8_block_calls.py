@@ -493,6 +493,19 @@ def test_operands_that_were_just_written(m, n, k):
         assert all(torch.equal(a, b) for a, b in zip(got, want[i % 2]))
 
 
+def test_copies_land_before_a_pair_that_gave_up_ends():
+    """The wait behind a role that gave up, for every number of stages that the two producers can have issued (0 to 9, either up to
+    four ahead); without a wait that runs out, and with the products as they were behind it."""
+    from alto_b200 import _lib as L
+    cases = sum(min(m, 4) + 5 for m in range(10))
+    for _ in range(3):
+        assert L.selftest_drain() == (0, cases)
+    assert L.status_read()[0] == 0
+    x, w = H.numbers((300, 528), BF, 1), H.numbers((272, 528), BF, 2, 0.1)
+    exact, bound = H.product_bound(H.quantize(x, "e4m3", -1)[2], H.quantize(w, "e4m3", None)[2], BF)
+    H.assert_within(FB._to_fp8_block_then_scaled_mm(x.cuda(), w.cuda()), exact, bound)
+
+
 def test_results_do_not_change_from_call_to_call():
     x, w, dy = torch.randn(2000, 1040, device="cuda", dtype=BF), torch.randn(784, 1040, device="cuda", dtype=BF), torch.randn(2000, 784, device="cuda", dtype=BF)
 
