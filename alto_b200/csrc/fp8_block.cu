@@ -470,13 +470,16 @@ __global__ void __launch_bounds__(256) fp8b_rows_kernel(const Fp8bRows q) {
     c1 = first;
     d = static_cast<char*>(d) + (int64_t)e * q.M * q.ldd * esz;
   } else if (q.offs != nullptr) {
-    // the running maximum of the ends (see Fp8bRun), so that no row has two experts: each warp for itself
+    // the running maximum of the ends (see Fp8bRun), so that no row has two experts: looked for by those that can have rows
+    // (20 rows of 1500 experts of 48 x 144: 18 us, 32 where every one looks)
     const auto cut = [&](int o) { return o < 0 ? 0 : o > q.M ? (int)q.M : o; };
-    int before = 0;
-    for (int i = lane; i < e; i += 32) before = max(before, cut(__ldg(q.offs + i)));
-    before = __reduce_max_sync(0xFFFFFFFFu, before);
-    row0 = before;
-    if (e < q.experts) row1 = max(before, cut(__ldg(q.offs + e)));
+    const int end = e < q.experts ? cut(__ldg(q.offs + e)) : (int)q.M;
+    int before = e > 0 ? cut(__ldg(q.offs + e - 1)) : 0;
+    if (end <= before) return;
+#pragma unroll 8
+    for (int i = lane; i < e - 1; i += 32) before = max(before, cut(__ldg(q.offs + i)));
+    row0 = __reduce_max_sync(0xFFFFFFFFu, before);
+    row1 = end;
   }
   const bool zeros = e == q.experts;      // rows behind the last expert
   const uint8_t* const b = q.b + (q.k_ranges || zeros ? 0 : (int64_t)e * q.N * q.K);
