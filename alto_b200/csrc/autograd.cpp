@@ -417,14 +417,40 @@ struct GradList {
   Tensor first;
   altob200_grad_list list = {};
 
+  size_t place(const void* p) const { return (reinterpret_cast<uintptr_t>(p) * 0x9E3779B97F4A7C15ull >> 20) & (seen.size() - 1); }
   // A tensor that is there twice would be scaled by two blocks at once: refused.
   void once(const void* p) {
-    size_t at = (reinterpret_cast<uintptr_t>(p) * 0x9E3779B97F4A7C15ull >> 20) & (seen.size() - 1);
+    size_t at = place(p);
     while (seen[at] != nullptr) {
       if (seen[at] == p) throw pybind11::value_error("clip_grads expects tensors that do not overlap: one is in the list twice");
       at = (at + 1) & (seen.size() - 1);
     }
     seen[at] = p;
+  }
+
+  bool is_written(const void* p) const {
+    size_t at = place(p);
+    while (seen[at] != nullptr && seen[at] != p) at = (at + 1) & (seen.size() - 1);
+    return seen[at] != nullptr;
+  }
+
+  // A gradient that another one is scaled into would be read while it is written.  False: it takes a look at each (lists that lie in
+  // memory one behind the other, each type for itself, need none).
+  bool apart(size_t n) const {
+    uintptr_t low[4] = {UINTPTR_MAX, UINTPTR_MAX, UINTPTR_MAX, UINTPTR_MAX}, high[4] = {0, 0, 0, 0};      // read and written, of either type
+    for (int type = 0; type < 2; ++type) {
+      uintptr_t rl = UINTPTR_MAX, rh = 0, wl = UINTPTR_MAX, wh = 0;
+      for (size_t i = 0; i < n; ++i) {
+        if ((dtypes[i] == ALTOB200_DT_F32) != (type == 1)) continue;
+        const uintptr_t r = reinterpret_cast<uintptr_t>(grads[i]), w = reinterpret_cast<uintptr_t>(outs[i]);
+        rl = std::min(rl, r), rh = std::max(rh, r), wl = std::min(wl, w), wh = std::max(wh, w);
+      }
+      low[2 * type] = rl, high[2 * type] = rh, low[2 * type + 1] = wl, high[2 * type + 1] = wh;
+    }
+    for (int r = 0; r < 4; r += 2)
+      for (int w = 1; w < 4; w += 2)
+        if (low[r] <= high[w] && low[w] <= high[r]) return false;
+    return true;
   }
 
   // The tensor of an object that the kernels can take, or null.  `keys`: those of the one before, which say the same of this one.
@@ -488,6 +514,10 @@ struct GradList {
       back.emplace_back(at::empty_like(g->is_non_overlapping_and_dense() ? *g : hold.back()), *o);
       outs[i] = back.back().first.mutable_data_ptr();
     }
+    if (others && !apart(n))
+      for (size_t i = 0; i < n; ++i)
+        if (sizes[i] != 0 && grads[i] != outs[i] && is_written(grads[i]) && grads[i] != THPVariable_Unpack(others_items[i]).const_data_ptr())
+          throw pybind11::value_error("clip_grads expects out to hold none of grads but in its own place");
     // what autograd has kept of a tensor that changes is no longer what it was
     for (size_t i = 0; writes && i < n; ++i)
       if (!written[i]->is_inference()) written[i]->bump_version();

@@ -166,8 +166,8 @@ def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0, group=Non
 @L.traced("clip_grads")
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None,
                group=None, error_if_nonfinite: bool = False) -> torch.Tensor:
-    """Scales the tensors (which do not overlap) to a common norm of at most ``max_norm``, in place or into ``out`` (others of the same
-    shapes and types); returns the norm before, an fp32 scalar.  Where nothing is clipped, tensors scaled in place are not
+    """Scales the tensors (which do not overlap) to a common norm of at most ``max_norm``, in place or into ``out`` (of the same
+    shapes and types: others, or the gradient itself in its own place); returns the norm before, an fp32 scalar.  Where nothing is clipped, tensors scaled in place are not
     written.  DTensors and ``group``: as ``grad_norm`` takes them; ``out`` is sharded like ``grads``, and a norm over ranks needs the call
     on all of them.  ``error_if_nonfinite`` waits for the norm and raises before anything is scaled."""
     inf, max_norm = _kind(norm_type), float(max_norm)

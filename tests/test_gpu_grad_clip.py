@@ -163,6 +163,21 @@ def test_a_tensor_that_is_listed_twice_and_versions():
         GC.clip_grads([torch.randn(100, device="cuda")], 1e-3)
 
 
+def test_gradients_that_others_are_scaled_into():
+    flat = torch.randn(64, device="cuda")
+    a, b, c, d = (flat[16 * i:16 * i + 16] for i in range(4))
+    before = flat.clone()
+    for grads, out in (([a, b], [b, a]), ([a, b], [c, a]), ([a, b, c], [d, b, a]), ([a, b.view(4, 4).t()], [c, a.view(4, 4).t()])):
+        with pytest.raises(ValueError, match="in its own place"):
+            GC.clip_grads(grads, 1e-3, out=out)
+    assert torch.equal(flat, before)
+    norm = GC.clip_grads([a, b, c], 1e-3, out=[a, d, c])          # in its own place, or into another
+    f = factor(float(norm), 1e-3)
+    assert torch.equal(b, before[16:32])
+    for got, src in ((a, before[:16]), (d, before[16:32]), (c, before[32:48])):
+        assert bool(((got.double() - src.double() * f).abs() <= src.double().abs() * f * 25 * 2.0 ** -24).all())
+
+
 def test_refusals():
     t = torch.ones(8, device="cuda")
     for bad, kind in (([t.half()], TypeError), ([t, t.cpu()], RuntimeError), ([t.to_sparse()], ValueError), ([t.long()], TypeError), ([t, None], TypeError)):
