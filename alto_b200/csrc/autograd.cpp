@@ -10,6 +10,7 @@
 //
 // The library stays free of torch: its entry points come as addresses from the handle that alto_b200/_lib.py holds.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -510,6 +511,7 @@ struct GradList {
         grads[i] = g->const_data_ptr();
       }
       if (!writes || (g->is_non_overlapping_and_dense() && o->strides() == g->strides())) continue;
+      at::assert_no_internal_overlap(*o);      // (before anything is scaled)
       // in the order of what is read
       back.emplace_back(at::empty_like(g->is_non_overlapping_and_dense() ? *g : hold.back()), *o);
       outs[i] = back.back().first.mutable_data_ptr();

@@ -178,6 +178,20 @@ def test_gradients_that_others_are_scaled_into():
         assert bool(((got.double() - src.double() * f).abs() <= src.double().abs() * f * 25 * 2.0 ** -24).all())
 
 
+def test_tensors_that_overlap_themselves():
+    t, one = torch.randn(16, device="cuda"), torch.randn(4, 1, device="cuda")
+    before, version = t.clone(), t._version
+    spread = one.expand(4, 5)
+    for grads, out in (([t, spread], None), ([t, one.repeat(1, 5)], [torch.empty_like(t), spread])):
+        with pytest.raises(RuntimeError, match="single memory location"):
+            GC.clip_grads(grads, 1e-3, out=out)
+        assert torch.equal(t, before) and t._version == version          # nothing was scaled before
+    into = [torch.empty_like(t), torch.empty(4, 5, device="cuda")]
+    norm = GC.clip_grads([t, spread], 1e-3, out=into)
+    assert abs(float(norm) - exact_norm([t, spread], False)) <= 1e-5
+    assert torch.equal(into[1], into[1][:, :1].expand(4, 5))
+
+
 def test_refusals():
     t = torch.ones(8, device="cuda")
     for bad, kind in (([t.half()], TypeError), ([t, t.cpu()], RuntimeError), ([t.to_sparse()], ValueError), ([t.long()], TypeError), ([t, None], TypeError)):
