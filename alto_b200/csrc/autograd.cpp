@@ -364,7 +364,8 @@ bool fp8_ends(const std::optional<Tensor>& offs, const Tensor& x, int64_t expert
 }
 std::optional<Tensor> fp8_try_serve(const Tensor& x, const Tensor& w_codes, const Tensor& w_scales, const std::optional<Tensor>& offs) {
   const int64_t dims = offs.has_value() ? 3 : 2;
-  if (!fp8_number(x) || x.dim() < 1 || (dims == 3 && x.dim() != 2) || (at::GradMode::is_enabled() && x.requires_grad())) return std::nullopt;
+  if (!fp8_number(x) || x.dim() < 1 || (dims == 3 && x.dim() != 2) || (at::GradMode::is_enabled() && (x.requires_grad() || w_scales.requires_grad())))
+    return std::nullopt;
   const bool e4 = w_codes.scalar_type() == at::kFloat8_e4m3fn;
   if ((!e4 && w_codes.scalar_type() != at::kFloat8_e5m2) || w_codes.dim() != dims || w_codes.device() != x.device()) return std::nullopt;
   const int64_t N = w_codes.size(-2), K = w_codes.size(-1);

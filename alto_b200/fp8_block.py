@@ -209,7 +209,7 @@ def _check_serving(name: str, x, w_codes, w_scales, dims: int) -> None:
         raise ValueError(f"{name} expects fp32 scales {want}, got {tuple(w_scales.shape)}, {w_scales.dtype}")
     if w_codes.device != x.device or w_scales.device != x.device:
         raise ValueError(f"{name} expects all tensors on one device")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if torch.is_grad_enabled() and (x.requires_grad or w_scales.requires_grad):
         raise RuntimeError(f"{name} has no gradient: codes of weights serve evaluation")
     if L.forward_mode() and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, w_scales)):
         raise RuntimeError(f"{name} has no forward-mode derivative")

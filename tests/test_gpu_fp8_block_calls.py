@@ -75,6 +75,21 @@ def test_refusals_of_linears():
             grouped._quantize_then_fp8_block_scaled_grouped_mm(a, bb, offs=o)
 
 
+@pytest.mark.parametrize("m", [4, 40])
+def test_a_gradient_of_the_scales_is_not_dropped(m):
+    x, w = torch.randn(m, 64, device="cuda", dtype=BF), torch.randn(48, 64, device="cuda", dtype=BF)
+    codes, scales = FB.convert_to_fp8_block(w, is_2d_block=True)
+    offs = torch.tensor([m], device="cuda", dtype=torch.int32)
+    calls = (lambda s: FB.fp8_block_linear(x, codes, s), lambda s: FB.fp8_block_grouped_linear(x, codes[None], s[None], offs))
+    wants = [call(scales) for call in calls]
+    scales.requires_grad_(True)
+    for call, want in zip(calls, wants):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(scales)
+        with torch.no_grad():
+            assert torch.equal(call(scales), want)
+
+
 def test_a_tangent_is_not_dropped():
     x, w = torch.randn(32, 64, device="cuda", dtype=BF), torch.randn(48, 64, device="cuda", dtype=BF)
     codes, scales = FB.convert_to_fp8_block(w, is_2d_block=True)
