@@ -99,6 +99,23 @@ def test_product(m, n, k, out, fmt):
     H.assert_within(got, *H.product_bound(va, vb, out), "squares on both sides")
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(300, 512, 2880), (513, 272, 1040), (1100, 1040, 400), (7, 144, 2880), (200, 2064, 272)])
+def test_product_with_scales_of_rows_in_either_order(m, n, k, out, fmt):
+    # as a quantizer writes them (a view of [blocks, rows]) and without gaps, which go through other kernels where rows are many
+    a, b = H.numbers((m, k), torch.float32, m + k), H.numbers((n, k), torch.float32, n, 0.1)
+    (ca, sa, va), (cb, sb, vb) = H.quantize(a, fmt, -1), H.quantize(b, fmt, -1)
+    exact, bound = H.product_bound(va, vb, out)
+    ca, sa, cb, sb = (t.cuda() for t in (ca, sa, cb, sb))
+    for left in (sa, sa.t().contiguous().t()):
+        for right in (sb, sb.t().contiguous().t()):
+            H.assert_within(FB.blockwise_fp8_gemm(ca, left, cb, right, output_dtype=out), exact, bound)
+    qb, ws = FB.convert_to_fp8_block(b.cuda(), fp8_format=fmt)
+    assert ws.stride() == (1, n) and torch.equal(ws, sb)
+    H.assert_within(FB.blockwise_fp8_gemm(ca, sa, qb, ws, output_dtype=out), exact, bound)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m", [1, 2, 8, 9, 16, 17, 40, 200])
 def test_serving(m, dtype):
