@@ -163,7 +163,9 @@ def _square_scales(s: torch.Tensor, transposed: bool = False) -> L.Fp8BlockScale
 def blockwise_fp8_gemm(a: torch.Tensor, a_s: torch.Tensor, b: torch.Tensor, b_s: torch.Tensor,
                        output_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a b^T for codes a [M, K] and b [N, K] of one format with fp32 scales [M or ceil(M / 128), ceil(K / 128)] and
-    [N or ceil(N / 128), ceil(K / 128)]; N and K multiples of 16."""
+    [N or ceil(N / 128), ceil(K / 128)]; N and K multiples of 16.  Scales of b's rows are best as ``convert_to_fp8_block`` returns them for
+    a matrix, neighbours along the rows: without gaps along K (a copy) they take the kernel of few rows, 4096 x 4096 x 4096 in
+    1500 us for 89."""
     if not (a.is_cuda and b.is_cuda and a_s.is_cuda and b_s.is_cuda):
         raise RuntimeError("blockwise_fp8_gemm runs on CUDA tensors only (no CPU fallback)")
     if a.dtype != b.dtype:
