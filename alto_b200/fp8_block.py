@@ -159,13 +159,18 @@ def _square_scales(s: torch.Tensor, transposed: bool = False) -> L.Fp8BlockScale
     return L.Fp8BlockScale(s.data_ptr(), c if transposed else r, r if transposed else c, s.stride(0), 7, 7)
 
 
+def _many(M: int, N: int) -> bool:
+    """Whether a product is not for the kernel of few rows, which takes scales in any order (16 rows, or two rounds of tiles of 32 x 32
+    on 148 SMs)."""
+    return M > 16 and -(-M // 32) * -(-N // 32) > 296
+
+
 @L.traced("blockwise_fp8_gemm")
 def blockwise_fp8_gemm(a: torch.Tensor, a_s: torch.Tensor, b: torch.Tensor, b_s: torch.Tensor,
                        output_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a b^T for codes a [M, K] and b [N, K] of one format with fp32 scales [M or ceil(M / 128), ceil(K / 128)] and
-    [N or ceil(N / 128), ceil(K / 128)]; N and K multiples of 16.  Scales of b's rows are best as ``convert_to_fp8_block`` returns them for
-    a matrix, neighbours along the rows: without gaps along K (a copy) they take the kernel of few rows, 4096 x 4096 x 4096 in
-    1500 us for 89."""
+    [N or ceil(N / 128), ceil(K / 128)]; N and K multiples of 16.  Scales lie in any order; those of b's rows that are not neighbours along
+    the rows, as ``convert_to_fp8_block`` returns them for a matrix, are copied into that order where rows are many."""
     if not (a.is_cuda and b.is_cuda and a_s.is_cuda and b_s.is_cuda):
         raise RuntimeError("blockwise_fp8_gemm runs on CUDA tensors only (no CPU fallback)")
     if a.dtype != b.dtype:
@@ -179,12 +184,16 @@ def blockwise_fp8_gemm(a: torch.Tensor, a_s: torch.Tensor, b: torch.Tensor, b_s:
     (M, K), N = a.shape, b.shape[0]
     if K % 16 != 0 or N % 16 != 0 or N == 0 or K == 0:
         raise ValueError(f"blockwise_fp8_gemm expects N and K in multiples of 16, got N={N}, K={K}")
-    sides = []
+    sides, kept = [], None
     for name, s, rows in (("a_s", a_s, M), ("b_s", b_s, N)):
         if s.dtype != torch.float32 or s.dim() != 2 or s.shape[1] != _blocks(K) or s.shape[0] not in (rows, _blocks(rows)):
             raise ValueError(f"blockwise_fp8_gemm expects fp32 scales {name} [{rows} or {_blocks(rows)}, {_blocks(K)}], got "
                              f"{tuple(s.shape)}, {s.dtype}")
-        sides.append(L.Fp8BlockScale(s.data_ptr(), s.stride(0), s.stride(1), 0, 0 if s.shape[0] == rows else 7, 7))
+        chunk = s.stride(1) if s.shape[1] > 1 else rows
+        if name == "b_s" and s.shape[0] == rows and _many(M, N) and (s.stride(0) != 1 or chunk % 4 != 0 or s.data_ptr() % 16 != 0):
+            s = kept = s.detach().t().clone(memory_format=torch.contiguous_format).t()
+            chunk = rows
+        sides.append(L.Fp8BlockScale(s.data_ptr(), s.stride(0), chunk, 0, 0 if s.shape[0] == rows else 7, 7))
     if any(t.device != a.device for t in (a_s, b, b_s)):
         raise ValueError("blockwise_fp8_gemm expects all tensors on one device")
     out = torch.empty((M, N), dtype=output_dtype, device=a.device)

@@ -116,6 +116,24 @@ def test_product_with_scales_of_rows_in_either_order(m, n, k, out, fmt):
     H.assert_within(FB.blockwise_fp8_gemm(ca, sa, qb, ws, output_dtype=out), exact, bound)
 
 
+@pytest.mark.parametrize("m,n,k", [(600, 1040, 128), (600, 1040, 96), (520, 2064, 1040), (40, 256, 272)])
+def test_every_order_of_the_scales_gives_the_same_bits(m, n, k):
+    a, b = H.numbers((m, k), torch.float32, m + k), H.numbers((n, k), torch.float32, n, 0.1)
+    (ca, sa, va), (cb, sb, vb) = H.quantize(a, "e4m3", -1), H.quantize(b, "e4m3", -1)
+    ca, sa, cb, sb = (t.cuda() for t in (ca, sa, cb, sb))
+    best = sb.t().contiguous().t()
+    want = FB.blockwise_fp8_gemm(ca, sa, cb, best, output_dtype=torch.float32)
+    H.assert_within(want, *H.product_bound(va, vb, torch.float32))
+    chunks = sb.shape[1]
+    gaps = torch.zeros(chunks, n + 3, device="cuda")[:, :n].t()           # neighbours along the rows, blocks an odd number apart
+    shifted = torch.zeros(chunks * n + 1, device="cuda")[1:].view(chunks, n).t()
+    spread = torch.zeros(n, 2 * chunks, device="cuda")[:, ::2]
+    for s in (sb, gaps, shifted, spread):
+        s.copy_(sb)
+        got = FB.blockwise_fp8_gemm(ca, sa, cb, s, output_dtype=torch.float32)
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m", [1, 2, 8, 9, 16, 17, 40, 200])
 def test_serving(m, dtype):
