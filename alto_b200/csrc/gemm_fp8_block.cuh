@@ -42,6 +42,7 @@ struct F8Args {
   const int32_t* offs;
   int mode, experts;
   int64_t k_rows;
+  int row_base;            // mode 1: of the experts' rows, those in front of A's
   void* d;
   int64_t ldd;
   int tiles_n, group_m;
@@ -228,7 +229,7 @@ __device__ __forceinline__ int f8_lists(const F8Args& a, int lane, uint32_t* uni
   int carry_end = 0, carry = 0;
   for (int e0 = 0; e0 < total; e0 += 32) {
     const int e = e0 + lane;
-    int end = e < a.experts ? __ldg(a.offs + e) : e == a.experts ? (int)limit : 0;
+    int end = e < a.experts ? max(__ldg(a.offs + e), 0) - a.row_base : e == a.experts ? (int)limit : 0;
     end = end < 0 ? 0 : (int64_t)end > limit ? (int)limit : end;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {

@@ -2000,7 +2000,8 @@ static int launch_fp8_block(const CUtensorMap& ta, const CUtensorMap& tb, const 
   return cudaLaunchKernelEx(&cfg, kernel, ta, tb, td, args) == cudaSuccess ? ALTOB200_OK : ALTOB200_ECUDA;
 }
 
-int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st) {
+// `row_base`: of the experts' rows, those in front of a->a's (mode 1).
+static int fp8_block_gemm_rows(const altob200_fp8_block_gemm_args* a, int64_t row_base, cudaStream_t st) {
   const bool b_rows = a->sb.row_shift == 0;
   if (a->a_dtype != -1 || a->K <= 0) return ALTOB200_EUNSUPPORTED;
   if (b_rows && (a->sb.row_stride != 1 || a->sb.chunk_stride % 4 != 0 || a->mode == 1 || (reinterpret_cast<uintptr_t>(a->sb.scales) & 15)))
@@ -2028,7 +2029,7 @@ int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st)
   g.M = a->M; g.N = a->N; g.K = a->K;
   g.sa = a->sa.scales; g.sa_row = a->sa.row_stride; g.sa_chunk = a->sa.chunk_stride; g.sa_shift = a->sa.row_shift;
   g.sb = a->sb.scales; g.sb_row = a->sb.row_stride; g.sb_chunk = a->sb.chunk_stride; g.sb_expert = a->mode == 1 ? a->sb.expert_stride : 0;
-  g.offs = a->offs; g.mode = a->mode; g.experts = a->mode == 0 ? 1 : a->experts; g.k_rows = a->k_rows;
+  g.offs = a->offs; g.row_base = (int)row_base; g.mode = a->mode; g.experts = a->mode == 0 ? 1 : a->experts; g.k_rows = a->k_rows;
   g.d = a->d; g.ldd = a->ldd;
   g.tiles_n = (int)tiles_n;
   g.group_m = 4;
@@ -2038,6 +2039,22 @@ int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st)
   g.wait_ns = wait_limit_ns();
   if (obf) return b_rows ? launch_fp8_block<true, true>(ta, tb, td, g, tiles, st) : launch_fp8_block<true, false>(ta, tb, td, g, tiles, st);
   return b_rows ? launch_fp8_block<false, true>(ta, tb, td, g, tiles, st) : launch_fp8_block<false, false>(ta, tb, td, g, tiles, st);
+}
+
+int fp8_block_gemm_tiles(const altob200_fp8_block_gemm_args* a, cudaStream_t st) {
+  // A launch lists MAX_UNITS units of 256 rows; where there are more, rows go in several: 1 050 000 past 8 x 1024 x 1024 in two.
+  const int64_t most = a->mode == 1 && a->experts + 2 <= CfgF8::MAX_RUNS ? (int64_t)(CfgF8::MAX_UNITS - a->experts - 1) * 256 : a->M;
+  if (a->M <= most) return fp8_block_gemm_rows(a, 0, st);
+  for (int64_t row = 0; row < a->M; row += most) {
+    altob200_fp8_block_gemm_args w = *a;
+    w.M = a->M - row < most ? a->M - row : most;
+    w.a = static_cast<const uint8_t*>(a->a) + row * a->K;
+    w.sa.scales = a->sa.scales + (row >> a->sa.row_shift) * a->sa.row_stride;
+    w.d = static_cast<char*>(a->d) + row * a->ldd * (a->out_dtype == ALTOB200_DT_BF16 ? 2 : 4);
+    const int rc = fp8_block_gemm_rows(&w, row, st);
+    if (rc != ALTOB200_OK) return rc;      // (the first one says whether the kernel takes the operands; the others are like it)
+  }
+  return ALTOB200_OK;
 }
 
 template <int NW, int J, bool E5M2>

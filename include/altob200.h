@@ -721,9 +721,8 @@ int altob200_fp8_block_dequantize(const void* codes, int32_t format, int64_t row
  * this one is the altob200_fp8_block_quantize of A, and B, sb and offs were complete before that one began; they may then be
  * read while it runs.  N and K are multiples of 16; codes lie without gaps; everything begins on 16 bytes.
  * Limits of the tensor-memory kernel, beyond which a product of many rows takes 16 to 28 times as long (the kernel of few rows is
- * left): mode 1, ceil(M / 256) + experts + 1 <= 4096 (some 1.04 million rows); modes 1 and 2, 1022 experts; a scale for every row of B
- * (sb.row_shift 0) with row_stride 1, chunk_stride a multiple of 4, scales on 16 bytes (as the quantizer writes them;
- * blockwise_fp8_gemm brings them into that order).
+ * left): modes 1 and 2, 1022 experts; a scale for every row of B (sb.row_shift 0) with row_stride 1, chunk_stride a multiple of 4,
+ * scales on 16 bytes (as the quantizer writes them; blockwise_fp8_gemm brings them into that order).
  */
 typedef struct altob200_fp8_block_gemm_args {
   int64_t M, N, K, lda, ldd, k_rows;

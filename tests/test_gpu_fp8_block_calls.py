@@ -370,6 +370,33 @@ def test_more_experts_than_a_list_holds(m):
     assert not bool(got[at:].any()) and not bool(y[at:].any()) and not bool(dx[at:].any())
 
 
+@pytest.mark.parametrize("ends", [[300, 1047700, 1049990], [1047552, 1047552, 1047600], [1048000, 5, 2 ** 30], [0, 0, 0]], ids=str)
+def test_more_rows_than_a_launch_lists(ends):
+    # 4096 units of 256 rows, 1 047 552 rows here, and those behind them
+    m, n, k, cut = 1_050_000, 48, 144, 500_000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = torch.randn(m, k, device="cuda", generator=g).to(BF), torch.randn(m, n, device="cuda", generator=g).to(BF)
+    w = H.numbers((3 * n, k), BF, 2, 0.1).cuda().view(3, n, k)
+    codes, scales = FB.convert_to_fp8_block(w, is_2d_block=True)
+    offs = torch.tensor(ends, device="cuda", dtype=torch.int32)
+
+    def run(rows, o):
+        xl = x[rows].requires_grad_(True)
+        y = grouped._quantize_then_fp8_block_scaled_grouped_mm(xl, w.transpose(1, 2), offs=o)
+        return FB.fp8_block_grouped_linear(x[rows], codes, scales, o), y, torch.autograd.grad(y, xl, dy[rows])[0]
+    whole = run(slice(0, m), offs)
+    for rows, o in ((slice(0, cut), offs.clamp(max=cut)), (slice(cut, m), in_order(offs, m).sub(cut).clamp(min=0))):
+        assert all(torch.equal(a[rows], b) for a, b in zip(whole, run(rows, o)))
+    at = 0
+    for e, end in enumerate(in_order(offs, m).tolist()):
+        rows = sorted({r for r in (at, at + 1, (at + end) // 2, 1047551, 1047552, end - 1) if at <= r < end})
+        wv = H.quantize(w[e].cpu(), "e4m3", None)[2]
+        for got, src, right in ((whole[0], x, wv), (whole[1], x, wv), (whole[2], dy, wv.T.contiguous())):
+            H.assert_within(got[rows], *H.product_bound(H.quantize(src[rows].cpu(), "e4m3", -1)[2], right, BF))
+        at = end
+    assert not any(bool(t[at:].any()) for t in whole)
+
+
 def test_offsets_past_thirty_two_bits():
     e, n, k = 34, 4096, 32768                                # 4.6 GB of codes
     codes = torch.empty(e, n, k, device="cuda", dtype=torch.float8_e4m3fn)
